@@ -40,6 +40,7 @@ typedef struct nh_qact nh_qact; /* rotated int8 activations resident in HBM (QAc
 typedef struct nh_weights nh_weights; /* every matmul weight of a .cact archive in HBM (QWeights) */
 typedef struct nh_model nh_model;     /* a loaded model for the decode step (Model) */
 typedef struct nh_session nh_session; /* one sequence's decoding state in HBM (Session) */
+typedef struct nh_kv4 nh_kv4;         /* a paged key/value cache held in 4 bits */
 
 /* ---- runtime ----------------------------------------------------------- */
 /* Select the device and prepare the code tables.  No reference counterpart
@@ -359,6 +360,116 @@ int nh_argmax(const float* x, int n, uint32_t* dst, void* stream);
  * caller cuts at EOS.  A step that fails resets the session to empty
  * (keeping its attention span), as a failed nh_forward_outputs does. */
 int nh_generate_greedy(nh_session* s, int steps, uint32_t* out, float* logits, void* stream);
+
+/* ---- a 4-bit key/value cache ------------------------------------------- */
+/* No reference counterpart: its sessions hold their own int8 keys and values
+ * (NatState, crates/needle-engine/src/infer.rs:966-1036).  This cache is shared
+ * by many sequences of any model, in pages, at 4 bits: per row and head, groups
+ * of 32 or 64 values with low = f16(min), step = f16((max - min) * f32(1/15))
+ * and codes rint((x - low) * (1 / step)) in 0..15; it holds low + step * code.
+ * Values past +-65504 are held as that; a group with a NaN or an infinity reads
+ * as NaN and reaches no other.
+ *
+ * A sequence is an id 0 .. seqs - 1.  nh_kv4_extend names the sequences of a
+ * step (the batch) and adds rows to them; nh_kv4_append stores the batch's keys
+ * and values of one layer, nh_kv4_attend attends with the batch's queries; rows
+ * lie one sequence after the other, in the order given to extend.  Any change to
+ * a sequence of the batch other than a longer life (fork, copy, compact,
+ * truncate, free) ends the batch.
+ *
+ * Who holds which page is known on the host: every call but append and attend
+ * works at once and reports at once (NH_ENOMEM: too few free pages or sequences;
+ * a refused call changes nothing), and is refused under stream capture.  append
+ * and attend read the batch from the device: captured, they follow the state
+ * that a later extend of the same rows outside the graph leaves.  The calls on
+ * one cache are queued on one stream, or ordered by the caller's events.  A
+ * cache belongs to the device it was made on. */
+#define NH_F32 0
+#define NH_F16 1
+#define NH_BF16 2
+/* layers x kv_heads heads of qk_dim keys and v_dim values (1 to 256 each);
+ * group 32 or 64; `pages` pages of `page` (32, 64, 128 or 256) positions; up to
+ * `seqs` sequences of up to `cap` positions (rounded up to pages).  One
+ * position of a layer's head takes W + 8 W / group bytes, W = 64, 128 or 256
+ * the smallest that holds both dims.  The only call that allocates. */
+int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int page, int pages, int seqs, int cap,
+               nh_kv4** c);
+int nh_kv4_free(nh_kv4* c);
+/* Bytes in HBM. */
+int64_t nh_kv4_bytes(const nh_kv4* c);
+/* Pages that no sequence holds. */
+int nh_kv4_free_pages(const nh_kv4* c);
+/* An empty sequence; returns its id. */
+int nh_kv4_seq_new(nh_kv4* c);
+int nh_kv4_seq_len(const nh_kv4* c, int seq);
+/* Gives the sequence's pages back (those that no branch shares). */
+int nh_kv4_seq_free(nh_kv4* c, int seq);
+/* Forgets positions len .. (rejected drafts; Session::rollback without its bound). */
+int nh_kv4_seq_truncate(nh_kv4* c, int seq, int len);
+/* n branches of seq (HOST ids) that share its pages; a branch extended within
+ * a shared page gets a copy of that page first.  No device work. */
+int nh_kv4_seq_fork(nh_kv4* c, int seq, int n, int* branches);
+/* A branch with a copy of every page; returns its id. */
+int nh_kv4_seq_copy(nh_kv4* c, int seq, void* stream);
+/* Sequence seqs[i] keeps counts[i] ranges of positions, ranges[2 j] <= p <
+ * ranges[2 j + 1] (ascending, apart; the sequences' ranges one after the
+ * other; all HOST), closed up in that order: a span's sink and ring, or a
+ * drafted tree's kept path.  Whole leading pages stay, the other kept rows
+ * move to fresh pages as they are (shared pages are not written).  Keys keep
+ * what was stored, a rotation by their first position among it. */
+int nh_kv4_seq_compact(nh_kv4* c, const int* seqs, int n, const int* counts, const int* ranges, void* stream);
+/* rows[i] (>= 0) more positions for each of n distinct sequences (HOST
+ * arrays), which become the batch.  The new positions hold nothing until
+ * append has stored them. */
+int nh_kv4_extend(nh_kv4* c, const int* seqs, const int* rows, int n, void* stream);
+/* The batch's rows. */
+int nh_kv4_rows(const nh_kv4* c);
+/* The batch's rows into one layer: DEVICE k[row * ldk + head * qk_dim + d] and
+ * v[row * ldv + head * v_dim + d] of `type` (a fused product's rows can be
+ * taken as they lie). */
+int nh_kv4_append(nh_kv4* c, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int type,
+                  void* stream);
+/* The values held: rows[i] positions from pos[i] of seqs[i] (HOST arrays) of
+ * one layer, or of every layer (-1), into DEVICE k [layer][row][head][qk_dim]
+ * and v [layer][row][head][v_dim] of `type`; returns the rows. */
+int nh_kv4_read(nh_kv4* c, int layer, const int* seqs, const int* pos, const int* rows, int n, void* k, void* v,
+                int type, void* stream);
+/* Attention of the batch's rows: DEVICE q[row * ldq + head * qk_dim + d] with
+ * `heads` query heads, each kv head shared by heads / kv_heads neighbours, into
+ * out[row * ldo + head * v_dim + d], both of `type`.  The row of position i
+ * sees keys j <= i, with a ring > 0 only j < sink or j > i - ring
+ * (Session::attend's span, crates/needle-engine/src/model.rs:62-66, by
+ * position).  lse (f32 [rows][heads], or NULL): the log of the summed
+ * exponentials, to join with other keys.  Scores, weights' sums and products
+ * are held in f32; f16 and bf16 calls round a weight to 11 bits, f32 calls
+ * carry 22.  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used
+ * by the work queued on `stream` only (its size depends on the batch's
+ * lengths: asked after the extend; 0: it may be NULL). */
+int64_t nh_kv4_attend_ws_bytes(const nh_kv4* c, int heads, int sink, int ring);
+int nh_kv4_attend(const nh_kv4* c, int layer, const void* q, int64_t ldq, int heads, float scale, int sink, int ring,
+                  void* out, int64_t ldo, float* lse, int type, void* ws, uint64_t ws_bytes, void* stream);
+
+/* ---- drafted tokens ----------------------------------------------------- */
+/* No reference counterpart (generate.rs:87-139 picks one token a step).
+ * Drafts against the target's probabilities p = softmax(logits / temperature):
+ * batch b's draft i, x = drafts[b n + i], is kept while u[b (n+1) + i] q(x) <
+ * p(x) with q(x) = probs[(b n + i) ldp + x] (probs NULL: a drafter without
+ * probabilities, q(x) = 1); `counts` (or NULL: n) says how many drafts of a
+ * sequence there are.  The token after the kept ones is drawn at the uniform
+ * u[b (n+1) + n], the first t whose cumulative weight exceeds u times the
+ * whole: of max(p - q, 0) where a draft was refused (p without x when probs is
+ * NULL, and p itself where nothing is left), else of p.  Temperature 0: a draft is
+ * kept if it is the argmax (nh_argmax), the next token is the argmax, and u may
+ * be NULL.  A NaN logit is never chosen; of a row without a finite or +inf
+ * logit token 0 is taken; a draft outside the vocabulary is refused.
+ * All DEVICE: logits[(b (n+1) + i) ldl + t] of `type` (row n: after the last
+ * draft), u f32, accepted[b] = kept drafts, tokens[b][n+1] = the kept drafts,
+ * the next token, then -1.  ws: 16-byte aligned, of
+ * nh_verify_drafts_ws_bytes bytes, used by the work queued on `stream` only. */
+int64_t nh_verify_drafts_ws_bytes(int batch, int n, int vocab);
+int nh_verify_drafts(const void* logits, int type, int64_t ldl, const int32_t* drafts, const int32_t* counts,
+                     const void* probs, int probs_type, int64_t ldp, const float* u, float temperature, int batch,
+                     int n, int vocab, int32_t* accepted, int32_t* tokens, void* ws, uint64_t ws_bytes, void* stream);
 
 /* ---- seeded inputs (host) ---------------------------------------------- */
 /* jax.random.normal for float32 from a threefry key, as

@@ -89,6 +89,25 @@ SIGNATURES = {
     "nh_session_head_logits_sparse": (I, [P, P, I, P, P]),
     "nh_generate_greedy": (I, [P, I, P, P, P]),
     "nh_argmax": (I, [P, I, P, P]),
+    "nh_kv4_new": (I, [I] * 9 + [P]),
+    "nh_kv4_free": (I, [P]),
+    "nh_kv4_bytes": (C.c_int64, [P]),
+    "nh_kv4_free_pages": (I, [P]),
+    "nh_kv4_seq_new": (I, [P]),
+    "nh_kv4_seq_len": (I, [P, I]),
+    "nh_kv4_seq_free": (I, [P, I]),
+    "nh_kv4_seq_truncate": (I, [P, I, I]),
+    "nh_kv4_seq_fork": (I, [P, I, I, P]),
+    "nh_kv4_seq_copy": (I, [P, I, P]),
+    "nh_kv4_seq_compact": (I, [P, P, I, P, P, P]),
+    "nh_kv4_extend": (I, [P, P, P, I, P]),
+    "nh_kv4_rows": (I, [P]),
+    "nh_kv4_append": (I, [P, I, P, P, C.c_int64, C.c_int64, I, P]),
+    "nh_kv4_read": (I, [P, I, P, P, P, I, P, P, I, P]),
+    "nh_kv4_attend_ws_bytes": (C.c_int64, [P, I, I, I]),
+    "nh_kv4_attend": (I, [P, I, P, C.c_int64, I, C.c_float, I, I, P, C.c_int64, P, I, P, C.c_uint64, P]),
+    "nh_verify_drafts_ws_bytes": (C.c_int64, [I, I, I]),
+    "nh_verify_drafts": (I, [P, I, C.c_int64, P, P, P, I, C.c_int64, P, C.c_float, I, I, I, P, P, P, C.c_uint64, P]),
     "nh_normal": (I, [C.c_uint32, C.c_uint32, C.c_uint64, P]),
     "nh_split": (I, [C.c_uint32, C.c_uint32, P]),
 }
@@ -684,3 +703,6 @@ def seeded_normals(sizes, seed: int = 0):
         key, sub = split(key)
         outs.append(normal(sub, n))
     return outs
+
+
+from .kv4 import KvCache4, verify_drafts  # noqa: E402,F401

@@ -1,0 +1,242 @@
+"""The 4-bit key/value cache and the check of drafted tokens over the C ABI
+(nh_kv4_* and nh_verify_drafts in include/needle_hip.h).  Neither has a
+counterpart in the reference."""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+
+import numpy as np
+import torch
+
+import needle_hip as nh
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # NH_F32, NH_F16, NH_BF16
+
+
+def _ints(v) -> np.ndarray:
+    a = np.asarray(v, dtype=np.int64).reshape(-1)
+    if a.size and (a.min() < -(1 << 31) or a.max() >= 1 << 31):
+        raise ValueError("not a 32-bit number")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def _on(stream):
+    """Allocations of the call come from the memory of the stream that uses them."""
+    return torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext()
+
+
+def _workspace(n: int, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+class KvCache4:
+    """A paged cache of keys and values in 4 bits, shared by many sequences
+    (nh_kv4).  A step: `extend` names its sequences and their new rows; then,
+    for every layer, `append` stores the rows' keys and values and `attend`
+    attends with their queries."""
+
+    def __init__(self, layers: int, kv_heads: int, qk_dim: int, v_dim: int, pages: int, seqs: int, cap: int,
+                 group: int = 32, page: int = 64):
+        lib = nh.load_library()
+        self.h = None
+        if torch.cuda.is_available():
+            nh.init()
+        h = C.c_void_p()
+        nh._check(lib.nh_kv4_new(int(layers), int(kv_heads), int(qk_dim), int(v_dim), int(group), int(page), int(pages),
+                                 int(seqs), int(cap), C.byref(h)))
+        self.h = h
+        self.layers, self.kv_heads, self.qk_dim, self.v_dim = int(layers), int(kv_heads), int(qk_dim), int(v_dim)
+        self.group, self.page, self.pages = int(group), int(page), int(pages)
+        self.device = torch.device("cuda", torch.cuda.current_device())
+
+    # ---- sequences
+    def new_seq(self) -> int:
+        """An empty sequence's id."""
+        return nh._check(nh._lib.nh_kv4_seq_new(self.h))
+
+    def length(self, seq: int) -> int:
+        return nh._check(nh._lib.nh_kv4_seq_len(self.h, int(seq)))
+
+    def free(self, seq: int):
+        """Gives back the pages that no branch shares."""
+        nh._check(nh._lib.nh_kv4_seq_free(self.h, int(seq)))
+
+    def truncate(self, seq: int, length: int):
+        """Forgets positions `length` and on."""
+        nh._check(nh._lib.nh_kv4_seq_truncate(self.h, int(seq), int(length)))
+
+    def fork(self, seq: int, n: int = 1) -> list:
+        """n branches that share the sequence's pages until they are written."""
+        out = np.zeros(max(int(n), 1), dtype=np.int32)
+        nh._check(nh._lib.nh_kv4_seq_fork(self.h, int(seq), int(n), nh._hptr(out)))
+        return out[:n].tolist()
+
+    def copy(self, seq: int, stream=None) -> int:
+        """A branch with pages of its own."""
+        return nh._check(nh._lib.nh_kv4_seq_copy(self.h, int(seq), nh._stream(stream)))
+
+    def compact(self, seqs, ranges, stream=None):
+        """Sequence seqs[i] keeps the positions of ranges[i], ascending (begin,
+        end) pairs, closed up."""
+        s = _ints(seqs)
+        if len(ranges) != s.size:
+            raise ValueError("one list of ranges for each sequence")
+        counts = _ints([len(r) for r in ranges])
+        flat = _ints([x for r in ranges for pair in r for x in pair])
+        if flat.size != 2 * int(counts.sum()):
+            raise ValueError("a range is a (begin, end) pair")
+        nh._check(nh._lib.nh_kv4_seq_compact(self.h, nh._hptr(s), s.size, nh._hptr(counts), nh._hptr(flat),
+                                             nh._stream(stream)))
+
+    @property
+    def free_pages(self) -> int:
+        return nh._check(nh._lib.nh_kv4_free_pages(self.h))
+
+    def bytes(self) -> int:
+        n = nh._lib.nh_kv4_bytes(self.h)
+        nh._check(-1 if n < 0 else 0)
+        return n
+
+    # ---- rows
+    def extend(self, seqs, rows, stream=None):
+        """rows[i] more positions for each sequence; they become the batch."""
+        s, r = _ints(seqs), _ints(rows)
+        if s.size != r.size:
+            raise ValueError("one number of rows for each sequence")
+        nh._check(nh._lib.nh_kv4_extend(self.h, nh._hptr(s), nh._hptr(r), s.size, nh._stream(stream)))
+
+    @property
+    def rows(self) -> int:
+        """The batch's rows."""
+        return nh._check(nh._lib.nh_kv4_rows(self.h))
+
+    def _rows_of(self, t: torch.Tensor, heads: int, dim: int, what: str) -> int:
+        """The row stride of [rows][heads][dim]; a row lies in one piece."""
+        if t.dim() != 3 or t.shape[1:] != (heads, dim) or t.shape[0] != self.rows:
+            raise ValueError(f"{what} is [{self.rows}][{heads}][{dim}], not {list(t.shape)}")
+        if t.device != self.device or t.dtype not in _TYPES:
+            raise ValueError(f"{what} is f32, f16 or bf16 on {self.device}")
+        if (dim > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != dim):
+            raise ValueError(f"a row of {what} is not contiguous")
+        return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, stream=None):
+        """The batch's keys [rows][kv_heads][qk_dim] and values [rows][kv_heads][v_dim]
+        into one layer; rows may be a view of a wider matrix's columns."""
+        ldk = self._rows_of(k, self.kv_heads, self.qk_dim, "k")
+        ldv = self._rows_of(v, self.kv_heads, self.v_dim, "v")
+        if k.dtype != v.dtype:
+            raise ValueError("k and v differ in type")
+        nh._check(nh._lib.nh_kv4_append(self.h, int(layer), k.data_ptr(), v.data_ptr(), ldk, ldv, _TYPES[k.dtype],
+                                        nh._stream(stream)))
+
+    def read(self, layer, seqs, starts, rows, dtype=torch.float32, stream=None):
+        """The values held: rows[i] positions from starts[i] of seqs[i], as (k
+        [rows][kv_heads][qk_dim], v [rows][kv_heads][v_dim]); with layer None of
+        every layer, [layers] in front."""
+        s, p, r = _ints(seqs), _ints(starts), _ints(rows)
+        if not s.size == p.size == r.size:
+            raise ValueError("one start and one number of rows for each sequence")
+        if dtype not in _TYPES:
+            raise ValueError("f32, f16 or bf16")
+        n = int(np.maximum(r, 0).sum(dtype=np.int64))
+        shape = (n, self.kv_heads) if layer is not None else (self.layers, n, self.kv_heads)
+        with _on(stream):
+            k = torch.empty((*shape, self.qk_dim), dtype=dtype, device=self.device)
+            v = torch.empty((*shape, self.v_dim), dtype=dtype, device=self.device)
+        if layer is not None and int(layer) < 0:
+            raise ValueError("no such layer")
+        nh._check(nh._lib.nh_kv4_read(self.h, -1 if layer is None else int(layer), nh._hptr(s), nh._hptr(p), nh._hptr(r),
+                                      s.size, k.data_ptr(), v.data_ptr(), _TYPES[dtype], nh._stream(stream)))
+        return k, v
+
+    def attend(self, layer: int, q: torch.Tensor, scale: float | None = None, sink: int = 0, ring: int = 0,
+               out: torch.Tensor | None = None, lse: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """Attention of the batch's queries [rows][heads][qk_dim] over their
+        sequences, each up to its own position; with a ring > 0 over the first
+        `sink` positions and its last `ring`.  Returns [rows][heads][v_dim] of
+        q's type (`out`, if given); lse (f32 [rows][heads]) takes the logs of
+        the summed exponentials.  scale: 1 / sqrt(qk_dim) unless given."""
+        heads = q.shape[1] if q.dim() == 3 else 0
+        ldq = self._rows_of(q, heads, self.qk_dim, "q")
+        with _on(stream):
+            if out is None:
+                out = torch.empty((q.shape[0], heads, self.v_dim), dtype=q.dtype, device=self.device)
+            ldo = self._rows_of(out, heads, self.v_dim, "out")
+            if out.dtype != q.dtype:
+                raise ValueError("q and out differ in type")
+            if lse is not None and (lse.dtype != torch.float32 or lse.shape != (q.shape[0], heads) or
+                                    not lse.is_contiguous() or lse.device != self.device):
+                raise ValueError("lse is a contiguous f32 [rows][heads]")
+            n = nh._lib.nh_kv4_attend_ws_bytes(self.h, heads, int(sink), int(ring))
+            if n < 0:
+                nh._check(int(n))
+            ws = _workspace(n, self.device)
+        nh._check(nh._lib.nh_kv4_attend(self.h, int(layer), q.data_ptr(), ldq, heads,
+                                        float(self.qk_dim ** -0.5 if scale is None else scale), int(sink), int(ring),
+                                        out.data_ptr(), ldo, _ptr(lse), _TYPES[q.dtype], _ptr(ws), n, nh._stream(stream)))
+        return out
+
+    def __del__(self):
+        if getattr(self, "h", None) and nh is not None and nh._lib is not None:
+            nh._lib.nh_kv4_free(self.h)
+        self.h = None
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor | None = None,
+                  probs: torch.Tensor | None = None, counts: torch.Tensor | None = None, temperature: float = 1.0,
+                  stream=None):
+    """Drafted tokens [batch][n] (int32) against the target's logits [batch][n +
+    1][vocab] from uniforms u [batch][n + 1] (nh_verify_drafts): (accepted
+    [batch], tokens [batch][n + 1]: the kept drafts, the next token, then -1),
+    int32.  probs [batch][n][vocab]: the drafter's probabilities (None: it has
+    none); counts [batch]: drafts of each sequence (None: n); temperature 0:
+    greedy.  Rows of logits and probs may be padded (a view of wider rows)."""
+    nh.init()
+    if logits.dim() != 3 or drafts.dim() != 2:
+        raise ValueError("logits are [batch][n + 1][vocab], drafts [batch][n]")
+    batch, rows, vocab = logits.shape
+    n = rows - 1
+    device = logits.device
+
+    def strided(t, what):
+        if t.dtype not in _TYPES or t.device != device or not t.is_cuda:
+            raise ValueError(f"{what}: f32, f16 or bf16 on the logits' device")
+        ld = t.stride(1) if t.shape[1] > 1 else t.stride(0) if t.shape[0] > 1 else t.shape[2]
+        if t.shape[2] > 1 and t.stride(2) != 1 or t.shape[0] > 1 and t.stride(0) != ld * t.shape[1]:
+            raise ValueError(f"the rows of {what} do not follow each other")
+        return max(ld, t.shape[2])
+
+    def plain(t, dtype, shape, what):
+        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on the logits' device")
+
+    ldl, ldp = strided(logits, "logits"), 0
+    plain(drafts, torch.int32, (batch, n), "drafts")
+    if u is not None:
+        plain(u, torch.float32, (batch, n + 1), "u")
+    if counts is not None:
+        plain(counts, torch.int32, (batch,), "counts")
+    if probs is not None:
+        if tuple(probs.shape) != (batch, n, vocab):
+            raise ValueError("probs are [batch][n][vocab]")
+        ldp = strided(probs, "probs") if probs.numel() else vocab
+    if device.index != torch.cuda.current_device():
+        raise ValueError("the tensors are on another device than the current one")
+    ws_bytes = nh._lib.nh_verify_drafts_ws_bytes(batch, n, vocab)
+    if ws_bytes < 0:
+        nh._check(int(ws_bytes))
+    with _on(stream):
+        accepted = torch.empty(batch, dtype=torch.int32, device=device)
+        tokens = torch.empty((batch, n + 1), dtype=torch.int32, device=device)
+        ws = _workspace(ws_bytes, device)
+    nh._check(nh._lib.nh_verify_drafts(logits.data_ptr(), _TYPES[logits.dtype], ldl, _ptr(drafts), _ptr(counts),
+                                       _ptr(probs), _TYPES[probs.dtype] if probs is not None else 0, ldp, _ptr(u),
+                                       float(temperature), batch, n, vocab, accepted.data_ptr(), tokens.data_ptr(),
+                                       _ptr(ws), ws_bytes, nh._stream(stream)))
+    return accepted, tokens
