@@ -205,8 +205,13 @@ int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int p
 
 int nh_kv4_free(nh_kv4* c) {
     if (!c) return NH_OK;
+    // A cache may be collected while this thread captures a graph of other
+    // work: in the relaxed mode the release does not end that capture.
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
     if (c->data) hipFree(c->data);
     if (c->state) hipFree(c->state);
+    if (relaxed) hipThreadExchangeStreamCaptureMode(&mode);
     delete c;
     return NH_OK;
 }
@@ -423,7 +428,7 @@ static int longest(const nh_kv4* c) {
 int64_t nh_kv4_attend_ws_bytes(const nh_kv4* c, int heads, int sink, int ring) {
     if (!c) return fail(NH_EINVAL, "null cache");
     if (int rc = check_attend(c, 0, heads, sink, ring)) return rc;
-    return (int64_t)nh::kv4_attend_ws(c->v, heads, sink, ring, longest(c));
+    return (int64_t)nh::kv4_attend_ws(c->v, c->book.batch_row0.data(), heads, sink, ring, longest(c));
 }
 
 int nh_kv4_attend(const nh_kv4* c, int layer, const void* q, int64_t ldq, int heads, float scale, int sink, int ring,
@@ -437,11 +442,11 @@ int nh_kv4_attend(const nh_kv4* c, int layer, const void* q, int64_t ldq, int he
     if (ldq < (int64_t)heads * c->v.dk || ldo < (int64_t)heads * c->v.dv)
         return fail(NH_EINVAL, "rows overlap: a row holds every head");
     const int most = longest(c);
-    const size_t need = nh::kv4_attend_ws(c->v, heads, sink, ring, most);
+    const size_t need = nh::kv4_attend_ws(c->v, c->book.batch_row0.data(), heads, sink, ring, most);
     if (need && (!ws || (uintptr_t)ws % 16 != 0)) return fail(NH_EINVAL, "no 16-byte aligned workspace");
     if (ws_bytes < need) return fail(NH_ESMALL, "the workspace is too small");
     nh::Kv4AttendArgs a{q, out, lse, type, layer, heads, sink, ring, ldq, ldo, scale, ws};
-    NH_TRY(nh::launch_kv4_attend(c->v, a, most, (hipStream_t)stream), "kv4 attention");
+    NH_TRY(nh::launch_kv4_attend(c->v, c->book.batch_row0.data(), a, most, (hipStream_t)stream), "kv4 attention");
     return NH_OK;
 }
 

@@ -19,8 +19,10 @@
 //                                  (i = 0 .. 3) at nibble i; it is the half
 //                                  t % 2 of dword ((t / 4) 16 + o) 2 NB +
 //                                  (t / 2 % 2) NB + b, NB = W / 64
-//   key scales   T x NG dwords     step in the low half, low in the high half
-//   value scales T x NG dwords
+//   key steps    T x NG f16
+//   key lows     T x NG f16
+//   value steps  T x NG f16
+//   value lows   f16 of (t, g) at (t / 4 NG + g) 4 + t % 4
 // That is the order in which a wavefront's MFMA operands want them: 16 lanes
 // (keys, or dims) by 4 lane groups kg, 8 codes of the summed index a dword,
 // and the two codes of a 16-bit half pair are one mask away (see the attention
@@ -51,7 +53,9 @@ struct Kv4View {
     __host__ __device__ size_t page_bytes() const { return block() * heads * layers; }
     __host__ __device__ uint32_t v_off() const { return (uint32_t)page() * width / 2; }
     __host__ __device__ uint32_t ks_off() const { return (uint32_t)page() * width; }
+    __host__ __device__ uint32_t kl_off() const { return (uint32_t)page() * (width + 2 * groups()); }
     __host__ __device__ uint32_t vs_off() const { return (uint32_t)page() * (width + 4 * groups()); }
+    __host__ __device__ uint32_t vl_off() const { return (uint32_t)page() * (width + 6 * groups()); }
 };
 
 // Values of the device's int32 state: (index, value) pairs.
@@ -101,8 +105,9 @@ hipError_t launch_kv4_append(const Kv4View& c, int layer, const void* k, const v
 // layer < 0: all, [layers][rows]; `rows` rows a layer in the output, this launch's from `row`.
 hipError_t launch_kv4_read(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,
                            int type, hipStream_t s);
-// Bytes of workspace an attention call of the batch needs; longest: the batch's longest sequence.
-size_t kv4_attend_ws(const Kv4View& c, int heads, int sink, int ring, int longest);
-hipError_t launch_kv4_attend(const Kv4View& c, const Kv4AttendArgs& a, int longest, hipStream_t s);
+// Bytes of workspace an attention call of the batch needs; row0: the host's copy
+// of the sequences' first rows; longest: the batch's longest sequence.
+size_t kv4_attend_ws(const Kv4View& c, const int* row0, int heads, int sink, int ring, int longest);
+hipError_t launch_kv4_attend(const Kv4View& c, const int* row0, const Kv4AttendArgs& a, int longest, hipStream_t s);
 
 }  // namespace nh

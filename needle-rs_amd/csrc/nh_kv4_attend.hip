@@ -2,96 +2,618 @@
 //
 //   o = sum_j softmax_j(scale q . k_j) v_j over the keys j <= i of row i's
 //   sequence; with a ring also j < sink or j > i - ring.
+//
+// With k_j = low + step c_j per group g, and the same of v_j:
+//   scale q . k_j = cq sum_g step_jg (q_g . c_jg) + sum_g low_jg (scale sum q_g)
+//   o = (sum_g sum_j (p_j step_jg) c_jg + sum_j p_j low_jg) / sum_j p_j
+// The two sums over low are matrix products of their own, with the lows as they
+// are stored: of the queries' sums (two f16 parts, 22 bits) and of the weights.
+// so the codes themselves are the matrix operands: a code 0 .. 15 under a
+// 16-bit mask is the f16 subnormal c 2^-24 (under the next nibble's mask 16 c
+// 2^-24), which the f16 MFMAs take exactly; unpacking is one AND for two
+// codes, and no value is dequantized.  The powers of two go into q and the
+// result.  The products are transposed, keys (or dims) by rows: S^T = K Q^T
+// leaves lane (row = lane % 16, kg = lane / 16) the scores of its row's keys 4 kg
+// + 0..3 of each 16, which is the operand that O^T = V^T P^T wants of that lane
+// (the order of the summed keys is free), so a weight never leaves its lane, and
+// a row's maximum, sum and correction are one lane's scalars.
+#include <algorithm>
+#include <type_traits>
+
 #include "nh_kv4_device.h"
 
 namespace nh {
 
-// One wavefront for each (row, head), 64 keys a step: a lane a key for the
-// scores, a lane a dim (and each 64th on) for the sums.
-template <int TYPE, int W>
-__global__ __launch_bounds__(64) void k_kv4_attend(Kv4View c, Kv4AttendArgs a) {
-    typedef typename Kv4Elem<TYPE>::T T;
-    __shared__ float qs[W];
-    __shared__ float ps[64];
-    __shared__ const uint8_t* blks[64];
-    const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y;
-    const int kvh = head / (a.heads / c.heads);
-    const int b = c.each ? row / c.each : kv4_entry(c.brow0, c.nb, row, lane);
-    const int seq = c.bseq[b];
-    const int i = c.len[seq] - c.brow0[b + 1] + row;
-    const T* q = reinterpret_cast<const T*>(a.q) + row * a.ldq + (int64_t)head * c.dk;
-    for (int d = lane; d < W; d += 64) qs[d] = d < c.dk ? Kv4Elem<TYPE>::get(q + d) : 0.0f;
-    __syncthreads();
-    float m = -__builtin_inff(), l = 0.0f, acc[W / 64] = {};
-    const int mask = c.page() - 1, ng = c.groups();
-    for (int j0 = 0; j0 <= i; j0 += 64) {
-        if (a.ring && j0 >= a.sink && j0 + 63 <= i - a.ring) continue;
-        const int j = j0 + lane;
-        const bool seen = j <= i && (!a.ring || j < a.sink || j > i - a.ring);
-        float s = -__builtin_inff();
-        const int pg = seen ? kv4_page(c, seq, j) : -1;
-        if (pg >= 0) {
-            const uint8_t* blk = kv4_block(c, pg, a.layer, kvh);
-            blks[lane] = blk;
-            const int slot = j & mask;
-            const uint32_t* codes = reinterpret_cast<const uint32_t*>(blk) + slot * (W / 8);
-            const uint32_t* scales = reinterpret_cast<const uint32_t*>(blk + c.ks_off()) + slot * ng;
-            s = 0.0f;
-            for (int t = 0; t * 8 < c.dk; ++t) {
-                const uint32_t w = codes[(t & 3) * (W / 32) + (t >> 2)], sc = scales[t * 8 / c.group];
-                for (int e = 0; e < 8; ++e) {
-                    const float k = __builtin_fmaf(kv4_step(sc), (float)((w >> (4 * ((e & 1) * 4 + (e >> 1)))) & 15u), kv4_low(sc));
-                    s = t * 8 + e < c.dk ? __builtin_fmaf(qs[t * 8 + e], k, s) : s;
-                }
-            }
-            s *= a.scale;
-        }
-        float most = s;
-        for (int h = 1; h < 64; h <<= 1) most = fmaxf(most, lane_xor(most, h, lane));
-        const float next = fmaxf(m, most);
-        const float keep = m == next ? 1.0f : expf(m - next);
-        const float p = pg >= 0 ? expf(s - next) : 0.0f;
-        m = next;
-        l = l * keep + p;
-        ps[lane] = p;
-        __syncthreads();
-        for (int x = 0; x < W / 64; ++x) {
-            const int d = 64 * x + lane, o = d & 15, n = (d & 63) >> 4;
-            acc[x] *= keep;
-            if (d >= c.dv) continue;
-            for (int y = 0; y < 64; ++y) {
-                const float w = ps[y];
-                if (w == 0.0f) continue;
-                const int slot = (j0 + y) & mask;
-                const uint16_t code = reinterpret_cast<const uint16_t*>(blks[y] + c.v_off())
-                    [(((slot >> 2) * 16 + o) * 2 * (W / 64) + ((slot >> 1) & 1) * (W / 64) + x) * 2 + (slot & 1)];
-                const uint32_t sc = reinterpret_cast<const uint32_t*>(blks[y] + c.vs_off())[slot * ng + d / c.group];
-                acc[x] = __builtin_fmaf(w, __builtin_fmaf(kv4_step(sc), (float)(code >> (4 * n) & 15), kv4_low(sc)), acc[x]);
-            }
-        }
-        __syncthreads();
-    }
-    for (int h = 1; h < 64; h <<= 1) l += lane_xor(l, h, lane);
-    T* out = reinterpret_cast<T*>(a.out) + row * a.ldo + (int64_t)head * c.dv;
-    const float r = 1.0f / l;
-    for (int x = 0; x < W / 64; ++x)
-        if (64 * x + lane < c.dv) Kv4Elem<TYPE>::put(out + 64 * x + lane, acc[x] * r);
-    if (a.lse && lane == 0) a.lse[(int64_t)row * a.heads + head] = m + logf(l);
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int KA_WAVES = 4;    // wavefronts of a workgroup, each every fourth chunk
+constexpr int KA_CHUNK = 32;   // keys of a step of a wavefront; a page holds whole chunks
+constexpr float KA_LOG2E = 1.44269504088896340736f;
+
+// The value of lane `I` of each row of 16 lanes (DPP row_newbcast).
+template <int I>
+__device__ __forceinline__ float row_bcast(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + I, 0xF, 0xF, true));
+}
+// Maximum and sum over the four lane groups of a row's lane.
+__device__ __forceinline__ float groups_max(float v) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const float y = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    const uint32_t z = __builtin_bit_cast(uint32_t, y);
+    auto b = __builtin_amdgcn_permlane16_swap(z, z, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const float y = __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
+    const uint32_t z = __builtin_bit_cast(uint32_t, y);
+    auto b = __builtin_amdgcn_permlane16_swap(z, z, false, false);
+    return __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
 }
 
-size_t kv4_attend_ws(const Kv4View&, int, int, int, int) { return 0; }
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float pow2i(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
+template <int I, int N, class F>
+__device__ __forceinline__ void static_for(F f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>());
+        static_for<I + 1, N>(f);
+    }
+}
+
+struct KaPlan {
+    int splits;      // key ranges of a sequence; more than one: partial results go to the workspace
+    int tiles_each;  // row tiles of every sequence when they are equal, else 0
+    int aligned;     // rows of q can be read 8 elements at a time
+};
+
+// The chunks that a tile of rows at positions lo .. hi sees: [0, ns) and [w, n).
+struct KaSpan {
+    int ns, w, n;
+    __device__ __forceinline__ KaSpan(int lo, int hi, int sink, int ring) {
+        n = hi / KA_CHUNK + 1;
+        ns = 0, w = 0;
+        if (ring) {
+            ns = min((int)(((int64_t)sink + KA_CHUNK - 1) / KA_CHUNK), n);
+            w = max(ns, max(0, lo - ring + 1) / KA_CHUNK);
+        }
+    }
+    __device__ __forceinline__ int count() const { return ns + n - w; }
+    __device__ __forceinline__ int at(int i) const { return i < ns ? i : i - ns + w; }
+};
+
+// What a lane loads of a chunk: two tiles of 16 keys.
+template <int W, int NG>
+struct KaChunk {
+    static constexpr int NS = (4 * NG + 15) / 16;
+    static constexpr int NL = (NG + 1) / 2;  // dwords of a key's lows
+    uint32_t k[2][W / 32], v[2][W / 32], kl[2][NL], vl[2][2];
+    uint16_t ks[2][NS], vs[2][NS];
+};
+
+template <int TYPE, int W, int G, int RT>
+__global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
+    typedef typename Kv4Elem<TYPE>::T T;
+    constexpr int NG = W / G, NB = W / 64, NJ = W / 32, GJ = G / 32, GI = G / 16;
+    constexpr int PARTS = TYPE == KV4_F32 ? 2 : 1;  // f16 halves of a query element and of a weight
+    typedef KaChunk<W, NG> Chunk;
+    constexpr int LD = W + 4;
+    __shared__ float so[KA_WAVES][16][LD];
+    __shared__ float sm[KA_WAVES][16], sl[KA_WAVES][16], spl[KA_WAVES][16][8];
+
+    const int tid = threadIdx.x, lane = tid & 63, o = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kvh = blockIdx.x % c.heads, per = a.heads / c.heads, split = blockIdx.y;
+
+    // The sequence and the rows of this tile.
+    int tile = blockIdx.x / c.heads, b;
+    if (plan.tiles_each) {
+        b = tile / plan.tiles_each;
+        tile -= b * plan.tiles_each;
+    } else {
+        b = 0;
+        for (int i = 0; i < c.nb; i += 64) {
+            int n = 0;
+            if (i + lane < c.nb) n = ((c.brow0[i + lane + 1] - c.brow0[i + lane]) * per + 16 * RT - 1) / (16 * RT);
+            int sum = n;  // tiles up to and with this lane's sequence
+#pragma unroll
+            for (int h = 1; h < 64; h <<= 1) {
+                const int x = __shfl_up(sum, h, 64);
+                if (lane >= h) sum += x;
+            }
+            const uint64_t before = __ballot(sum <= tile && i + lane < c.nb);
+            const int skip = __popcll(before);
+            const int last = __shfl(sum, skip ? skip - 1 : 0, 64);
+            b += skip;
+            if (skip) tile -= last;
+            if (skip < 64) break;
+        }
+        b = __builtin_amdgcn_readfirstlane(b);
+        tile = __builtin_amdgcn_readfirstlane(tile);
+    }
+    if (b >= c.nb) return;
+    const int row0 = c.brow0[b], nrows = c.brow0[b + 1] - row0;
+    const int seq = c.bseq[b], len = c.len[seq];
+    const int first = len - nrows, r0 = tile * 16 * RT;
+    if (first < 0 || r0 >= nrows * per) return;  // (a state that no extend of this shape leaves)
+    const int r1 = min(r0 + 16 * RT, nrows * per) - 1;
+    const int plo = first + r0 / per, phi = first + r1 / per;
+
+    // The queries: f16 operands scaled by a power of two to just under 2^15,
+    // elements 2, 3, 6, 7 of 8 by 1/16 for their codes' 16; the sums of each group.
+    h8 q[RT][PARTS][NJ];
+    h8 qs[RT];
+    float cq[RT];
+    int pos[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = min(r0 + rt * 16 + o, r1), t = r / per;
+        pos[rt] = first + t;
+        const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(row0 + t) * a.ldq + (int64_t)(kvh * per + r - t * per) * c.dk;
+        float x[NJ][8], most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int d = j * 32 + kg * 8;
+            if (plan.aligned) {
+                typedef T Vec __attribute__((ext_vector_type(8)));
+                Vec y = {};
+                if (d < c.dk) y = *reinterpret_cast<const Vec*>(src + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][e] = (float)y[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][e] = d + e < c.dk ? Kv4Elem<TYPE>::get(src + d + e) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[j][e]));
+        }
+        most = groups_max(most);
+        const int ef = max((int)(__builtin_bit_cast(uint32_t, most) >> 23 & 255u), 15);
+        const float up = __builtin_bit_cast(float, (uint32_t)(268 - ef) << 23);
+        // scores: (2^18 sum step z + low . qs) cq, z = 2^-24 up (q . c), qs = 2^-6 up sum q
+        cq[rt] = (a.scale * KA_LOG2E * 64.0f) * __builtin_bit_cast(float, (uint32_t)(ef - 14) << 23);
+        qs[rt] = h8{};
+        static_for<0, NG>([&](auto GG) {
+            constexpr int g = GG.value;
+            float s = 0.0f;
+#pragma unroll
+            for (int j = g * GJ; j < (g + 1) * GJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s += x[j][e] * up;
+            s = groups_sum(s) * 0.015625f;
+            const _Float16 hi = (_Float16)s, lo = (_Float16)(s - (float)hi);
+            qs[rt][g] = kg == 0 ? hi : kg == 1 ? lo : (_Float16)0.0f;
+        });
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = x[j][e] * up, f = e & 2 ? 0.0625f : 1.0f;
+                const _Float16 hi = (_Float16)y;
+                q[rt][0][j][e] = (_Float16)((float)hi * f);
+                if constexpr (PARTS == 2) q[rt][1][j][e] = (_Float16)((y - (float)hi) * f);
+            }
+    }
+
+    f32x4 acc[RT][W / 16];
+    f32x4 accl[RT];  // 2^15 sum_j p_j low_jg: group 4 kg + r
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -__builtin_inff();
+        l[rt] = 0.0f;
+        accl[rt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < W / 16; ++i) acc[rt][i] = f32x4{0, 0, 0, 0};
+    }
+    // The weights are kept as 2^15 p, and with their steps as the f16 operand
+    // 2^15 p step / 2^eref, 2^eref above every step seen so far: at most 2^15,
+    // and exact to 11 bits down to 2^-29 of it.
+    int eref = -24;
+
+    const KaSpan span(plo, phi, a.sink, a.ring);
+    const int per_split = max((span.count() + plan.splits - 1) / plan.splits, KA_WAVES);
+    const int c0 = split * per_split, c1 = min(c0 + per_split, span.count());
+
+    const int* table = c.table + (size_t)seq * c.table_ld;
+    auto page_of = [&](int i) { return i < c1 ? table[span.at(i) * KA_CHUNK >> c.page_log2] : 0; };
+    const uint32_t sidx = o & (4 * NG - 1);
+    auto load = [&](Chunk& x, int i, int pg) {
+        const int slot = span.at(i) * KA_CHUNK & (c.page() - 1);
+        // (a page id comes from the cache's own table; a bad one is not followed)
+        const uint8_t* blk = kv4_block(c, (unsigned)pg < (unsigned)c.pages ? pg : 0, a.layer, kvh);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t ko = (uint32_t)(slot + 16 * t + o) * (W / 2) + kg * (W / 8);
+            const uint32_t vo = c.v_off() + ((uint32_t)((slot >> 2) + 4 * t + kg) * 16 + o) * (8 * NB);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) x.k[t][j] = reinterpret_cast<const uint32_t*>(blk + ko)[j];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) x.v[t][j] = reinterpret_cast<const uint32_t*>(blk + vo)[j];
+            const uint32_t so = ((uint32_t)(slot + 16 * t + 4 * kg) * NG + sidx) * 2;
+#pragma unroll
+            for (int n = 0; n < Chunk::NS; ++n) {
+                x.ks[t][n] = kv4_half(blk, c.ks_off() + so + 32 * n);
+                x.vs[t][n] = kv4_half(blk, c.vs_off() + so + 32 * n);
+            }
+            const uint32_t kl = c.kl_off() + (uint32_t)(slot + 16 * t + o) * NG * 2;
+            if constexpr (NG == 1)
+                x.kl[t][0] = kv4_half(blk, kl);
+            else
+#pragma unroll
+                for (int n = 0; n < NG / 2; ++n) x.kl[t][n] = reinterpret_cast<const uint32_t*>(blk + kl)[n];
+            const uint32_t vl = c.vl_off() + ((uint32_t)((slot >> 2) + 4 * t + kg) * NG + (o & (NG - 1))) * 8;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) x.vl[t][n] = reinterpret_cast<const uint32_t*>(blk + vl)[n];
+        }
+    };
+
+    auto compute = [&](const Chunk& x, int i) {
+        const int key0 = span.at(i) * KA_CHUNK;
+        const bool whole = key0 + KA_CHUNK - 1 <= plo &&
+                           (!a.ring || key0 + KA_CHUNK - 1 < a.sink || key0 > phi - a.ring);
+        // The steps' reference: raised (a wavefront at a time) when a step passes it.
+        uint32_t top = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < Chunk::NS; ++n) {
+                const uint32_t s = x.vs[t][n];
+                const int key = key0 + 16 * t + 4 * kg + (int)(sidx + 16 * n) / NG;
+                if (s < 0x7c00u && key <= phi) top = max(top, s);
+            }
+        // step < 2^(e - 14) for the f16 exponent field e (subnormals below 2^-14)
+        if (__any((int)(top >> 10) - 14 > eref)) {
+            int e = (int)(top >> 10) - 14;
+#pragma unroll
+            for (int h = 1; h < 64; h <<= 1) e = max(e, __shfl_xor(e, h, 64));
+            const float down = pow2i(max(eref - e, -126));
+            eref = __builtin_amdgcn_readfirstlane(e);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int k = 0; k < W / 16; ++k) acc[rt][k] *= down;
+        }
+        const float wscale = pow2i(-eref);
+        float kstep[2][Chunk::NS], vstep[2][Chunk::NS];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < Chunk::NS; ++n) {
+                kstep[t][n] = f16_value(x.ks[t][n]) * 262144.0f;
+                vstep[t][n] = f16_value(x.vs[t][n]) * wscale;
+            }
+        h8 ka[2][NJ];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t w = x.k[t][j], z = w >> 8;
+                const u32x4 y = {w & 0x000f000fu, w & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u};
+                ka[t][j] = __builtin_bit_cast(h8, y);
+            }
+        h8 pw[RT][NG][PARTS];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const bool fresh = m[rt] == -__builtin_inff();  // no key seen yet
+            const float base = fresh ? 0.0f : m[rt];
+            float s[2][4];  // 15 + log2 of the weight against the maximum so far
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                u32x4 y = {};
+#pragma unroll
+                for (int n = 0; n < Chunk::NL; ++n) y[n] = x.kl[t][n];
+                f32x4 lows = {0, 0, 0, 0};
+                lows = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, y), qs[rt], lows, 0, 0, 0);
+                f32x4 z[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    z[g] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int j = g * GJ; j < (g + 1) * GJ; ++j)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p)
+                            z[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[t][j], q[rt][p][j], z[g], 0, 0, 0);
+                }
+                static_for<0, 4>([&](auto R) {
+                    constexpr int r = R.value;
+                    float sum = lows[r];
+                    static_for<0, NG>([&](auto GG) {
+                        constexpr int g = GG.value, at = r * NG + g;
+                        sum = __builtin_fmaf(row_bcast<at % 16>(kstep[t][at / 16]), z[g][r], sum);
+                    });
+                    s[t][r] = __builtin_fmaf(sum, cq[rt], 15.0f - base);
+                });
+            }
+            bool seen[2][4];
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = key0 + 16 * t + 4 * kg + r;
+                        seen[t][r] = j <= pos[rt] && (!a.ring || j < a.sink || j > pos[rt] - a.ring);
+                        s[t][r] = seen[t][r] ? s[t][r] : -__builtin_inff();
+                    }
+            }
+            float most = s[0][0];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) most = fmaxf(most, s[k / 4][k % 4]);
+            most = groups_max(most);
+            if (__any(most > 15.0f || fresh)) {
+                // A new maximum (the first: whatever it is).
+                const float over = most == -__builtin_inff() ? 0.0f : fresh ? most - 15.0f : fmaxf(most - 15.0f, 0.0f);
+                const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
+                m[rt] = fresh && most == -__builtin_inff() ? m[rt] : base + over;
+                l[rt] *= keep;
+                accl[rt] *= keep;
+#pragma unroll
+                for (int k = 0; k < W / 16; ++k) acc[rt][k] *= keep;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[k / 4][k % 4] -= over;
+            }
+            float p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                p[k] = __builtin_amdgcn_exp2f(s[k / 4][k % 4]);
+                l[rt] += p[k];
+            }
+            // Two numbers to f16 at a time; f32 calls carry what that rounds off.
+            auto halves = [&](const float* w, h8* to) {
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) {
+                    const f32x2 y = {w[k], w[k + 1]};
+                    const h2 hi = __builtin_convertvector(y, h2);
+                    to[0][k] = hi[0], to[0][k + 1] = hi[1];
+                    if constexpr (PARTS == 2) {
+                        to[1][k] = (_Float16)(w[k] - (float)hi[0]);
+                        to[1][k + 1] = (_Float16)(w[k + 1] - (float)hi[1]);
+                    }
+                }
+            };
+            h8 pp[PARTS];
+            halves(p, pp);
+            const u32x4 vl = {x.vl[0][0], x.vl[0][1], x.vl[1][0], x.vl[1][1]};
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k)
+                accl[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vl), pp[k], accl[rt], 0, 0, 0);
+            static_for<0, NG>([&](auto GG) {
+                constexpr int g = GG.value;
+                float w[8];
+                static_for<0, 8>([&](auto K) {
+                    constexpr int k = K.value, at = (k % 4) * NG + g;
+                    w[k] = p[k] * row_bcast<at % 16>(vstep[k / 4][at / 16]);
+                });
+                if (!whole)  // (a step may be NaN: a hidden key's weight is none)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) w[k] = seen[k / 4][k % 4] ? w[k] : 0.0f;
+                halves(w, pw[rt][g]);
+            });
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            // dword (token pair, n) of each quad: dims 64 n + 16 i + o for i = 0 .. 3
+            const uint32_t w[4] = {x.v[0][n], x.v[0][NB + n], x.v[1][n], x.v[1][NB + n]};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                u32x4 y;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = (i & 2 ? w[k] >> 8 : w[k]) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+                const h8 va = __builtin_bit_cast(h8, y);
+                const int d = 4 * n + i;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p)
+                        acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pw[rt][d / GI][p], acc[rt][d], 0, 0, 0);
+            }
+        }
+    };
+
+    // The next chunk's loads are issued before this one's arithmetic, its page
+    // id one step earlier still.
+    {
+        Chunk x, y;
+        int i = c0 + wave;
+        int pg = page_of(i);
+        if (i < c1) load(x, i, pg);
+        pg = page_of(i + KA_WAVES);
+        for (; i < c1; i += 2 * KA_WAVES) {
+            const int i1 = i + KA_WAVES, i2 = i1 + KA_WAVES;
+            if (i1 < c1) load(y, i1, pg);
+            pg = page_of(i2);
+            compute(x, i);
+            if (i1 >= c1) break;
+            if (i2 < c1) load(x, i2, pg);
+            pg = page_of(i2 + KA_WAVES);
+            compute(y, i1);
+        }
+    }
+
+    // The wavefronts' sums joined, 16 rows at a time.
+    const float unit = pow2i(24 - 15 + eref);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        l[rt] = groups_sum(l[rt]);
+        if (l[rt] != l[rt]) m[rt] = l[rt];  // NaN scores: the row's, whatever other ranges hold
+        if (rt) __syncthreads();
+        if (kg == 0) sm[wave][o] = m[rt], sl[wave][o] = l[rt] * 0x1p-15f;
+        if (4 * kg < NG) *reinterpret_cast<f32x4*>(&spl[wave][o][4 * kg]) = accl[rt] * 0x1p-15f;
+        __syncthreads();
+        float most = sm[0][o];
+#pragma unroll
+        for (int w = 1; w < KA_WAVES; ++w) most = fmaxf(most, sm[w][o]);
+        const float base = most == -__builtin_inff() ? 0.0f : most;
+        const float f = __builtin_amdgcn_exp2f(m[rt] - base);
+#pragma unroll
+        for (int i = 0; i < W / 16; ++i) {
+            const float u = i & 1 ? unit * 0.0625f : unit, low = spl[wave][o][i / GI];
+            f32x4 y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = (acc[rt][i][r] * u + low) * f;
+            *reinterpret_cast<f32x4*>(&so[wave][o][16 * i + 4 * kg]) = y;
+        }
+        __syncthreads();
+        for (int x = tid; x < 16 * W; x += KA_WAVES * 64) {
+            const int rr = x / W, d = x % W, r = r0 + rt * 16 + rr;
+            if (r > r1 || d >= c.dv) continue;
+            float top = sm[0][rr];
+#pragma unroll
+            for (int w = 1; w < KA_WAVES; ++w) top = fmaxf(top, sm[w][rr]);
+            const float zero = top == -__builtin_inff() ? 0.0f : top;
+            float sum = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < KA_WAVES; ++w) {
+                sum = __builtin_fmaf(sl[w][rr], __builtin_amdgcn_exp2f(sm[w][rr] - zero), sum);
+                v += so[w][rr][d];
+            }
+            const int t = r / per, head = kvh * per + r - t * per;
+            const int64_t row = row0 + t;
+            if (plan.splits == 1) {
+                Kv4Elem<TYPE>::put(reinterpret_cast<T*>(a.out) + row * a.ldo + (int64_t)head * c.dv + d, v / sum);
+                if (a.lse && d == 0) a.lse[row * a.heads + head] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
+            } else {
+                const int64_t at = ((int64_t)split * c.rows + row) * a.heads + head;
+                float* ml = reinterpret_cast<float*>(a.ws);
+                ml[2 * ((int64_t)plan.splits * c.rows * a.heads) + at * c.dv + d] = v;
+                if (d == 0) ml[2 * at] = top, ml[2 * at + 1] = sum;
+            }
+        }
+    }
+}
+
+// The key ranges' partial results of one (row, head), joined by a workgroup: the
+// ranges' factors first, then a wavefront every fourth range, eight loads at a
+// time (one wavefront in turn over the 256 ranges of a long sequence took 170 us).
+constexpr int KA_SPLITS = 512;
 template <int TYPE>
-static hipError_t attend_typed(const Kv4View& c, const Kv4AttendArgs& a, hipStream_t s) {
-    auto kern = c.width == 64 ? k_kv4_attend<TYPE, 64> : c.width == 128 ? k_kv4_attend<TYPE, 128> : k_kv4_attend<TYPE, 256>;
-    hipLaunchKernelGGL(kern, dim3(c.rows, a.heads), dim3(64), 0, s, c, a);
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, int splits) {
+    typedef typename Kv4Elem<TYPE>::T T;
+    __shared__ float f[KA_SPLITS], sv[4][256], st[4], ss[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t n = (int64_t)c.rows * a.heads, at = blockIdx.x;
+    const float* ml = reinterpret_cast<const float*>(a.ws);
+    const float* po = ml + 2 * n * splits + at * c.dv;
+    float top = -__builtin_inff();
+    for (int s = tid; s < splits; s += 256) {
+        f[s] = ml[2 * (s * n + at)];
+        top = fmaxf(top, f[s]);
+    }
+#pragma unroll
+    for (int h = 1; h < 64; h <<= 1) top = fmaxf(top, lane_xor(top, h, lane));
+    if (lane == 0) st[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(st[0], st[1]), fmaxf(st[2], st[3]));
+    const float zero = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+    for (int s = tid; s < splits; s += 256) {
+        f[s] = __builtin_amdgcn_exp2f(f[s] - zero);  // 0: a range without keys, which wrote no sums
+        sum += f[s] == 0.0f ? 0.0f : ml[2 * (s * n + at) + 1] * f[s];
+    }
+#pragma unroll
+    for (int h = 1; h < 64; h <<= 1) sum += lane_xor(sum, h, lane);
+    if (lane == 0) ss[wave] = sum;
+    __syncthreads();
+    sum = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+    for (int x = 0; x * 64 < c.dv; ++x) {
+        const int d = x * 64 + lane;
+        float v = 0.0f;
+        for (int s0 = wave; s0 < splits; s0 += 32) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = s0 + 4 * k < splits && d < c.dv ? po[(s0 + 4 * k) * n * c.dv + d] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float g = s0 + 4 * k < splits ? f[s0 + 4 * k] : 0.0f;
+                v = g == 0.0f ? v : __builtin_fmaf(y[k], g, v);
+            }
+        }
+        sv[wave][d & 255] = v;
+    }
+    __syncthreads();
+    if (tid < c.dv) {
+        T* out = reinterpret_cast<T*>(a.out) + at / a.heads * a.ldo + at % a.heads * c.dv;
+        Kv4Elem<TYPE>::put(out + tid, ((sv[0][tid] + sv[1][tid]) + (sv[2][tid] + sv[3][tid])) / sum);
+    }
+    if (a.lse && tid == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
+}
+
+// Row tiles of the batch, 16 RT rows (tokens by query heads of a kv head) each.
+static int64_t tiles_of(const Kv4View& c, const int* row0, int per, int rt, int* each) {
+    int64_t n = 0;
+    *each = 0;
+    if (c.each) {
+        *each = (int)(((int64_t)c.each * per + 16 * rt - 1) / (16 * rt));
+        return (int64_t)*each * c.nb;
+    }
+    for (int b = 0; b < c.nb; ++b) n += ((int64_t)(row0[b + 1] - row0[b]) * per + 16 * rt - 1) / (16 * rt);
+    return n;
+}
+
+static int row_tiles(const Kv4View& c, int per) {
+    // Two tiles a wavefront once a sequence fills them: the keys are unpacked once for both.
+    return c.width <= 128 && (int64_t)(c.rows / (c.nb ? c.nb : 1)) * per > 16 ? 2 : 1;
+}
+
+static int splits_of(const Kv4View& c, const int* row0, int heads, int sink, int ring, int longest) {
+    const int per = heads / c.heads;
+    int each;
+    const int64_t base = tiles_of(c, row0, per, row_tiles(c, per), &each) * c.heads;
+    const int64_t keys = ring ? std::min<int64_t>(longest, (int64_t)sink + ring + c.rows + 2 * KA_CHUNK) : longest;
+    const int64_t chunks = (keys + KA_CHUNK - 1) / KA_CHUNK;
+    // Two workgroups a CU, as many as their registers let run, but at least
+    // four steps for each wavefront of a range. (64 sequences of 4096 to 8192
+    // keys, 8 kv heads: 512 workgroups 129 us, 1024 139, 2048 146; 131,072 keys:
+    // 42, 46, 55 us. Two or one step instead of four: 1060 visible keys 41 and
+    // 60 us for 31.)
+    const int64_t want = std::min<int64_t>(base > 0 ? (512 + base - 1) / base : 1, KA_SPLITS);
+    return (int)std::max<int64_t>(1, std::min(want, chunks / (4 * KA_WAVES)));
+}
+
+size_t kv4_attend_ws(const Kv4View& c, const int* row0, int heads, int sink, int ring, int longest) {
+    const int s = splits_of(c, row0, heads, sink, ring, longest);
+    return s > 1 ? (size_t)s * c.rows * heads * (c.dv + 2) * 4 : 0;
+}
+
+template <int TYPE, int W, int G>
+static hipError_t attend_shaped(const Kv4View& c, const int* row0, const Kv4AttendArgs& a, int longest, hipStream_t s) {
+    const int per = a.heads / c.heads, rt = row_tiles(c, per);
+    const size_t es = sizeof(typename Kv4Elem<TYPE>::T);
+    KaPlan plan;
+    const int64_t tiles = tiles_of(c, row0, per, rt, &plan.tiles_each);
+    plan.splits = splits_of(c, row0, a.heads, a.sink, a.ring, longest);
+    plan.aligned = c.dk % 8 == 0 && (uintptr_t)a.q % 16 == 0 && a.ldq * es % 16 == 0 && c.dk * es % 16 == 0;
+    if (tiles * c.heads > 0x7fffffff || (int64_t)c.rows * a.heads > 0x7fffffff) return hipErrorInvalidValue;
+    auto kern = k_kv4_attend<TYPE, W, G, 1>;
+    if constexpr (W <= 128)
+        if (rt == 2) kern = k_kv4_attend<TYPE, W, G, 2>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * c.heads), plan.splits), dim3(KA_WAVES * 64), 0, s, c, a, plan);
+    if (plan.splits > 1) {
+        hipLaunchKernelGGL(k_kv4_join<TYPE>, dim3((unsigned)(c.rows * a.heads)), dim3(256), 0, s, c, a, plan.splits);
+    }
     return hipGetLastError();
 }
 
-hipError_t launch_kv4_attend(const Kv4View& c, const Kv4AttendArgs& a, int, hipStream_t s) {
-    return a.type == KV4_F32   ? attend_typed<KV4_F32>(c, a, s)
-           : a.type == KV4_F16 ? attend_typed<KV4_F16>(c, a, s)
-                               : attend_typed<KV4_BF16>(c, a, s);
+template <int TYPE>
+static hipError_t attend_typed(const Kv4View& c, const int* row0, const Kv4AttendArgs& a, int longest, hipStream_t s) {
+    if (c.group == 32)
+        return c.width == 64    ? attend_shaped<TYPE, 64, 32>(c, row0, a, longest, s)
+               : c.width == 128 ? attend_shaped<TYPE, 128, 32>(c, row0, a, longest, s)
+                                : attend_shaped<TYPE, 256, 32>(c, row0, a, longest, s);
+    return c.width == 64    ? attend_shaped<TYPE, 64, 64>(c, row0, a, longest, s)
+           : c.width == 128 ? attend_shaped<TYPE, 128, 64>(c, row0, a, longest, s)
+                            : attend_shaped<TYPE, 256, 64>(c, row0, a, longest, s);
+}
+
+hipError_t launch_kv4_attend(const Kv4View& c, const int* row0, const Kv4AttendArgs& a, int longest, hipStream_t s) {
+    return a.type == KV4_F32   ? attend_typed<KV4_F32>(c, row0, a, longest, s)
+           : a.type == KV4_F16 ? attend_typed<KV4_F16>(c, row0, a, longest, s)
+                               : attend_typed<KV4_BF16>(c, row0, a, longest, s);
 }
 
 }  // namespace nh

@@ -28,9 +28,20 @@ struct Kv4Elem<KV4_BF16> {
     static __device__ __forceinline__ void put(T* p, float v) { *p = (__bf16)v; }
 };
 
-// Half of a scale dword: step (low half) or low (high half) as f32.
-__device__ __forceinline__ float kv4_step(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)w); }
-__device__ __forceinline__ float kv4_low(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)); }
+__device__ __forceinline__ float f16_value(uint32_t bits) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+
+// Where the step and the low of (slot, group) lie in a block, in bytes from
+// its start: keys, values.
+__device__ __forceinline__ uint32_t kv4_k_scale(const Kv4View& c, int slot, int g) { return c.ks_off() + 2 * (slot * c.groups() + g); }
+__device__ __forceinline__ uint32_t kv4_k_low(const Kv4View& c, int slot, int g) { return c.kl_off() + 2 * (slot * c.groups() + g); }
+__device__ __forceinline__ uint32_t kv4_v_scale(const Kv4View& c, int slot, int g) { return c.vs_off() + 2 * (slot * c.groups() + g); }
+__device__ __forceinline__ uint32_t kv4_v_low(const Kv4View& c, int slot, int g) {
+    return c.vl_off() + 2 * (((slot >> 2) * c.groups() + g) * 4 + (slot & 3));
+}
+__device__ __forceinline__ uint16_t& kv4_half(uint8_t* blk, uint32_t at) { return *reinterpret_cast<uint16_t*>(blk + at); }
+__device__ __forceinline__ uint16_t kv4_half(const uint8_t* blk, uint32_t at) { return *reinterpret_cast<const uint16_t*>(blk + at); }
 
 // The batch entry that holds `row`: the count of entries that end at or
 // before it (row0 ascends; an entry without rows is passed over).  One load

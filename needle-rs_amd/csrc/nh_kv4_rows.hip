@@ -19,7 +19,7 @@ hipError_t launch_kv4_patch(int* state, const Kv4Patch& p, hipStream_t s) {
 // ------------------------------------------------------------------- rows
 // Of one group: low, step and the reciprocal the codes are taken with.
 struct Kv4Group {
-    uint32_t scales;  // step | low << 16
+    uint16_t sb, lb;  // step and low as stored
     float low, inv;   // inv 0: every code is 0
 };
 __device__ __forceinline__ Kv4Group kv4_group(float mn, float mx, bool bad) {
@@ -32,13 +32,9 @@ __device__ __forceinline__ Kv4Group kv4_group(float mn, float mx, bool bad) {
     Kv4Group g;
     g.low = (float)low;
     g.inv = step > (_Float16)0.0f ? 1.0f / (float)step : 0.0f;
-    uint32_t sb = __builtin_bit_cast(uint16_t, step), lb = __builtin_bit_cast(uint16_t, low);
-    if (bad) {
-        sb = 0x7e00u;
-        lb = 0;
-        g.inv = 0.0f;
-    }
-    g.scales = sb | lb << 16;
+    g.sb = bad ? (uint16_t)0x7e00u : __builtin_bit_cast(uint16_t, step);
+    g.lb = bad ? (uint16_t)0 : __builtin_bit_cast(uint16_t, low);
+    if (bad) g.inv = 0.0f;
     return g;
 }
 __device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Group& g) {
@@ -82,8 +78,10 @@ __device__ __forceinline__ void kv4_store_k(const Kv4View& c, const typename Kv4
             if (t * 8 + e < c.dk) w |= kv4_code(v[e], g) << (4 * ((e & 1) * 4 + (e >> 1)));
         if (t < W / 8) {
             reinterpret_cast<uint32_t*>(blk + (size_t)slot * (W / 2))[(t & 3) * (W / 32) + (t >> 2)] = w;
-            if (t % per == 0)
-                reinterpret_cast<uint32_t*>(blk + c.ks_off())[slot * c.groups() + t / per] = g.scales;
+            if (t % per == 0) {
+                kv4_half(blk, kv4_k_scale(c, slot, t / per)) = g.sb;
+                kv4_half(blk, kv4_k_low(c, slot, t / per)) = g.lb;
+            }
         }
     }
 }
@@ -98,7 +96,6 @@ __device__ __forceinline__ void kv4_store_v(const Kv4View& c, const typename Kv4
     float v[W / 16];
 #pragma unroll
     for (int i = 0; i < W / 16; ++i) v[i] = 16 * i + o < c.dv ? Kv4Elem<TYPE>::get(x + 16 * i + o) : 0.0f;
-    uint32_t* scales = reinterpret_cast<uint32_t*>(blk + c.vs_off()) + slot * c.groups();
     // `gi` dims of each lane to a group: 2 or 4
     auto group = [&](int i0, int gi) {
         float mn = __builtin_inff(), mx = -__builtin_inff();
@@ -120,7 +117,10 @@ __device__ __forceinline__ void kv4_store_v(const Kv4View& c, const typename Kv4
 #pragma unroll
         for (int i = i0; i < i0 + gi; ++i)
             if (16 * i + o < c.dv) half[i / 4] |= (uint16_t)(kv4_code(v[i], g) << (4 * (i & 3)));
-        if (o == 0) scales[i0 / gi] = g.scales;
+        if (o == 0) {
+            kv4_half(blk, kv4_v_scale(c, slot, i0 / gi)) = g.sb;
+            kv4_half(blk, kv4_v_low(c, slot, i0 / gi)) = g.lb;
+        }
     };
     if (c.group == 32) {
 #pragma unroll
@@ -197,34 +197,33 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, Kv4Span
     const int head = (int)(u % quads) * 4 + (lane >> 4);
     if (pg < 0 || head >= c.heads) return;
     const uint8_t* blk = kv4_block(c, pg, layer0 + (int)blockIdx.y, head);
-    const int slot = pos & (c.page() - 1), ng = c.groups();
+    const int slot = pos & (c.page() - 1);
     const int64_t at = ((int64_t)blockIdx.y * rows + row_at + row) * c.heads + head;
     if (u < quads) {
-        const uint32_t* scales = reinterpret_cast<const uint32_t*>(blk + c.ks_off()) + slot * ng;
 #pragma unroll
         for (int t0 = 0; t0 < W / 8; t0 += 16) {
             const int t = t0 + o;
             if (t * 8 >= c.dk) continue;
             const uint32_t code = reinterpret_cast<const uint32_t*>(blk + (size_t)slot * (W / 2))[(t & 3) * (W / 32) + (t >> 2)];
-            const uint32_t sc = scales[t * 8 / c.group];
+            const int g = t * 8 / c.group;
+            const float step = f16_value(kv4_half(blk, kv4_k_scale(c, slot, g))), low = f16_value(kv4_half(blk, kv4_k_low(c, slot, g)));
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (t * 8 + e < c.dk)
                     Kv4Elem<TYPE>::put(k + at * c.dk + t * 8 + e,
-                                       __builtin_fmaf(kv4_step(sc), (float)((code >> (4 * ((e & 1) * 4 + (e >> 1)))) & 15u),
-                                                      kv4_low(sc)));
+                                       __builtin_fmaf(step, (float)((code >> (4 * ((e & 1) * 4 + (e >> 1)))) & 15u), low));
         }
     } else {
-        const uint32_t* scales = reinterpret_cast<const uint32_t*>(blk + c.vs_off()) + slot * ng;
         const uint16_t* codes = reinterpret_cast<const uint16_t*>(blk + c.v_off()) +
                                 (((slot >> 2) * 16 + o) * 2 * NB + ((slot >> 1) & 1) * NB) * 2 + (slot & 1);
 #pragma unroll
         for (int i = 0; i < W / 16; ++i) {
             const int d = 16 * i + o;
             if (d >= c.dv) continue;
-            const uint32_t sc = scales[d / c.group];
+            const int g = d / c.group;
             const uint32_t code = (uint32_t)codes[2 * (i >> 2)] >> (4 * (i & 3)) & 15u;
-            Kv4Elem<TYPE>::put(v + at * c.dv + d, __builtin_fmaf(kv4_step(sc), (float)code, kv4_low(sc)));
+            Kv4Elem<TYPE>::put(v + at * c.dv + d, __builtin_fmaf(f16_value(kv4_half(blk, kv4_v_scale(c, slot, g))), (float)code,
+                                                                 f16_value(kv4_half(blk, kv4_v_low(c, slot, g)))));
         }
     }
 }
@@ -294,8 +293,10 @@ __global__ __launch_bounds__(256) void k_kv4_runs(Kv4View c, const int* __restri
                    (((s1 >> 2) * 16 + l) * 2 * nb + ((s1 >> 1) & 1) * nb) * 2 + (s1 & 1);
     for (int b = 0; b < nb; ++b) zv[2 * b] = av[2 * b];
     if (l < ng) {
-        reinterpret_cast<uint32_t*>(z + c.ks_off())[s1 * ng + l] = reinterpret_cast<const uint32_t*>(a + c.ks_off())[s0 * ng + l];
-        reinterpret_cast<uint32_t*>(z + c.vs_off())[s1 * ng + l] = reinterpret_cast<const uint32_t*>(a + c.vs_off())[s0 * ng + l];
+        kv4_half(z, kv4_k_scale(c, s1, l)) = kv4_half(a, kv4_k_scale(c, s0, l));
+        kv4_half(z, kv4_k_low(c, s1, l)) = kv4_half(a, kv4_k_low(c, s0, l));
+        kv4_half(z, kv4_v_scale(c, s1, l)) = kv4_half(a, kv4_v_scale(c, s0, l));
+        kv4_half(z, kv4_v_low(c, s1, l)) = kv4_half(a, kv4_v_low(c, s0, l));
     }
 }
 

@@ -428,6 +428,22 @@ def test_changes_are_refused_under_capture(nh):
     torch.cuda.synchronize()
 
 
+def test_a_cache_is_freed_during_a_capture(nh):
+    """The collector may run inside a capture: a cache that goes there leaves the graph whole."""
+    c = nh.KvCache4(1, 1, 64, 64, pages=4, seqs=3, cap=64)
+    x = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x.add_(1)
+        del c
+        x.add_(2)
+    for i in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert x.tolist() == [3.0 * (i + 1)] * 4
+
+
 def test_a_captured_step_follows_the_cache(nh):
     """append and attention of a step captured once, replayed after each extend (other lengths, a page border,
     a fork's copied page), with eager work between; every replay against the eager call."""
