@@ -2,8 +2,8 @@
 // HBM allocation, the book of who holds them (nh_kv4_book.h) and its mirror
 // on the device.
 //
-// The mirror is an int32 array: the sequences' page ids and lengths, and the
-// batch (its sequences and their first rows).  The host keeps a copy of what
+// The mirror is an int32 array: the sequences' page ids, and the batch (its
+// sequences, their rows and lengths).  The host keeps a copy of what
 // it sent and sends what changed as kernel arguments, so a step of a decoding
 // loop is one small launch, no host memory has to outlive the call, and every
 // kernel after it on the stream sees the new state.  Append and attention read
@@ -30,7 +30,7 @@ struct nh_kv4 {
     int* state = nullptr;
     size_t n_state = 0;
     // where the mirror's parts start
-    size_t o_table = 0, o_len = 0, o_bseq = 0, o_brow0 = 0, o_fresh = 0;
+    size_t o_table = 0, o_batch = 0, o_fresh = 0;
     std::vector<int> sent;  // the mirror's values but the tables' and the fresh ids'
     nh::Kv4Patch patch{};   // values not sent yet
 };
@@ -105,7 +105,7 @@ int put(nh_kv4* c, size_t at, int v, hipStream_t st) {
 
 // A value of the mirror that the host remembers: sent when it changed.
 int put_changed(nh_kv4* c, size_t at, int v, hipStream_t st) {
-    int& old = c->sent[at - c->o_len];
+    int& old = c->sent[at - c->o_batch];
     if (old == v) return NH_OK;
     old = v;
     return put(c, at, v, st);
@@ -158,7 +158,7 @@ int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int p
     if (seqs < 1 || seqs > 65536) return fail(NH_EINVAL, "1 to 65536 sequences");
     if (cap < 1 || cap > (1 << 30)) return fail(NH_EINVAL, "a sequence's capacity is 1 to 2^30 positions");
     const int64_t ld = ((int64_t)cap + page - 1) / page;
-    if (ld * seqs + 3 * (int64_t)seqs + 1 + pages > (int64_t)UINT32_MAX / 4)
+    if (ld * seqs + 4 * (int64_t)seqs + 4 + pages > (int64_t)UINT32_MAX / 4)
         return fail(NH_EINVAL, "the sequences' page tables are too large");
     if (!nh::ready()) return fail(NH_ESTATE, "nh_init has not been called");
     return guarded([&]() -> int {
@@ -175,12 +175,10 @@ int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int p
         c->seqs = seqs;
         c->book.init(page, pages, seqs, cap);
         c->o_table = 0;
-        c->o_len = (size_t)ld * seqs;
-        c->o_bseq = c->o_len + seqs;
-        c->o_brow0 = c->o_bseq + seqs;
-        c->o_fresh = c->o_brow0 + seqs + 1;
+        c->o_batch = ((size_t)ld * seqs + 3) / 4 * 4;  // (an entry is one 16-byte load)
+        c->o_fresh = c->o_batch + 4 * (size_t)seqs;
         c->n_state = c->o_fresh + pages;
-        c->sent.assign(c->o_fresh - c->o_len, 0);
+        c->sent.assign(c->o_fresh - c->o_batch, 0);
         const size_t bytes = (size_t)pages * v.page_bytes();
         hipError_t e = hipMalloc(&c->data, bytes);
         if (e == hipSuccess) e = hipMalloc(&c->state, c->n_state * 4);
@@ -195,9 +193,7 @@ int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int p
         }
         v.data = c->data;
         v.table = c->state + c->o_table;
-        v.len = c->state + c->o_len;
-        v.bseq = c->state + c->o_bseq;
-        v.brow0 = c->state + c->o_brow0;
+        v.batch = c->state + c->o_batch;
         *h = c.release();
         return NH_OK;
     });
@@ -343,9 +339,9 @@ int nh_kv4_extend(nh_kv4* c, const int* seqs, const int* rows, int n, void* stre
         c->v.each = n ? rows[0] : 0;
         for (int i = 0; i < n; ++i) {
             if (int rc = sync_table(c, seqs[i], st)) return rc;
-            if (int rc = put_changed(c, c->o_len + seqs[i], c->book.seqs[seqs[i]].len, st)) return rc;
-            if (int rc = put_changed(c, c->o_bseq + i, seqs[i], st)) return rc;
-            if (int rc = put_changed(c, c->o_brow0 + i + 1, row0[i + 1], st)) return rc;
+            const int entry[4] = {seqs[i], row0[i], row0[i + 1], c->book.seqs[seqs[i]].len};
+            for (int k = 0; k < 4; ++k)
+                if (int rc = put_changed(c, c->o_batch + 4 * (size_t)i + k, entry[k], st)) return rc;
             if (rows[i] != rows[0]) c->v.each = 0;
         }
         return flush(c, st);

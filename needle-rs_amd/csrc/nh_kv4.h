@@ -11,23 +11,24 @@
 // Rows are stored `width` wide: 64, 128 or 256, the smallest that holds both
 // head dims (dims past a head's own have code 0 and are never read out).
 // A page holds `page` positions of every layer and head; the block of one
-// (page, layer, head) is, with T = page, W = width and NG = W / group:
-//   key codes    T x W / 2 bytes   dword (t, kg, j) at t W/2 + (kg W/32 + j) 4
-//                                  holds dims 32 j + 8 kg + e (e = 0 .. 7) at
-//                                  nibble (e % 2) 4 + e / 2
-//   value codes  T x W / 2 bytes   ushort (t, o, b) holds dims 64 b + 16 i + o
-//                                  (i = 0 .. 3) at nibble i; it is the half
-//                                  t % 2 of dword ((t / 4) 16 + o) 2 NB +
-//                                  (t / 2 % 2) NB + b, NB = W / 64
-//   key steps    T x NG f16
-//   key lows     T x NG f16
-//   value steps  T x NG f16
-//   value lows   f16 of (t, g) at (t / 4 NG + g) 4 + t % 4
-// That is the order in which a wavefront's MFMA operands want them: 16 lanes
-// (keys, or dims) by 4 lane groups kg, 8 codes of the summed index a dword,
-// and the two codes of a 16-bit half pair are one mask away (see the attention
-// kernel).  No position shares a byte with another, so rows are written
-// without reading their neighbours.
+// (page, layer, head) is page / 32 chunks of 32 positions, one after the other.
+// A chunk, with W = width, NG = W / group and slot = position % 32, is what a
+// wavefront of the attention kernel takes in one step, in the order in which its
+// lanes hold it (lane = 16 kg + o, 16 bytes a lane and piece, so a piece is one
+// load of 1 KiB):
+//   key codes    W / 64 pieces: lane (o = slot % 16, kg), dword u = slot / 16
+//                (W / 32) + j of the lane's W / 16 dwords holds dims 32 j + 8 kg + e
+//                (e = 0 .. 7) at nibble (e % 2) 4 + e / 2
+//   value codes  W / 64 pieces: lane (o, kg = slot / 4 % 4), half slot % 2 of dword u =
+//                slot / 16 (W / 32) + (slot / 2 % 2) NB + b, NB = W / 64, holds dims
+//                64 b + 16 i + o (i = 0 .. 3) at nibble i
+//   key steps    32 x NG f16
+//   key lows     32 x NG f16
+//   value steps  32 x NG f16
+//   value lows   f16 of (slot, g) at (slot / 4 NG + g) 4 + slot % 4
+// Of a lane's 8 codes a dword, the two of a 16-bit half pair are one mask away
+// from an MFMA operand (see the attention kernel).  No position shares a byte
+// with another, so rows are written without reading their neighbours.
 #pragma once
 
 #include "nh_internal.h"
@@ -38,24 +39,22 @@ enum Kv4Type { KV4_F32 = 0, KV4_F16 = 1, KV4_BF16 = 2 };  // NH_F32 ..
 
 constexpr int KV4_LANES = 16;
 
+struct Kv4Entry {
+    int seq, row0, row1, len;
+};
+
 struct Kv4View {
     uint8_t* data;       // [pages][layers][heads] blocks
     const int* table;    // [seqs][table_ld] page ids
-    const int* len;      // [seqs]
-    const int* bseq;     // [nb] the batch's sequences
-    const int* brow0;    // [nb + 1] their first rows
+    const int* batch;    // [nb] of (sequence, first row, end row, length): Kv4Entry
     int table_ld, pages, layers, heads, dk, dv, width, group, page_log2;
     int nb, rows, each;  // the batch; each: rows of every sequence when they are equal, else 0
     __host__ __device__ int page() const { return 1 << page_log2; }
     __host__ __device__ int groups() const { return width / group; }
-    // bytes of one (page, layer, head)
-    __host__ __device__ size_t block() const { return (size_t)page() * (width + 8 * groups()); }
+    // bytes of 32 positions, and of one (page, layer, head)
+    __host__ __device__ uint32_t chunk() const { return 32u * (width + 8 * groups()); }
+    __host__ __device__ size_t block() const { return (size_t)(page() / 32) * chunk(); }
     __host__ __device__ size_t page_bytes() const { return block() * heads * layers; }
-    __host__ __device__ uint32_t v_off() const { return (uint32_t)page() * width / 2; }
-    __host__ __device__ uint32_t ks_off() const { return (uint32_t)page() * width; }
-    __host__ __device__ uint32_t kl_off() const { return (uint32_t)page() * (width + 2 * groups()); }
-    __host__ __device__ uint32_t vs_off() const { return (uint32_t)page() * (width + 4 * groups()); }
-    __host__ __device__ uint32_t vl_off() const { return (uint32_t)page() * (width + 6 * groups()); }
 };
 
 // Values of the device's int32 state: (index, value) pairs.

@@ -103,6 +103,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
     constexpr int PARTS = TYPE == KV4_F32 ? 2 : 1;  // f16 halves of a query element and of a weight
     typedef KaChunk<W, NG> Chunk;
     constexpr int LD = W + 4;
+    constexpr uint32_t CB = 32 * (W + 8 * NG);
     __shared__ float so[KA_WAVES][16][LD];
     __shared__ float sm[KA_WAVES][16], sl[KA_WAVES][16], spl[KA_WAVES][16][8];
 
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         b = 0;
         for (int i = 0; i < c.nb; i += 64) {
             int n = 0;
-            if (i + lane < c.nb) n = ((c.brow0[i + lane + 1] - c.brow0[i + lane]) * per + 16 * RT - 1) / (16 * RT);
+            if (i + lane < c.nb) n = ((c.batch[4 * (i + lane) + 2] - c.batch[4 * (i + lane) + 1]) * per + 16 * RT - 1) / (16 * RT);
             int sum = n;  // tiles up to and with this lane's sequence
 #pragma unroll
             for (int h = 1; h < 64; h <<= 1) {
@@ -137,9 +138,9 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         tile = __builtin_amdgcn_readfirstlane(tile);
     }
     if (b >= c.nb) return;
-    const int row0 = c.brow0[b], nrows = c.brow0[b + 1] - row0;
-    const int seq = c.bseq[b], len = c.len[seq];
-    const int first = len - nrows, r0 = tile * 16 * RT;
+    const Kv4Entry entry = kv4_batch(c, b);
+    const int row0 = entry.row0, nrows = entry.row1 - row0, seq = entry.seq;
+    const int first = entry.len - nrows, r0 = tile * 16 * RT;
     if (first < 0 || r0 >= nrows * per) return;  // (a state that no extend of this shape leaves)
     const int r1 = min(r0 + 16 * RT, nrows * per) - 1;
     const int plo = first + r0 / per, phi = first + r1 / per;
@@ -217,6 +218,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
     int eref = -24;
 
     const KaSpan span(plo, phi, a.sink, a.ring);
+    const int sink = a.ring ? a.sink : 0x7fffffff, ring = a.ring;
     const int per_split = max((span.count() + plan.splits - 1) / plan.splits, KA_WAVES);
     const int c0 = split * per_split, c1 = min(c0 + per_split, span.count());
 
@@ -227,36 +229,43 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         const int slot = span.at(i) * KA_CHUNK & (c.page() - 1);
         // (a page id comes from the cache's own table; a bad one is not followed)
         const uint8_t* blk = kv4_block(c, (unsigned)pg < (unsigned)c.pages ? pg : 0, a.layer, kvh);
+        blk += (uint32_t)(slot >> 5) * CB;
+        // (the lane's 2 W / 32 dwords of each, 16 bytes a piece)
+#pragma unroll
+        for (int u = 0; u < 2 * NJ; u += 4) {
+            const u32x4 k = *reinterpret_cast<const u32x4*>(blk + (u >> 2) * 1024 + lane * 16);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(blk + 16 * W + (u >> 2) * 1024 + lane * 16);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                x.k[(u + n) / NJ][(u + n) % NJ] = k[n];
+                x.v[(u + n) / NJ][(u + n) % NJ] = v[n];
+            }
+        }
+        const uint8_t* scales = blk + 32 * W;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const uint32_t ko = (uint32_t)(slot + 16 * t + o) * (W / 2) + kg * (W / 8);
-            const uint32_t vo = c.v_off() + ((uint32_t)((slot >> 2) + 4 * t + kg) * 16 + o) * (8 * NB);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) x.k[t][j] = reinterpret_cast<const uint32_t*>(blk + ko)[j];
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) x.v[t][j] = reinterpret_cast<const uint32_t*>(blk + vo)[j];
-            const uint32_t so = ((uint32_t)(slot + 16 * t + 4 * kg) * NG + sidx) * 2;
+            const uint32_t so = ((uint32_t)(16 * t + 4 * kg) * NG + sidx) * 2;
 #pragma unroll
             for (int n = 0; n < Chunk::NS; ++n) {
-                x.ks[t][n] = kv4_half(blk, c.ks_off() + so + 32 * n);
-                x.vs[t][n] = kv4_half(blk, c.vs_off() + so + 32 * n);
+                x.ks[t][n] = kv4_half(scales, so + 32 * n);
+                x.vs[t][n] = kv4_half(scales, 128 * NG + so + 32 * n);
             }
-            const uint32_t kl = c.kl_off() + (uint32_t)(slot + 16 * t + o) * NG * 2;
+            const uint32_t kl = 64 * NG + (uint32_t)(16 * t + o) * NG * 2;
             if constexpr (NG == 1)
-                x.kl[t][0] = kv4_half(blk, kl);
+                x.kl[t][0] = kv4_half(scales, kl);
             else
 #pragma unroll
-                for (int n = 0; n < NG / 2; ++n) x.kl[t][n] = reinterpret_cast<const uint32_t*>(blk + kl)[n];
-            const uint32_t vl = c.vl_off() + ((uint32_t)((slot >> 2) + 4 * t + kg) * NG + (o & (NG - 1))) * 8;
+                for (int n = 0; n < NG / 2; ++n) x.kl[t][n] = kv4_word(scales, kl + 4 * n);
+            const uint32_t vl = 192 * NG + ((uint32_t)(4 * t + kg) * NG + (o & (NG - 1))) * 8;
 #pragma unroll
-            for (int n = 0; n < 2; ++n) x.vl[t][n] = reinterpret_cast<const uint32_t*>(blk + vl)[n];
+            for (int n = 0; n < 2; ++n) x.vl[t][n] = kv4_word(scales, vl + 4 * n);
         }
     };
 
     auto compute = [&](const Chunk& x, int i) {
         const int key0 = span.at(i) * KA_CHUNK;
         const bool whole = key0 + KA_CHUNK - 1 <= plo &&
-                           (!a.ring || key0 + KA_CHUNK - 1 < a.sink || key0 > phi - a.ring);
+                           (key0 + KA_CHUNK - 1 < sink || key0 > phi - ring);
         // The steps' reference: raised (a wavefront at a time) when a step passes it.
         uint32_t top = 0;
 #pragma unroll
@@ -337,7 +346,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int j = key0 + 16 * t + 4 * kg + r;
-                        seen[t][r] = j <= pos[rt] && (!a.ring || j < a.sink || j > pos[rt] - a.ring);
+                        seen[t][r] = (j <= pos[rt]) & ((j < sink) | (j > pos[rt] - ring));
                         s[t][r] = seen[t][r] ? s[t][r] : -__builtin_inff();
                     }
             }
@@ -415,23 +424,25 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         }
     };
 
-    // The next chunk's loads are issued before this one's arithmetic, its page
-    // id one step earlier still.
+    // The loads of the next two chunks are in flight during this one's
+    // arithmetic, the page id of the third is on its way.
     {
-        Chunk x, y;
+        Chunk x[3];
         int i = c0 + wave;
-        int pg = page_of(i);
-        if (i < c1) load(x, i, pg);
-        pg = page_of(i + KA_WAVES);
-        for (; i < c1; i += 2 * KA_WAVES) {
-            const int i1 = i + KA_WAVES, i2 = i1 + KA_WAVES;
-            if (i1 < c1) load(y, i1, pg);
-            pg = page_of(i2);
-            compute(x, i);
-            if (i1 >= c1) break;
-            if (i2 < c1) load(x, i2, pg);
-            pg = page_of(i2 + KA_WAVES);
-            compute(y, i1);
+        auto fetch = [&](Chunk& to, int at, int pg) {
+            if (at < c1) load(to, at, pg);
+        };
+        int p0 = page_of(i), p1 = page_of(i + KA_WAVES), p2 = page_of(i + 2 * KA_WAVES);
+        fetch(x[0], i, p0);
+        fetch(x[1], i + KA_WAVES, p1);
+        while (i < c1) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k, i += KA_WAVES) {
+                if (i >= c1) break;
+                fetch(x[(k + 2) % 3], i + 2 * KA_WAVES, p2);
+                p2 = page_of(i + 3 * KA_WAVES);
+                compute(x[k], i);
+            }
         }
     }
 

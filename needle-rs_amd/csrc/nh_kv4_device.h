@@ -32,25 +32,51 @@ __device__ __forceinline__ float f16_value(uint32_t bits) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
-// Where the step and the low of (slot, group) lie in a block, in bytes from
-// its start: keys, values.
-__device__ __forceinline__ uint32_t kv4_k_scale(const Kv4View& c, int slot, int g) { return c.ks_off() + 2 * (slot * c.groups() + g); }
-__device__ __forceinline__ uint32_t kv4_k_low(const Kv4View& c, int slot, int g) { return c.kl_off() + 2 * (slot * c.groups() + g); }
-__device__ __forceinline__ uint32_t kv4_v_scale(const Kv4View& c, int slot, int g) { return c.vs_off() + 2 * (slot * c.groups() + g); }
-__device__ __forceinline__ uint32_t kv4_v_low(const Kv4View& c, int slot, int g) {
-    return c.vl_off() + 2 * (((slot >> 2) * c.groups() + g) * 4 + (slot & 3));
+// Where things of position `slot` of a page lie in its block, in bytes from the
+// block's start: the dword of key dims 8 t .. 8 t + 7, the half of value dims
+// 64 b + 16 i + o, the group's steps and lows.
+__device__ __forceinline__ uint32_t kv4_chunk_at(const Kv4View& c, int slot) { return (uint32_t)(slot >> 5) * c.chunk(); }
+__device__ __forceinline__ uint32_t kv4_lane_dword(int lane, int u) { return (uint32_t)(u >> 2) * 1024 + lane * 16 + (u & 3) * 4; }
+__device__ __forceinline__ uint32_t kv4_k_dword(const Kv4View& c, int slot, int t) {
+    return kv4_chunk_at(c, slot) + kv4_lane_dword((t & 3) * 16 + (slot & 15), (slot >> 4 & 1) * (c.width / 32) + (t >> 2));
 }
+__device__ __forceinline__ uint32_t kv4_v_half(const Kv4View& c, int slot, int o, int b) {
+    return kv4_chunk_at(c, slot) + 16 * c.width +
+           kv4_lane_dword((slot >> 2 & 3) * 16 + o, (slot >> 4 & 1) * (c.width / 32) + (slot >> 1 & 1) * (c.width / 64) + b) +
+           2 * (slot & 1);
+}
+__device__ __forceinline__ uint32_t kv4_scale_at(const Kv4View& c, int slot, int array) {
+    return kv4_chunk_at(c, slot) + 32 * c.width + array * 64 * c.groups();
+}
+__device__ __forceinline__ uint32_t kv4_k_scale(const Kv4View& c, int slot, int g) {
+    return kv4_scale_at(c, slot, 0) + 2 * ((slot & 31) * c.groups() + g);
+}
+__device__ __forceinline__ uint32_t kv4_k_low(const Kv4View& c, int slot, int g) {
+    return kv4_scale_at(c, slot, 1) + 2 * ((slot & 31) * c.groups() + g);
+}
+__device__ __forceinline__ uint32_t kv4_v_scale(const Kv4View& c, int slot, int g) {
+    return kv4_scale_at(c, slot, 2) + 2 * ((slot & 31) * c.groups() + g);
+}
+__device__ __forceinline__ uint32_t kv4_v_low(const Kv4View& c, int slot, int g) {
+    return kv4_scale_at(c, slot, 3) + 2 * (((slot >> 2 & 7) * c.groups() + g) * 4 + (slot & 3));
+}
+__device__ __forceinline__ uint32_t& kv4_word(uint8_t* blk, uint32_t at) { return *reinterpret_cast<uint32_t*>(blk + at); }
+__device__ __forceinline__ uint32_t kv4_word(const uint8_t* blk, uint32_t at) { return *reinterpret_cast<const uint32_t*>(blk + at); }
 __device__ __forceinline__ uint16_t& kv4_half(uint8_t* blk, uint32_t at) { return *reinterpret_cast<uint16_t*>(blk + at); }
 __device__ __forceinline__ uint16_t kv4_half(const uint8_t* blk, uint32_t at) { return *reinterpret_cast<const uint16_t*>(blk + at); }
 
-// The batch entry that holds `row`: the count of entries that end at or
-// before it (row0 ascends; an entry without rows is passed over).  One load
-// for each 64 entries, the wavefront together; row is the same in every lane.
-__device__ __forceinline__ int kv4_entry(const int* __restrict__ row0, int nb, int row, int lane) {
+// The entry that holds `row`, of entries whose rows end at ends[i * stride]: the
+// count of those that end at or before it (an entry without rows is passed
+// over).  One load for each 64 entries, the wavefront together; row is the same
+// in every lane.
+__device__ __forceinline__ int kv4_entry(const int* __restrict__ ends, int stride, int n, int row, int lane) {
     int b = 0;
-    for (int i = 0; i < nb; i += 64)
-        b += __popcll(__ballot(i + lane < nb && row0[i + lane + 1] <= row));
-    return b < nb ? b : nb - 1;
+    for (int i = 0; i < n; i += 64) b += __popcll(__ballot(i + lane < n && ends[(i + lane) * stride] <= row));
+    return b < n ? b : n - 1;
+}
+__device__ __forceinline__ Kv4Entry kv4_batch(const Kv4View& c, int b) {
+    const int4 e = reinterpret_cast<const int4*>(c.batch)[b];
+    return Kv4Entry{e.x, e.y, e.z, e.w};
 }
 
 // Where position `pos` of sequence `seq` lies: its page id, or -1 outside the

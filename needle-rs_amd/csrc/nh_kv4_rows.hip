@@ -77,7 +77,7 @@ __device__ __forceinline__ void kv4_store_k(const Kv4View& c, const typename Kv4
         for (int e = 0; e < 8; ++e)
             if (t * 8 + e < c.dk) w |= kv4_code(v[e], g) << (4 * ((e & 1) * 4 + (e >> 1)));
         if (t < W / 8) {
-            reinterpret_cast<uint32_t*>(blk + (size_t)slot * (W / 2))[(t & 3) * (W / 32) + (t >> 2)] = w;
+            kv4_word(blk, kv4_k_dword(c, slot, t)) = w;
             if (t % per == 0) {
                 kv4_half(blk, kv4_k_scale(c, slot, t / per)) = g.sb;
                 kv4_half(blk, kv4_k_low(c, slot, t / per)) = g.lb;
@@ -129,10 +129,8 @@ __device__ __forceinline__ void kv4_store_v(const Kv4View& c, const typename Kv4
 #pragma unroll
         for (int g = 0; g < W / 64; ++g) group(4 * g, 4);
     }
-    uint16_t* codes = reinterpret_cast<uint16_t*>(blk + c.v_off()) +
-                      (((slot >> 2) * 16 + o) * 2 * NB + ((slot >> 1) & 1) * NB) * 2 + (slot & 1);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) codes[2 * b] = half[b];
+    for (int b = 0; b < NB; ++b) kv4_half(blk, kv4_v_half(c, slot, o, b)) = half[b];
 }
 
 // A wavefront takes four heads' keys, or values, of one row.
@@ -146,10 +144,9 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4View c, int layer, const 
     const int row = (int)(w / (2 * quads));
     const uint32_t u = w % (2 * quads);
     if (row >= c.rows) return;
-    const int b = c.each ? row / c.each : kv4_entry(c.brow0, c.nb, row, lane);
-    const int seq = c.bseq[b];
-    const int pos = c.len[seq] - c.brow0[b + 1] + row;
-    const int pg = pos < 0 ? -1 : kv4_page(c, seq, pos);
+    const Kv4Entry e = kv4_batch(c, c.each ? row / c.each : kv4_entry(c.batch + 2, 4, c.nb, row, lane));
+    const int pos = e.len - e.row1 + row;
+    const int pg = pos < 0 ? -1 : kv4_page(c, e.seq, pos);
     const int head = (int)(u % quads) * 4 + (lane >> 4);
     if (pg < 0 || head >= c.heads) return;
     uint8_t* blk = kv4_block(c, pg, layer, head);
@@ -184,14 +181,13 @@ template <int TYPE, int W>
 __global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, Kv4Spans p, int64_t rows, int64_t row_at,
                                                   typename Kv4Elem<TYPE>::T* __restrict__ k,
                                                   typename Kv4Elem<TYPE>::T* __restrict__ v) {
-    constexpr int NB = W / 64;
     const int lane = threadIdx.x & 63, o = lane & 15;
     const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 6);
     const uint32_t quads = (c.heads + 3) / 4;
     const int row = (int)(w / (2 * quads));
     const uint32_t u = w % (2 * quads);
     if (row >= p.row0[p.n]) return;
-    const int b = kv4_entry(p.row0, p.n, row, lane);
+    const int b = kv4_entry(p.row0 + 1, 1, p.n, row, lane);
     const int pos = p.pos[b] + row - p.row0[b];
     const int pg = kv4_page(c, p.seq[b], pos);
     const int head = (int)(u % quads) * 4 + (lane >> 4);
@@ -204,7 +200,7 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, Kv4Span
         for (int t0 = 0; t0 < W / 8; t0 += 16) {
             const int t = t0 + o;
             if (t * 8 >= c.dk) continue;
-            const uint32_t code = reinterpret_cast<const uint32_t*>(blk + (size_t)slot * (W / 2))[(t & 3) * (W / 32) + (t >> 2)];
+            const uint32_t code = kv4_word(blk, kv4_k_dword(c, slot, t));
             const int g = t * 8 / c.group;
             const float step = f16_value(kv4_half(blk, kv4_k_scale(c, slot, g))), low = f16_value(kv4_half(blk, kv4_k_low(c, slot, g)));
 #pragma unroll
@@ -214,14 +210,12 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, Kv4Span
                                        __builtin_fmaf(step, (float)((code >> (4 * ((e & 1) * 4 + (e >> 1)))) & 15u), low));
         }
     } else {
-        const uint16_t* codes = reinterpret_cast<const uint16_t*>(blk + c.v_off()) +
-                                (((slot >> 2) * 16 + o) * 2 * NB + ((slot >> 1) & 1) * NB) * 2 + (slot & 1);
 #pragma unroll
         for (int i = 0; i < W / 16; ++i) {
             const int d = 16 * i + o;
             if (d >= c.dv) continue;
             const int g = d / c.group;
-            const uint32_t code = (uint32_t)codes[2 * (i >> 2)] >> (4 * (i & 3)) & 15u;
+            const uint32_t code = (uint32_t)kv4_half(blk, kv4_v_half(c, slot, o, i >> 2)) >> (4 * (i & 3)) & 15u;
             Kv4Elem<TYPE>::put(v + at * c.dv + d, __builtin_fmaf(f16_value(kv4_half(blk, kv4_v_scale(c, slot, g))), (float)code,
                                                                  f16_value(kv4_half(blk, kv4_v_low(c, slot, g)))));
         }
@@ -284,14 +278,8 @@ __global__ __launch_bounds__(256) void k_kv4_runs(Kv4View c, const int* __restri
     const int mask = c.page() - 1, s0 = src & mask, s1 = dst & mask, W = c.width, nb = W / 64, ng = c.groups();
     const uint8_t* a = kv4_block(c, from, (int)blockIdx.y, (int)blockIdx.z);
     uint8_t* z = kv4_block(c, to, (int)blockIdx.y, (int)blockIdx.z);
-    const uint32_t* ak = reinterpret_cast<const uint32_t*>(a) + s0 * (W / 8);
-    uint32_t* zk = reinterpret_cast<uint32_t*>(z) + s1 * (W / 8);
-    for (int t = l; t < W / 8; t += 16) zk[t] = ak[t];
-    const uint16_t* av = reinterpret_cast<const uint16_t*>(a + c.v_off()) +
-                         (((s0 >> 2) * 16 + l) * 2 * nb + ((s0 >> 1) & 1) * nb) * 2 + (s0 & 1);
-    uint16_t* zv = reinterpret_cast<uint16_t*>(z + c.v_off()) +
-                   (((s1 >> 2) * 16 + l) * 2 * nb + ((s1 >> 1) & 1) * nb) * 2 + (s1 & 1);
-    for (int b = 0; b < nb; ++b) zv[2 * b] = av[2 * b];
+    for (int t = l; t < W / 8; t += 16) kv4_word(z, kv4_k_dword(c, s1, t)) = kv4_word(a, kv4_k_dword(c, s0, t));
+    for (int b = 0; b < nb; ++b) kv4_half(z, kv4_v_half(c, s1, l, b)) = kv4_half(a, kv4_v_half(c, s0, l, b));
     if (l < ng) {
         kv4_half(z, kv4_k_scale(c, s1, l)) = kv4_half(a, kv4_k_scale(c, s0, l));
         kv4_half(z, kv4_k_low(c, s1, l)) = kv4_half(a, kv4_k_low(c, s0, l));
