@@ -298,7 +298,7 @@ int nh_kv4_seq_compact(nh_kv4* c, const int* seqs, int n, const int* counts, con
         if (!rc) rc = flush(c, st);
         nh::Kv4Runs r;
         r.n = 0;
-        r.row0[0] = 0;
+        r.unit0[0] = 0;
         for (size_t m = 0; m < p.moves.size() && !rc; ++m) {
             const nh::Kv4Book::Move& mv = p.moves[m];
             r.seq[r.n] = seqs[mv.seq];
@@ -306,8 +306,8 @@ int nh_kv4_seq_compact(nh_kv4* c, const int* seqs, int n, const int* counts, con
             r.dst[r.n] = mv.dst;
             r.count[r.n] = mv.count;
             r.fresh[r.n] = (int)c->o_fresh + at[mv.seq];
-            r.row0[r.n + 1] = r.row0[r.n] + mv.count;
-            if (++r.n == nh::Kv4Runs::MAX || m + 1 == p.moves.size() || r.row0[r.n] > (1 << 28)) {
+            r.unit0[r.n + 1] = r.unit0[r.n] + nh::kv4_chunks(mv.dst, mv.count);
+            if (++r.n == nh::Kv4Runs::MAX || m + 1 == p.moves.size() || r.unit0[r.n] > (1 << 26)) {
                 const hipError_t e = nh::launch_kv4_runs(c->v, c->state, r, st);
                 if (e != hipSuccess) rc = hip_fail(e, "kv4 compaction");
                 r.n = 0;
@@ -361,7 +361,7 @@ int nh_kv4_append(nh_kv4* c, int layer, const void* k, const void* v, int64_t ld
     if (!k || !v) return fail(NH_EINVAL, "null argument");
     if (ldk < (int64_t)c->v.heads * c->v.dk || ldv < (int64_t)c->v.heads * c->v.dv)
         return fail(NH_EINVAL, "rows overlap: a row holds every head");
-    NH_TRY(nh::launch_kv4_append(c->v, layer, k, v, ldk, ldv, type, (hipStream_t)stream), "kv4 append");
+    NH_TRY(nh::launch_kv4_append(c->v, c->book.batch_row0.data(), layer, k, v, ldk, ldv, type, (hipStream_t)stream), "kv4 append");
     return NH_OK;
 }
 
@@ -391,12 +391,13 @@ int nh_kv4_read(nh_kv4* c, int layer, const int* seqs, const int* pos, const int
         int64_t row = 0;
         for (int i = 0; i < n;) {
             p.n = 0;
-            p.row0[0] = 0;
+            p.row0[0] = p.unit0[0] = 0;
             for (; i < n && p.n < nh::Kv4Spans::MAX; ++i) {
                 if (!rows[i]) continue;
                 p.seq[p.n] = seqs[i];
                 p.pos[p.n] = pos[i];
                 p.row0[p.n + 1] = p.row0[p.n] + rows[i];
+                p.unit0[p.n + 1] = p.unit0[p.n] + nh::kv4_chunks(pos[i], rows[i]);
                 ++p.n;
             }
             if (!p.n) break;

@@ -21,7 +21,7 @@
 //                (e = 0 .. 7) at nibble (e % 2) 4 + e / 2
 //   value codes  W / 64 pieces: lane (o, kg = slot / 4 % 4), half slot % 2 of dword u =
 //                slot / 16 (W / 32) + (slot / 2 % 2) NB + b, NB = W / 64, holds dims
-//                64 b + 16 i + o (i = 0 .. 3) at nibble i
+//                64 b + 32 (i / 2) + 2 o + i % 2 (i = 0 .. 3) at nibble i
 //   key steps    32 x NG f16
 //   key lows     32 x NG f16
 //   value steps  32 x NG f16
@@ -71,19 +71,23 @@ struct Kv4Pairs {
     int from[MAX], to[MAX];
 };
 // Rows to read: entry i is rows row0[i] .. row0[i + 1] - 1 of the output,
-// positions pos[i] .. of sequence seq[i].
+// positions pos[i] .. of sequence seq[i]; unit0: the first of the chunks that
+// they lie in, in the launch.
 struct Kv4Spans {
-    static constexpr int MAX = 255;
+    static constexpr int MAX = 240;
     int n;
-    int seq[MAX], pos[MAX], row0[MAX + 1];
+    int seq[MAX], pos[MAX], row0[MAX + 1], unit0[MAX + 1];
 };
+// The chunks of 32 that positions pos .. pos + n - 1 lie in.
+__host__ __device__ inline int kv4_chunks(int pos, int n) { return n ? ((pos + n - 1) >> 5) - (pos >> 5) + 1 : 0; }
 // Runs of positions to move into fresh pages: positions src .. of sequence
 // seq to positions dst .. counted from fresh page 0 of that sequence, whose
-// ids are at state[fresh ..]; row0: the run's first position in the launch.
+// ids are at state[fresh ..]; unit0: the first of the chunks that the run
+// writes into, in the launch.
 struct Kv4Runs {
     static constexpr int MAX = 160;
     int n;
-    int seq[MAX], src[MAX], dst[MAX], count[MAX], fresh[MAX], row0[MAX + 1];
+    int seq[MAX], src[MAX], dst[MAX], count[MAX], fresh[MAX], unit0[MAX + 1];
 };
 
 struct Kv4AttendArgs {
@@ -99,7 +103,7 @@ struct Kv4AttendArgs {
 hipError_t launch_kv4_patch(int* state, const Kv4Patch& p, hipStream_t s);
 hipError_t launch_kv4_pairs(const Kv4View& c, const Kv4Pairs& p, hipStream_t s);
 hipError_t launch_kv4_runs(const Kv4View& c, const int* state, const Kv4Runs& r, hipStream_t s);
-hipError_t launch_kv4_append(const Kv4View& c, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int type,
+hipError_t launch_kv4_append(const Kv4View& c, const int* row0, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int type,
                              hipStream_t s);
 // layer < 0: all, [layers][rows]; `rows` rows a layer in the output, this launch's from `row`.
 hipError_t launch_kv4_read(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,

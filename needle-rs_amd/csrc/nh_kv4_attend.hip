@@ -117,25 +117,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         b = tile / plan.tiles_each;
         tile -= b * plan.tiles_each;
     } else {
-        b = 0;
-        for (int i = 0; i < c.nb; i += 64) {
-            int n = 0;
-            if (i + lane < c.nb) n = ((c.batch[4 * (i + lane) + 2] - c.batch[4 * (i + lane) + 1]) * per + 16 * RT - 1) / (16 * RT);
-            int sum = n;  // tiles up to and with this lane's sequence
-#pragma unroll
-            for (int h = 1; h < 64; h <<= 1) {
-                const int x = __shfl_up(sum, h, 64);
-                if (lane >= h) sum += x;
-            }
-            const uint64_t before = __ballot(sum <= tile && i + lane < c.nb);
-            const int skip = __popcll(before);
-            const int last = __shfl(sum, skip ? skip - 1 : 0, 64);
-            b += skip;
-            if (skip) tile -= last;
-            if (skip < 64) break;
-        }
-        b = __builtin_amdgcn_readfirstlane(b);
-        tile = __builtin_amdgcn_readfirstlane(tile);
+        b = kv4_find(c, tile, lane, [&](const Kv4Entry& e) { return ((e.row1 - e.row0) * per + 16 * RT - 1) / (16 * RT); });
     }
     if (b >= c.nb) return;
     const Kv4Entry entry = kv4_batch(c, b);
@@ -406,7 +388,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            // dword (token pair, n) of each quad: dims 64 n + 16 i + o for i = 0 .. 3
+            // dword (token pair, n) of each quad: dims 64 n + 32 (i / 2) + 2 o + i % 2
             const uint32_t w[4] = {x.v[0][n], x.v[0][NB + n], x.v[1][n], x.v[1][NB + n]};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -462,12 +444,19 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         const float base = most == -__builtin_inff() ? 0.0f : most;
         const float f = __builtin_amdgcn_exp2f(m[rt] - base);
 #pragma unroll
-        for (int i = 0; i < W / 16; ++i) {
-            const float u = i & 1 ? unit * 0.0625f : unit, low = spl[wave][o][i / GI];
-            f32x4 y;
+        for (int i = 0; i < W / 16; i += 2) {
+            // products i, i + 1: dims 16 i + 8 kg + 2 r, and the ones after them
+            const float low = spl[wave][o][i / GI];
+            f32x4 y, z;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = (acc[rt][i][r] * u + low) * f;
-            *reinterpret_cast<f32x4*>(&so[wave][o][16 * i + 4 * kg]) = y;
+            for (int r = 0; r < 2; ++r) {
+                y[2 * r] = (acc[rt][i][r] * unit + low) * f;
+                y[2 * r + 1] = (acc[rt][i + 1][r] * (unit * 0.0625f) + low) * f;
+                z[2 * r] = (acc[rt][i][r + 2] * unit + low) * f;
+                z[2 * r + 1] = (acc[rt][i + 1][r + 2] * (unit * 0.0625f) + low) * f;
+            }
+            *reinterpret_cast<f32x4*>(&so[wave][o][16 * i + 8 * kg]) = y;
+            *reinterpret_cast<f32x4*>(&so[wave][o][16 * i + 8 * kg + 4]) = z;
         }
         __syncthreads();
         for (int x = tid; x < 16 * W; x += KA_WAVES * 64) {

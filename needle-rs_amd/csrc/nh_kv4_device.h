@@ -32,47 +32,64 @@ __device__ __forceinline__ float f16_value(uint32_t bits) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
-// Where things of position `slot` of a page lie in its block, in bytes from the
-// block's start: the dword of key dims 8 t .. 8 t + 7, the half of value dims
-// 64 b + 16 i + o, the group's steps and lows.
-__device__ __forceinline__ uint32_t kv4_chunk_at(const Kv4View& c, int slot) { return (uint32_t)(slot >> 5) * c.chunk(); }
-__device__ __forceinline__ uint32_t kv4_lane_dword(int lane, int u) { return (uint32_t)(u >> 2) * 1024 + lane * 16 + (u & 3) * 4; }
-__device__ __forceinline__ uint32_t kv4_k_dword(const Kv4View& c, int slot, int t) {
-    return kv4_chunk_at(c, slot) + kv4_lane_dword((t & 3) * 16 + (slot & 15), (slot >> 4 & 1) * (c.width / 32) + (t >> 2));
-}
-__device__ __forceinline__ uint32_t kv4_v_half(const Kv4View& c, int slot, int o, int b) {
-    return kv4_chunk_at(c, slot) + 16 * c.width +
-           kv4_lane_dword((slot >> 2 & 3) * 16 + o, (slot >> 4 & 1) * (c.width / 32) + (slot >> 1 & 1) * (c.width / 64) + b) +
-           2 * (slot & 1);
-}
-__device__ __forceinline__ uint32_t kv4_scale_at(const Kv4View& c, int slot, int array) {
-    return kv4_chunk_at(c, slot) + 32 * c.width + array * 64 * c.groups();
-}
-__device__ __forceinline__ uint32_t kv4_k_scale(const Kv4View& c, int slot, int g) {
-    return kv4_scale_at(c, slot, 0) + 2 * ((slot & 31) * c.groups() + g);
-}
-__device__ __forceinline__ uint32_t kv4_k_low(const Kv4View& c, int slot, int g) {
-    return kv4_scale_at(c, slot, 1) + 2 * ((slot & 31) * c.groups() + g);
-}
-__device__ __forceinline__ uint32_t kv4_v_scale(const Kv4View& c, int slot, int g) {
-    return kv4_scale_at(c, slot, 2) + 2 * ((slot & 31) * c.groups() + g);
-}
-__device__ __forceinline__ uint32_t kv4_v_low(const Kv4View& c, int slot, int g) {
-    return kv4_scale_at(c, slot, 3) + 2 * (((slot >> 2 & 7) * c.groups() + g) * 4 + (slot & 3));
-}
-__device__ __forceinline__ uint32_t& kv4_word(uint8_t* blk, uint32_t at) { return *reinterpret_cast<uint32_t*>(blk + at); }
-__device__ __forceinline__ uint32_t kv4_word(const uint8_t* blk, uint32_t at) { return *reinterpret_cast<const uint32_t*>(blk + at); }
-__device__ __forceinline__ uint16_t& kv4_half(uint8_t* blk, uint32_t at) { return *reinterpret_cast<uint16_t*>(blk + at); }
-__device__ __forceinline__ uint16_t kv4_half(const uint8_t* blk, uint32_t at) { return *reinterpret_cast<const uint16_t*>(blk + at); }
+// Where the things of position `slot` (0 .. 31) of a chunk lie, in bytes from
+// the chunk's start: the dword of key dims 8 t .. 8 t + 7; the byte of value
+// dims 2 x, 2 x + 1; a group's steps and lows.
+template <int W, int G>
+struct Kv4Lay {
+    static constexpr int NG = W / G, NB = W / 64, NJ = W / 32;
+    static constexpr uint32_t CHUNK = 32 * (W + 8 * NG);
+    static __device__ __forceinline__ uint32_t lane_dword(int lane, int u) { return (uint32_t)(u >> 2) * 1024 + lane * 16 + (u & 3) * 4; }
+    static __device__ __forceinline__ uint32_t k_dword(int slot, int t) {
+        return lane_dword((t & 3) * 16 + (slot & 15), (slot >> 4) * NJ + (t >> 2));
+    }
+    static __device__ __forceinline__ uint32_t v_half(int slot, int o, int b) {
+        return 16 * W + lane_dword((slot >> 2 & 3) * 16 + o, (slot >> 4) * NJ + (slot >> 1 & 1) * NB + b) + 2 * (slot & 1);
+    }
+    static __device__ __forceinline__ uint32_t v_byte(int slot, int x) { return v_half(slot, x & 15, x >> 5) + (x >> 4 & 1); }
+    static __device__ __forceinline__ uint32_t k_step(int slot, int g) { return 32 * W + 2 * (slot * NG + g); }
+    static __device__ __forceinline__ uint32_t k_low(int slot, int g) { return 32 * W + 64 * NG + 2 * (slot * NG + g); }
+    static __device__ __forceinline__ uint32_t v_step(int slot, int g) { return 32 * W + 128 * NG + 2 * (slot * NG + g); }
+    static __device__ __forceinline__ uint32_t v_low(int slot, int g) {
+        return 32 * W + 192 * NG + 2 * (((slot >> 2) * NG + g) * 4 + (slot & 3));
+    }
+};
+__device__ __forceinline__ uint32_t& kv4_word(uint8_t* p, uint32_t at) { return *reinterpret_cast<uint32_t*>(p + at); }
+__device__ __forceinline__ uint32_t kv4_word(const uint8_t* p, uint32_t at) { return *reinterpret_cast<const uint32_t*>(p + at); }
+__device__ __forceinline__ uint16_t& kv4_half(uint8_t* p, uint32_t at) { return *reinterpret_cast<uint16_t*>(p + at); }
+__device__ __forceinline__ uint16_t kv4_half(const uint8_t* p, uint32_t at) { return *reinterpret_cast<const uint16_t*>(p + at); }
 
-// The entry that holds `row`, of entries whose rows end at ends[i * stride]: the
-// count of those that end at or before it (an entry without rows is passed
-// over).  One load for each 64 entries, the wavefront together; row is the same
-// in every lane.
-__device__ __forceinline__ int kv4_entry(const int* __restrict__ ends, int stride, int n, int row, int lane) {
+// The entry whose units (ascending, from first[i]) hold `unit`; the wavefront
+// together, unit the same in every lane.
+__device__ __forceinline__ int kv4_span(const int* __restrict__ first, int n, int unit, int lane) {
     int b = 0;
-    for (int i = 0; i < n; i += 64) b += __popcll(__ballot(i + lane < n && ends[(i + lane) * stride] <= row));
+    for (int i = 0; i < n; i += 64) b += __popcll(__ballot(i + lane < n && first[i + lane + 1] <= unit));
     return b < n ? b : n - 1;
+}
+// The batch entry whose units(entry) hold `unit`, which becomes that entry's own;
+// c.nb past the last.  The wavefront together.
+template <class F>
+__device__ __forceinline__ int kv4_find(const Kv4View& c, int& unit, int lane, F units) {
+    int b = 0;
+    for (int i = 0; i < c.nb; i += 64) {
+        int sum = 0;
+        if (i + lane < c.nb) {
+            const int4 e = reinterpret_cast<const int4*>(c.batch)[i + lane];
+            sum = units(Kv4Entry{e.x, e.y, e.z, e.w});
+        }
+#pragma unroll
+        for (int h = 1; h < 64; h <<= 1) {
+            const int x = __shfl_up(sum, h, 64);
+            if (lane >= h) sum += x;
+        }
+        const int skip = __popcll(__ballot(sum <= unit && i + lane < c.nb));
+        const int last = __shfl(sum, skip ? skip - 1 : 0, 64);
+        b += skip;
+        if (skip) unit -= last;
+        if (skip < 64) break;
+    }
+    unit = __builtin_amdgcn_readfirstlane(unit);
+    return __builtin_amdgcn_readfirstlane(b);
 }
 __device__ __forceinline__ Kv4Entry kv4_batch(const Kv4View& c, int b) {
     const int4 e = reinterpret_cast<const int4*>(c.batch)[b];

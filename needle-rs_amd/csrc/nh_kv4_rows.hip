@@ -42,201 +42,260 @@ __device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Group& g) {
     return (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f);
 }
 
-// One row of one head by 16 lanes, keys: dword t (dims 8 t ..) by lane t % 16;
-// the group's range over 4 or 8 neighbouring lanes.
-template <int TYPE, int W>
-__device__ __forceinline__ void kv4_store_k(const Kv4View& c, const typename Kv4Elem<TYPE>::T* __restrict__ x, uint8_t* blk,
-                                            int slot, int lane) {
-    const int l = lane & 15, per = c.group / 8;
+// A workgroup's rows are those of one head in one chunk of 32 positions: their
+// codes are put together in LDS as the chunk has them, and go out 16 bytes a
+// thread if the rows fill the chunk, else piece by piece (the other positions'
+// bytes are not touched).  16 lanes take a row, 8 dims each (twice at 256), its
+// groups' ranges over 4 or 8 neighbouring lanes.
+template <int TYPE, int W, int G, bool VALUES>
+__device__ __forceinline__ void kv4_pack_row(const typename Kv4Elem<TYPE>::T* __restrict__ x, int dim, bool vec, uint8_t* img,
+                                             int slot, int lane, bool live) {
+    typedef typename Kv4Elem<TYPE>::T T;
+    typedef T Vec __attribute__((ext_vector_type(8)));
+    typedef Kv4Lay<W, G> L;
 #pragma unroll
     for (int t0 = 0; t0 < W / 8; t0 += 16) {
-        const int t = t0 + l;
+        const int t = t0 + (lane & 15), d = t * 8;
         float v[8];
-        float mn = __builtin_inff(), mx = -__builtin_inff();
-        bool bad = false;
+        if (vec && live && d < dim) {  // (dim is a multiple of 8)
+            const Vec y = *reinterpret_cast<const Vec*>(x + d);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const bool in = t * 8 + e < c.dk;
-            const float r = in ? Kv4Elem<TYPE>::get(x + t * 8 + e) : 0.0f;
-            bad |= !(fabsf(r) < __builtin_inff());
-            v[e] = fminf(fmaxf(r, -65504.0f), 65504.0f);
-            if (in) mn = fminf(mn, v[e]), mx = fmaxf(mx, v[e]);
+            for (int e = 0; e < 8; ++e) v[e] = (float)y[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = live && d + e < dim ? Kv4Elem<TYPE>::get(x + d + e) : 0.0f;
         }
-        int nb = bad;
-#pragma unroll
-        for (int h = 1; h < 8; h <<= 1) {
-            if (h * 8 >= c.group) break;
-            mn = fminf(mn, lane_xor(mn, h, lane));
-            mx = fmaxf(mx, lane_xor(mx, h, lane));
-            nb |= __float_as_int(lane_xor(__int_as_float(nb), h, lane));
-        }
-        if (mn > mx) mn = mx = 0.0f;  // a group of padding
-        const Kv4Group g = kv4_group(mn, mx, nb != 0);
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (t * 8 + e < c.dk) w |= kv4_code(v[e], g) << (4 * ((e & 1) * 4 + (e >> 1)));
-        if (t < W / 8) {
-            kv4_word(blk, kv4_k_dword(c, slot, t)) = w;
-            if (t % per == 0) {
-                kv4_half(blk, kv4_k_scale(c, slot, t / per)) = g.sb;
-                kv4_half(blk, kv4_k_low(c, slot, t / per)) = g.lb;
-            }
-        }
-    }
-}
-
-// Values: lane o holds dims 16 i + o; the group's range over i and the 16 lanes.
-template <int TYPE, int W>
-__device__ __forceinline__ void kv4_store_v(const Kv4View& c, const typename Kv4Elem<TYPE>::T* __restrict__ x, uint8_t* blk,
-                                            int slot, int lane) {
-    constexpr int NB = W / 64;
-    const int o = lane & 15;
-    uint16_t half[NB] = {};
-    float v[W / 16];
-#pragma unroll
-    for (int i = 0; i < W / 16; ++i) v[i] = 16 * i + o < c.dv ? Kv4Elem<TYPE>::get(x + 16 * i + o) : 0.0f;
-    // `gi` dims of each lane to a group: 2 or 4
-    auto group = [&](int i0, int gi) {
         float mn = __builtin_inff(), mx = -__builtin_inff();
         int bad = 0;
 #pragma unroll
-        for (int i = i0; i < i0 + gi; ++i) {
-            bad |= !(fabsf(v[i]) < __builtin_inff());
-            v[i] = fminf(fmaxf(v[i], -65504.0f), 65504.0f);
-            if (16 * i + o < c.dv) mn = fminf(mn, v[i]), mx = fmaxf(mx, v[i]);
+        for (int e = 0; e < 8; ++e) {
+            bad |= !(fabsf(v[e]) < __builtin_inff());
+            v[e] = fminf(fmaxf(v[e], -65504.0f), 65504.0f);
+            if (d + e < dim) mn = fminf(mn, v[e]), mx = fmaxf(mx, v[e]);
         }
 #pragma unroll
-        for (int h = 1; h < 16; h <<= 1) {
+        for (int h = 1; h < G / 8; h <<= 1) {
             mn = fminf(mn, lane_xor(mn, h, lane));
             mx = fmaxf(mx, lane_xor(mx, h, lane));
             bad |= __float_as_int(lane_xor(__int_as_float(bad), h, lane));
         }
-        if (mn > mx) mn = mx = 0.0f;
+        if (mn > mx) mn = mx = 0.0f;  // a group of padding
         const Kv4Group g = kv4_group(mn, mx, bad != 0);
+        uint32_t code[8];
 #pragma unroll
-        for (int i = i0; i < i0 + gi; ++i)
-            if (16 * i + o < c.dv) half[i / 4] |= (uint16_t)(kv4_code(v[i], g) << (4 * (i & 3)));
-        if (o == 0) {
-            kv4_half(blk, kv4_v_scale(c, slot, i0 / gi)) = g.sb;
-            kv4_half(blk, kv4_v_low(c, slot, i0 / gi)) = g.lb;
+        for (int e = 0; e < 8; ++e) code[e] = d + e < dim ? kv4_code(v[e], g) : 0;
+        if (!live || t >= W / 8) continue;
+        if constexpr (VALUES) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) img[L::v_byte(slot, t * 4 + e / 2)] = (uint8_t)(code[e] | code[e + 1] << 4);
+        } else {
+            uint32_t w = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w |= code[e] << (4 * ((e & 1) * 4 + (e >> 1)));
+            kv4_word(img, L::k_dword(slot, t)) = w;
         }
-    };
-    if (c.group == 32) {
-#pragma unroll
-        for (int g = 0; g < W / 32; ++g) group(2 * g, 2);
-    } else {
-#pragma unroll
-        for (int g = 0; g < W / 64; ++g) group(4 * g, 4);
+        if (t % (G / 8) == 0) {
+            const int n = t / (G / 8);
+            kv4_half(img, VALUES ? L::v_step(slot, n) : L::k_step(slot, n)) = g.sb;
+            kv4_half(img, VALUES ? L::v_low(slot, n) : L::k_low(slot, n)) = g.lb;
+        }
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) kv4_half(blk, kv4_v_half(c, slot, o, b)) = half[b];
 }
 
-// A wavefront takes four heads' keys, or values, of one row.
-template <int TYPE, int W>
+// Positions lo .. hi of a chunk from `img` to `to` (two images of one layout), by
+// the whole workgroup.
+template <int W, int G, int THREADS>
+__device__ __forceinline__ void kv4_put_chunk(const uint8_t* img, uint8_t* to, int lo, int hi, int tid) {
+    typedef Kv4Lay<W, G> L;
+    if (lo == 0 && hi == 31) {
+        for (uint32_t i = tid; i < L::CHUNK / 16; i += THREADS)
+            reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(img)[i];
+        return;
+    }
+    // Key dwords, value halves, the four scales of a group: pieces of one position.
+    constexpr int KD = W / 8, VH = W / 4, PIECES = KD + VH + 4 * L::NG;
+    for (int i = tid; i < (hi - lo + 1) * PIECES; i += THREADS) {
+        const int slot = lo + i / PIECES, p = i % PIECES;
+        if (p < KD) {
+            const uint32_t at = L::k_dword(slot, p);
+            kv4_word(to, at) = kv4_word(img, at);
+        } else {
+            const int x = p - KD - VH, g = x >> 2;
+            const uint32_t at = p < KD + VH    ? L::v_half(slot, (p - KD) & 15, (p - KD) >> 4)
+                                : (x & 3) == 0 ? L::k_step(slot, g)
+                                : (x & 3) == 1 ? L::k_low(slot, g)
+                                : (x & 3) == 2 ? L::v_step(slot, g)
+                                               : L::v_low(slot, g);
+            kv4_half(to, at) = kv4_half(img, at);
+        }
+    }
+}
+
+struct Kv4Rows {  // the rows of an append, or of a read
+    int64_t ldk, ldv;
+    int veck, vecv;  // rows of k, of v can be taken 8 elements at a time
+    int each;        // chunks of every sequence, when all have the same rows (the most), else 0
+};
+
+__host__ __device__ inline int kv4_most_chunks(int rows) { return rows ? (rows + 30) / 32 + 1 : 0; }
+
+template <int TYPE, int W, int G>
 __global__ __launch_bounds__(256) void k_kv4_append(Kv4View c, int layer, const typename Kv4Elem<TYPE>::T* __restrict__ k,
-                                                    const typename Kv4Elem<TYPE>::T* __restrict__ v, int64_t ldk,
-                                                    int64_t ldv) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t quads = (c.heads + 3) / 4;
-    const int row = (int)(w / (2 * quads));
-    const uint32_t u = w % (2 * quads);
-    if (row >= c.rows) return;
-    const Kv4Entry e = kv4_batch(c, c.each ? row / c.each : kv4_entry(c.batch + 2, 4, c.nb, row, lane));
-    const int pos = e.len - e.row1 + row;
-    const int pg = pos < 0 ? -1 : kv4_page(c, e.seq, pos);
-    const int head = (int)(u % quads) * 4 + (lane >> 4);
-    if (pg < 0 || head >= c.heads) return;
-    uint8_t* blk = kv4_block(c, pg, layer, head);
-    const int slot = pos & (c.page() - 1);
-    if (u < quads)
-        kv4_store_k<TYPE, W>(c, k + row * ldk + (int64_t)head * c.dk, blk, slot, lane);
-    else
-        kv4_store_v<TYPE, W>(c, v + row * ldv + (int64_t)head * c.dv, blk, slot, lane);
+                                                    const typename Kv4Elem<TYPE>::T* __restrict__ v, Kv4Rows a) {
+    typedef Kv4Lay<W, G> L;
+    __shared__ __align__(16) uint8_t img[L::CHUNK];
+    const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.x % c.heads;
+    int unit = blockIdx.x / c.heads, b;
+    if (a.each) {
+        b = unit / a.each;
+        unit -= b * a.each;
+    } else
+        b = kv4_find(c, unit, lane, [](const Kv4Entry& e) { return kv4_most_chunks(e.row1 - e.row0); });
+    if (b >= c.nb) return;
+    const Kv4Entry e = kv4_batch(c, b);
+    const int first = e.len - (e.row1 - e.row0);  // the position of row row0
+    const int pos0 = ((first >> 5) + unit) << 5, lo = max(first - pos0, 0), hi = min(e.len - 1 - pos0, 31);
+    if (first < 0 || lo > hi) return;
+    const int pg = kv4_page(c, e.seq, pos0);
+    if (pg < 0) return;
+#pragma unroll 1
+    for (int s0 = lo; s0 <= hi; s0 += 16) {
+        const int slot = s0 + (tid >> 4);
+        const bool live = slot <= hi;
+        const int64_t row = e.row0 + (live ? pos0 + slot - first : 0);
+        kv4_pack_row<TYPE, W, G, false>(k + row * a.ldk + (int64_t)head * c.dk, c.dk, a.veck, img, slot, lane, live);
+        kv4_pack_row<TYPE, W, G, true>(v + row * a.ldv + (int64_t)head * c.dv, c.dv, a.vecv, img, slot, lane, live);
+    }
+    __syncthreads();
+    uint8_t* to = kv4_block(c, pg, layer, head) + (uint32_t)((pos0 & (c.page() - 1)) >> 5) * L::CHUNK;
+    kv4_put_chunk<W, G, 256>(img, to, lo, hi, tid);
 }
 
 template <int TYPE>
-static hipError_t append_typed(const Kv4View& c, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv,
-                               hipStream_t s) {
+static bool can_take8(const void* p, int64_t ld, int dim) {
+    const size_t es = sizeof(typename Kv4Elem<TYPE>::T);
+    return dim % 8 == 0 && (uintptr_t)p % 16 == 0 && ld * es % 16 == 0;
+}
+
+template <int TYPE, int G>
+static hipError_t append_typed(const Kv4View& c, const int* row0, int layer, const void* k, const void* v, int64_t ldk,
+                               int64_t ldv, hipStream_t s) {
     typedef const typename Kv4Elem<TYPE>::T* P;
-    const uint64_t blocks = ((uint64_t)c.rows * 2 * ((c.heads + 3) / 4) + 3) / 4;
-    if (blocks > 0x3fffffffu) return hipErrorInvalidValue;
-    auto kern = c.width == 64 ? k_kv4_append<TYPE, 64> : c.width == 128 ? k_kv4_append<TYPE, 128> : k_kv4_append<TYPE, 256>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, s, c, layer, (P)k, (P)v, ldk, ldv);
+    Kv4Rows a{ldk, ldv, can_take8<TYPE>(k, ldk, c.dk), can_take8<TYPE>(v, ldv, c.dv), kv4_most_chunks(c.each)};
+    int64_t units = (int64_t)a.each * c.nb;
+    if (!a.each)
+        for (int b = 0; b < c.nb; ++b) units += kv4_most_chunks(row0[b + 1] - row0[b]);
+    if (units * c.heads > 0x7fffffff) return hipErrorInvalidValue;
+    auto kern = c.width == 64    ? k_kv4_append<TYPE, 64, G>
+                : c.width == 128 ? k_kv4_append<TYPE, 128, G>
+                                 : k_kv4_append<TYPE, 256, G>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(units * c.heads)), dim3(256), 0, s, c, layer, (P)k, (P)v, a);
     return hipGetLastError();
 }
 
-hipError_t launch_kv4_append(const Kv4View& c, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int type,
-                             hipStream_t s) {
-    return type == KV4_F32   ? append_typed<KV4_F32>(c, layer, k, v, ldk, ldv, s)
-           : type == KV4_F16 ? append_typed<KV4_F16>(c, layer, k, v, ldk, ldv, s)
-                             : append_typed<KV4_BF16>(c, layer, k, v, ldk, ldv, s);
+template <int TYPE>
+static hipError_t append_typed(const Kv4View& c, const int* row0, int layer, const void* k, const void* v, int64_t ldk,
+                               int64_t ldv, hipStream_t s) {
+    return c.group == 32 ? append_typed<TYPE, 32>(c, row0, layer, k, v, ldk, ldv, s)
+                         : append_typed<TYPE, 64>(c, row0, layer, k, v, ldk, ldv, s);
 }
 
-// The values held, a wavefront as in the store.  step * code is exact in f32,
-// so the fma rounds once, as the product and the sum do.
-template <int TYPE, int W>
-__global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, Kv4Spans p, int64_t rows, int64_t row_at,
-                                                  typename Kv4Elem<TYPE>::T* __restrict__ k,
-                                                  typename Kv4Elem<TYPE>::T* __restrict__ v) {
-    const int lane = threadIdx.x & 63, o = lane & 15;
-    const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t quads = (c.heads + 3) / 4;
-    const int row = (int)(w / (2 * quads));
-    const uint32_t u = w % (2 * quads);
-    if (row >= p.row0[p.n]) return;
-    const int b = kv4_entry(p.row0 + 1, 1, p.n, row, lane);
-    const int pos = p.pos[b] + row - p.row0[b];
-    const int pg = kv4_page(c, p.seq[b], pos);
-    const int head = (int)(u % quads) * 4 + (lane >> 4);
-    if (pg < 0 || head >= c.heads) return;
-    const uint8_t* blk = kv4_block(c, pg, layer0 + (int)blockIdx.y, head);
-    const int slot = pos & (c.page() - 1);
-    const int64_t at = ((int64_t)blockIdx.y * rows + row_at + row) * c.heads + head;
-    if (u < quads) {
+hipError_t launch_kv4_append(const Kv4View& c, const int* row0, int layer, const void* k, const void* v, int64_t ldk,
+                             int64_t ldv, int type, hipStream_t s) {
+    return type == KV4_F32   ? append_typed<KV4_F32>(c, row0, layer, k, v, ldk, ldv, s)
+           : type == KV4_F16 ? append_typed<KV4_F16>(c, row0, layer, k, v, ldk, ldv, s)
+                             : append_typed<KV4_BF16>(c, row0, layer, k, v, ldk, ldv, s);
+}
+
+// Eight dims of a row of keys, or of values, out of a chunk's image.  step * code
+// is exact in f32, so the fma rounds once, as the product and the sum do.
+template <int TYPE, int W, int G, bool VALUES>
+__device__ __forceinline__ void kv4_unpack8(const uint8_t* img, int slot, int t, typename Kv4Elem<TYPE>::T* __restrict__ to,
+                                            int dim, bool vec) {
+    typedef typename Kv4Elem<TYPE>::T T;
+    typedef T Vec __attribute__((ext_vector_type(8)));
+    typedef Kv4Lay<W, G> L;
+    const int g = t * 8 / G;
+    const float step = f16_value(kv4_half(img, VALUES ? L::v_step(slot, g) : L::k_step(slot, g)));
+    const float low = f16_value(kv4_half(img, VALUES ? L::v_low(slot, g) : L::k_low(slot, g)));
+    uint32_t code[8];
+    if constexpr (VALUES) {
 #pragma unroll
-        for (int t0 = 0; t0 < W / 8; t0 += 16) {
-            const int t = t0 + o;
-            if (t * 8 >= c.dk) continue;
-            const uint32_t code = kv4_word(blk, kv4_k_dword(c, slot, t));
-            const int g = t * 8 / c.group;
-            const float step = f16_value(kv4_half(blk, kv4_k_scale(c, slot, g))), low = f16_value(kv4_half(blk, kv4_k_low(c, slot, g)));
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (t * 8 + e < c.dk)
-                    Kv4Elem<TYPE>::put(k + at * c.dk + t * 8 + e,
-                                       __builtin_fmaf(step, (float)((code >> (4 * ((e & 1) * 4 + (e >> 1)))) & 15u), low));
+        for (int e = 0; e < 8; e += 2) {
+            const uint32_t y = img[L::v_byte(slot, t * 4 + e / 2)];
+            code[e] = y & 15u;
+            code[e + 1] = y >> 4;
         }
     } else {
+        const uint32_t w = kv4_word(img, L::k_dword(slot, t));
 #pragma unroll
-        for (int i = 0; i < W / 16; ++i) {
-            const int d = 16 * i + o;
-            if (d >= c.dv) continue;
-            const int g = d / c.group;
-            const uint32_t code = (uint32_t)kv4_half(blk, kv4_v_half(c, slot, o, i >> 2)) >> (4 * (i & 3)) & 15u;
-            Kv4Elem<TYPE>::put(v + at * c.dv + d, __builtin_fmaf(f16_value(kv4_half(blk, kv4_v_scale(c, slot, g))), (float)code,
-                                                                 f16_value(kv4_half(blk, kv4_v_low(c, slot, g)))));
-        }
+        for (int e = 0; e < 8; ++e) code[e] = w >> (4 * ((e & 1) * 4 + (e >> 1))) & 15u;
     }
+    Vec y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        T z;
+        Kv4Elem<TYPE>::put(&z, __builtin_fmaf(step, (float)code[e], low));
+        y[e] = z;
+    }
+    if (vec)
+        *reinterpret_cast<Vec*>(to + t * 8) = y;
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (t * 8 + e < dim) to[t * 8 + e] = y[e];
+}
+
+// A workgroup reads one head's rows of one chunk: the chunk to LDS, 16 bytes a
+// thread, then 8 dims a lane out of it.
+template <int TYPE, int W, int G>
+__global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, Kv4Spans p, int64_t rows, int64_t row_at,
+                                                  typename Kv4Elem<TYPE>::T* __restrict__ k,
+                                                  typename Kv4Elem<TYPE>::T* __restrict__ v, Kv4Rows a) {
+    typedef Kv4Lay<W, G> L;
+    __shared__ __align__(16) uint8_t img[L::CHUNK];
+    const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.x % c.heads;
+    const int unit = blockIdx.x / c.heads, b = kv4_span(p.unit0, p.n, unit, lane);
+    const int first = p.pos[b], end = first + p.row0[b + 1] - p.row0[b];
+    const int pos0 = ((first >> 5) + unit - p.unit0[b]) << 5, lo = max(first - pos0, 0), hi = min(end - 1 - pos0, 31);
+    const int pg = kv4_page(c, p.seq[b], pos0);
+    if (pg < 0) return;
+    const uint8_t* from = kv4_block(c, pg, layer0 + (int)blockIdx.y, head) + (uint32_t)((pos0 & (c.page() - 1)) >> 5) * L::CHUNK;
+    for (uint32_t i = tid; i < L::CHUNK / 16; i += 256)
+        reinterpret_cast<uint4*>(img)[i] = reinterpret_cast<const uint4*>(from)[i];
+    __syncthreads();
+    const int64_t row = (int64_t)blockIdx.y * rows + row_at + p.row0[b] + (pos0 - first);  // of slot 0
+    for (int i = tid; i < (hi - lo + 1) * (W / 8); i += 256) {
+        const int slot = lo + i / (W / 8), t = i % (W / 8);
+        const int64_t at = (row + slot) * c.heads + head;
+        if (t * 8 < c.dk) kv4_unpack8<TYPE, W, G, false>(img, slot, t, k + at * c.dk, c.dk, a.veck);
+        if (t * 8 < c.dv) kv4_unpack8<TYPE, W, G, true>(img, slot, t, v + at * c.dv, c.dv, a.vecv);
+    }
+}
+
+template <int TYPE, int G>
+static hipError_t read_typed(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,
+                             hipStream_t s) {
+    typedef typename Kv4Elem<TYPE>::T* P;
+    const Kv4Rows a{0, 0, can_take8<TYPE>(k, c.dk, c.dk), can_take8<TYPE>(v, c.dv, c.dv), 0};
+    const int64_t blocks = (int64_t)p.unit0[p.n] * c.heads;
+    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    auto kern = c.width == 64 ? k_kv4_read<TYPE, 64, G> : c.width == 128 ? k_kv4_read<TYPE, 128, G> : k_kv4_read<TYPE, 256, G>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks, layer < 0 ? c.layers : 1), dim3(256), 0, s, c, layer < 0 ? 0 : layer, p,
+                       rows, row, (P)k, (P)v, a);
+    return hipGetLastError();
 }
 
 template <int TYPE>
 static hipError_t read_typed(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,
                              hipStream_t s) {
-    typedef typename Kv4Elem<TYPE>::T* P;
-    const uint64_t blocks = ((uint64_t)p.row0[p.n] * 2 * ((c.heads + 3) / 4) + 3) / 4;
-    if (blocks > 0x3fffffffu) return hipErrorInvalidValue;
-    auto kern = c.width == 64 ? k_kv4_read<TYPE, 64> : c.width == 128 ? k_kv4_read<TYPE, 128> : k_kv4_read<TYPE, 256>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks, layer < 0 ? c.layers : 1), dim3(256), 0, s, c, layer < 0 ? 0 : layer, p,
-                       rows, row, (P)k, (P)v);
-    return hipGetLastError();
+    return c.group == 32 ? read_typed<TYPE, 32>(c, layer, p, rows, row, k, v, s)
+                         : read_typed<TYPE, 64>(c, layer, p, rows, row, k, v, s);
 }
 
 hipError_t launch_kv4_read(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,
                            int type, hipStream_t s) {
-    static_assert(sizeof(Kv4Spans) <= 3600, "the argument segment");
+    static_assert(sizeof(Kv4Spans) <= 3900, "the argument segment");
     return type == KV4_F32   ? read_typed<KV4_F32>(c, layer, p, rows, row, k, v, s)
            : type == KV4_F16 ? read_typed<KV4_F16>(c, layer, p, rows, row, k, v, s)
                              : read_typed<KV4_BF16>(c, layer, p, rows, row, k, v, s);
@@ -258,42 +317,51 @@ hipError_t launch_kv4_pairs(const Kv4View& c, const Kv4Pairs& p, hipStream_t s) 
     return hipGetLastError();
 }
 
-// One position of one (layer, head) by 16 lanes, four positions a wavefront.
-// The fresh pages belong to this sequence alone and no position shares a byte
-// with another, so the order of the moves does not matter.
-__global__ __launch_bounds__(256) void k_kv4_runs(Kv4View c, const int* __restrict__ state, Kv4Runs r) {
-    const int lane = threadIdx.x & 63, l = lane & 15;
-    const int64_t i = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4);
-    if (i >= r.row0[r.n]) return;
-    int lo = 0, hi = r.n - 1;  // the run that holds position i of the launch
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (r.row0[mid] <= i) lo = mid;
-        else hi = mid - 1;
+// A workgroup writes one run's positions of one chunk of a fresh page, for one
+// (layer, head): gathered into LDS, then stored as an append stores them.  The
+// fresh pages belong to this sequence alone and no position shares a byte with
+// another, so the order of the moves does not matter.
+template <int W, int G>
+__global__ __launch_bounds__(128) void k_kv4_runs(Kv4View c, const int* __restrict__ state, Kv4Runs r) {
+    typedef Kv4Lay<W, G> L;
+    __shared__ __align__(16) uint8_t img[L::CHUNK];
+    const int tid = threadIdx.x, lane = tid & 63, l = tid & 15;
+    const int unit = blockIdx.x, m = kv4_span(r.unit0, r.n, unit, lane);
+    const int dst = r.dst[m], pos0 = ((dst >> 5) + unit - r.unit0[m]) << 5;
+    const int lo = max(dst - pos0, 0), hi = min(dst + r.count[m] - 1 - pos0, 31), src0 = r.src[m] - dst + pos0;
+    const int to = state[r.fresh[m] + (pos0 >> c.page_log2)], mask = c.page() - 1;
+    for (int slot = lo + (tid >> 4); slot <= hi; slot += 8) {
+        const int src = src0 + slot, from = kv4_page(c, r.seq[m], src);
+        if (from < 0) continue;
+        const uint8_t* a = kv4_block(c, from, (int)blockIdx.y, (int)blockIdx.z) + (uint32_t)((src & mask) >> 5) * L::CHUNK;
+        const int s = src & 31;
+#pragma unroll
+        for (int t = l; t < W / 8; t += 16) kv4_word(img, L::k_dword(slot, t)) = kv4_word(a, L::k_dword(s, t));
+#pragma unroll
+        for (int b = 0; b < L::NB; ++b) kv4_half(img, L::v_half(slot, l, b)) = kv4_half(a, L::v_half(s, l, b));
+        if (l < L::NG) {
+            kv4_half(img, L::k_step(slot, l)) = kv4_half(a, L::k_step(s, l));
+            kv4_half(img, L::k_low(slot, l)) = kv4_half(a, L::k_low(s, l));
+            kv4_half(img, L::v_step(slot, l)) = kv4_half(a, L::v_step(s, l));
+            kv4_half(img, L::v_low(slot, l)) = kv4_half(a, L::v_low(s, l));
+        }
     }
-    const int off = (int)i - r.row0[lo];
-    const int src = r.src[lo] + off, dst = r.dst[lo] + off;
-    const int from = kv4_page(c, r.seq[lo], src), to = state[r.fresh[lo] + (dst >> c.page_log2)];
-    if (from < 0) return;
-    const int mask = c.page() - 1, s0 = src & mask, s1 = dst & mask, W = c.width, nb = W / 64, ng = c.groups();
-    const uint8_t* a = kv4_block(c, from, (int)blockIdx.y, (int)blockIdx.z);
-    uint8_t* z = kv4_block(c, to, (int)blockIdx.y, (int)blockIdx.z);
-    for (int t = l; t < W / 8; t += 16) kv4_word(z, kv4_k_dword(c, s1, t)) = kv4_word(a, kv4_k_dword(c, s0, t));
-    for (int b = 0; b < nb; ++b) kv4_half(z, kv4_v_half(c, s1, l, b)) = kv4_half(a, kv4_v_half(c, s0, l, b));
-    if (l < ng) {
-        kv4_half(z, kv4_k_scale(c, s1, l)) = kv4_half(a, kv4_k_scale(c, s0, l));
-        kv4_half(z, kv4_k_low(c, s1, l)) = kv4_half(a, kv4_k_low(c, s0, l));
-        kv4_half(z, kv4_v_scale(c, s1, l)) = kv4_half(a, kv4_v_scale(c, s0, l));
-        kv4_half(z, kv4_v_low(c, s1, l)) = kv4_half(a, kv4_v_low(c, s0, l));
-    }
+    __syncthreads();
+    uint8_t* z = kv4_block(c, to, (int)blockIdx.y, (int)blockIdx.z) + (uint32_t)((pos0 & mask) >> 5) * L::CHUNK;
+    kv4_put_chunk<W, G, 128>(img, z, lo, hi, tid);
+}
+
+template <int G>
+static hipError_t launch_runs(const Kv4View& c, const int* state, const Kv4Runs& r, hipStream_t s) {
+    auto kern = c.width == 64 ? k_kv4_runs<64, G> : c.width == 128 ? k_kv4_runs<128, G> : k_kv4_runs<256, G>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)r.unit0[r.n], c.layers, c.heads), dim3(128), 0, s, c, state, r);
+    return hipGetLastError();
 }
 
 hipError_t launch_kv4_runs(const Kv4View& c, const int* state, const Kv4Runs& r, hipStream_t s) {
     static_assert(sizeof(Kv4Runs) <= 3900, "the argument segment");
-    const int64_t n = r.row0[r.n];
-    if (n <= 0) return hipSuccess;
-    hipLaunchKernelGGL(k_kv4_runs, dim3((unsigned)((n + 15) / 16), c.layers, c.heads), dim3(256), 0, s, c, state, r);
-    return hipGetLastError();
+    if (r.unit0[r.n] <= 0) return hipSuccess;
+    return c.group == 32 ? launch_runs<32>(c, state, r, s) : launch_runs<64>(c, state, r, s);
 }
 
 }  // namespace nh
