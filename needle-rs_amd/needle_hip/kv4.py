@@ -3,10 +3,10 @@
 counterpart in the reference."""
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes as C
 
-import numpy as np
 import torch
 
 import needle_hip as nh
@@ -14,20 +14,19 @@ import needle_hip as nh
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # NH_F32, NH_F16, NH_BF16
 
 
-def _ints(v) -> np.ndarray:
-    a = np.asarray(v, dtype=np.int64).reshape(-1)
-    if a.size and (a.min() < -(1 << 31) or a.max() >= 1 << 31):
-        raise ValueError("not a 32-bit number")
-    return np.ascontiguousarray(a, dtype=np.int32)
+def _ints(v):
+    """(the numbers as C ints, their address, their count); the array keeps them alive."""
+    try:
+        a = array.array("i", v)
+    except (OverflowError, TypeError) as e:
+        raise ValueError(f"not a list of 32-bit numbers: {e}") from None
+    at, n = a.buffer_info()
+    return a, at, n
 
 
 def _on(stream):
     """Allocations of the call come from the memory of the stream that uses them."""
     return torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext()
-
-
-def _workspace(n: int, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
 
 
 def _ptr(t):
@@ -53,6 +52,8 @@ class KvCache4:
         self.layers, self.kv_heads, self.qk_dim, self.v_dim = int(layers), int(kv_heads), int(qk_dim), int(v_dim)
         self.group, self.page, self.pages = int(group), int(page), int(pages)
         self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index
+        self._rows = 0  # the batch's
 
     # ---- sequences
     def new_seq(self) -> int:
@@ -65,33 +66,38 @@ class KvCache4:
     def free(self, seq: int):
         """Gives back the pages that no branch shares."""
         nh._check(nh._lib.nh_kv4_seq_free(self.h, int(seq)))
+        self._rows = self.rows  # (the batch may be over)
 
     def truncate(self, seq: int, length: int):
         """Forgets positions `length` and on."""
         nh._check(nh._lib.nh_kv4_seq_truncate(self.h, int(seq), int(length)))
+        self._rows = self.rows
 
     def fork(self, seq: int, n: int = 1) -> list:
         """n branches that share the sequence's pages until they are written."""
-        out = np.zeros(max(int(n), 1), dtype=np.int32)
-        nh._check(nh._lib.nh_kv4_seq_fork(self.h, int(seq), int(n), nh._hptr(out)))
-        return out[:n].tolist()
+        out = (C.c_int * max(int(n), 1))()
+        nh._check(nh._lib.nh_kv4_seq_fork(self.h, int(seq), int(n), C.addressof(out)))
+        self._rows = self.rows
+        return out[:n]
 
     def copy(self, seq: int, stream=None) -> int:
         """A branch with pages of its own."""
-        return nh._check(nh._lib.nh_kv4_seq_copy(self.h, int(seq), nh._stream(stream)))
+        made = nh._check(nh._lib.nh_kv4_seq_copy(self.h, int(seq), nh._stream(stream)))
+        self._rows = self.rows
+        return made
 
     def compact(self, seqs, ranges, stream=None):
         """Sequence seqs[i] keeps the positions of ranges[i], ascending (begin,
         end) pairs, closed up."""
-        s = _ints(seqs)
-        if len(ranges) != s.size:
+        if len(ranges) != len(seqs):
             raise ValueError("one list of ranges for each sequence")
-        counts = _ints([len(r) for r in ranges])
-        flat = _ints([x for r in ranges for pair in r for x in pair])
-        if flat.size != 2 * int(counts.sum()):
+        if any(len(pair) != 2 for r in ranges for pair in r):
             raise ValueError("a range is a (begin, end) pair")
-        nh._check(nh._lib.nh_kv4_seq_compact(self.h, nh._hptr(s), s.size, nh._hptr(counts), nh._hptr(flat),
-                                             nh._stream(stream)))
+        s, ps, n = _ints(seqs)
+        counts, pc, _ = _ints([len(r) for r in ranges])
+        flat, pf, _ = _ints([x for r in ranges for pair in r for x in pair])
+        nh._check(nh._lib.nh_kv4_seq_compact(self.h, ps, n, pc, pf, nh._stream(stream)))
+        self._rows = self.rows
 
     @property
     def free_pages(self) -> int:
@@ -105,10 +111,12 @@ class KvCache4:
     # ---- rows
     def extend(self, seqs, rows, stream=None):
         """rows[i] more positions for each sequence; they become the batch."""
-        s, r = _ints(seqs), _ints(rows)
-        if s.size != r.size:
+        s, ps, n = _ints(seqs)
+        r, pr, m = _ints(rows)
+        if n != m:
             raise ValueError("one number of rows for each sequence")
-        nh._check(nh._lib.nh_kv4_extend(self.h, nh._hptr(s), nh._hptr(r), s.size, nh._stream(stream)))
+        nh._check(nh._lib.nh_kv4_extend(self.h, ps, pr, n, nh._stream(stream)))
+        self._rows = sum(r)
 
     @property
     def rows(self) -> int:
@@ -117,13 +125,15 @@ class KvCache4:
 
     def _rows_of(self, t: torch.Tensor, heads: int, dim: int, what: str) -> int:
         """The row stride of [rows][heads][dim]; a row lies in one piece."""
-        if t.dim() != 3 or t.shape[1:] != (heads, dim) or t.shape[0] != self.rows:
-            raise ValueError(f"{what} is [{self.rows}][{heads}][{dim}], not {list(t.shape)}")
-        if t.device != self.device or t.dtype not in _TYPES:
+        n = self._rows
+        if t.shape != (n, heads, dim):
+            raise ValueError(f"{what} is [{n}][{heads}][{dim}], not {list(t.shape)}")
+        if t.get_device() != self._index or t.dtype not in _TYPES:
             raise ValueError(f"{what} is f32, f16 or bf16 on {self.device}")
-        if (dim > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != dim):
+        ld, of_head, of_dim = t.stride()
+        if (dim > 1 and of_dim != 1) or (heads > 1 and of_head != dim):
             raise ValueError(f"a row of {what} is not contiguous")
-        return t.stride(0) if t.shape[0] > 1 else heads * dim
+        return ld if n > 1 else heads * dim
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, stream=None):
         """The batch's keys [rows][kv_heads][qk_dim] and values [rows][kv_heads][v_dim]
@@ -139,20 +149,22 @@ class KvCache4:
         """The values held: rows[i] positions from starts[i] of seqs[i], as (k
         [rows][kv_heads][qk_dim], v [rows][kv_heads][v_dim]); with layer None of
         every layer, [layers] in front."""
-        s, p, r = _ints(seqs), _ints(starts), _ints(rows)
-        if not s.size == p.size == r.size:
+        s, ps, count = _ints(seqs)
+        p, pp, m = _ints(starts)
+        r, pr, m2 = _ints(rows)
+        if not count == m == m2:
             raise ValueError("one start and one number of rows for each sequence")
         if dtype not in _TYPES:
             raise ValueError("f32, f16 or bf16")
-        n = int(np.maximum(r, 0).sum(dtype=np.int64))
+        if layer is not None and int(layer) < 0:
+            raise ValueError("no such layer")
+        n = sum(x for x in r if x > 0)
         shape = (n, self.kv_heads) if layer is not None else (self.layers, n, self.kv_heads)
         with _on(stream):
             k = torch.empty((*shape, self.qk_dim), dtype=dtype, device=self.device)
             v = torch.empty((*shape, self.v_dim), dtype=dtype, device=self.device)
-        if layer is not None and int(layer) < 0:
-            raise ValueError("no such layer")
-        nh._check(nh._lib.nh_kv4_read(self.h, -1 if layer is None else int(layer), nh._hptr(s), nh._hptr(p), nh._hptr(r),
-                                      s.size, k.data_ptr(), v.data_ptr(), _TYPES[dtype], nh._stream(stream)))
+        nh._check(nh._lib.nh_kv4_read(self.h, -1 if layer is None else int(layer), ps, pp, pr, count, k.data_ptr(),
+                                      v.data_ptr(), _TYPES[dtype], nh._stream(stream)))
         return k, v
 
     def attend(self, layer: int, q: torch.Tensor, scale: float | None = None, sink: int = 0, ring: int = 0,
@@ -162,7 +174,7 @@ class KvCache4:
         `sink` positions and its last `ring`.  Returns [rows][heads][v_dim] of
         q's type (`out`, if given); lse (f32 [rows][heads]) takes the logs of
         the summed exponentials.  scale: 1 / sqrt(qk_dim) unless given."""
-        heads = q.shape[1] if q.dim() == 3 else 0
+        heads = q.shape[1] if len(q.shape) == 3 else 0
         ldq = self._rows_of(q, heads, self.qk_dim, "q")
         with _on(stream):
             if out is None:
@@ -171,12 +183,12 @@ class KvCache4:
             if out.dtype != q.dtype:
                 raise ValueError("q and out differ in type")
             if lse is not None and (lse.dtype != torch.float32 or lse.shape != (q.shape[0], heads) or
-                                    not lse.is_contiguous() or lse.device != self.device):
+                                    not lse.is_contiguous() or lse.get_device() != self._index):
                 raise ValueError("lse is a contiguous f32 [rows][heads]")
             n = nh._lib.nh_kv4_attend_ws_bytes(self.h, heads, int(sink), int(ring))
             if n < 0:
                 nh._check(int(n))
-            ws = _workspace(n, self.device)
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
         nh._check(nh._lib.nh_kv4_attend(self.h, int(layer), q.data_ptr(), ldq, heads,
                                         float(self.qk_dim ** -0.5 if scale is None else scale), int(sink), int(ring),
                                         out.data_ptr(), ldo, _ptr(lse), _TYPES[q.dtype], _ptr(ws), n, nh._stream(stream)))
@@ -197,23 +209,25 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor | 
     int32.  probs [batch][n][vocab]: the drafter's probabilities (None: it has
     none); counts [batch]: drafts of each sequence (None: n); temperature 0:
     greedy.  Rows of logits and probs may be padded (a view of wider rows)."""
-    nh.init()
-    if logits.dim() != 3 or drafts.dim() != 2:
+    if not nh._ready:
+        nh.init()
+    if len(logits.shape) != 3 or len(drafts.shape) != 2:
         raise ValueError("logits are [batch][n + 1][vocab], drafts [batch][n]")
     batch, rows, vocab = logits.shape
-    n = rows - 1
-    device = logits.device
+    n, index = rows - 1, logits.get_device()
 
     def strided(t, what):
-        if t.dtype not in _TYPES or t.device != device or not t.is_cuda:
+        if t.dtype not in _TYPES or t.get_device() != index or index < 0:
             raise ValueError(f"{what}: f32, f16 or bf16 on the logits' device")
-        ld = t.stride(1) if t.shape[1] > 1 else t.stride(0) if t.shape[0] > 1 else t.shape[2]
-        if t.shape[2] > 1 and t.stride(2) != 1 or t.shape[0] > 1 and t.stride(0) != ld * t.shape[1]:
+        b, r, v = t.shape
+        sb, sr, sv = t.stride()
+        ld = sr if r > 1 else sb if b > 1 else v
+        if v > 1 and sv != 1 or b > 1 and sb != ld * r:
             raise ValueError(f"the rows of {what} do not follow each other")
-        return max(ld, t.shape[2])
+        return max(ld, v)
 
     def plain(t, dtype, shape, what):
-        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
             raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on the logits' device")
 
     ldl, ldp = strided(logits, "logits"), 0
@@ -223,18 +237,19 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor | 
     if counts is not None:
         plain(counts, torch.int32, (batch,), "counts")
     if probs is not None:
-        if tuple(probs.shape) != (batch, n, vocab):
+        if probs.shape != (batch, n, vocab):
             raise ValueError("probs are [batch][n][vocab]")
         ldp = strided(probs, "probs") if probs.numel() else vocab
-    if device.index != torch.cuda.current_device():
+    if index != torch.cuda.current_device():
         raise ValueError("the tensors are on another device than the current one")
     ws_bytes = nh._lib.nh_verify_drafts_ws_bytes(batch, n, vocab)
     if ws_bytes < 0:
         nh._check(int(ws_bytes))
     with _on(stream):
-        accepted = torch.empty(batch, dtype=torch.int32, device=device)
-        tokens = torch.empty((batch, n + 1), dtype=torch.int32, device=device)
-        ws = _workspace(ws_bytes, device)
+        # (one allocation for both results and one for the workspace, which goes back at the end)
+        both = torch.empty(batch * (n + 2), dtype=torch.int32, device=logits.device)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
+    accepted, tokens = both[:batch], both[batch:].view(batch, n + 1)
     nh._check(nh._lib.nh_verify_drafts(logits.data_ptr(), _TYPES[logits.dtype], ldl, _ptr(drafts), _ptr(counts),
                                        _ptr(probs), _TYPES[probs.dtype] if probs is not None else 0, ldp, _ptr(u),
                                        float(temperature), batch, n, vocab, accepted.data_ptr(), tokens.data_ptr(),
