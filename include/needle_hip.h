@@ -441,8 +441,8 @@ int nh_kv4_read(nh_kv4* c, int layer, const int* seqs, const int* pos, const int
  * (Session::attend's span, crates/needle-engine/src/model.rs:62-66, by
  * position).  lse (f32 [rows][heads], or NULL): the log of the summed
  * exponentials, to join with other keys.  Scores, weights' sums and products
- * are held in f32; f16 and bf16 calls round a weight to 11 bits, f32 calls
- * carry 22.  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used
+ * are held in f32; f16 and bf16 calls round a weight to 11 bits (of many rows
+ * also a key's and a value's step x code), f32 calls carry 22.  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used
  * by the work queued on `stream` only (its size depends on the batch's
  * lengths: asked after the extend; 0: it may be NULL). */
 int64_t nh_kv4_attend_ws_bytes(const nh_kv4* c, int heads, int sink, int ring);

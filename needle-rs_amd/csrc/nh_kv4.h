@@ -24,8 +24,8 @@
 //                64 b + 32 (i / 2) + 2 o + i % 2 (i = 0 .. 3) at nibble i
 //   key steps    32 x NG f16
 //   key lows     32 x NG f16
-//   value steps  32 x NG f16
-//   value lows   f16 of (slot, g) at (slot / 4 NG + g) 4 + slot % 4
+//   value steps  f16 of (slot, g) at (slot / 4 NG + g) 4 + slot % 4
+//   value lows   as the value steps
 // Of a lane's 8 codes a dword, the two of a 16-bit half pair are one mask away
 // from an MFMA operand (see the attention kernel).  No position shares a byte
 // with another, so rows are written without reading their neighbours.

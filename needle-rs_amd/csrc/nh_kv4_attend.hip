@@ -70,6 +70,7 @@ struct KaPlan {
     int splits;      // key ranges of a sequence; more than one: partial results go to the workspace
     int tiles_each;  // row tiles of every sequence when they are equal, else 0
     int aligned;     // rows of q can be read 8 elements at a time
+    int out_aligned; // rows of out can be written 4 elements at a time
 };
 
 // The chunks that a tile of rows at positions lo .. hi sees: [0, ns) and [w, n).
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
 #pragma unroll
             for (int n = 0; n < Chunk::NS; ++n) {
                 const uint32_t s = x.vs[t][n];
-                const int key = key0 + 16 * t + 4 * kg + (int)(sidx + 16 * n) / NG;
+                const int key = key0 + 16 * t + 4 * kg + (int)(sidx & 3);
                 if (s < 0x7c00u && key <= phi) top = max(top, s);
             }
         // step < 2^(e - 14) for the f16 exponent field e (subnormals below 2^-14)
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
                 constexpr int g = GG.value;
                 float w[8];
                 static_for<0, 8>([&](auto K) {
-                    constexpr int k = K.value, at = (k % 4) * NG + g;
+                    constexpr int k = K.value, at = g * 4 + k % 4;
                     w[k] = p[k] * row_bcast<at % 16>(vstep[k / 4][at / 16]);
                 });
                 if (!whole)  // (a step may be NaN: a hidden key's weight is none)
@@ -487,6 +488,383 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
     }
 }
 
+// ------------------------------------------------------------------ prompts
+// Many rows: a workgroup of eight wavefronts takes 256 rows, 32 a wavefront, and
+// the chunks' codes are turned into f16 operands once for all of them, through
+// LDS, two chunks in turn.  Keys and values are kept as step x code there, in
+// units of a power of two above the largest step (one more AND-and-multiply for
+// two codes; rounded to 11 bits), their lows go through the same small products
+// as above, so the rounding is relative to a group's range and not to its
+// offset.  32 x 32 MFMAs: a lane holds 16 scores of its row, the other half of
+// them is 32 lanes away.  The weights' sum is one more row of the lows' product.
+constexpr int KP_WAVES = 8;
+constexpr int KP_ROWS = 32 * KP_WAVES;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ float halves_max(float v) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+}
+
+template <int TYPE, int W, int G>
+__global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
+    typedef typename Kv4Elem<TYPE>::T T;
+    typedef Kv4Lay<W, G> L;
+    constexpr int NG = L::NG, NJ = W / 32, NX = W / 16, ND = W / 32;
+    struct Image {  // a chunk's operands, 16 bytes a lane each
+        u32x4 k[NX][64], kl[64], v[ND][2][64], vl[2][64];
+    };
+    __shared__ Image img[2];
+
+    const int tid = threadIdx.x, lane = tid & 63, o = lane & 15, kg = lane >> 4, half = lane >> 5, m32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kvh = blockIdx.x % c.heads, per = a.heads / c.heads, split = blockIdx.y;
+    int tile = blockIdx.x / c.heads, b;
+    if (plan.tiles_each) {
+        b = tile / plan.tiles_each;
+        tile = plan.tiles_each - 1 - (tile - b * plan.tiles_each);  // the longest first
+    } else
+        b = kv4_find(c, tile, lane, [&](const Kv4Entry& e) { return ((e.row1 - e.row0) * per + KP_ROWS - 1) / KP_ROWS; });
+    if (b >= c.nb) return;
+    const Kv4Entry entry = kv4_batch(c, b);
+    const int row0 = entry.row0, nrows = entry.row1 - row0, first = entry.len - nrows, r0 = tile * KP_ROWS;
+    if (first < 0 || r0 >= nrows * per) return;
+    const int r1 = min(r0 + KP_ROWS, nrows * per) - 1;
+    const int plo = first + r0 / per, phi = first + r1 / per;
+    const int w0 = min(r0 + wave * 32, r1), w1 = min(w0 + 31, r1);  // this wavefront's rows
+    const int wlo = first + w0 / per, whi = first + w1 / per;
+    const int sink = a.ring ? a.sink : 0x7fffffff, ring = a.ring;
+
+    // The queries, as in the kernel above.
+    h8 q[NX], qs = {};
+    const int r = min(r0 + wave * 32 + m32, r1), token = r / per, pos = first + token;
+    float ck, cl;
+    {
+        const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(row0 + token) * a.ldq + (int64_t)(kvh * per + r - token * per) * c.dk;
+        float most = 0.0f, sums[NG] = {};
+        T x[NX][8];
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+            const int d = 16 * j + 8 * half;
+            typedef T Vec __attribute__((ext_vector_type(8)));
+            if (plan.aligned) {
+                Vec y = {};
+                if (d < c.dk) y = *reinterpret_cast<const Vec*>(src + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][e] = y[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][e] = d + e < c.dk ? src[d + e] : (T)0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)x[j][e]));
+        }
+        most = halves_max(most);
+        const int ef = max((int)(__builtin_bit_cast(uint32_t, most) >> 23 & 255u), 15);
+        const float up = __builtin_bit_cast(float, (uint32_t)(268 - ef) << 23);
+        cl = (a.scale * KA_LOG2E * 64.0f) * __builtin_bit_cast(float, (uint32_t)(ef - 14) << 23);
+        ck = cl * 16.0f;
+#pragma unroll
+        for (int j = 0; j < NX; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = (float)x[j][e] * up;
+                sums[j * 16 / G] += y;
+                q[j][e] = (_Float16)(y * (e & 2 ? 0.0625f : 1.0f));
+            }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const float s = (sums[g] + __shfl_xor(sums[g], 32, 64)) * 0.015625f;
+            const _Float16 hi = (_Float16)s, lo = (_Float16)(s - (float)hi);
+            qs[g] = half == 0 ? hi : lo;
+        }
+    }
+
+    f32x16 acc[ND], accl = {};
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+    float m = -__builtin_inff();
+    int kref = -24, vref = -24;  // 2^ref is above every step so far
+
+    const KaSpan span(plo, phi, a.sink, a.ring);
+    const int per_split = (span.count() + plan.splits - 1) / plan.splits;
+    const int c0 = split * per_split, c1 = min(c0 + per_split, span.count());
+    const int* table = c.table + (size_t)entry.seq * c.table_ld;
+    auto page_of = [&](int i) { return i < c1 ? table[span.at(i) * KA_CHUNK >> c.page_log2] : 0; };
+
+    // What this wavefront turns into operands: key dword (kt, kj), value dwords
+    // (vt, vn) under nibbles 2 vi, 2 vi + 1; a few wavefronts also the lows.
+    constexpr int UNITS = W == 128 ? 8 : 4;
+    const bool does_k = W == 128 || wave < UNITS, does_v = W == 128 || wave >= UNITS;
+    const int ku = wave % UNITS, kt = ku / NJ, kj = ku % NJ;
+    const int vt = ku & 1, vn = W == 128 ? ku >> 1 & 1 : 0, vi = W == 128 ? ku >> 2 : ku >> 1;
+    struct Raw {
+        uint32_t k, v[2], vs[2], low[2], ks_top, vs_top;
+        uint16_t ks;
+    };
+    auto load = [&](Raw& x, int i, int pg) {
+        const int slot = span.at(i) * KA_CHUNK & (c.page() - 1);
+        const uint8_t* p = kv4_block(c, (unsigned)pg < (unsigned)c.pages ? pg : 0, a.layer, kvh) + (uint32_t)(slot >> 5) * L::CHUNK;
+        if (does_k) {
+            x.k = kv4_word(p, L::lane_dword(lane, kt * NJ + kj));
+            x.ks = kv4_half(p, L::k_step(16 * kt + o, kj * 32 / G));
+        }
+        if (does_v) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) x.v[t] = kv4_word(p, 16 * W + L::lane_dword(lane, vt * NJ + t * L::NB + vn));
+#pragma unroll
+            for (int t = 0; t < 2; ++t) x.vs[t] = kv4_word(p, L::v_step(16 * vt + 4 * kg + 2 * t, (64 * vn + 32 * vi) / G));
+        }
+        // (two steps a lane, every wavefront the same, for the references)
+        const uint32_t x2 = 2 * (lane & (16 * NG - 1));
+        x.ks_top = kv4_word(p, 32 * W + 2 * x2);
+        x.vs_top = kv4_word(p, 32 * W + 128 * NG + 2 * x2);
+        if (wave < 4) {  // value lows of keys 16 y + 8 w + 4 half .., y = wave / 2, w = wave % 2
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                x.low[t] = kv4_word(p, L::v_low(16 * (wave >> 1) + 8 * (wave & 1) + 4 * half + 2 * t, m32 & (NG - 1)));
+        } else if (wave == 4) {  // key lows
+            if constexpr (NG == 1)
+                x.low[0] = kv4_half(p, L::k_low(m32, 0));
+            else
+#pragma unroll
+                for (int t = 0; t < NG / 2; ++t) x.low[t] = kv4_word(p, L::k_low(m32, 2 * t));
+        }
+    };
+    // The references raised where a step passes them (the same in every
+    // wavefront); true: a value step is NaN.
+    float vmul = 0.0f, kmul = 0.0f, vdown = 1.0f;
+    auto refer = [&](const Raw& x, int i) {
+        const int key0 = span.at(i) * KA_CHUNK;
+        const uint32_t x2 = 2 * (lane & (16 * NG - 1));
+        uint32_t kt2 = 0, vt2 = 0;
+        bool nan = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t k = x.ks_top >> (16 * t) & 0xffffu, v = x.vs_top >> (16 * t) & 0xffffu;
+            const int kkey = key0 + (int)(x2 + t) / NG, vkey = key0 + (int)(x2 / (4 * NG)) * 4 + (int)((x2 + t) & 3);
+            if (kkey <= phi && k < 0x7c00u) kt2 = max(kt2, k);
+            if (vkey <= phi && v < 0x7c00u) vt2 = max(vt2, v);
+            nan |= vkey <= phi && v >= 0x7c00u;
+        }
+        vdown = 1.0f;
+        if (__any((int)(kt2 >> 10) - 14 > kref || (int)(vt2 >> 10) - 14 > vref)) {
+            int ke = (int)(kt2 >> 10) - 14, ve = (int)(vt2 >> 10) - 14;
+#pragma unroll
+            for (int h = 1; h < 64; h <<= 1) {
+                ke = max(ke, __shfl_xor(ke, h, 64));
+                ve = max(ve, __shfl_xor(ve, h, 64));
+            }
+            ke = max(__builtin_amdgcn_readfirstlane(ke), kref);
+            ve = max(__builtin_amdgcn_readfirstlane(ve), vref);
+            vdown = pow2i(max(vref - ve, -126));
+            kref = ke;
+            vref = ve;
+        }
+        kmul = pow2i(14 - kref);
+        vmul = pow2i(14 - vref);
+        return __any(nan) != 0;
+    };
+    // Codes under a mask times scaled steps: c 2^-24 x step 2^(14 - ref) (16 times
+    // that under the upper mask), two at a time.
+    auto times = [](uint32_t codes, uint32_t steps) {
+        const h2 y = __builtin_bit_cast(h2, codes) * __builtin_bit_cast(h2, steps);
+        return __builtin_bit_cast(uint32_t, y);
+    };
+    auto unpack = [&](const Raw& x, int i, Image& to) {
+        const int key0 = span.at(i) * KA_CHUNK;
+        if (does_k) {
+            float s = f16_value(x.ks) * kmul;
+            s = s > 65504.0f ? 65504.0f : s;  // (a hidden key's; NaN stays, a key's reader has to see it)
+            const h2 s2 = {(_Float16)s, (_Float16)s};
+            const uint32_t sw = __builtin_bit_cast(uint32_t, s2), w = x.k, z = w >> 8;
+            const u32x4 y = {times(w & 0x000f000fu, sw), times(w & 0x00f000f0u, sw), times(z & 0x000f000fu, sw),
+                             times(z & 0x00f000f0u, sw)};
+            to.k[2 * kj + (kg >> 1)][(kg & 1) * 32 + 16 * kt + o] = y;
+        }
+        if (does_v) {
+            uint32_t sw[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                // (hidden keys' steps, and NaN, count as 0: what a NaN does to its readers comes with the weights)
+                const int key = key0 + 16 * vt + 4 * kg + 2 * t;
+                const float s0 = f16_value(x.vs[t]) * vmul, s1 = f16_value(x.vs[t] >> 16) * vmul;
+                const h2 s2 = {(_Float16)(key <= phi && s0 == s0 ? s0 : 0.0f), (_Float16)(key + 1 <= phi && s1 == s1 ? s1 : 0.0f)};
+                sw[t] = __builtin_bit_cast(uint32_t, s2);
+            }
+            const uint32_t w0 = vi ? x.v[0] >> 8 : x.v[0], w1 = vi ? x.v[1] >> 8 : x.v[1];
+            const uint2 even = {times(w0 & 0x000f000fu, sw[0]), times(w1 & 0x000f000fu, sw[1])};
+            const uint2 odd = {times(w0 & 0x00f000f0u, sw[0]), times(w1 & 0x00f000f0u, sw[1])};
+            uint2* out = reinterpret_cast<uint2*>(&to.v[2 * vn + vi][vt][(kg & 1) * 32 + 2 * o]) + (kg >> 1);
+            out[0] = even;
+            out[2] = odd;
+        }
+        if (wave < 4) {
+            const bool one = m32 == 8;
+            const uint2 y = {one ? 0x3c003c00u : x.low[0], one ? 0x3c003c00u : x.low[1]};
+            reinterpret_cast<uint2*>(&to.vl[wave >> 1][lane])[wave & 1] = y;
+        } else if (wave == 4) {
+            u32x4 y = {};
+#pragma unroll
+            for (int t = 0; t < (NG + 1) / 2; ++t) y[t] = x.low[t];
+            to.kl[lane] = y;
+        }
+    };
+
+    auto compute = [&](const Image& x, int i, float kscale, bool nan) {
+        const int key0 = span.at(i) * KA_CHUNK;
+        if (key0 > whi || (key0 >= sink && key0 + KA_CHUNK - 1 <= wlo - ring)) return;  // nothing for these rows
+        const bool whole = key0 + KA_CHUNK - 1 <= wlo && (key0 + KA_CHUNK - 1 < sink || key0 > whi - ring);
+        f32x16 z = {}, low = {};
+        low = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x.kl[lane]), qs, low, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < NX; ++j)
+            z = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x.k[j][lane]), q[j], z, 0, 0, 0);
+        const bool fresh = m == -__builtin_inff();
+        const float zero = fresh ? 0.0f : m, cz = ck * kscale;
+        float s[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(z[e], cz, __builtin_fmaf(low[e], cl, 15.0f - zero));
+        bool seen[16];
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
+                seen[e] = (j <= pos) & ((j < sink) | (j > pos - ring));
+                s[e] = seen[e] ? s[e] : -__builtin_inff();
+            }
+        }
+        float most = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
+        most = halves_max(most);
+        if (__any(most > 15.0f || fresh)) {
+            const float over = most == -__builtin_inff() ? 0.0f : fresh ? most - 15.0f : fmaxf(most - 15.0f, 0.0f);
+            const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
+            m = fresh && most == -__builtin_inff() ? m : zero + over;
+            accl *= keep;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[d] *= keep;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] -= over;
+        }
+        h8 p[2];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            const f32x2 y = {__builtin_amdgcn_exp2f(s[e]), __builtin_amdgcn_exp2f(s[e + 1])};
+            const h2 w = __builtin_convertvector(y, h2);
+            p[e >> 3][e & 7] = w[0], p[e >> 3][(e & 7) + 1] = w[1];
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            accl = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x.vl[y][lane]), p[y], accl, 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x.v[d][y][lane]), p[y], acc[d], 0, 0, 0);
+        }
+        if (nan) {
+            // A NaN value: the rows that see it are NaN in its group.
+            const uint8_t* at = kv4_block(c, table[key0 >> c.page_log2], a.layer, kvh) + (uint32_t)((key0 & (c.page() - 1)) >> 5) * L::CHUNK;
+            for (int g = 0; g < NG; ++g) {
+                int hit = 0;
+                for (int e = 0; e < 16; ++e) {
+                    const int j = 8 * (e >> 2) + 4 * half + (e & 3), key = key0 + j;
+                    const bool see = key <= pos && (key < sink || key > pos - ring);
+                    if (see && (kv4_half(at, L::v_step(j, g)) & 0x7fffu) > 0x7c00u) hit = 1;
+                }
+                hit |= __shfl_xor(hit, 32, 64);
+                const float add = hit ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    if (d * 32 / G == g) acc[d] += add;
+            }
+        }
+    };
+
+    // Loads two chunks ahead, operands one: a chunk's image is written while the
+    // one before it is used, one barrier a chunk.
+    {
+        Raw x;
+        float kscale[2];
+        bool nan[2];
+        int pg = page_of(c0 + 1);
+        if (c0 < c1) {
+            load(x, c0, page_of(c0));
+            nan[0] = refer(x, c0);
+            kscale[0] = pow2i(kref);
+            unpack(x, c0, img[0]);
+        }
+        if (c0 + 1 < c1) load(x, c0 + 1, pg);
+        pg = page_of(c0 + 2);
+        __syncthreads();
+        for (int i = c0; i < c1; ++i) {
+            const int now = (i - c0) & 1;
+            float down = 1.0f;
+            if (i + 1 < c1) {
+                nan[now ^ 1] = refer(x, i + 1);
+                kscale[now ^ 1] = pow2i(kref);
+                down = vdown;
+                unpack(x, i + 1, img[now ^ 1]);
+                if (i + 2 < c1) load(x, i + 2, pg);
+                pg = page_of(i + 3);
+            }
+            compute(img[now], i, kscale[now], nan[now]);
+            if (down != 1.0f) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d) acc[d] *= down;
+            }
+            __syncthreads();
+        }
+    }
+
+    // Row `m32` of the lows' product is in reg m % 4 + 4 (m / 8) of half m / 4 % 2.
+    const float l = __shfl(accl[4], m32, 64);  // m = 8
+    if (l != l) m = l;
+    const float unit = pow2i(10 + vref);
+    if (r0 + wave * 32 + m32 > r1) return;
+    const int64_t row = row0 + token, head = kvh * per + r - token * per;
+    const bool last = plan.splits == 1;
+    const float scale = last ? 1.0f / l : 0x1p-15f;
+    T* out = reinterpret_cast<T*>(a.out) + row * a.ldo + head * c.dv;
+    const int64_t at = ((int64_t)split * c.rows + row) * a.heads + head;
+    float* ml = reinterpret_cast<float*>(a.ws);
+    float* po = ml + 2 * ((int64_t)plan.splits * c.rows * a.heads) + at * c.dv;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        constexpr int GD = G / 32;
+        const float low = __shfl(accl[d / GD], m32, 64);  // (NG <= 4: m = d / GD is in the lower half)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int dim = 32 * d + 8 * (e >> 2) + 4 * half;
+            float y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = (acc[d][e + k] * (k & 1 ? unit * 0.0625f : unit) + low) * scale;
+            if (last) {
+                typedef T Vec4 __attribute__((ext_vector_type(4)));
+                if (plan.out_aligned && dim + 4 <= c.dv) {
+                    Vec4 z;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) z[k] = (T)y[k];
+                    *reinterpret_cast<Vec4*>(out + dim) = z;
+                } else
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (dim + k < c.dv) out[dim + k] = (T)y[k];
+            } else
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (dim + k < c.dv) po[dim + k] = y[k];
+        }
+    }
+    if (half == 0) {
+        if (last) {
+            if (a.lse) a.lse[row * a.heads + head] = (m + __builtin_amdgcn_logf(l * 0x1p-15f)) * 0.69314718055994530942f;
+        } else
+            ml[2 * at] = m, ml[2 * at + 1] = l * 0x1p-15f;
+    }
+}
+
 // The key ranges' partial results of one (row, head), joined by a workgroup: the
 // ranges' factors first, then a wavefront every fourth range, eight loads at a
 // time (one wavefront in turn over the 256 ranges of a long sequence took 170 us).
@@ -543,27 +921,30 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, in
     if (a.lse && tid == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
 }
 
-// Row tiles of the batch, 16 RT rows (tokens by query heads of a kv head) each.
-static int64_t tiles_of(const Kv4View& c, const int* row0, int per, int rt, int* each) {
-    int64_t n = 0;
-    *each = 0;
-    if (c.each) {
-        *each = (int)(((int64_t)c.each * per + 16 * rt - 1) / (16 * rt));
-        return (int64_t)*each * c.nb;
-    }
-    for (int b = 0; b < c.nb; ++b) n += ((int64_t)(row0[b + 1] - row0[b]) * per + 16 * rt - 1) / (16 * rt);
-    return n;
-}
+// The shape of a call: which kernel, rows of its tiles, key ranges.
+struct KaShape {
+    bool prompt;
+    int rows, tiles_each, splits;
+    int64_t tiles;
+};
 
-static int row_tiles(const Kv4View& c, int per) {
-    // Two tiles a wavefront once a sequence fills them: the keys are unpacked once for both.
-    return c.width <= 128 && (int64_t)(c.rows / (c.nb ? c.nb : 1)) * per > 16 ? 2 : 1;
-}
-
-static int splits_of(const Kv4View& c, const int* row0, int heads, int sink, int ring, int longest) {
+static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, int sink, int ring, int longest) {
     const int per = heads / c.heads;
-    int each;
-    const int64_t base = tiles_of(c, row0, per, row_tiles(c, per), &each) * c.heads;
+    const int64_t mean = c.nb ? (int64_t)c.rows * per / c.nb : 0;  // rows of a sequence for a kv head
+    KaShape s;
+    // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at
+    // 256 dims its sums do not fit the registers.
+    s.prompt = type != KV4_F32 && c.width <= 128 && mean >= 128;
+    // Two tiles of 16 a wavefront once a sequence fills them: the keys are unpacked once for both.
+    s.rows = s.prompt ? KP_ROWS : c.width <= 128 && mean > 16 ? 32 : 16;
+    s.tiles_each = 0;
+    s.tiles = 0;
+    if (c.each) {
+        s.tiles_each = (int)(((int64_t)c.each * per + s.rows - 1) / s.rows);
+        s.tiles = (int64_t)s.tiles_each * c.nb;
+    } else
+        for (int b = 0; b < c.nb; ++b) s.tiles += ((int64_t)(row0[b + 1] - row0[b]) * per + s.rows - 1) / s.rows;
+    const int64_t base = s.tiles * c.heads;
     const int64_t keys = ring ? std::min<int64_t>(longest, (int64_t)sink + ring + c.rows + 2 * KA_CHUNK) : longest;
     const int64_t chunks = (keys + KA_CHUNK - 1) / KA_CHUNK;
     // Two workgroups a CU, as many as their registers let run, but at least
@@ -571,31 +952,43 @@ static int splits_of(const Kv4View& c, const int* row0, int heads, int sink, int
     // keys, 8 kv heads: 512 workgroups 129 us, 1024 139, 2048 146; 131,072 keys:
     // 42, 46, 55 us. Two or one step instead of four: 1060 visible keys 41 and
     // 60 us for 31.)
-    const int64_t want = std::min<int64_t>(base > 0 ? (512 + base - 1) / base : 1, KA_SPLITS);
-    return (int)std::max<int64_t>(1, std::min(want, chunks / (4 * KA_WAVES)));
+    const int64_t want = std::min<int64_t>(base > 0 ? ((s.prompt ? 256 : 512) + base - 1) / base : 1, KA_SPLITS);
+    s.splits = (int)std::max<int64_t>(1, std::min(want, chunks / (s.prompt ? 16 : 4 * KA_WAVES)));
+    return s;
 }
 
 size_t kv4_attend_ws(const Kv4View& c, const int* row0, int heads, int sink, int ring, int longest) {
-    const int s = splits_of(c, row0, heads, sink, ring, longest);
+    // (enough for a call of any type)
+    const int s = std::max(shape_of(c, row0, KV4_F32, heads, sink, ring, longest).splits,
+                           shape_of(c, row0, KV4_F16, heads, sink, ring, longest).splits);
     return s > 1 ? (size_t)s * c.rows * heads * (c.dv + 2) * 4 : 0;
 }
 
 template <int TYPE, int W, int G>
 static hipError_t attend_shaped(const Kv4View& c, const int* row0, const Kv4AttendArgs& a, int longest, hipStream_t s) {
-    const int per = a.heads / c.heads, rt = row_tiles(c, per);
+    const KaShape shape = shape_of(c, row0, TYPE, a.heads, a.sink, a.ring, longest);
     const size_t es = sizeof(typename Kv4Elem<TYPE>::T);
     KaPlan plan;
-    const int64_t tiles = tiles_of(c, row0, per, rt, &plan.tiles_each);
-    plan.splits = splits_of(c, row0, a.heads, a.sink, a.ring, longest);
+    plan.tiles_each = shape.tiles_each;
+    plan.splits = shape.splits;
     plan.aligned = c.dk % 8 == 0 && (uintptr_t)a.q % 16 == 0 && a.ldq * es % 16 == 0 && c.dk * es % 16 == 0;
-    if (tiles * c.heads > 0x7fffffff || (int64_t)c.rows * a.heads > 0x7fffffff) return hipErrorInvalidValue;
-    auto kern = k_kv4_attend<TYPE, W, G, 1>;
-    if constexpr (W <= 128)
-        if (rt == 2) kern = k_kv4_attend<TYPE, W, G, 2>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * c.heads), plan.splits), dim3(KA_WAVES * 64), 0, s, c, a, plan);
-    if (plan.splits > 1) {
-        hipLaunchKernelGGL(k_kv4_join<TYPE>, dim3((unsigned)(c.rows * a.heads)), dim3(256), 0, s, c, a, plan.splits);
+    plan.out_aligned = c.dv % 4 == 0 && (uintptr_t)a.out % 16 == 0 && a.ldo * es % 16 == 0;
+    if (shape.tiles * c.heads > 0x7fffffff || (int64_t)c.rows * a.heads > 0x7fffffff) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(shape.tiles * c.heads), plan.splits);
+    bool done = false;
+    if constexpr (W <= 128 && TYPE != KV4_F32)
+        if (shape.prompt) {
+            hipLaunchKernelGGL((k_kv4_prompt<TYPE, W, G>), grid, dim3(KP_WAVES * 64), 0, s, c, a, plan);
+            done = true;
+        }
+    if (!done) {
+        auto kern = k_kv4_attend<TYPE, W, G, 1>;
+        if constexpr (W <= 128)
+            if (shape.rows == 32) kern = k_kv4_attend<TYPE, W, G, 2>;
+        hipLaunchKernelGGL(kern, grid, dim3(KA_WAVES * 64), 0, s, c, a, plan);
     }
+    if (plan.splits > 1)
+        hipLaunchKernelGGL(k_kv4_join<TYPE>, dim3((unsigned)(c.rows * a.heads)), dim3(256), 0, s, c, a, plan.splits);
     return hipGetLastError();
 }
 

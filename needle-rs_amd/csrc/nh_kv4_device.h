@@ -49,7 +49,9 @@ struct Kv4Lay {
     static __device__ __forceinline__ uint32_t v_byte(int slot, int x) { return v_half(slot, x & 15, x >> 5) + (x >> 4 & 1); }
     static __device__ __forceinline__ uint32_t k_step(int slot, int g) { return 32 * W + 2 * (slot * NG + g); }
     static __device__ __forceinline__ uint32_t k_low(int slot, int g) { return 32 * W + 64 * NG + 2 * (slot * NG + g); }
-    static __device__ __forceinline__ uint32_t v_step(int slot, int g) { return 32 * W + 128 * NG + 2 * (slot * NG + g); }
+    static __device__ __forceinline__ uint32_t v_step(int slot, int g) {
+        return 32 * W + 128 * NG + 2 * (((slot >> 2) * NG + g) * 4 + (slot & 3));
+    }
     static __device__ __forceinline__ uint32_t v_low(int slot, int g) {
         return 32 * W + 192 * NG + 2 * (((slot >> 2) * NG + g) * 4 + (slot & 3));
     }

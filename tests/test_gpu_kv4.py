@@ -222,6 +222,11 @@ def attend_case(nh, lens, rows, kv, per, qk, v, group, page, dtype, sink=0, ring
         # the log of a sum of weights that are each off by the scores' bound
         size = np.abs(x).sum(-1).max() * np.abs(k).max() * abs(s)
         off = (qk + 16) * 2.0 ** -24 * size * 2 + (n + 64) * 2.0 ** -23 + 2.0 ** -22 * np.abs(want_lse)
+        if dtype != "f32" and max(qk, v) <= 128 and sum(rows) * per // len(rows) >= 128:
+            # Calls of many rows round step x code of a key to 11 bits, half a step 2^-12 of at most
+            # the group's range, 2 max |k|: a score moves by scale sum |q| 2^-11 max |k| at most, and so
+            # the log of the sum; each weight, rounded to 11 bits and summed so, by 2^-12 of itself.
+            off = off + 2.0 ** -11 * size + 2.0 ** -12
         assert np.all(np.abs(plain(lse[at:at + r]) - want_lse) <= off)
         at += r
     return c, ids, o
@@ -259,6 +264,66 @@ def test_attend_long(nh, dtype):
 def test_attend_long_prompt_rows(nh):
     attend_case(nh, [1500, 700], [800, 300], 2, 2, 128, 128, 32, 64, "bf16")
     attend_case(nh, [1500, 700], [800, 300], 2, 2, 64, 64, 64, 64, "f32", sink=10, ring=200)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("kv,per,qk,v,group,page", [(1, 1, 64, 64, 32, 32), (2, 4, 48, 64, 64, 32), (2, 3, 45, 51, 32, 64),
+                                                    (2, 4, 128, 128, 64, 64), (1, 8, 80, 96, 32, 128), (1, 2, 128, 72, 32, 64)])
+def test_attend_prompts(nh, kv, per, qk, v, group, page, dtype):
+    """Rows by the hundred, ragged, from the first position on and after others, with and without a span."""
+    attend_case(nh, [300, 517, 33, 260], [300, 129, 33, 200], kv, per, qk, v, group, page, dtype)
+    attend_case(nh, [410], [257], kv, per, qk, v, group, page, dtype, sink=5, ring=70)
+    attend_case(nh, [900, 900], [256, 256], kv, per, qk, v, group, page, dtype, sink=130, ring=300)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attend_prompt_scales(nh, dtype):
+    for spread, scale in ((1e-3, None), (50.0, 0.01), (1.0, -0.2), (1.0, 0.0), (3.0, 1.0)):
+        attend_case(nh, [350], [290], 2, 2, 64, 64, 32, 32, dtype, scale=scale, spread=spread)
+
+
+def test_prompt_nan_reaches_its_readers_only(nh):
+    rng = np.random.default_rng(19)
+    n = 400
+    k, v, q = (rows_of(rng, n, 2, 64, "bf16") for _ in range(3))
+    v2, k2, q2 = v.clone(), k.clone(), q.clone()
+    v2[140, 1, 40] = float("nan")
+    k2[300, 0, 3] = float("inf")
+    q2[10, 0, 5] = float("nan")
+    outs = []
+    for kk, vv, qq in ((k, v, q), (k, v2, q), (k2, v, q), (k, v, q2)):
+        c = nh.KvCache4(1, 2, 64, 64, pages=14, seqs=1, cap=n, page=32)
+        s = c.new_seq()
+        c.extend([s], [n])
+        c.append(0, kk.cuda(), vv.cuda())
+        outs.append(plain(c.attend(0, qq.cuda(), ring=50)))
+    assert not np.isnan(outs[0]).any()
+    for got, seen in ((outs[1], (slice(140, 190), 1, slice(32, 64))), (outs[2], (slice(300, 350), 0, slice(0, 64))),
+                      (outs[3], (10, 0, slice(0, 64)))):
+        spoiled = np.zeros((n, 2, 64), bool)
+        spoiled[seen] = True
+        assert np.array_equal(np.isnan(got), spoiled)
+        assert np.array_equal(got[~spoiled], outs[0][~spoiled])
+
+
+def test_prompt_rows_do_not_depend_on_hidden_rows(nh):
+    """Rows of a page that were written after this sequence's end (another's, larger, or NaN) change no bit."""
+    rng = np.random.default_rng(23)
+    k, v, q = (rows_of(rng, 161, 1, 128, "bf16").cuda() for _ in range(3))
+    outs = []
+    for stale in (None, 3000.0, float("nan")):
+        c = nh.KvCache4(1, 1, 128, 128, pages=3, seqs=1, cap=192, page=64)
+        if stale is not None:
+            s = c.new_seq()
+            c.extend([s], [192])
+            x = torch.full((192, 1, 128), stale, device="cuda") * torch.randn(192, 1, 128, device="cuda")
+            c.append(0, x, x)
+            c.free(s)
+        s = c.new_seq()
+        c.extend([s], [161])
+        c.append(0, k, v)
+        outs.append(c.attend(0, q))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
