@@ -536,10 +536,88 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
     const int wlo = first + w0 / per, whi = first + w1 / per;
     const int sink = a.ring ? a.sink : 0x7fffffff, ring = a.ring;
 
-    // The queries, as in the kernel above.
-    h8 q[NX], qs = {};
     const int r = min(r0 + wave * 32 + m32, r1), token = r / per, pos = first + token;
-    float ck, cl;
+    f32x16 acc[ND], accl = {};
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+    float m = -__builtin_inff();
+
+    const KaSpan span(plo, phi, a.sink, a.ring);
+    const int per_split = (span.count() + plan.splits - 1) / plan.splits;
+    const int c0 = split * per_split, c1 = min(c0 + per_split, span.count());
+    const int* table = c.table + (size_t)entry.seq * c.table_ld;
+    const uint8_t* layer = kv4_block(c, 0, a.layer, kvh);
+    const size_t page_bytes = c.page_bytes();
+    const int mask = c.page() - 1;
+    auto page_of = [&](int i) { return i < c1 ? table[span.at(i) * KA_CHUNK >> c.page_log2] : 0; };
+    auto chunk_at = [&](int i, int pg) {
+        const int slot = span.at(i) * KA_CHUNK & mask;
+        return layer + ((unsigned)pg < (unsigned)c.pages ? pg : 0) * page_bytes + (uint32_t)(slot >> 5) * L::CHUNK;
+    };
+
+    // The references: powers of two above every step of the keys (and values)
+    // of this range, and whether a value is NaN.  One look at the steps ahead of
+    // the loop: inside it they took a third of the instructions.
+    int kref, vref;
+    bool nan;
+    {
+        const uint32_t x2 = 2 * (lane & (16 * NG - 1));  // two steps a lane
+        uint32_t top[2] = {0, 0};
+        bool bad = false;
+        constexpr int DEEP = 8;
+        for (int i0 = c0 + wave; i0 < c1; i0 += DEEP * KP_WAVES) {
+            // (past the end: the last chunk again, so that every load is in flight at once)
+            int pg[DEEP];
+            uint32_t w[DEEP][2];
+#pragma unroll
+            for (int x = 0; x < DEEP; ++x) pg[x] = page_of(min(i0 + x * KP_WAVES, c1 - 1));
+#pragma unroll
+            for (int x = 0; x < DEEP; ++x) {
+                const uint8_t* p = chunk_at(min(i0 + x * KP_WAVES, c1 - 1), pg[x]);
+                w[x][0] = kv4_word(p, 32 * W + 2 * x2);
+                w[x][1] = kv4_word(p, 32 * W + 128 * NG + 2 * x2);
+            }
+#pragma unroll
+            for (int x = 0; x < DEEP; ++x) {
+                const int key0 = span.at(min(i0 + x * KP_WAVES, c1 - 1)) * KA_CHUNK;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t k = w[x][0] >> (16 * t) & 0xffffu, v = w[x][1] >> (16 * t) & 0xffffu;
+                    const int kkey = key0 + (int)(x2 + t) / NG, vkey = key0 + (int)(x2 / (4 * NG)) * 4 + (int)((x2 + t) & 3);
+                    top[0] = max(top[0], (kkey <= phi) & (k < 0x7c00u) ? k : 0u);
+                    top[1] = max(top[1], (vkey <= phi) & (v < 0x7c00u) ? v : 0u);
+                    bad |= (vkey <= phi) & (v >= 0x7c00u);
+                }
+            }
+        }
+        __shared__ uint32_t st[2][KP_WAVES];
+        __shared__ int sbad[KP_WAVES];
+#pragma unroll
+        for (int h = 1; h < 64; h <<= 1) {
+            top[0] = max(top[0], (uint32_t)__shfl_xor((int)top[0], h, 64));
+            top[1] = max(top[1], (uint32_t)__shfl_xor((int)top[1], h, 64));
+        }
+        const bool any = __any(bad);
+        if (lane == 0) st[0][wave] = top[0], st[1][wave] = top[1], sbad[wave] = any;
+        __syncthreads();
+        int bads = 0;
+#pragma unroll
+        for (int w = 0; w < KP_WAVES; ++w) {
+            top[0] = max(top[0], st[0][w]);
+            top[1] = max(top[1], st[1][w]);
+            bads |= sbad[w];
+        }
+        kref = __builtin_amdgcn_readfirstlane((int)(top[0] >> 10)) - 14;
+        vref = __builtin_amdgcn_readfirstlane((int)(top[1] >> 10)) - 14;
+        nan = __builtin_amdgcn_readfirstlane(bads) != 0;
+    }
+    const float kmul = pow2i(14 - kref), vmul = pow2i(14 - vref);
+
+    // The queries, scaled to just under 2^5, and their sums in units that make the
+    // lows' product another term of the scores' own accumulator: scores are z cz,
+    // z = up (q . step c) 2^(-10 - ref) + low (up sum q 2^(-10 - ref)).
+    h8 q[NX], qs = {};
+    float cz;
     {
         const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(row0 + token) * a.ldq + (int64_t)(kvh * per + r - token * per) * c.dk;
         float most = 0.0f, sums[NG] = {};
@@ -562,9 +640,8 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
         }
         most = halves_max(most);
         const int ef = max((int)(__builtin_bit_cast(uint32_t, most) >> 23 & 255u), 15);
-        const float up = __builtin_bit_cast(float, (uint32_t)(268 - ef) << 23);
-        cl = (a.scale * KA_LOG2E * 64.0f) * __builtin_bit_cast(float, (uint32_t)(ef - 14) << 23);
-        ck = cl * 16.0f;
+        const float up = __builtin_bit_cast(float, (uint32_t)(258 - ef) << 23);
+        cz = (a.scale * KA_LOG2E) * pow2i(10 + kref) * __builtin_bit_cast(float, (uint32_t)(ef - 4) << 23);
 #pragma unroll
         for (int j = 0; j < NX; ++j)
 #pragma unroll
@@ -575,23 +652,11 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
             }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const float s = (sums[g] + __shfl_xor(sums[g], 32, 64)) * 0.015625f;
+            const float s = (sums[g] + __shfl_xor(sums[g], 32, 64)) * pow2i(-10 - kref);
             const _Float16 hi = (_Float16)s, lo = (_Float16)(s - (float)hi);
             qs[g] = half == 0 ? hi : lo;
         }
     }
-
-    f32x16 acc[ND], accl = {};
-#pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
-    float m = -__builtin_inff();
-    int kref = -24, vref = -24;  // 2^ref is above every step so far
-
-    const KaSpan span(plo, phi, a.sink, a.ring);
-    const int per_split = (span.count() + plan.splits - 1) / plan.splits;
-    const int c0 = split * per_split, c1 = min(c0 + per_split, span.count());
-    const int* table = c.table + (size_t)entry.seq * c.table_ld;
-    auto page_of = [&](int i) { return i < c1 ? table[span.at(i) * KA_CHUNK >> c.page_log2] : 0; };
 
     // What this wavefront turns into operands: key dword (kt, kj), value dwords
     // (vt, vn) under nibbles 2 vi, 2 vi + 1; a few wavefronts also the lows.
@@ -599,72 +664,38 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
     const bool does_k = W == 128 || wave < UNITS, does_v = W == 128 || wave >= UNITS;
     const int ku = wave % UNITS, kt = ku / NJ, kj = ku % NJ;
     const int vt = ku & 1, vn = W == 128 ? ku >> 1 & 1 : 0, vi = W == 128 ? ku >> 2 : ku >> 1;
+    const uint32_t at_k = L::lane_dword(lane, kt * NJ + kj), at_ks = L::k_step(16 * kt + o, kj * 32 / G);
+    const uint32_t at_v = 16 * W + L::lane_dword(lane, vt * NJ + vn);
+    const uint32_t at_vs = L::v_step(16 * vt + 4 * kg, (64 * vn + 32 * vi) / G);
+    // value lows of keys 16 y + 8 w + 4 half .., y = wave / 2, w = wave % 2; key lows by wavefront 4
+    const uint32_t at_low = wave < 4 ? L::v_low(16 * (wave >> 1) + 8 * (wave & 1) + 4 * half, m32 & (NG - 1)) : L::k_low(m32, 0);
     struct Raw {
-        uint32_t k, v[2], vs[2], low[2], ks_top, vs_top;
+        uint32_t k, v[2], vs[2], low[2];
         uint16_t ks;
     };
     auto load = [&](Raw& x, int i, int pg) {
-        const int slot = span.at(i) * KA_CHUNK & (c.page() - 1);
-        const uint8_t* p = kv4_block(c, (unsigned)pg < (unsigned)c.pages ? pg : 0, a.layer, kvh) + (uint32_t)(slot >> 5) * L::CHUNK;
+        const uint8_t* p = chunk_at(i, pg);
         if (does_k) {
-            x.k = kv4_word(p, L::lane_dword(lane, kt * NJ + kj));
-            x.ks = kv4_half(p, L::k_step(16 * kt + o, kj * 32 / G));
+            x.k = kv4_word(p, at_k);
+            x.ks = kv4_half(p, at_ks);
         }
         if (does_v) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) x.v[t] = kv4_word(p, 16 * W + L::lane_dword(lane, vt * NJ + t * L::NB + vn));
-#pragma unroll
-            for (int t = 0; t < 2; ++t) x.vs[t] = kv4_word(p, L::v_step(16 * vt + 4 * kg + 2 * t, (64 * vn + 32 * vi) / G));
-        }
-        // (two steps a lane, every wavefront the same, for the references)
-        const uint32_t x2 = 2 * (lane & (16 * NG - 1));
-        x.ks_top = kv4_word(p, 32 * W + 2 * x2);
-        x.vs_top = kv4_word(p, 32 * W + 128 * NG + 2 * x2);
-        if (wave < 4) {  // value lows of keys 16 y + 8 w + 4 half .., y = wave / 2, w = wave % 2
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                x.low[t] = kv4_word(p, L::v_low(16 * (wave >> 1) + 8 * (wave & 1) + 4 * half + 2 * t, m32 & (NG - 1)));
-        } else if (wave == 4) {  // key lows
-            if constexpr (NG == 1)
-                x.low[0] = kv4_half(p, L::k_low(m32, 0));
-            else
-#pragma unroll
-                for (int t = 0; t < NG / 2; ++t) x.low[t] = kv4_word(p, L::k_low(m32, 2 * t));
-        }
-    };
-    // The references raised where a step passes them (the same in every
-    // wavefront); true: a value step is NaN.
-    float vmul = 0.0f, kmul = 0.0f, vdown = 1.0f;
-    auto refer = [&](const Raw& x, int i) {
-        const int key0 = span.at(i) * KA_CHUNK;
-        const uint32_t x2 = 2 * (lane & (16 * NG - 1));
-        uint32_t kt2 = 0, vt2 = 0;
-        bool nan = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const uint32_t k = x.ks_top >> (16 * t) & 0xffffu, v = x.vs_top >> (16 * t) & 0xffffu;
-            const int kkey = key0 + (int)(x2 + t) / NG, vkey = key0 + (int)(x2 / (4 * NG)) * 4 + (int)((x2 + t) & 3);
-            if (kkey <= phi && k < 0x7c00u) kt2 = max(kt2, k);
-            if (vkey <= phi && v < 0x7c00u) vt2 = max(vt2, v);
-            nan |= vkey <= phi && v >= 0x7c00u;
-        }
-        vdown = 1.0f;
-        if (__any((int)(kt2 >> 10) - 14 > kref || (int)(vt2 >> 10) - 14 > vref)) {
-            int ke = (int)(kt2 >> 10) - 14, ve = (int)(vt2 >> 10) - 14;
-#pragma unroll
-            for (int h = 1; h < 64; h <<= 1) {
-                ke = max(ke, __shfl_xor(ke, h, 64));
-                ve = max(ve, __shfl_xor(ve, h, 64));
+            for (int t = 0; t < 2; ++t) {
+                x.v[t] = kv4_word(p, at_v + 4 * t * L::NB);
+                x.vs[t] = kv4_word(p, at_vs + 4 * t);
             }
-            ke = max(__builtin_amdgcn_readfirstlane(ke), kref);
-            ve = max(__builtin_amdgcn_readfirstlane(ve), vref);
-            vdown = pow2i(max(vref - ve, -126));
-            kref = ke;
-            vref = ve;
         }
-        kmul = pow2i(14 - kref);
-        vmul = pow2i(14 - vref);
-        return __any(nan) != 0;
+        if (wave < 5) {
+            if constexpr (NG == 4) {
+                x.low[0] = kv4_word(p, at_low);
+                x.low[1] = kv4_word(p, at_low + 4);
+            } else {
+                // (a key's lows take 2 NG bytes)
+                x.low[0] = NG == 1 && wave == 4 ? kv4_half(p, at_low) : kv4_word(p, at_low);
+                x.low[1] = wave < 4 ? kv4_word(p, at_low + 4) : 0;
+            }
+        }
     };
     // Codes under a mask times scaled steps: c 2^-24 x step 2^(14 - ref) (16 times
     // that under the upper mask), two at a time.
@@ -684,14 +715,19 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
             to.k[2 * kj + (kg >> 1)][(kg & 1) * 32 + 16 * kt + o] = y;
         }
         if (does_v) {
+            float s[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[t] = f16_value(x.vs[t >> 1] >> (16 * (t & 1))) * vmul;
+            // (hidden keys' steps, and NaN, count as 0: what a NaN does to its readers comes after the products)
+            if (nan || key0 + KA_CHUNK - 1 > phi) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) s[t] = key0 + 16 * vt + 4 * kg + t <= phi && s[t] == s[t] ? s[t] : 0.0f;
+            }
             uint32_t sw[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                // (hidden keys' steps, and NaN, count as 0: what a NaN does to its readers comes with the weights)
-                const int key = key0 + 16 * vt + 4 * kg + 2 * t;
-                const float s0 = f16_value(x.vs[t]) * vmul, s1 = f16_value(x.vs[t] >> 16) * vmul;
-                const h2 s2 = {(_Float16)(key <= phi && s0 == s0 ? s0 : 0.0f), (_Float16)(key + 1 <= phi && s1 == s1 ? s1 : 0.0f)};
-                sw[t] = __builtin_bit_cast(uint32_t, s2);
+                const f32x2 y = {s[2 * t], s[2 * t + 1]};
+                sw[t] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, h2));
             }
             const uint32_t w0 = vi ? x.v[0] >> 8 : x.v[0], w1 = vi ? x.v[1] >> 8 : x.v[1];
             const uint2 even = {times(w0 & 0x000f000fu, sw[0]), times(w1 & 0x000f000fu, sw[1])};
@@ -705,116 +741,97 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
             const uint2 y = {one ? 0x3c003c00u : x.low[0], one ? 0x3c003c00u : x.low[1]};
             reinterpret_cast<uint2*>(&to.vl[wave >> 1][lane])[wave & 1] = y;
         } else if (wave == 4) {
-            u32x4 y = {};
-#pragma unroll
-            for (int t = 0; t < (NG + 1) / 2; ++t) y[t] = x.low[t];
+            const u32x4 y = {x.low[0], NG == 4 ? x.low[1] : 0, 0, 0};
             to.kl[lane] = y;
         }
     };
 
-    auto compute = [&](const Image& x, int i, float kscale, bool nan) {
-        const int key0 = span.at(i) * KA_CHUNK;
-        if (key0 > whi || (key0 >= sink && key0 + KA_CHUNK - 1 <= wlo - ring)) return;  // nothing for these rows
-        const bool whole = key0 + KA_CHUNK - 1 <= wlo && (key0 + KA_CHUNK - 1 < sink || key0 > whi - ring);
-        f32x16 z = {}, low = {};
-        low = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x.kl[lane]), qs, low, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < NX; ++j)
-            z = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x.k[j][lane]), q[j], z, 0, 0, 0);
-        const bool fresh = m == -__builtin_inff();
-        const float zero = fresh ? 0.0f : m, cz = ck * kscale;
-        float s[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(z[e], cz, __builtin_fmaf(low[e], cl, 15.0f - zero));
-        bool seen[16];
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
-                seen[e] = (j <= pos) & ((j < sink) | (j > pos - ring));
-                s[e] = seen[e] ? s[e] : -__builtin_inff();
-            }
-        }
-        float most = s[0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
-        most = halves_max(most);
-        if (__any(most > 15.0f || fresh)) {
-            const float over = most == -__builtin_inff() ? 0.0f : fresh ? most - 15.0f : fmaxf(most - 15.0f, 0.0f);
-            const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
-            m = fresh && most == -__builtin_inff() ? m : zero + over;
-            accl *= keep;
-#pragma unroll
-            for (int d = 0; d < ND; ++d) acc[d] *= keep;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] -= over;
-        }
-        h8 p[2];
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            const f32x2 y = {__builtin_amdgcn_exp2f(s[e]), __builtin_amdgcn_exp2f(s[e + 1])};
-            const h2 w = __builtin_convertvector(y, h2);
-            p[e >> 3][e & 7] = w[0], p[e >> 3][(e & 7) + 1] = w[1];
-        }
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            accl = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x.vl[y][lane]), p[y], accl, 0, 0, 0);
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x.v[d][y][lane]), p[y], acc[d], 0, 0, 0);
-        }
-        if (nan) {
-            // A NaN value: the rows that see it are NaN in its group.
-            const uint8_t* at = kv4_block(c, table[key0 >> c.page_log2], a.layer, kvh) + (uint32_t)((key0 & (c.page() - 1)) >> 5) * L::CHUNK;
-            for (int g = 0; g < NG; ++g) {
-                int hit = 0;
-                for (int e = 0; e < 16; ++e) {
-                    const int j = 8 * (e >> 2) + 4 * half + (e & 3), key = key0 + j;
-                    const bool see = key <= pos && (key < sink || key > pos - ring);
-                    if (see && (kv4_half(at, L::v_step(j, g)) & 0x7fffu) > 0x7c00u) hit = 1;
-                }
-                hit |= __shfl_xor(hit, 32, 64);
-                const float add = hit ? __builtin_nanf("") : 0.0f;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    if (d * 32 / G == g) acc[d] += add;
-            }
-        }
-    };
-
-    // Loads two chunks ahead, operands one: a chunk's image is written while the
-    // one before it is used, one barrier a chunk.
-    {
+    // Loads run two chunks ahead, operands one: a chunk's image is written between
+    // the two products of the one before it (the vector units have work while the
+    // scores' chain of products runs), one barrier a chunk.  Past the end the last
+    // chunk is loaded and written again, so that no branch cuts the instructions
+    // in pieces.
+    if (c0 < c1) {
         Raw x;
-        float kscale[2];
-        bool nan[2];
-        int pg = page_of(c0 + 1);
-        if (c0 < c1) {
-            load(x, c0, page_of(c0));
-            nan[0] = refer(x, c0);
-            kscale[0] = pow2i(kref);
-            unpack(x, c0, img[0]);
-        }
-        if (c0 + 1 < c1) load(x, c0 + 1, pg);
-        pg = page_of(c0 + 2);
+        const int end = c1 - 1;
+        load(x, c0, page_of(c0));
+        unpack(x, c0, img[0]);
+        load(x, min(c0 + 1, end), page_of(min(c0 + 1, end)));
+        int pg = page_of(min(c0 + 2, end));
         __syncthreads();
         for (int i = c0; i < c1; ++i) {
-            const int now = (i - c0) & 1;
-            float down = 1.0f;
-            if (i + 1 < c1) {
-                nan[now ^ 1] = refer(x, i + 1);
-                kscale[now ^ 1] = pow2i(kref);
-                down = vdown;
-                unpack(x, i + 1, img[now ^ 1]);
-                if (i + 2 < c1) load(x, i + 2, pg);
-                pg = page_of(i + 3);
-            }
-            compute(img[now], i, kscale[now], nan[now]);
-            if (down != 1.0f) {
+            const Image& now = img[(i - c0) & 1];
+            const int key0 = span.at(i) * KA_CHUNK;
+            f32x16 z = {};
+            z = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.kl[lane]), qs, z, 0, 0, 0);
 #pragma unroll
-                for (int d = 0; d < ND; ++d) acc[d] *= down;
+            for (int j = 0; j < NX; ++j)
+                z = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.k[j][lane]), q[j], z, 0, 0, 0);
+            unpack(x, min(i + 1, end), img[((i - c0) & 1) ^ 1]);
+            load(x, min(i + 2, end), pg);
+            pg = page_of(min(i + 3, end));
+            const bool fresh = m == -__builtin_inff();
+            const float zero = fresh ? 0.0f : m;
+            float s[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(z[e], cz, 15.0f - zero);
+            if (!(key0 + KA_CHUNK - 1 <= wlo && (key0 + KA_CHUNK - 1 < sink || key0 > whi - ring))) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
+                    s[e] = (j <= pos) & ((j < sink) | (j > pos - ring)) ? s[e] : -__builtin_inff();
+                }
+            }
+            float most = s[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
+            most = halves_max(most);
+            if (__any(most > 15.0f || fresh)) {
+                const float over = most == -__builtin_inff() ? 0.0f : fresh ? most - 15.0f : fmaxf(most - 15.0f, 0.0f);
+                const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
+                m = fresh && most == -__builtin_inff() ? m : zero + over;
+                accl *= keep;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) acc[d] *= keep;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] -= over;
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                h8 p;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const f32x2 w = {__builtin_amdgcn_exp2f(s[8 * y + e]), __builtin_amdgcn_exp2f(s[8 * y + e + 1])};
+                    const h2 w2 = __builtin_convertvector(w, h2);
+                    p[e] = w2[0], p[e + 1] = w2[1];
+                }
+                accl = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.vl[y][lane]), p, accl, 0, 0, 0);
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.v[d][y][lane]), p, acc[d], 0, 0, 0);
             }
             __syncthreads();
+        }
+    }
+    if (nan) {
+        // NaN values: the rows that see one are NaN in its group.
+        int hit[NG] = {};
+        for (int i = c0; i < c1; ++i) {
+            const int key0 = span.at(i) * KA_CHUNK;
+            const uint8_t* at = chunk_at(i, page_of(i));
+            for (int e = 0; e < 16; ++e) {
+                const int j = 16 * half + e, key = key0 + j;
+                if (key <= pos && (key < sink || key > pos - ring))
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) hit[g] |= (kv4_half(at, L::v_step(j, g)) & 0x7fffu) > 0x7c00u;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            hit[g] |= __shfl_xor(hit[g], 32, 64);
+            const float add = hit[g] ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+            for (int d = g * (G / 32); d < (g + 1) * (G / 32); ++d) acc[d] += add;
         }
     }
 
