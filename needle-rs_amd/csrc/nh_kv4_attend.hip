@@ -515,7 +515,7 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
     struct Image {  // a chunk's operands, 16 bytes a lane each
         u32x4 k[NX][64], kl[64], v[ND][2][64], vl[2][64];
     };
-    __shared__ Image img[2];
+    __shared__ Image img[2][2];
 
     const int tid = threadIdx.x, lane = tid & 63, o = lane & 15, kg = lane >> 4, half = lane >> 5, m32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -746,70 +746,92 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
         }
     };
 
-    // Loads run two chunks ahead, operands one: a chunk's image is written between
-    // the two products of the one before it (the vector units have work while the
-    // scores' chain of products runs), one barrier a chunk.  Past the end the last
-    // chunk is loaded and written again, so that no branch cuts the instructions
-    // in pieces.
+    // Two chunks a step.  Their loads run two steps ahead, their operands one: a
+    // step's images are written while the one before is used, one barrier a step.
+    // The second chunk's scores are started before the first one's weights are
+    // worked out, and so on, so that the matrix unit has work under the vector
+    // unit's.  Past the end the last chunk is loaded and written again (its keys
+    // count as hidden), so that fewer branches cut the instructions in pieces.
     if (c0 < c1) {
-        Raw x;
+        Raw x[2];
         const int end = c1 - 1;
-        load(x, c0, page_of(c0));
-        unpack(x, c0, img[0]);
-        load(x, min(c0 + 1, end), page_of(min(c0 + 1, end)));
-        int pg = page_of(min(c0 + 2, end));
+        int pg[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            load(x[u], min(c0 + u, end), page_of(min(c0 + u, end)));
+            unpack(x[u], min(c0 + u, end), img[0][u]);
+            load(x[u], min(c0 + 2 + u, end), page_of(min(c0 + 2 + u, end)));
+            pg[u] = page_of(min(c0 + 4 + u, end));
+        }
         __syncthreads();
-        for (int i = c0; i < c1; ++i) {
-            const Image& now = img[(i - c0) & 1];
-            const int key0 = span.at(i) * KA_CHUNK;
-            f32x16 z = {};
-            z = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.kl[lane]), qs, z, 0, 0, 0);
+        int turn = 0;
+        for (int i = c0; i < c1; i += 2, turn ^= 1) {
+            f32x16 z[2];
+            auto scores = [&](int u) {
+                const Image& now = img[turn][u];
+                z[u] = f32x16{};
+                z[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.kl[lane]), qs, z[u], 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < NX; ++j)
-                z = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.k[j][lane]), q[j], z, 0, 0, 0);
-            unpack(x, min(i + 1, end), img[((i - c0) & 1) ^ 1]);
-            load(x, min(i + 2, end), pg);
-            pg = page_of(min(i + 3, end));
-            const bool fresh = m == -__builtin_inff();
-            const float zero = fresh ? 0.0f : m;
-            float s[16];
+                for (int j = 0; j < NX; ++j)
+                    z[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.k[j][lane]), q[j], z[u], 0, 0, 0);
+            };
+            auto next = [&](int u) {
+                unpack(x[u], min(i + 2 + u, end), img[turn ^ 1][u]);
+                load(x[u], min(i + 4 + u, end), pg[u]);
+                pg[u] = page_of(min(i + 6 + u, end));
+            };
+            auto weigh = [&](int u) {
+                const Image& now = img[turn][u];
+                const int key0 = span.at(min(i + u, end)) * KA_CHUNK;
+                const bool live = i + u < c1;
+                const bool fresh = m == -__builtin_inff();
+                const float zero = fresh ? 0.0f : m;
+                float s[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(z[e], cz, 15.0f - zero);
-            if (!(key0 + KA_CHUNK - 1 <= wlo && (key0 + KA_CHUNK - 1 < sink || key0 > whi - ring))) {
+                for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(z[u][e], cz, 15.0f - zero);
+                if (!(live && key0 + KA_CHUNK - 1 <= wlo && (key0 + KA_CHUNK - 1 < sink || key0 > whi - ring))) {
+                    const int top = live ? pos : -1;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
-                    s[e] = (j <= pos) & ((j < sink) | (j > pos - ring)) ? s[e] : -__builtin_inff();
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
+                        s[e] = (j <= top) & ((j < sink) | (j > pos - ring)) ? s[e] : -__builtin_inff();
+                    }
                 }
-            }
-            float most = s[0];
+                float most = s[0];
 #pragma unroll
-            for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
-            most = halves_max(most);
-            if (__any(most > 15.0f || fresh)) {
-                const float over = most == -__builtin_inff() ? 0.0f : fresh ? most - 15.0f : fmaxf(most - 15.0f, 0.0f);
-                const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
-                m = fresh && most == -__builtin_inff() ? m : zero + over;
-                accl *= keep;
+                for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
+                most = halves_max(most);
+                if (__any(most > 15.0f || fresh)) {
+                    const float over = most == -__builtin_inff() ? 0.0f : fresh ? most - 15.0f : fmaxf(most - 15.0f, 0.0f);
+                    const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
+                    m = fresh && most == -__builtin_inff() ? m : zero + over;
+                    accl *= keep;
 #pragma unroll
-                for (int d = 0; d < ND; ++d) acc[d] *= keep;
+                    for (int d = 0; d < ND; ++d) acc[d] *= keep;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] -= over;
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                h8 p;
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const f32x2 w = {__builtin_amdgcn_exp2f(s[8 * y + e]), __builtin_amdgcn_exp2f(s[8 * y + e + 1])};
-                    const h2 w2 = __builtin_convertvector(w, h2);
-                    p[e] = w2[0], p[e + 1] = w2[1];
+                    for (int e = 0; e < 16; ++e) s[e] -= over;
                 }
-                accl = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.vl[y][lane]), p, accl, 0, 0, 0);
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.v[d][y][lane]), p, acc[d], 0, 0, 0);
-            }
+                for (int y = 0; y < 2; ++y) {
+                    h8 p;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const f32x2 w = {__builtin_amdgcn_exp2f(s[8 * y + e]), __builtin_amdgcn_exp2f(s[8 * y + e + 1])};
+                        const h2 w2 = __builtin_convertvector(w, h2);
+                        p[e] = w2[0], p[e + 1] = w2[1];
+                    }
+                    accl = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.vl[y][lane]), p, accl, 0, 0, 0);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, now.v[d][y][lane]), p, acc[d], 0, 0, 0);
+                }
+            };
+            scores(0);
+            next(0);
+            scores(1);
+            weigh(0);
+            next(1);
+            weigh(1);
             __syncthreads();
         }
     }
