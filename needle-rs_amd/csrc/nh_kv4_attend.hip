@@ -28,7 +28,6 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int KA_WAVES = 4;    // wavefronts of a workgroup, each every fourth chunk
 constexpr int KA_CHUNK = 32;   // keys of a step of a wavefront; a page holds whole chunks
 constexpr float KA_LOG2E = 1.44269504088896340736f;
 
@@ -97,16 +96,17 @@ struct KaChunk {
     uint16_t ks[2][NS], vs[2][NS];
 };
 
-template <int TYPE, int W, int G, int RT>
-__global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
+// NW wavefronts a workgroup, each every NW-th chunk of the range; RT tiles of 16 rows.
+template <int TYPE, int W, int G, int RT, int NW>
+__global__ __launch_bounds__(NW * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
     typedef typename Kv4Elem<TYPE>::T T;
     constexpr int NG = W / G, NB = W / 64, NJ = W / 32, GJ = G / 32, GI = G / 16;
     constexpr int PARTS = TYPE == KV4_F32 ? 2 : 1;  // f16 halves of a query element and of a weight
     typedef KaChunk<W, NG> Chunk;
     constexpr int LD = W + 4;
     constexpr uint32_t CB = 32 * (W + 8 * NG);
-    __shared__ float so[KA_WAVES][16][LD];
-    __shared__ float sm[KA_WAVES][16], sl[KA_WAVES][16], spl[KA_WAVES][16][8];
+    __shared__ float so[NW][16][LD];
+    __shared__ float sm[NW][16], sl[NW][16], spl[NW][16][8];
 
     const int tid = threadIdx.x, lane = tid & 63, o = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
 
     const KaSpan span(plo, phi, a.sink, a.ring);
     const int sink = a.ring ? a.sink : 0x7fffffff, ring = a.ring;
-    const int per_split = max((span.count() + plan.splits - 1) / plan.splits, KA_WAVES);
+    const int per_split = max((span.count() + plan.splits - 1) / plan.splits, NW);
     const int c0 = split * per_split, c1 = min(c0 + per_split, span.count());
 
     const int* table = c.table + (size_t)seq * c.table_ld;
@@ -415,15 +415,15 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         auto fetch = [&](Chunk& to, int at, int pg) {
             if (at < c1) load(to, at, pg);
         };
-        int p0 = page_of(i), p1 = page_of(i + KA_WAVES), p2 = page_of(i + 2 * KA_WAVES);
+        int p0 = page_of(i), p1 = page_of(i + NW), p2 = page_of(i + 2 * NW);
         fetch(x[0], i, p0);
-        fetch(x[1], i + KA_WAVES, p1);
+        fetch(x[1], i + NW, p1);
         while (i < c1) {
 #pragma unroll
-            for (int k = 0; k < 3; ++k, i += KA_WAVES) {
+            for (int k = 0; k < 3; ++k, i += NW) {
                 if (i >= c1) break;
-                fetch(x[(k + 2) % 3], i + 2 * KA_WAVES, p2);
-                p2 = page_of(i + 3 * KA_WAVES);
+                fetch(x[(k + 2) % 3], i + 2 * NW, p2);
+                p2 = page_of(i + 3 * NW);
                 compute(x[k], i);
             }
         }
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
         __syncthreads();
         float most = sm[0][o];
 #pragma unroll
-        for (int w = 1; w < KA_WAVES; ++w) most = fmaxf(most, sm[w][o]);
+        for (int w = 1; w < NW; ++w) most = fmaxf(most, sm[w][o]);
         const float base = most == -__builtin_inff() ? 0.0f : most;
         const float f = __builtin_amdgcn_exp2f(m[rt] - base);
 #pragma unroll
@@ -460,16 +460,16 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv4_attend(Kv4View c, Kv4Atte
             *reinterpret_cast<f32x4*>(&so[wave][o][16 * i + 8 * kg + 4]) = z;
         }
         __syncthreads();
-        for (int x = tid; x < 16 * W; x += KA_WAVES * 64) {
+        for (int x = tid; x < 16 * W; x += NW * 64) {
             const int rr = x / W, d = x % W, r = r0 + rt * 16 + rr;
             if (r > r1 || d >= c.dv) continue;
             float top = sm[0][rr];
 #pragma unroll
-            for (int w = 1; w < KA_WAVES; ++w) top = fmaxf(top, sm[w][rr]);
+            for (int w = 1; w < NW; ++w) top = fmaxf(top, sm[w][rr]);
             const float zero = top == -__builtin_inff() ? 0.0f : top;
             float sum = 0.0f, v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < KA_WAVES; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 sum = __builtin_fmaf(sl[w][rr], __builtin_amdgcn_exp2f(sm[w][rr] - zero), sum);
                 v += so[w][rr][d];
             }
@@ -960,10 +960,10 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, in
     if (a.lse && tid == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
 }
 
-// The shape of a call: which kernel, rows of its tiles, key ranges.
+// The shape of a call: which kernel, its rows a tile and wavefronts, key ranges.
 struct KaShape {
     bool prompt;
-    int rows, tiles_each, splits;
+    int rows, waves, tiles_each, splits;
     int64_t tiles;
 };
 
@@ -974,8 +974,7 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
     // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at
     // 256 dims its sums do not fit the registers.
     s.prompt = type != KV4_F32 && c.width <= 128 && mean >= 128;
-    // Two tiles of 16 a wavefront once a sequence fills them: the keys are unpacked once for both.
-    s.rows = s.prompt ? KP_ROWS : c.width <= 128 && mean > 16 ? 32 : 16;
+    s.rows = s.prompt ? KP_ROWS : c.width == 64 && mean > 16 ? 32 : 16;
     s.tiles_each = 0;
     s.tiles = 0;
     if (c.each) {
@@ -984,15 +983,16 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
     } else
         for (int b = 0; b < c.nb; ++b) s.tiles += ((int64_t)(row0[b + 1] - row0[b]) * per + s.rows - 1) / s.rows;
     const int64_t base = s.tiles * c.heads;
+    s.waves = s.prompt ? KP_WAVES : s.rows == 16 && c.width <= 128 && base <= 256 ? 8 : 4;
     const int64_t keys = ring ? std::min<int64_t>(longest, (int64_t)sink + ring + c.rows + 2 * KA_CHUNK) : longest;
     const int64_t chunks = (keys + KA_CHUNK - 1) / KA_CHUNK;
-    // Two workgroups a CU, as many as their registers let run, but at least
+    // Eight wavefronts a CU, as many as their registers let run, but at least
     // four steps for each wavefront of a range. (64 sequences of 4096 to 8192
     // keys, 8 kv heads: 512 workgroups 129 us, 1024 139, 2048 146; 131,072 keys:
     // 42, 46, 55 us. Two or one step instead of four: 1060 visible keys 41 and
     // 60 us for 31.)
-    const int64_t want = std::min<int64_t>(base > 0 ? ((s.prompt ? 256 : 512) + base - 1) / base : 1, KA_SPLITS);
-    s.splits = (int)std::max<int64_t>(1, std::min(want, chunks / (s.prompt ? 16 : 4 * KA_WAVES)));
+    const int64_t want = std::min<int64_t>(base > 0 ? ((s.waves == 4 ? 512 : 256) + base - 1) / base : 1, KA_SPLITS);
+    s.splits = (int)std::max<int64_t>(1, std::min(want, chunks / (s.prompt ? 16 : 4 * s.waves)));
     return s;
 }
 
@@ -1021,10 +1021,12 @@ static hipError_t attend_shaped(const Kv4View& c, const int* row0, const Kv4Atte
             done = true;
         }
     if (!done) {
-        auto kern = k_kv4_attend<TYPE, W, G, 1>;
+        auto kern = k_kv4_attend<TYPE, W, G, 1, 4>;
         if constexpr (W <= 128)
-            if (shape.rows == 32) kern = k_kv4_attend<TYPE, W, G, 2>;
-        hipLaunchKernelGGL(kern, grid, dim3(KA_WAVES * 64), 0, s, c, a, plan);
+            if (shape.waves == 8) kern = k_kv4_attend<TYPE, W, G, 1, 8>;
+        if constexpr (W == 64)
+            if (shape.rows == 32) kern = k_kv4_attend<TYPE, W, G, 2, 4>;
+        hipLaunchKernelGGL(kern, grid, dim3(shape.waves * 64), 0, s, c, a, plan);
     }
     if (plan.splits > 1)
         hipLaunchKernelGGL(k_kv4_join<TYPE>, dim3((unsigned)(c.rows * a.heads)), dim3(256), 0, s, c, a, plan.splits);
