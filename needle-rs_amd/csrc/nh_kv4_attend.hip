@@ -98,10 +98,20 @@ struct KaChunk {
 
 // NW wavefronts a workgroup, each every NW-th chunk of the range; RT tiles of 16 rows.
 template <int TYPE, int W, int G, int RT, int NW>
-__global__ __launch_bounds__(NW * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
+__global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
     typedef typename Kv4Elem<TYPE>::T T;
     constexpr int NG = W / G, NB = W / 64, NJ = W / 32, GJ = G / 32, GI = G / 16;
     constexpr int PARTS = TYPE == KV4_F32 ? 2 : 1;  // f16 halves of a query element and of a weight
+    // The MFMAs take a subnormal as it is, but line its products up by the exponent
+    // of the smallest normal number: up to 2^-17 of the largest product is cut off
+    // (2^-20 with normal operands, both measured).  Calls that carry 22 bits bring
+    // their codes up by 2^14 first, one more instruction for two codes.
+    constexpr int UP = PARTS == 2 ? 14 : 0;
+    auto operand = [](u32x4 y) {
+        h8 z = __builtin_bit_cast(h8, y);
+        if constexpr (PARTS == 2) z *= (_Float16)16384.0f;
+        return z;
+    };
     typedef KaChunk<W, NG> Chunk;
     constexpr int LD = W + 4;
     constexpr uint32_t CB = 32 * (W + 8 * NG);
@@ -159,7 +169,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs
         most = groups_max(most);
         const int ef = max((int)(__builtin_bit_cast(uint32_t, most) >> 23 & 255u), 15);
         const float up = __builtin_bit_cast(float, (uint32_t)(268 - ef) << 23);
-        // scores: (2^18 sum step z + low . qs) cq, z = 2^-24 up (q . c), qs = 2^-6 up sum q
+        // scores: (2^(18 - UP) sum step z + low . qs) cq, z = 2^(UP - 24) up (q . c), qs = 2^-6 up sum q
         cq[rt] = (a.scale * KA_LOG2E * 64.0f) * __builtin_bit_cast(float, (uint32_t)(ef - 14) << 23);
         qs[rt] = h8{};
         static_for<0, NG>([&](auto GG) {
@@ -277,7 +287,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int n = 0; n < Chunk::NS; ++n) {
-                kstep[t][n] = f16_value(x.ks[t][n]) * 262144.0f;
+                kstep[t][n] = f16_value(x.ks[t][n]) * pow2i(18 - UP);
                 vstep[t][n] = f16_value(x.vs[t][n]) * wscale;
             }
         h8 ka[2][NJ];
@@ -287,7 +297,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs
             for (int j = 0; j < NJ; ++j) {
                 const uint32_t w = x.k[t][j], z = w >> 8;
                 const u32x4 y = {w & 0x000f000fu, w & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u};
-                ka[t][j] = __builtin_bit_cast(h8, y);
+                ka[t][j] = operand(y);
             }
         h8 pw[RT][NG][PARTS];
 #pragma unroll
@@ -396,7 +406,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs
                 u32x4 y;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) y[k] = (i & 2 ? w[k] >> 8 : w[k]) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
-                const h8 va = __builtin_bit_cast(h8, y);
+                const h8 va = operand(y);
                 const int d = 4 * n + i;
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
@@ -430,7 +440,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv4_attend(Kv4View c, Kv4AttendArgs
     }
 
     // The wavefronts' sums joined, 16 rows at a time.
-    const float unit = pow2i(24 - 15 + eref);
+    const float unit = pow2i(24 - 15 - UP + eref);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         l[rt] = groups_sum(l[rt]);

@@ -24,9 +24,12 @@ def _ints(v):
     return a, at, n
 
 
+_here = contextlib.nullcontext()
+
+
 def _on(stream):
     """Allocations of the call come from the memory of the stream that uses them."""
-    return torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext()
+    return torch.cuda.stream(stream) if stream is not None else _here
 
 
 def _ptr(t):
@@ -200,6 +203,23 @@ class KvCache4:
         self.h = None
 
 
+def _row_stride(t, index, what):
+    """Elements from one row of [batch][rows][vocab] to the next."""
+    if t.dtype not in _TYPES or t.get_device() != index or index < 0:
+        raise ValueError(f"{what}: f32, f16 or bf16 on the logits' device")
+    b, r, v = t.shape
+    sb, sr, sv = t.stride()
+    ld = sr if r > 1 else sb if b > 1 else v
+    if v > 1 and sv != 1 or b > 1 and sb != ld * r:
+        raise ValueError(f"the rows of {what} do not follow each other")
+    return max(ld, v)
+
+
+def _plain(t, dtype, shape, index, what):
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on the logits' device")
+
+
 def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor | None = None,
                   probs: torch.Tensor | None = None, counts: torch.Tensor | None = None, temperature: float = 1.0,
                   stream=None):
@@ -216,40 +236,25 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor | 
     batch, rows, vocab = logits.shape
     n, index = rows - 1, logits.get_device()
 
-    def strided(t, what):
-        if t.dtype not in _TYPES or t.get_device() != index or index < 0:
-            raise ValueError(f"{what}: f32, f16 or bf16 on the logits' device")
-        b, r, v = t.shape
-        sb, sr, sv = t.stride()
-        ld = sr if r > 1 else sb if b > 1 else v
-        if v > 1 and sv != 1 or b > 1 and sb != ld * r:
-            raise ValueError(f"the rows of {what} do not follow each other")
-        return max(ld, v)
-
-    def plain(t, dtype, shape, what):
-        if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
-            raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on the logits' device")
-
-    ldl, ldp = strided(logits, "logits"), 0
-    plain(drafts, torch.int32, (batch, n), "drafts")
+    ldl, ldp = _row_stride(logits, index, "logits"), 0
+    _plain(drafts, torch.int32, (batch, n), index, "drafts")
     if u is not None:
-        plain(u, torch.float32, (batch, n + 1), "u")
+        _plain(u, torch.float32, (batch, n + 1), index, "u")
     if counts is not None:
-        plain(counts, torch.int32, (batch,), "counts")
+        _plain(counts, torch.int32, (batch,), index, "counts")
     if probs is not None:
         if probs.shape != (batch, n, vocab):
             raise ValueError("probs are [batch][n][vocab]")
-        ldp = strided(probs, "probs") if probs.numel() else vocab
+        ldp = _row_stride(probs, index, "probs") if probs.numel() else vocab
     if index != torch.cuda.current_device():
         raise ValueError("the tensors are on another device than the current one")
     ws_bytes = nh._lib.nh_verify_drafts_ws_bytes(batch, n, vocab)
     if ws_bytes < 0:
         nh._check(int(ws_bytes))
     with _on(stream):
-        # (one allocation for both results and one for the workspace, which goes back at the end)
-        both = torch.empty(batch * (n + 2), dtype=torch.int32, device=logits.device)
+        accepted = torch.empty(batch, dtype=torch.int32, device=logits.device)
+        tokens = torch.empty((batch, n + 1), dtype=torch.int32, device=logits.device)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
-    accepted, tokens = both[:batch], both[batch:].view(batch, n + 1)
     nh._check(nh._lib.nh_verify_drafts(logits.data_ptr(), _TYPES[logits.dtype], ldl, _ptr(drafts), _ptr(counts),
                                        _ptr(probs), _TYPES[probs.dtype] if probs is not None else 0, ldp, _ptr(u),
                                        float(temperature), batch, n, vocab, accepted.data_ptr(), tokens.data_ptr(),

@@ -333,6 +333,19 @@ def test_attend_scales(nh, dtype):
         attend_case(nh, [150, 40], [3, 1], 2, 2, 64, 64, 32, 32, dtype, scale=scale, spread=spread)
 
 
+@pytest.mark.parametrize("qk,v,group,n", [(48, 64, 32, 300), (128, 128, 32, 1000), (128, 128, 64, 90), (256, 256, 64, 200)])
+def test_f32_calls_carry_22_bits(nh, qk, v, group, n):
+    """f32 results to 1e-5 of their size.  A score is a sum of some ten matrix products, each cut off at 2^-20.6 of its
+    largest term (measured; a term here is up to some 40, over the scale of 1 / sqrt(qk) some 4), so off by a few
+    2^-19 at random, and weights and parts carry 2^-22: 1e-5 is five times that.  Codes taken as subnormals gave 4e-5."""
+    rng = np.random.default_rng(qk + n)
+    c, ids, ks, vs = filled(nh, rng, [n], 2, qk, v, group, 32, "f32", last=[1])
+    q = rows_of(rng, 1, 12, qk, "f32")
+    o = plain(c.attend(0, q.cuda())).astype(np.float64)
+    want, _ = ref.attend(plain(q), ref.quantize(plain(ks[0][0]), group), ref.quantize(plain(vs[0][0]), group), qk ** -0.5)
+    assert np.linalg.norm(o - want) <= 1e-5 * np.linalg.norm(want)
+
+
 def test_attend_does_not_depend_on_the_batch(nh):
     """A sequence's result is the same bits beside other sequences whose values are larger."""
     rng = np.random.default_rng(2)
