@@ -635,6 +635,43 @@ class Session:
         _check(_lib.nh_generate_greedy(self.h, int(steps), _hptr(out), _dptr(logits), _stream(stream)))
         return out[:steps].copy(), logits
 
+    def verify_drafts(self, drafts, u=None, temperature: float = 0.0, probs=None, stream=None):
+        """A step of drafted decoding (no reference counterpart): up to 32 drafted
+        tokens are fed as one chunk after what the session holds, checked against
+        its logits (verify_drafts below; temperature 0: greedy, else u f32 [n + 1]
+        uniforms and probs [n][out_rows] the drafter's probabilities or None), the
+        refused ones rolled back, and the next token fed.  Returns the new tokens
+        (the kept drafts and the next one), all of them in the session, whose
+        logits are those after the last.  The drafts' rows take the prefill
+        combine, a step the decode combine, so a near tie may be picked
+        otherwise than by steps.  Under a span a refused draft has taken the KV
+        slot of the position a ring before it, as any rolled back position has."""
+        toks = np.ascontiguousarray(np.asarray(drafts, dtype=np.uint32).reshape(-1))
+        n, width = toks.size, self.model.out_rows
+        if n > 32:
+            raise ValueError("a session rolls back at most 32 drafts")
+        if len(self) + n + 1 > self.cap:
+            raise ValueError("the drafts and the next token do not fit the session's capacity")
+        # (all that the check could refuse, before anything is fed)
+        if not 0.0 <= temperature < float("inf") or temperature > 0.0 and u is None:
+            raise NeedleHipError(-1, "a temperature is 0 (greedy), or positive with uniforms")
+        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream()):
+            target = torch.empty((1, n + 1, width), dtype=torch.float32, device="cuda")
+            x = torch.from_numpy(toks.view(np.int32)).cuda().view(1, n)
+            if u is not None:
+                u = torch.as_tensor(u, dtype=torch.float32).to(target.device).reshape(1, n + 1)
+            if probs is not None:
+                probs = probs.reshape(1, n, width)
+            _check(_lib.nh_forward(self.h, _hptr(toks), 0, _dptr(target), _stream()))
+            if n:
+                _check(_lib.nh_forward_outputs(self.h, _hptr(toks), n, OUT_ALL_LOGITS, target[0, 1].data_ptr(), n * width,
+                                               _stream()))
+            tokens = verify_drafts(target, x, u, probs=probs, temperature=temperature)[1]
+            new = [t for t in tokens[0].tolist() if t >= 0]
+            self.rollback(n + 1 - len(new))
+            self.forward(new[-1:])
+        return new
+
     def __del__(self):
         if getattr(self, "h", None) and _lib is not None:
             _lib.nh_session_free(self.h)
