@@ -202,9 +202,14 @@ __global__ __launch_bounds__(VR_THREADS) void k_verify_rows(VerifyArgs a) {
             const float e = __builtin_amdgcn_exp2f(t);
             const float w = __builtin_fmaf(e, r * 0.69314718055994530942f, e);
             // (not for NaN, infinite arguments, or weights below 2^-126)
-            sum += l == m ? 1.0f : t > -126.0f ? w : 0.0f;
+            sum += t > -126.0f ? w : 0.0f;
         }
-        if (!(m > -__builtin_inff())) sum = 0.0f;
+        if (fabsf(m) == __builtin_inff()) {
+            // Infinite logits share the whole; a slice of -inf and NaN has none.
+            sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < VR_EACH; ++k) sum += m > 0.0f && v[k] == m ? 1.0f : 0.0f;
+        }
         const double s = wave_sum((double)sum);
         if (lane == 0) ss[wave] = s;
         __syncthreads();
@@ -307,12 +312,11 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
         const int out = refused && !RESIDUE ? s_out : -1;
         const float un = u[n];
         const VerifySlice* sl = a.slices + (row0 + kept) * a.nslices;
-        // The weights of a thread's neighbours t .. t + VP_EACH - 1.
-        auto weigh = [&](int t, bool left, double* w) {
+        // A thread's neighbours t .. t + VP_EACH - 1: the logits, and what the drafter gave them; then their weights.
+        auto fetch = [&](int t, bool left, float* l, float* d) {
             typedef T VecT __attribute__((ext_vector_type(VP_EACH)));
             typedef P VecP __attribute__((ext_vector_type(VP_EACH)));
             const bool whole = t + VP_EACH <= a.vocab;
-            float l[VP_EACH], d[VP_EACH];
             if (whole && a.aligned) {
                 const VecT y = *reinterpret_cast<const VecT*>(x + t);
 #pragma unroll
@@ -331,6 +335,8 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
                     for (int k = 0; k < VP_EACH; ++k) d[k] = t + k < a.vocab ? Kv4Elem<PT>::get(q + t + k) : 0.0f;
                 }
             }
+        };
+        auto weigh = [&](int t, bool left, const float* l, const float* d, double* w) {
             double s = 0.0;
             verify_weights<VP_EACH>(l, m, a.c, w);
 #pragma unroll
@@ -347,9 +353,14 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
         };
         // A slice's weights, and their sum over the workgroup in wavefront order.
         auto weigh_slice = [&](int k, bool left) {
+            // (every strip's loads are issued first)
+            float l[SUB][VP_EACH], d[SUB][VP_EACH];
             double s = 0.0, w[VP_EACH];
-#pragma unroll 1
-            for (int y = 0; y < SUB; ++y) s += weigh(k * VR_SLICE + (y * VP_THREADS + tid) * VP_EACH, left, w);
+            const int t = k * VR_SLICE + tid * VP_EACH;
+#pragma unroll
+            for (int y = 0; y < SUB; ++y) fetch(t + y * VP_THREADS * VP_EACH, left, l[y], d[y]);
+#pragma unroll
+            for (int y = 0; y < SUB; ++y) s += weigh(t + y * VP_THREADS * VP_EACH, left, l[y], d[y], w);
             s = wave_sum(s);
             __syncthreads();
             if (lane == 0) ss[0][wave] = s;
@@ -436,9 +447,11 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
                 double before = 0.0;
 #pragma unroll 1
                 for (int y = 0; y < SUB; ++y) {
+                    float l[VP_EACH], d[VP_EACH];
                     double w[VP_EACH];
                     const int t0 = (y * VP_THREADS + tid) * VP_EACH;
-                    const double s = weigh(at * VR_SLICE + t0, left, w), z = wave_scan(s);
+                    fetch(at * VR_SLICE + t0, left, l, d);
+                    const double s = weigh(at * VR_SLICE + t0, left, l, d, w), z = wave_scan(s);
                     if (lane == 63) ss[y & 1][wave] = z;
                     __syncthreads();
                     double run = before + (z - s);
