@@ -381,8 +381,9 @@ int nh_generate_greedy(nh_session* s, int steps, uint32_t* out, float* logits, v
  * works at once and reports at once (NH_ENOMEM: too few free pages or sequences;
  * a refused call changes nothing), and is refused under stream capture.  append
  * and attend read the batch from the device: captured, they follow the state
- * that a later extend of the same rows outside the graph leaves.  The calls on
- * one cache are queued on one stream, or ordered by the caller's events.  A
+ * that a later extend of the same rows outside the graph leaves (after an extend
+ * of more rows, or where the batch is over and its pages have changed hands,
+ * a replay touches nothing).  The calls on one cache are queued on one stream, or ordered by the caller's events.  A
  * cache belongs to the device it was made on. */
 #define NH_F32 0
 #define NH_F16 1

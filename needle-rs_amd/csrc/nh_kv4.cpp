@@ -33,6 +33,7 @@ struct nh_kv4 {
     size_t o_table = 0, o_batch = 0, o_fresh = 0;
     std::vector<int> sent;  // the mirror's values but the tables' and the fresh ids'
     nh::Kv4Patch patch{};   // values not sent yet
+    int entries = 0;        // batch entries that the device holds
 };
 
 namespace {
@@ -132,6 +133,23 @@ int copy_pages(nh_kv4* c, const std::vector<std::pair<int, int>>& copies, hipStr
     return NH_OK;
 }
 
+// The device's batch entries from `n` on are emptied (queued), so that a step
+// captured for them, replayed without an extend of its own, touches no page
+// that has changed hands.
+int drop_entries(nh_kv4* c, int n, hipStream_t st) {
+    for (int i = n; i < c->entries; ++i)
+        for (int k = 0; k < 4; ++k)
+            if (int rc = put_changed(c, c->o_batch + 4 * (size_t)i + k, 0, st)) return rc;
+    c->entries = std::min(c->entries, n);
+    return NH_OK;
+}
+// Before pages are handed out under no batch (one that is over, or none).
+int drop_batch(nh_kv4* c, hipStream_t st) {
+    if (!c->book.batch_seq.empty() || !c->entries) return NH_OK;
+    if (int rc = drop_entries(c, 0, st)) return rc;
+    return flush(c, st);
+}
+
 // The batch of the last extend, as the kernels see it.
 int check_batch(const nh_kv4* c, int layer) {
     if (layer < 0 || layer >= c->v.layers) return fail(NH_EINVAL, "no such layer");
@@ -160,13 +178,15 @@ int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int p
     const int64_t ld = ((int64_t)cap + page - 1) / page;
     if (ld * seqs + 4 * (int64_t)seqs + 4 + pages > (int64_t)UINT32_MAX / 4)
         return fail(NH_EINVAL, "the sequences' page tables are too large");
+    const int wide = std::max(qk_dim, v_dim), width = wide <= 64 ? 64 : wide <= 128 ? 128 : 256;
+    if ((double)pages * page * layers * kv_heads * (width + 8 * (width / group)) > 0x1p46)
+        return fail(NH_EINVAL, "the pages are larger than any device's memory");
     if (!nh::ready()) return fail(NH_ESTATE, "nh_init has not been called");
     return guarded([&]() -> int {
         auto c = std::make_unique<nh_kv4>();
         NH_TRY(hipGetDevice(&c->device), "hipGetDevice");
         nh::Kv4View& v = c->v;
-        const int wide = std::max(qk_dim, v_dim);
-        v.width = wide <= 64 ? 64 : wide <= 128 ? 128 : 256;
+        v.width = width;
         v.group = group;
         v.layers = layers, v.heads = kv_heads, v.dk = qk_dim, v.dv = v_dim;
         v.page_log2 = page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : 8;
@@ -267,7 +287,9 @@ int nh_kv4_seq_copy(nh_kv4* c, int seq, void* stream) {
         std::vector<std::pair<int, int>> copies;
         int to = -1;
         if (int rc = c->book.copy(seq, &to, &copies)) return refused(c, rc);
-        if (int rc = copy_pages(c, copies, st)) {
+        int rc = drop_batch(c, st);
+        if (!rc) rc = copy_pages(c, copies, st);
+        if (rc) {
             c->book.free_seq(to);
             return rc;
         }
@@ -287,7 +309,11 @@ int nh_kv4_seq_compact(nh_kv4* c, const int* seqs, int n, const int* counts, con
         if (int rc = c->book.compact(seqs, n, counts, ranges, &p)) return refused(c, rc);
         // The sources' tables and the fresh pages' ids, then the moves.
         std::vector<int> at(n, 0);
-        int rc = NH_OK, fresh = 0;
+        // (a sequence of the batch that gets shorter ends it)
+        bool over = c->book.batch_seq.empty();
+        for (int i = 0; i < n; ++i)
+            for (int b : c->book.batch_seq) over |= b == seqs[i] && c->book.seqs[seqs[i]].len != p.len[i];
+        int rc = over ? drop_entries(c, 0, st) : NH_OK, fresh = 0;
         for (int i = 0; i < n && !rc; ++i) {
             at[i] = fresh;
             if (p.fresh[i].empty()) continue;
@@ -344,6 +370,8 @@ int nh_kv4_extend(nh_kv4* c, const int* seqs, const int* rows, int n, void* stre
                 if (int rc = put_changed(c, c->o_batch + 4 * (size_t)i + k, entry[k], st)) return rc;
             if (rows[i] != rows[0]) c->v.each = 0;
         }
+        if (int rc = drop_entries(c, n, st)) return rc;
+        c->entries = n;
         return flush(c, st);
     });
 }

@@ -406,6 +406,104 @@ def test_nan_reaches_its_readers_only(nh):
     assert np.array_equal(outs[2][~spoiled], outs[0][~spoiled])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_ragged_sequences(nh, dtype):
+    """More sequences than a wavefront has lanes, of 0 to 9 rows each; more spans than one launch reads."""
+    rng = np.random.default_rng(31)
+    lens = [int(x) for x in rng.integers(0, 90, 150)]
+    rows = [int(min(n, x)) for n, x in zip(lens, rng.integers(0, 10, 150))]
+    c, ids, _ = attend_case(nh, lens, rows, 1, 2, 64, 64, 32, 32, dtype)
+    pick = [int(x) for x in rng.integers(0, 150, 400)]
+    begin = [int(rng.integers(0, lens[i] + 1)) for i in pick]
+    count = [int(rng.integers(0, lens[i] - b + 1)) for i, b in zip(pick, begin)]
+    k, v = c.read(0, [ids[i] for i in pick], begin, count)
+    whole_k, whole_v = c.read(0, ids, [0] * 150, lens)
+    first = np.concatenate(([0], np.cumsum(lens)))
+    at = [first[i] + b + j for i, b, n in zip(pick, begin, count) for j in range(n)]
+    assert torch.equal(k, whole_k[at]) and torch.equal(v, whole_v[at])
+
+
+def test_a_long_sequence_is_copied_and_closed_up(nh):
+    """More pages than one launch's arguments name: tables, copies, compaction of 40,000 positions."""
+    rng = np.random.default_rng(37)
+    n = 40000
+    c, ids, ks, vs = filled(nh, rng, [n], 1, 64, 64, 64, 32, "f16", extra_pages=2600, seqs=3, last=[2])
+    t = c.copy(ids[0])
+    c.compact([t], [[(3, 20000), (20001, n)]])
+    keep = [i for i in range(3, n) if i != 20000]
+    k, v = c.read(0, [t], [0], [n - 4])
+    a, b = c.read(0, ids, [0], [n])
+    assert torch.equal(k, a[keep]) and torch.equal(v, b[keep])
+    assert np.array_equal(plain(a), ref.quantize(plain(ks[0][0]), 64).astype(np.float32))
+    c.extend([t], [1])
+    x = rows_of(rng, 1, 1, 64, "f16")
+    c.append(0, x.cuda(), x.cuda())
+    q = rows_of(rng, 1, 4, 64, "f16")
+    o = plain(c.attend(0, q.cuda()))
+    kk, vv = (np.concatenate((plain(y), ref.quantize(plain(x), 64))) for y in (k, v))
+    want, _ = ref.attend(plain(q), kk, vv, 0.125)
+    assert np.all(np.abs(o - want) <= ref.attend_bound(plain(q), kk, vv, want, 0.125, "f16"))
+
+
+def test_a_replay_of_another_shape_does_nothing(nh):
+    """A step captured for two rows, replayed after an extend of five: neither the rows nor the cache are touched."""
+    rng = np.random.default_rng(41)
+    c, ids, _, _ = filled(nh, rng, [40], 1, 64, 64, 32, 32, "bf16", extra_pages=4, last=[2])
+    x, q = rows_of(rng, 2, 1, 64, "bf16").cuda(), rows_of(rng, 2, 2, 64, "bf16").cuda()
+    out = torch.zeros(2, 2, 64, device="cuda", dtype=torch.bfloat16)
+    c.attend(0, q, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.append(0, x, x)
+        c.attend(0, q, out=out)
+    c.extend(ids, [5])
+    y = rows_of(rng, 5, 1, 64, "bf16").cuda()
+    c.append(0, y, y)
+    before = c.read(0, ids, [0], [45])
+    out.fill_(3.0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert bool((out == 3.0).all())
+    for a, b in zip(before, c.read(0, ids, [0], [45])):
+        assert torch.equal(a, b)
+
+
+def test_a_replay_after_pages_changed_hands_does_nothing(nh):
+    """A captured step whose sequences are gone, and one whose second sequence is: what took their pages stays as it is."""
+    rng = np.random.default_rng(43)
+    c, ids, _, _ = filled(nh, rng, [64, 64, 50], 1, 64, 64, 32, 32, "bf16", extra_pages=2, last=[1, 1, 0])
+    x, q = rows_of(rng, 3, 1, 64, "bf16").cuda(), rows_of(rng, 3, 2, 64, "bf16").cuda()
+    out = torch.zeros(3, 2, 64, device="cuda", dtype=torch.bfloat16)
+    c.extend(ids, [1, 1, 1])
+    c.append(0, x, x)
+    c.attend(0, q, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.append(0, x, x)
+        c.attend(0, q, out=out)
+    for change in ("extend", "copy", "compact"):
+        if change == "extend":
+            c.free(ids[1])
+            c.extend([ids[0]], [0])
+            t = ids[2]
+        else:
+            c.extend([i for i in ids if i != ids[1]], [1, 1])
+            c.append(0, x[:2], x[:2])
+            c.truncate(ids[0], 33)
+            t = c.copy(ids[2])
+            if change == "compact":
+                c.compact([t], [[(7, 40)]])
+        before = c.read(0, [ids[0], t], [0, 0], [c.length(ids[0]), c.length(t)])
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(before, c.read(0, [ids[0], t], [0, 0], [c.length(ids[0]), c.length(t)])):
+            assert torch.equal(a, b), change
+        if change != "extend":
+            c.free(t)
+
+
 def test_refusals(nh):
     c = nh.KvCache4(2, 2, 48, 64, pages=3, seqs=2, cap=90, page=32)
     k, v = torch.zeros(4, 2, 48, device="cuda"), torch.zeros(4, 2, 64, device="cuda")

@@ -26,7 +26,8 @@ def new(**over):
                                   dict(qk_dim=257), dict(v_dim=0), dict(v_dim=300), dict(group=16), dict(group=128),
                                   dict(page=16), dict(page=33), dict(page=512), dict(pages=0), dict(pages=-1),
                                   dict(pages=1 << 29), dict(seqs=0), dict(seqs=70000), dict(cap=0), dict(cap=-5),
-                                  dict(cap=(1 << 30) + 1), dict(seqs=65536, cap=1 << 30)])
+                                  dict(cap=(1 << 30) + 1), dict(seqs=65536, cap=1 << 30),
+                                  dict(layers=4096, kv_heads=1024, pages=1 << 28)])
 def test_shapes(over):
     assert new(**over) == EINVAL
     assert nh.load_library().nh_last_error()
