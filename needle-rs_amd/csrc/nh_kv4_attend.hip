@@ -492,7 +492,7 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
                 const int64_t at = ((int64_t)split * c.rows + row) * a.heads + head;
                 float* ml = reinterpret_cast<float*>(a.ws);
                 ml[2 * ((int64_t)plan.splits * c.rows * a.heads) + at * c.dv + d] = v;
-                if (d == 0) ml[2 * at] = top, ml[2 * at + 1] = sum;
+                if (d == 0) ml[2 * at] = sum == sum ? top : sum, ml[2 * at + 1] = sum;
             }
         }
     }
@@ -917,7 +917,7 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
         if (last) {
             if (a.lse) a.lse[row * a.heads + head] = (m + __builtin_amdgcn_logf(l * 0x1p-15f)) * 0.69314718055994530942f;
         } else
-            ml[2 * at] = m, ml[2 * at + 1] = l * 0x1p-15f;
+            ml[2 * at] = l == l ? m : l, ml[2 * at + 1] = l * 0x1p-15f;
     }
 }
 
@@ -946,8 +946,10 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, in
     const float zero = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f;
     for (int s = tid; s < splits; s += 256) {
-        f[s] = __builtin_amdgcn_exp2f(f[s] - zero);  // 0: a range without keys, which wrote no sums
-        sum += f[s] == 0.0f ? 0.0f : ml[2 * (s * n + at) + 1] * f[s];
+        // -1: a range without keys, which wrote no sums.  NaN: scores were, and the row's results are.
+        const float g = f[s] == -__builtin_inff() ? -1.0f : __builtin_amdgcn_exp2f(f[s] - zero);
+        f[s] = g;
+        sum += g < 0.0f ? 0.0f : ml[2 * (s * n + at) + 1] * g;
     }
 #pragma unroll
     for (int h = 1; h < 64; h <<= 1) sum += lane_xor(sum, h, lane);
@@ -963,8 +965,8 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, in
             for (int k = 0; k < 8; ++k) y[k] = s0 + 4 * k < splits && d < c.dv ? po[(s0 + 4 * k) * n * c.dv + d] : 0.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float g = s0 + 4 * k < splits ? f[s0 + 4 * k] : 0.0f;
-                v = g == 0.0f ? v : __builtin_fmaf(y[k], g, v);
+                const float g = s0 + 4 * k < splits ? f[s0 + 4 * k] : -1.0f;
+                v = g < 0.0f ? v : __builtin_fmaf(y[k], g, v);
             }
         }
         sv[wave][d & 255] = v;

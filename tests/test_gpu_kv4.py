@@ -381,6 +381,39 @@ def test_stale_pages_are_not_seen(nh):
     assert np.all(np.abs(o - want) <= ref.attend_bound(plain(q), a, b, want, 0.125, "f32"))
 
 
+@pytest.mark.parametrize("rows", [1, 160])
+def test_nan_reaches_its_readers_over_ranges_of_keys(nh, rows):
+    """A long sequence's keys are attended in ranges.  A NaN key spoils the rows that see it, a NaN value its group
+    of them, a NaN query its own row, also where that range's other weights vanish beside another one's."""
+    rng = np.random.default_rng(12)
+    n, at = 6000, 300
+    k, v = (rows_of(rng, n, 1, 64, "bf16") for _ in range(2))
+    q = rows_of(rng, rows, 2, 64, "bf16")
+    k[5000] = 60.0 * torch.sign(q[-1, 0])  # takes all of the weight of the last row's first head
+    k2, v2, q2 = k.clone(), v.clone(), q.clone()
+    k2[at, 0, 7] = float("nan")
+    v2[at, 0, 40] = float("nan")
+    q2[0, 1, 5] = float("nan")
+    outs = []
+    for kk, vv, qq in ((k, v, q), (k2, v, q), (k, v2, q), (k, v, q2)):
+        c = nh.KvCache4(1, 1, 64, 64, pages=200, seqs=1, cap=8192, page=64)
+        s = c.new_seq()
+        c.extend([s], [n - rows])
+        c.append(0, kk[: n - rows].cuda(), vv[: n - rows].cuda())
+        c.extend([s], [rows])
+        c.append(0, kk[n - rows :].cuda(), vv[n - rows :].cuda())
+        lse = torch.empty((rows, 2), device="cuda")
+        outs.append([plain(x) for x in (c.attend(0, qq.cuda(), scale=1.0, lse=lse), lse)])
+    assert not np.isnan(outs[0][0]).any() and not np.isnan(outs[0][1]).any()
+    assert np.isnan(outs[1][0]).all() and np.isnan(outs[1][1]).all()
+    assert np.isnan(outs[2][0][..., 32:]).all() and not np.isnan(outs[2][0][..., :32]).any()
+    assert np.array_equal(outs[2][1], outs[0][1])
+    spoiled = np.zeros((rows, 2), bool)
+    spoiled[0, 1] = True
+    assert np.array_equal(np.isnan(outs[3][1]), spoiled)
+    assert np.array_equal(np.isnan(outs[3][0]).all(-1), spoiled) and np.array_equal(np.isnan(outs[3][0]).any(-1), spoiled)
+
+
 def test_nan_reaches_its_readers_only(nh):
     """A NaN value in a row: outputs of the rows that see it are NaN in its group, all others are as without it;
     the window hides it from later rows.  A NaN query spoils its own row and head."""
