@@ -382,9 +382,10 @@ int nh_generate_greedy(nh_session* s, int steps, uint32_t* out, float* logits, v
  * a refused call changes nothing), and is refused under stream capture.  append
  * and attend read the batch from the device: captured, they follow the state
  * that a later extend of the same rows outside the graph leaves (after an extend
- * of more rows, or where the batch is over and its pages have changed hands,
- * a replay touches nothing).  The calls on one cache are queued on one stream, or ordered by the caller's events.  A
- * cache belongs to the device it was made on. */
+ * of more rows, or where the batch is over and its pages have changed hands, a
+ * replay reads and writes no page, and what it leaves in `out` says nothing).  The
+ * calls on one cache are queued on one stream, or ordered by the caller's
+ * events.  A cache belongs to the device it was made on. */
 #define NH_F32 0
 #define NH_F16 1
 #define NH_BF16 2
@@ -442,13 +443,18 @@ int nh_kv4_read(nh_kv4* c, int layer, const int* seqs, const int* pos, const int
  * (Session::attend's span, crates/needle-engine/src/model.rs:62-66, by
  * position).  lse (f32 [rows][heads], or NULL): the log of the summed
  * exponentials, to join with other keys.  Scores, weights' sums and products
- * are held in f32; f16 and bf16 calls round a weight to 11 bits (of many rows
- * also a key's and a value's step x code), f32 calls carry 22.  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used
- * by the work queued on `stream` only (its size depends on the batch's
- * lengths: asked after the extend; 0: it may be NULL). */
+ * are held in f32; f32 and f16 calls carry 22 bits of a weight, bf16 calls 11
+ * (f16 and bf16 calls of many rows 11 of it and of a key's and a value's step x
+ * code).  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used by
+ * the work queued on `stream` only (its size depends on the batch's lengths:
+ * asked after the extend; 0: it may be NULL). */
 int64_t nh_kv4_attend_ws_bytes(const nh_kv4* c, int heads, int sink, int ring);
 int nh_kv4_attend(const nh_kv4* c, int layer, const void* q, int64_t ldq, int heads, float scale, int sink, int ring,
                   void* out, int64_t ldo, float* lse, int type, void* ws, uint64_t ws_bytes, void* stream);
+/* No reference counterpart (a test hook): attention by the kernel of few rows
+ * (1), by that of many where it takes the call's type and dims (2), or by the
+ * one that the shapes make the quicker (0, as made). */
+int nh_kv4_debug_kernel(nh_kv4* c, int kernel);
 
 /* ---- drafted tokens ----------------------------------------------------- */
 /* No reference counterpart (generate.rs:87-139 picks one token a step).

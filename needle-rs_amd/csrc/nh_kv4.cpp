@@ -450,6 +450,13 @@ static int longest(const nh_kv4* c) {
     return n;
 }
 
+int nh_kv4_debug_kernel(nh_kv4* c, int kernel) {
+    if (!c) return fail(NH_EINVAL, "null cache");
+    if (kernel < 0 || kernel > 2) return fail(NH_EINVAL, "0, 1 or 2");
+    c->v.kernel = kernel;
+    return NH_OK;
+}
+
 int64_t nh_kv4_attend_ws_bytes(const nh_kv4* c, int heads, int sink, int ring) {
     if (!c) return fail(NH_EINVAL, "null cache");
     if (int rc = check_attend(c, 0, heads, sink, ring)) return rc;

@@ -49,6 +49,7 @@ struct Kv4View {
     const int* batch;    // [nb] of (sequence, first row, end row, length): Kv4Entry
     int table_ld, pages, layers, heads, dk, dv, width, group, page_log2;
     int nb, rows, each;  // the batch; each: rows of every sequence when they are equal, else 0
+    int kernel;          // nh_kv4_debug_kernel
     __host__ __device__ int page() const { return 1 << page_log2; }
     __host__ __device__ int groups() const { return width / group; }
     // bytes of 32 positions, and of one (page, layer, head)

@@ -7,7 +7,7 @@
 //   scale q . k_j = cq sum_g step_jg (q_g . c_jg) + sum_g low_jg (scale sum q_g)
 //   o = (sum_g sum_j (p_j step_jg) c_jg + sum_j p_j low_jg) / sum_j p_j
 // The two sums over low are matrix products of their own, with the lows as they
-// are stored: of the queries' sums (two f16 parts, 22 bits) and of the weights.
+// are stored: of the queries' sums (two f16 parts, 22 bits) and of the weights,
 // so the codes themselves are the matrix operands: a code 0 .. 15 under a
 // 16-bit mask is the f16 subnormal c 2^-24 (under the next nibble's mask 16 c
 // 2^-24), which the f16 MFMAs take exactly; unpacking is one AND for two
@@ -17,6 +17,13 @@
 // + 0..3 of each 16, which is the operand that O^T = V^T P^T wants of that lane
 // (the order of the summed keys is free), so a weight never leaves its lane, and
 // a row's maximum, sum and correction are one lane's scalars.
+//
+// Bound by the codes' bytes where keys are many: 64 sequences of 4,096 to 8,192
+// keys, 8 kv heads of 128 under 32, bf16 (511 MB): 110 us, 4.65 TB/s, what a
+// large copy reaches.  A wavefront's 32 keys cost about 300 vector instructions
+// (masks, steps, exponentials) beside 19 MFMAs, 0.87 us a SIMD, so where one
+// sequence has all the keys the two are about equal: 131,072 keys (151 MB) 36 us
+// and 5 for the join.  Few keys are latency: 374 of them 7.5 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -101,7 +108,11 @@ template <int TYPE, int W, int G, int RT, int NW>
 __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
     typedef typename Kv4Elem<TYPE>::T T;
     constexpr int NG = W / G, NB = W / 64, NJ = W / 32, GJ = G / 32, GI = G / 16;
-    constexpr int PARTS = TYPE == KV4_F32 ? 2 : 1;  // f16 halves of a query element and of a weight
+    constexpr int PARTS = TYPE == KV4_F32 ? 2 : 1;   // f16 halves of a query element
+    // ..  and of a weight.  One leaves up to three roundings of an f16 output (4.6e-4
+    // of it instead of 2.1e-4, 20 keys; 131,072 keys: 38.6 us, 41.0 with two), but
+    // a tenth of a bf16 output's one.
+    constexpr int WPARTS = TYPE == KV4_BF16 ? 1 : 2;
     // The MFMAs take a subnormal as it is, but line its products up by the exponent
     // of the smallest normal number: up to 2^-17 of the largest product is cut off
     // (2^-20 with normal operands, both measured).  Calls that carry 22 bits bring
@@ -299,7 +310,7 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
                 const u32x4 y = {w & 0x000f000fu, w & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u};
                 ka[t][j] = operand(y);
             }
-        h8 pw[RT][NG][PARTS];
+        h8 pw[RT][NG][WPARTS];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const bool fresh = m[rt] == -__builtin_inff();  // no key seen yet
@@ -365,24 +376,24 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
                 p[k] = __builtin_amdgcn_exp2f(s[k / 4][k % 4]);
                 l[rt] += p[k];
             }
-            // Two numbers to f16 at a time; f32 calls carry what that rounds off.
+            // Two numbers to f16 at a time; f32 and f16 calls carry what that rounds off.
             auto halves = [&](const float* w, h8* to) {
 #pragma unroll
                 for (int k = 0; k < 8; k += 2) {
                     const f32x2 y = {w[k], w[k + 1]};
                     const h2 hi = __builtin_convertvector(y, h2);
                     to[0][k] = hi[0], to[0][k + 1] = hi[1];
-                    if constexpr (PARTS == 2) {
+                    if constexpr (WPARTS == 2) {
                         to[1][k] = (_Float16)(w[k] - (float)hi[0]);
                         to[1][k + 1] = (_Float16)(w[k + 1] - (float)hi[1]);
                     }
                 }
             };
-            h8 pp[PARTS];
+            h8 pp[WPARTS];
             halves(p, pp);
             const u32x4 vl = {x.vl[0][0], x.vl[0][1], x.vl[1][0], x.vl[1][1]};
 #pragma unroll
-            for (int k = 0; k < PARTS; ++k)
+            for (int k = 0; k < WPARTS; ++k)
                 accl[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vl), pp[k], accl[rt], 0, 0, 0);
             static_for<0, NG>([&](auto GG) {
                 constexpr int g = GG.value;
@@ -411,7 +422,7 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p)
+                    for (int p = 0; p < WPARTS; ++p)
                         acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pw[rt][d / GI][p], acc[rt][d], 0, 0, 0);
             }
         }
@@ -507,6 +518,13 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
 // as above, so the rounding is relative to a group's range and not to its
 // offset.  32 x 32 MFMAs: a lane holds 16 scores of its row, the other half of
 // them is 32 lanes away.  The weights' sum is one more row of the lows' product.
+//
+// Two sequences' 2,000 rows after 6,000 keys, 32 heads over 8 of 128, bf16 (427
+// GFLOP): 575 us, 743 TFLOP/s; the kernel above takes 1,450, an operand's masks,
+// steps and lows serving 16 rows there and 256 here.  A large library product
+// runs at 1,130 to 1,180.  The matrix cores are busy 37 % of the time, the vector
+// units (exponentials, maxima, weights to f16) 42 %, one wavefront's chain of
+// scores, maximum, weights and sums being what neither hides from the other.
 constexpr int KP_WAVES = 8;
 constexpr int KP_ROWS = 32 * KP_WAVES;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -979,6 +997,41 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, in
     if (a.lse && tid == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
 }
 
+// The same for few ranges, a thread an element of the output: many rows are many
+// elements, and a workgroup a (row, head) would mostly wait for its barriers (32,768
+// of two ranges).
+constexpr int KA_FEW = 8;
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_kv4_join_few(Kv4View c, Kv4AttendArgs a, int splits) {
+    typedef typename Kv4Elem<TYPE>::T T;
+    const int64_t n = (int64_t)c.rows * a.heads, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n * c.dv) return;
+    const int64_t at = i / c.dv;
+    const int d = (int)(i - at * c.dv);
+    const float* ml = reinterpret_cast<const float*>(a.ws);
+    const float* po = ml + 2 * n * splits + i;
+    float m[KA_FEW], l[KA_FEW], v[KA_FEW], top = -__builtin_inff();
+#pragma unroll
+    for (int s = 0; s < KA_FEW; ++s) {
+        const int64_t x = s < splits ? s : 0;
+        m[s] = s < splits ? ml[2 * (x * n + at)] : -__builtin_inff();
+        l[s] = ml[2 * (x * n + at) + 1];
+        v[s] = po[x * n * c.dv];
+        top = fmaxf(top, m[s]);
+    }
+    const float zero = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KA_FEW; ++s) {
+        const float g = __builtin_amdgcn_exp2f(m[s] - zero);
+        const bool some = m[s] != -__builtin_inff();  // (a range without keys wrote no sums)
+        sum = some ? __builtin_fmaf(l[s], g, sum) : sum;
+        o = some ? __builtin_fmaf(v[s], g, o) : o;
+    }
+    Kv4Elem<TYPE>::put(reinterpret_cast<T*>(a.out) + at / a.heads * a.ldo + at % a.heads * c.dv + d, o / sum);
+    if (a.lse && d == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
+}
+
 // The shape of a call: which kernel, its rows a tile and wavefronts, key ranges.
 struct KaShape {
     bool prompt;
@@ -986,33 +1039,80 @@ struct KaShape {
     int64_t tiles;
 };
 
-static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, int sink, int ring, int longest) {
-    const int per = heads / c.heads;
-    const int64_t mean = c.nb ? (int64_t)c.rows * per / c.nb : 0;  // rows of a sequence for a kv head
-    KaShape s;
-    // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at
-    // 256 dims its sums do not fit the registers.
-    s.prompt = type != KV4_F32 && c.width <= 128 && mean >= 128;
-    s.rows = s.prompt ? KP_ROWS : c.width == 64 && mean > 16 ? 32 : 16;
+static void tiles_of(const Kv4View& c, const int* row0, int per, int rows, KaShape& s) {
+    s.rows = rows;
     s.tiles_each = 0;
     s.tiles = 0;
     if (c.each) {
-        s.tiles_each = (int)(((int64_t)c.each * per + s.rows - 1) / s.rows);
+        s.tiles_each = (int)(((int64_t)c.each * per + rows - 1) / rows);
         s.tiles = (int64_t)s.tiles_each * c.nb;
     } else
-        for (int b = 0; b < c.nb; ++b) s.tiles += ((int64_t)(row0[b + 1] - row0[b]) * per + s.rows - 1) / s.rows;
+        for (int b = 0; b < c.nb; ++b) s.tiles += ((int64_t)(row0[b + 1] - row0[b]) * per + rows - 1) / rows;
+}
+
+// Which kernel is the quicker depends on the rows, the keys and how both fill the
+// chip, so both are estimated, in us, from what was measured of each at 128 (64)
+// dims of bf16:
+//  rows   4 in all and 4 a round of 512 workgroups of four wavefronts (256 of
+//         eight), 1.74 (1.8) a step of a wavefront: 32 keys of 16 (32) rows
+//  prompt 18 in all (the references, the first images), 1.3 (1.0) for 32 keys of
+//         256 rows, a workgroup a CU
+//  join   4, and the partial results' bytes there and back at 2 TB/s
+// One sequence of 4,000 keys and 32 heads over 8, 128 dims, rows / prompt: 128 rows
+// 33 / 63, 256 60 / 71, 512 112 / 98, 1,024 224 / 162, 2,048 480 / 265; 16 sequences'
+// 32 rows 110 / 109, 64 rows 204 / 139; 500 keys' 1,024 rows 80 / 80, 2,048 190 / 124.
+static double ka_join_us(const Kv4View& c, int heads, int64_t splits) {
+    return splits > 1 ? 4.0 + (double)c.rows * heads * (double)splits * (c.dv + 2) * 8 / 2e6 : 0.0;
+}
+
+static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, int sink, int ring, int longest) {
+    const int per = heads / c.heads;
+    const int64_t tokens = c.nb ? (c.rows + c.nb - 1) / c.nb : 0, mean = c.nb ? (int64_t)c.rows * per / c.nb : 0;
+    // The chunks that a tile of `rows` rows sees: the last tile's, and a middle one's.
+    auto chunks_of = [&](int rows, bool middle) -> int64_t {
+        const int64_t keys = longest - (middle ? tokens / 2 : 0), wide = std::min<int64_t>(tokens, rows / per + 1);
+        return ((ring ? std::min<int64_t>(keys, (int64_t)sink + ring + wide + 2 * KA_CHUNK) : keys) + KA_CHUNK - 1) / KA_CHUNK;
+    };
+    KaShape s;
+    s.prompt = false;
+    // Two tiles of rows a wavefront where their sums fit the registers beside the loads.
+    tiles_of(c, row0, per, c.width == 64 && mean > 16 ? 32 : 16, s);
     const int64_t base = s.tiles * c.heads;
-    s.waves = s.prompt ? KP_WAVES : s.rows == 16 && c.width <= 128 && base <= 256 ? 8 : 4;
-    const int64_t keys = ring ? std::min<int64_t>(longest, (int64_t)sink + ring + c.rows + 2 * KA_CHUNK) : longest;
-    const int64_t chunks = (keys + KA_CHUNK - 1) / KA_CHUNK;
+    s.waves = s.rows == 16 && c.width <= 128 && base <= 256 ? 8 : 4;
+    const int64_t chunks = chunks_of(s.rows, false);
     // Eight wavefronts a CU, as many as their registers let run, but at least
     // four steps for each wavefront of a range. (64 sequences of 4096 to 8192
     // keys, 8 kv heads: 512 workgroups 129 us, 1024 139, 2048 146; 131,072 keys:
     // 42, 46, 55 us. Two or one step instead of four: 1060 visible keys 41 and
-    // 60 us for 31.)
-    const int64_t want = std::min<int64_t>(base > 0 ? ((s.waves == 4 ? 512 : 256) + base - 1) / base : 1, KA_SPLITS);
-    s.splits = (int)std::max<int64_t>(1, std::min(want, chunks / (s.prompt ? 16 : 4 * s.waves)));
-    return s;
+    // 60 us for 31.  All of that with four wavefronts, an earlier build.)  Eight
+    // of one workgroup meet in LDS and not in the workspace, so half as many
+    // ranges are joined: 1060 keys of 128 (sequence, head) tiles 15.4 us for 27.9,
+    // 131,072 keys of 8 38.7 for 41.5.  With more than 256 tiles every CU has its
+    // eight wavefronts without it.
+    const int64_t slots = s.waves == 4 ? 512 : 256;
+    const int64_t want = std::min<int64_t>(base > 0 ? (slots + base - 1) / base : 1, KA_SPLITS);
+    s.splits = (int)std::max<int64_t>(1, std::min(want, chunks / (4 * s.waves)));
+
+    // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at
+    // 256 dims its sums do not fit the registers.
+    if (type == KV4_F32 || c.width > 128 || c.kernel == 1 || base == 0) return s;
+    const int64_t steps = (chunks_of(s.rows, true) + s.splits * s.waves - 1) / (s.splits * s.waves);
+    const double step = s.rows == 32 ? 1.8 : c.width == 64 ? 0.9 : 1.74;
+    const double plain = 4.0 + std::max(1.0, (double)(base * s.splits) / (double)slots) * (4.0 + (double)steps * step) +
+                         ka_join_us(c, heads, s.splits);
+    KaShape p;
+    p.prompt = true;
+    p.waves = KP_WAVES;
+    tiles_of(c, row0, per, KP_ROWS, p);
+    const int64_t most = chunks_of(KP_ROWS, false), middle = chunks_of(KP_ROWS, true);
+    const double each = c.width == 64 ? 1.0 : 1.3;
+    double best = 0.0;
+    for (int64_t n = 1; n <= KA_FEW * 4 && (n == 1 || most / n >= 16); ++n) {
+        const int64_t rounds = (p.tiles * c.heads * n + 255) / 256;
+        const double us = 18.0 + (double)rounds * (double)(((rounds == 1 ? most : middle) + n - 1) / n) * each + ka_join_us(c, heads, n);
+        if (n == 1 || us < best) best = us, p.splits = (int)n;
+    }
+    return best < plain || c.kernel == 2 ? p : s;
 }
 
 size_t kv4_attend_ws(const Kv4View& c, const int* row0, int heads, int sink, int ring, int longest) {
@@ -1047,8 +1147,11 @@ static hipError_t attend_shaped(const Kv4View& c, const int* row0, const Kv4Atte
             if (shape.rows == 32) kern = k_kv4_attend<TYPE, W, G, 2, 4>;
         hipLaunchKernelGGL(kern, grid, dim3(shape.waves * 64), 0, s, c, a, plan);
     }
-    if (plan.splits > 1)
+    if (plan.splits > KA_FEW)
         hipLaunchKernelGGL(k_kv4_join<TYPE>, dim3((unsigned)(c.rows * a.heads)), dim3(256), 0, s, c, a, plan.splits);
+    else if (plan.splits > 1)
+        hipLaunchKernelGGL(k_kv4_join_few<TYPE>, dim3((unsigned)(((int64_t)c.rows * a.heads * c.dv + 255) / 256)), dim3(256), 0, s, c, a,
+                           plan.splits);
     return hipGetLastError();
 }
 

@@ -104,6 +104,7 @@ SIGNATURES = {
     "nh_kv4_rows": (I, [P]),
     "nh_kv4_append": (I, [P, I, P, P, C.c_int64, C.c_int64, I, P]),
     "nh_kv4_read": (I, [P, I, P, P, P, I, P, P, I, P]),
+    "nh_kv4_debug_kernel": (I, [P, I]),
     "nh_kv4_attend_ws_bytes": (C.c_int64, [P, I, I, I]),
     "nh_kv4_attend": (I, [P, I, P, C.c_int64, I, C.c_float, I, I, P, C.c_int64, P, I, P, C.c_uint64, P]),
     "nh_verify_drafts_ws_bytes": (C.c_int64, [I, I, I]),

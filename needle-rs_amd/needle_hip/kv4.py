@@ -197,6 +197,10 @@ class KvCache4:
                                         out.data_ptr(), ldo, _ptr(lse), _TYPES[q.dtype], _ptr(ws), n, nh._stream(stream)))
         return out
 
+    def debug_kernel(self, kernel: int):
+        """Attention by one of its kernels (nh_kv4_debug_kernel); tests only."""
+        nh._check(nh._lib.nh_kv4_debug_kernel(self.h, int(kernel)))
+
     def __del__(self):
         if getattr(self, "h", None) and nh is not None and nh._lib is not None:
             nh._lib.nh_kv4_free(self.h)

@@ -201,11 +201,13 @@ def test_many_single_positions_compact(nh):
         assert np.array_equal(plain(v), want)
 
 
-def attend_case(nh, lens, rows, kv, per, qk, v, group, page, dtype, sink=0, ring=0, scale=None, spread=1.0, seed=0):
+def attend_case(nh, lens, rows, kv, per, qk, v, group, page, dtype, sink=0, ring=0, scale=None, spread=1.0, seed=0,
+                kernel=0):
     rng = np.random.default_rng(seed + 100 * qk + v)
     c, ids, ks, vs = filled(nh, rng, lens, kv, qk, v, group, page, dtype, last=rows, spread=spread)
     q = rows_of(rng, sum(rows), kv * per, qk, dtype)
     lse = torch.full((sum(rows), kv * per), 9.0, device="cuda")
+    c.debug_kernel(kernel)
     o = c.attend(0, q.cuda(), scale=scale, sink=sink, ring=ring, lse=lse)
     assert o.dtype == T[dtype] and o.shape == (sum(rows), kv * per, v)
     s = qk ** -0.5 if scale is None else scale
@@ -222,7 +224,7 @@ def attend_case(nh, lens, rows, kv, per, qk, v, group, page, dtype, sink=0, ring
         # the log of a sum of weights that are each off by the scores' bound
         size = np.abs(x).sum(-1).max() * np.abs(k).max() * abs(s)
         off = (qk + 16) * 2.0 ** -24 * size * 2 + (n + 64) * 2.0 ** -23 + 2.0 ** -22 * np.abs(want_lse)
-        if dtype != "f32" and max(qk, v) <= 128 and sum(rows) * per // len(rows) >= 128:
+        if dtype != "f32" and max(qk, v) <= 128 and kernel != 1:
             # Calls of many rows round step x code of a key to 11 bits, half a step 2^-12 of at most
             # the group's range, 2 max |k|: a score moves by scale sum |q| 2^-11 max |k| at most, and so
             # the log of the sum; each weight, rounded to 11 bits and summed so, by 2^-12 of itself.
@@ -266,20 +268,36 @@ def test_attend_long_prompt_rows(nh):
     attend_case(nh, [1500, 700], [800, 300], 2, 2, 64, 64, 64, 64, "f32", sink=10, ring=200)
 
 
+@pytest.mark.parametrize("kernel", [1, 2])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("kv,per,qk,v,group,page", [(1, 1, 64, 64, 32, 32), (2, 4, 48, 64, 64, 32), (2, 3, 45, 51, 32, 64),
                                                     (2, 4, 128, 128, 64, 64), (1, 8, 80, 96, 32, 128), (1, 2, 128, 72, 32, 64)])
-def test_attend_prompts(nh, kv, per, qk, v, group, page, dtype):
-    """Rows by the hundred, ragged, from the first position on and after others, with and without a span."""
-    attend_case(nh, [300, 517, 33, 260], [300, 129, 33, 200], kv, per, qk, v, group, page, dtype)
-    attend_case(nh, [410], [257], kv, per, qk, v, group, page, dtype, sink=5, ring=70)
-    attend_case(nh, [900, 900], [256, 256], kv, per, qk, v, group, page, dtype, sink=130, ring=300)
+def test_attend_prompts(nh, kv, per, qk, v, group, page, dtype, kernel):
+    """Rows by the hundred, ragged, from the first position on and after others, with and without a span, by
+    either kernel."""
+    attend_case(nh, [300, 517, 33, 260], [300, 129, 33, 200], kv, per, qk, v, group, page, dtype, kernel=kernel)
+    attend_case(nh, [410], [257], kv, per, qk, v, group, page, dtype, sink=5, ring=70, kernel=kernel)
+    attend_case(nh, [900, 900], [256, 256], kv, per, qk, v, group, page, dtype, sink=130, ring=300, kernel=kernel)
+    attend_case(nh, [1700, 3], [12, 1], kv, per, qk, v, group, page, dtype, kernel=kernel)
+
+
+def test_the_rule_takes_either_kernel(nh):
+    """Few rows, or short ones, go to the one kernel, long prompts to the other."""
+    rng = np.random.default_rng(41)
+    for n, rows, which in ((700, 100, 1), (4000, 16, 1), (2100, 1700, 2)):
+        c, _, _, _ = filled(nh, rng, [n], 8, 128, 128, 32, 64, "bf16", last=[rows])
+        q = rows_of(rng, rows, 32, 128, "bf16").cuda()
+        outs = []
+        for kernel in (0, 1, 2):
+            c.debug_kernel(kernel)
+            outs.append(c.attend(0, q))
+        assert torch.equal(outs[0], outs[which]) and not torch.equal(outs[0], outs[3 - which])
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_attend_prompt_scales(nh, dtype):
     for spread, scale in ((1e-3, None), (50.0, 0.01), (1.0, -0.2), (1.0, 0.0), (3.0, 1.0)):
-        attend_case(nh, [350], [290], 2, 2, 64, 64, 32, 32, dtype, scale=scale, spread=spread)
+        attend_case(nh, [350], [290], 2, 2, 64, 64, 32, 32, dtype, scale=scale, spread=spread, kernel=2)
 
 
 def test_prompt_nan_reaches_its_readers_only(nh):
@@ -293,6 +311,7 @@ def test_prompt_nan_reaches_its_readers_only(nh):
     outs = []
     for kk, vv, qq in ((k, v, q), (k, v2, q), (k2, v, q), (k, v, q2)):
         c = nh.KvCache4(1, 2, 64, 64, pages=14, seqs=1, cap=n, page=32)
+        c.debug_kernel(2)
         s = c.new_seq()
         c.extend([s], [n])
         c.append(0, kk.cuda(), vv.cuda())
@@ -313,6 +332,7 @@ def test_prompt_rows_do_not_depend_on_hidden_rows(nh):
     outs = []
     for stale in (None, 3000.0, float("nan")):
         c = nh.KvCache4(1, 1, 128, 128, pages=3, seqs=1, cap=192, page=64)
+        c.debug_kernel(2)
         if stale is not None:
             s = c.new_seq()
             c.extend([s], [192])
@@ -381,8 +401,8 @@ def test_stale_pages_are_not_seen(nh):
     assert np.all(np.abs(o - want) <= ref.attend_bound(plain(q), a, b, want, 0.125, "f32"))
 
 
-@pytest.mark.parametrize("rows", [1, 160])
-def test_nan_reaches_its_readers_over_ranges_of_keys(nh, rows):
+@pytest.mark.parametrize("rows,kernel", [(1, 1), (160, 1), (160, 2), (1, 2)])
+def test_nan_reaches_its_readers_over_ranges_of_keys(nh, rows, kernel):
     """A long sequence's keys are attended in ranges.  A NaN key spoils the rows that see it, a NaN value its group
     of them, a NaN query its own row, also where that range's other weights vanish beside another one's."""
     rng = np.random.default_rng(12)
@@ -397,6 +417,7 @@ def test_nan_reaches_its_readers_over_ranges_of_keys(nh, rows):
     outs = []
     for kk, vv, qq in ((k, v, q), (k2, v, q), (k, v2, q), (k, v, q2)):
         c = nh.KvCache4(1, 1, 64, 64, pages=200, seqs=1, cap=8192, page=64)
+        c.debug_kernel(kernel)
         s = c.new_seq()
         c.extend([s], [n - rows])
         c.append(0, kk[: n - rows].cuda(), vv[: n - rows].cuda())
