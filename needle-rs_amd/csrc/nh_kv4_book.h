@@ -176,7 +176,7 @@ struct Kv4Book {
         for (int i = 0; i < n; ++i) {
             const Seq& q = seqs[s[i]];
             need += pages_of(q.len + rows[i]) - (int)q.table.size();
-            if (rows[i] && q.len % page) {
+            if (rows[i] && q.len % page && refs[q.table.back()] > 1) {
                 const int p = q.table.back();
                 size_t j = 0;
                 while (j < shared.size() && shared[j].first != p) ++j;
