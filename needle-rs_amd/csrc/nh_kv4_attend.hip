@@ -1075,29 +1075,38 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
     };
     KaShape s;
     s.prompt = false;
-    // Two tiles of rows a wavefront where their sums fit the registers beside the loads.
-    tiles_of(c, row0, per, c.width == 64 && mean > 16 ? 32 : 16, s);
+    // Two tiles of rows a wavefront where their sums fit the registers beside the
+    // loads, and there are tiles for every CU's eight wavefronts without it (2 kv
+    // heads, 4000 keys: 96 tiles of 16 17.6 us, half as many of 32 21.3; 384 36.4 and
+    // 47.3; 1024 about the same).
+    tiles_of(c, row0, per, 16, s);
+    if (c.width == 64 && mean > 16 && s.tiles * c.heads > 512) tiles_of(c, row0, per, 32, s);
     const int64_t base = s.tiles * c.heads;
     s.waves = s.rows == 16 && c.width <= 128 && base <= 256 ? 8 : 4;
+    // The workgroups that run at once: eight wavefronts a CU, as many as their
+    // registers let run (four at 256 dims).  Eight of one workgroup meet in LDS and
+    // not in the workspace, so half as many ranges are joined: 1060 keys of 256 tiles
+    // 15.4 us for 27.9, 131,072 keys of 8 38.7 for 41.5.  With more than 256 tiles
+    // every CU has its eight without it.
+    const int64_t slots = s.waves == 8 || c.width == 256 ? 256 : 512;
     const int64_t chunks = chunks_of(s.rows, false);
-    // Eight wavefronts a CU, as many as their registers let run.  Eight of one
-    // workgroup meet in LDS and not in the workspace, so half as many ranges are
-    // joined: 1060 keys of 128 (sequence, head) tiles 15.4 us for 27.9, 131,072 keys of
-    // 8 38.7 for 41.5.  With more than 256 tiles every CU has its eight without it.
-    // More ranges than that do not pay (64 sequences of 4096 to 8192 keys, 8 kv heads:
-    // 512 workgroups of four 129 us, 1024 139, 2048 146), nor a second workgroup of
-    // eight for a few CUs (240 tiles of 1000 keys 15.3 us, 480 22.7).  A wavefront of
-    // eight has two steps at least (8 tiles of 4000 keys 12.4 us, with four 16.7; 16000
-    // keys 14.3 and 17.1), of four, whose join is larger beside its work, four.
-    const int64_t want = base == 0 ? 1 : std::min<int64_t>(s.waves == 8 ? std::max<int64_t>(1, 256 / base) : (511 + base) / base, KA_SPLITS);
-    s.splits = (int)std::max<int64_t>(1, std::min(want, chunks / ((s.waves == 8 ? 2 : 4) * s.waves)));
+    // Ranges as the slots allow: a second round for some costs more than slots that
+    // stay empty (240 tiles of 1000 keys, 8 wavefronts: 14.9 us, in two ranges each
+    // 22.7; 400 of 4000 keys, 4 wavefronts: 56 and 64; 192 of 256 dims 62 and 84), but
+    // for long keys where hardly half of them are taken (304 tiles of 4000 keys: 57 and
+    // 54, of 64 dims 39 and 33; of 1000 keys 22 and 26).  A wavefront of eight has two
+    // steps at least (8 tiles of 4000 keys 12.4 us, with four 16.7; 16000 keys 14.3 and
+    // 17.1), of four, whose join is larger beside its work, four.
+    int64_t want = base ? std::max<int64_t>(1, slots / base) : 1;
+    if (s.waves == 4 && want == 1 && base * 8 < slots * 5 && chunks >= 64) want = 2;
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, KA_SPLITS), chunks / ((s.waves == 8 ? 2 : 4) * s.waves)));
 
     // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at
     // 256 dims its sums do not fit the registers.
     if (type == KV4_F32 || c.width > 128 || c.kernel == 1 || base == 0) return s;
     const int64_t steps = (chunks_of(s.rows, true) + s.splits * s.waves - 1) / (s.splits * s.waves);
     const double step = s.rows == 32 ? 1.8 : c.width == 64 ? 0.9 : 1.74;
-    const double plain = 4.0 + std::max(1.0, (double)(base * s.splits) / (s.waves == 8 ? 256.0 : 512.0)) * (4.0 + (double)steps * step) +
+    const double plain = 4.0 + std::max(1.0, (double)(base * s.splits) / (double)slots) * (4.0 + (double)steps * step) +
                          ka_join_us(c, heads, s.splits);
     KaShape p;
     p.prompt = true;
