@@ -383,7 +383,9 @@ int nh_generate_greedy(nh_session* s, int steps, uint32_t* out, float* logits, v
  * and attend read the batch from the device: captured, they follow the state
  * that a later extend of the same rows outside the graph leaves (after an extend
  * of more rows, or where the batch is over and its pages have changed hands, a
- * replay reads and writes no page, and what it leaves in `out` says nothing).  The
+ * replay reads and writes no page, and what it leaves in `out` says nothing).
+ * A captured attend keeps the split of its work that suits the lengths it was
+ * captured at: right at any length, quickest near them.  The
  * calls on one cache are queued on one stream, or ordered by the caller's
  * events.  A cache belongs to the device it was made on. */
 #define NH_F32 0

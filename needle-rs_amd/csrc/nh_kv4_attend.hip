@@ -22,8 +22,8 @@
 // keys, 8 kv heads of 128 under 32, bf16 (511 MB): 110 us, 4.65 TB/s, what a
 // large copy reaches.  A wavefront's 32 keys cost about 300 vector instructions
 // (masks, steps, exponentials) beside 19 MFMAs, 0.87 us a SIMD, so where one
-// sequence has all the keys the two are about equal: 131,072 keys (151 MB) 36 us
-// and 5 for the join.  Few keys are latency: 374 of them 7.5 us.
+// sequence has all the keys the two are about equal: 131,072 keys (151 MB, f16) 41
+// us with the join.  Few keys are latency: 374 of them 7.8 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -1086,7 +1086,7 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
     // The workgroups that run at once: eight wavefronts a CU, as many as their
     // registers let run (four at 256 dims).  Eight of one workgroup meet in LDS and
     // not in the workspace, so half as many ranges are joined: 1060 keys of 256 tiles
-    // 15.4 us for 27.9, 131,072 keys of 8 38.7 for 41.5.  With more than 256 tiles
+    // 15.4 us for 27.9, 131,072 keys of 8 38.7 for 41.5 (weights of one part).  With more than 256 tiles
     // every CU has its eight without it.
     const int64_t slots = s.waves == 8 || c.width == 256 ? 256 : 512;
     const int64_t chunks = chunks_of(s.rows, false);

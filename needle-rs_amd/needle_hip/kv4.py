@@ -181,10 +181,11 @@ class KvCache4:
         ldq = self._rows_of(q, heads, self.qk_dim, "q")
         with _on(stream):
             if out is None:
-                out = torch.empty((q.shape[0], heads, self.v_dim), dtype=q.dtype, device=self.device)
-            ldo = self._rows_of(out, heads, self.v_dim, "out")
-            if out.dtype != q.dtype:
-                raise ValueError("q and out differ in type")
+                out, ldo = torch.empty((self._rows, heads, self.v_dim), dtype=q.dtype, device=self.device), heads * self.v_dim
+            else:
+                ldo = self._rows_of(out, heads, self.v_dim, "out")
+                if out.dtype != q.dtype:
+                    raise ValueError("q and out differ in type")
             if lse is not None and (lse.dtype != torch.float32 or lse.shape != (q.shape[0], heads) or
                                     not lse.is_contiguous() or lse.get_device() != self._index):
                 raise ValueError("lse is a contiguous f32 [rows][heads]")
