@@ -1098,7 +1098,7 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
     // steps at least (8 tiles of 4000 keys 12.4 us, with four 16.7; 16000 keys 14.3 and
     // 17.1), of four, whose join is larger beside its work, four.
     int64_t want = base ? std::max<int64_t>(1, slots / base) : 1;
-    if (s.waves == 4 && want == 1 && base * 8 < slots * 5 && chunks >= 64) want = 2;
+    if (slots == 512 && want == 1 && base * 8 < slots * 5 && chunks >= 64) want = 2;  // (two workgroups share a CU)
     s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, KA_SPLITS), chunks / ((s.waves == 8 ? 2 : 4) * s.waves)));
 
     // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at
