@@ -217,6 +217,9 @@ def _row_stride(t, index, what):
     ld = sr if r > 1 else sb if b > 1 else v
     if v > 1 and sv != 1 or b > 1 and sb != ld * r:
         raise ValueError(f"the rows of {what} do not follow each other")
+    if ld < v and b * r:
+        # (one row expanded to many holds fewer elements than rows of v would)
+        raise ValueError(f"the rows of {what} repeat or overlap: make them contiguous")
     return max(ld, v)
 
 
@@ -233,7 +236,8 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor | 
     [batch], tokens [batch][n + 1]: the kept drafts, the next token, then -1),
     int32.  probs [batch][n][vocab]: the drafter's probabilities (None: it has
     none); counts [batch]: drafts of each sequence (None: n); temperature 0:
-    greedy.  Rows of logits and probs may be padded (a view of wider rows)."""
+    greedy.  Rows of logits and probs may be padded (a view of wider rows), not
+    repeated (an expanded row)."""
     if not nh._ready:
         nh.init()
     if len(logits.shape) != 3 or len(drafts.shape) != 2:
