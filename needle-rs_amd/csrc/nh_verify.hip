@@ -235,7 +235,7 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
     typedef typename Kv4Elem<PT>::T P;
     __shared__ double s_sum, ss[2][VP_WAVES];
     __shared__ float s_max;
-    __shared__ int s_kept, s_best, s_slice, s_pick, s_last, s_out;
+    __shared__ int s_kept, s_best, s_slice, s_pick, s_last, s_left, s_out;
     __shared__ double s_goal, s_part[64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
     const int b = RESIDUE ? blockIdx.x / a.nslices : blockIdx.x, mine = RESIDUE ? blockIdx.x % a.nslices : 0;
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
                 if (lane == 0) {
                     s_slice = at;
                     s_goal = goal - at_before;
-                    s_last = left;
+                    s_left = left;  // (not s_last: a wavefront may still be reading it)
                     s_pick = VR_SLICE;
                     s_best = -1;
                 }
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
             const int at = s_slice;
             if (at >= 0) {
                 // Inside the slice, a strip at a time: the threads' sums scanned.
-                left = s_last;
+                left = s_left;
                 double before = 0.0;
 #pragma unroll 1
                 for (int y = 0; y < SUB; ++y) {
