@@ -306,6 +306,7 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
     }
     __syncthreads();
     const int kept = s_kept;
+    int pick = GREEDY ? s_best : 0;
     if constexpr (!GREEDY) {
         const double sum = s_sum, scale = sum > 0.0 ? 1.0 / sum : 0.0;
         const float m = s_max;
@@ -385,7 +386,6 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
             __syncthreads();
             if (!s_last) return;
         }
-        int pick = 0;
         if (sum > 0.0) {
             bool left = refused;  // draw from what the draft left, from all of p if that is nothing
             double out_slice = 0.0;
@@ -477,12 +477,11 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
                     if (before > s_goal) break;  // (the same in every thread)
                 }
                 __syncthreads();
+                // (the same in every thread, each in a register of its own: slower wavefronts still read s_best)
                 pick = at * VR_SLICE + max(s_pick < VR_SLICE ? s_pick : s_best, 0);
             }
         }
-        s_best = pick;  // (every thread the same)
     }
-    const int pick = s_best;
     for (int i = tid; i <= n; i += VP_THREADS)
         a.tokens[row0 + i] = i < kept ? drafts[i] : i == kept ? pick : -1;
     if (tid == 0) a.accepted[b] = kept;

@@ -18,3 +18,21 @@ def test_all_drafts_kept_with_probabilities(nh, vocab):
         u[:, 2] = np.random.default_rng(vocab + k).random(24).astype(np.float32)
         kept, _ = check(nh, logits, drafts, u, q)
         assert (kept == 2).all()
+
+
+@pytest.mark.parametrize("with_probs", [False, True])
+@pytest.mark.parametrize("vocab", [300, 5000, 20000])
+def test_uniforms_past_the_whole(nh, vocab, with_probs):
+    """No cumulative weight passes the goal: the last token that weighs anything, wherever its slice begins."""
+    logits, drafts, u, q = case(vocab, 24, 1, vocab, 1.0, with_probs)
+    last = np.random.default_rng(vocab).integers(vocab // 2, vocab, 24)
+    for b in range(24):
+        logits[b, :, last[b] + 1:] = -np.inf
+        if with_probs:
+            q[b, 0, last[b]] = 0.0  # (so that it is left of the target when the draft is refused)
+    drafts[:, 0] = 0
+    u[:, 0] = np.where(np.arange(24) % 2, 0.0, 1.0)  # kept and refused in turn
+    for past in (1.0, 1.5, 4.0):
+        u[:, 1] = past
+        kept, tokens = check(nh, logits, drafts, u, q)
+        assert np.array_equal(tokens[np.arange(24), kept], last)
