@@ -474,7 +474,9 @@ int nh_kv4_debug_kernel(nh_kv4* c, int kernel);
  * All DEVICE: logits[(b (n+1) + i) ldl + t] of `type` (row n: after the last
  * draft), u f32, accepted[b] = kept drafts, tokens[b][n+1] = the kept drafts,
  * the next token, then -1.  ws: 16-byte aligned, of
- * nh_verify_drafts_ws_bytes bytes, used by the work queued on `stream` only. */
+ * nh_verify_drafts_ws_bytes bytes, used by the work queued on `stream` only.
+ * NH_EINVAL from 2^22 sequences or 2^24 slices of up to 4,096 logits of a row
+ * on: more than a launch takes. */
 int64_t nh_verify_drafts_ws_bytes(int batch, int n, int vocab);
 int nh_verify_drafts(const void* logits, int type, int64_t ldl, const int32_t* drafts, const int32_t* counts,
                      const void* probs, int probs_type, int64_t ldp, const float* u, float temperature, int batch,

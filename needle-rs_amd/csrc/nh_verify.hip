@@ -529,7 +529,8 @@ int fail(int code, const std::string& msg) {
 int check_sizes(int batch, int n, int vocab) {
     if (batch < 0 || n < 0 || n > 1024 || vocab < 1 || vocab > (1 << 30))
         return fail(NH_EINVAL, "a batch of 0 to 1024 drafts over 1 to 2^30 tokens");
-    if ((int64_t)batch * (n + 1) > (1 << 24) || (int64_t)batch * (n + 1) * nh::slices_of(vocab) > (1 << 30))
+    // (a launch takes fewer than 2^32 threads: a workgroup of 256 a slice of a row, one of 1024 a sequence)
+    if ((int64_t)batch * (n + 1) * nh::slices_of(vocab) >= (1 << 24) || batch >= (1 << 22))
         return fail(NH_EINVAL, "too many rows");
     return NH_OK;
 }

@@ -3,6 +3,7 @@ stepping a row of the vocabulary at a time, would read past the end of."""
 import pytest
 import torch
 
+import needle_hip as nh
 from needle_hip import kv4
 
 
@@ -50,8 +51,16 @@ def test_rows_that_are_taken(shape, stride, ld):
     assert kv4._row_stride(View(shape, stride), 0, "probs") == ld
 
 
+@pytest.mark.parametrize("batch,n,vocab", [(1 << 22, 0, 5), (1 << 21, 7, 5), (1 << 14, 1023, 5), (1 << 18, 1, 1 << 17)])
+def test_batches_that_no_launch_takes_are_refused(batch, n, vocab):
+    """2^32 threads and more: a workgroup of 256 for each 4,096 logits of a row, one of 1,024 for each sequence."""
+    f = nh.load_library().nh_verify_drafts_ws_bytes
+    assert f(batch, n, vocab) == -1
+    assert f(batch - 1, n, vocab) > 0
+
+
 @pytest.mark.gpu
-def test_an_expanded_row_is_refused(nh):
+def test_an_expanded_row_is_refused(nh):  # noqa: F811
     """A uniform drafter as one expanded row, and a target's row for every position."""
     b, n, v = 2, 3, 1000
     logits = torch.zeros(b, n + 1, v, device="cuda")
