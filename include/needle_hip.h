@@ -466,7 +466,7 @@ int nh_kv4_debug_kernel(nh_kv4* c, int kernel);
  * probabilities, q(x) = 1); `counts` (or NULL: n) says how many drafts of a
  * sequence there are.  The token after the kept ones is drawn at the uniform
  * u[b (n+1) + n], the first t whose cumulative weight exceeds u times the
- * whole: of max(p - q, 0) where a draft was refused (p without x when probs is
+ * whole (the last that weighs anything for u >= 1): of max(p - q, 0) where a draft was refused (p without x when probs is
  * NULL, and p itself where nothing is left), else of p.  Temperature 0: a draft is
  * kept if it is the argmax (nh_argmax), the next token is the argmax, and u may
  * be NULL.  A NaN logit is never chosen; of a row without a finite or +inf

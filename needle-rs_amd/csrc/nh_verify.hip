@@ -426,7 +426,9 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
                     }
                     if (seek) break;
                     if (before > 0.0) {
-                        goal = (double)un * before;
+                        // (no sum passes a uniform of 1: not left to the whole's last bits, which the
+                        // walk within a slice, by 64-bit weights, does not share)
+                        goal = un < 1.0f ? (double)un * before : (double)__builtin_inff();
                         seek = true;
                     } else if (left) {
                         left = false;
