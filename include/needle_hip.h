@@ -381,9 +381,11 @@ int nh_generate_greedy(nh_session* s, int steps, uint32_t* out, float* logits, v
  * works at once and reports at once (NH_ENOMEM: too few free pages or sequences;
  * a refused call changes nothing), and is refused under stream capture.  append
  * and attend read the batch from the device: captured, they follow the state
- * that a later extend of the same rows outside the graph leaves (after an extend
- * of more rows, or where the batch is over and its pages have changed hands, a
- * replay reads and writes no page, and what it leaves in `out` says nothing).
+ * that a later extend outside the graph leaves, of any sequences with the same
+ * rows one after the other (after an extend of other rows, or where the batch is
+ * over and its pages have changed hands, a replay reads and writes no page, and
+ * what it leaves in `out` says nothing).  A fork does no device work: a replay
+ * between it and the next extend writes the batch's rows, which the branch shares.
  * A captured attend keeps the split of its work that suits the lengths it was
  * captured at: right at any length, quickest near them.  The
  * calls on one cache are queued on one stream, or ordered by the caller's

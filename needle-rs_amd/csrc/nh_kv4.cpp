@@ -3,12 +3,13 @@
 // on the device.
 //
 // The mirror is an int32 array: the sequences' page ids, and the batch (its
-// sequences, their rows and lengths).  The host keeps a copy of what
+// shape, its sequences, their rows and lengths).  The host keeps a copy of what
 // it sent and sends what changed as kernel arguments, so a step of a decoding
 // loop is one small launch, no host memory has to outlive the call, and every
 // kernel after it on the stream sees the new state.  Append and attention read
 // the batch from the mirror: captured in a graph, they follow the state that
-// an extend outside the graph leaves.
+// an extend outside the graph leaves if it has the shape that they were
+// captured at, and do nothing under any other.
 #include <math.h>
 
 #include <algorithm>
@@ -33,7 +34,6 @@ struct nh_kv4 {
     size_t o_table = 0, o_batch = 0, o_fresh = 0;
     std::vector<int> sent;  // the mirror's values but the tables' and the fresh ids'
     nh::Kv4Patch patch{};   // values not sent yet
-    int entries = 0;        // batch entries that the device holds
 };
 
 namespace {
@@ -133,21 +133,28 @@ int copy_pages(nh_kv4* c, const std::vector<std::pair<int, int>>& copies, hipStr
     return NH_OK;
 }
 
-// The device's batch entries from `n` on are emptied (queued), so that a step
-// captured for them, replayed without an extend of its own, touches no page
-// that has changed hands.
-int drop_entries(nh_kv4* c, int n, hipStream_t st) {
-    for (int i = n; i < c->entries; ++i)
-        for (int k = 0; k < 4; ++k)
-            if (int rc = put_changed(c, c->o_batch + 4 * (size_t)i + k, 0, st)) return rc;
-    c->entries = std::min(c->entries, n);
-    return NH_OK;
+// The shape that the device's batch has (queued): a launch made for another
+// one, replayed from a captured step, touches no page.
+int put_shape(nh_kv4* c, int lo, int hi, hipStream_t st) {
+    if (int rc = put_changed(c, c->o_batch, lo, st)) return rc;
+    return put_changed(c, c->o_batch + 1, hi, st);
 }
 // Before pages are handed out under no batch (one that is over, or none).
 int drop_batch(nh_kv4* c, hipStream_t st) {
-    if (!c->book.batch_seq.empty() || !c->entries) return NH_OK;
-    if (int rc = drop_entries(c, 0, st)) return rc;
+    if (!c->book.batch_seq.empty()) return NH_OK;
+    if (int rc = put_shape(c, 0, 0, st)) return rc;
     return flush(c, st);
+}
+// The shape of n sequences' rows: a 64-bit FNV-1a hash, (0, 0) left out.  Two
+// shapes of one hash would share a grid, not run out of bounds: every kernel
+// checks its rows and pages besides.
+void shape_of_rows(const int* rows, int n, int* shape) {
+    uint64_t h = 0xcbf29ce484222325ull;
+    for (int i = 0; i < n; ++i)
+        for (int k = 0; k < 32; k += 8) h = (h ^ ((uint32_t)rows[i] >> k & 255u)) * 0x100000001b3ull;
+    if (!h) h = 1;
+    shape[0] = (int)(uint32_t)h;
+    shape[1] = (int)(uint32_t)(h >> 32);
 }
 
 // The batch of the last extend, as the kernels see it.
@@ -176,7 +183,7 @@ int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int p
     if (seqs < 1 || seqs > 65536) return fail(NH_EINVAL, "1 to 65536 sequences");
     if (cap < 1 || cap > (1 << 30)) return fail(NH_EINVAL, "a sequence's capacity is 1 to 2^30 positions");
     const int64_t ld = ((int64_t)cap + page - 1) / page;
-    if (ld * seqs + 4 * (int64_t)seqs + 4 + pages > (int64_t)UINT32_MAX / 4)
+    if (ld * seqs + 4 * (int64_t)seqs + 8 + pages > (int64_t)UINT32_MAX / 4)
         return fail(NH_EINVAL, "the sequences' page tables are too large");
     const int wide = std::max(qk_dim, v_dim), width = wide <= 64 ? 64 : wide <= 128 ? 128 : 256;
     if ((double)pages * page * layers * kv_heads * (width + 8 * (width / group)) > 0x1p46)
@@ -195,8 +202,8 @@ int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int p
         c->seqs = seqs;
         c->book.init(page, pages, seqs, cap);
         c->o_table = 0;
-        c->o_batch = ((size_t)ld * seqs + 3) / 4 * 4;  // (an entry is one 16-byte load)
-        c->o_fresh = c->o_batch + 4 * (size_t)seqs;
+        c->o_batch = ((size_t)ld * seqs + 3) / 4 * 4;  // the shape, then the entries, 16 bytes each
+        c->o_fresh = c->o_batch + 4 + 4 * (size_t)seqs;
         c->n_state = c->o_fresh + pages;
         c->sent.assign(c->o_fresh - c->o_batch, 0);
         const size_t bytes = (size_t)pages * v.page_bytes();
@@ -213,7 +220,7 @@ int nh_kv4_new(int layers, int kv_heads, int qk_dim, int v_dim, int group, int p
         }
         v.data = c->data;
         v.table = c->state + c->o_table;
-        v.batch = c->state + c->o_batch;
+        v.batch = c->state + c->o_batch + 4;
         *h = c.release();
         return NH_OK;
     });
@@ -309,11 +316,7 @@ int nh_kv4_seq_compact(nh_kv4* c, const int* seqs, int n, const int* counts, con
         if (int rc = c->book.compact(seqs, n, counts, ranges, &p)) return refused(c, rc);
         // The sources' tables and the fresh pages' ids, then the moves.
         std::vector<int> at(n, 0);
-        // (a sequence of the batch that gets shorter ends it)
-        bool over = c->book.batch_seq.empty();
-        for (int i = 0; i < n; ++i)
-            for (int b : c->book.batch_seq) over |= b == seqs[i] && c->book.seqs[seqs[i]].len != p.len[i];
-        int rc = over ? drop_entries(c, 0, st) : NH_OK, fresh = 0;
+        int rc = NH_OK, fresh = 0;
         for (int i = 0; i < n && !rc; ++i) {
             at[i] = fresh;
             if (p.fresh[i].empty()) continue;
@@ -344,7 +347,7 @@ int nh_kv4_seq_compact(nh_kv4* c, const int* seqs, int n, const int* counts, con
             return rc;
         }
         c->book.compacted(seqs, n, p);
-        return NH_OK;
+        return drop_batch(c, st);  // (over already, or by a sequence of it that got shorter)
     });
 }
 
@@ -363,15 +366,15 @@ int nh_kv4_extend(nh_kv4* c, const int* seqs, const int* rows, int n, void* stre
         c->v.nb = n;
         c->v.rows = row0.back();
         c->v.each = n ? rows[0] : 0;
+        shape_of_rows(rows, n, c->v.shape);
+        if (int rc = put_shape(c, c->v.shape[0], c->v.shape[1], st)) return rc;
         for (int i = 0; i < n; ++i) {
             if (int rc = sync_table(c, seqs[i], st)) return rc;
             const int entry[4] = {seqs[i], row0[i], row0[i + 1], c->book.seqs[seqs[i]].len};
             for (int k = 0; k < 4; ++k)
-                if (int rc = put_changed(c, c->o_batch + 4 * (size_t)i + k, entry[k], st)) return rc;
+                if (int rc = put_changed(c, c->o_batch + 4 + 4 * (size_t)i + k, entry[k], st)) return rc;
             if (rows[i] != rows[0]) c->v.each = 0;
         }
-        if (int rc = drop_entries(c, n, st)) return rc;
-        c->entries = n;
         return flush(c, st);
     });
 }

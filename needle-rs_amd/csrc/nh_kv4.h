@@ -46,9 +46,10 @@ struct Kv4Entry {
 struct Kv4View {
     uint8_t* data;       // [pages][layers][heads] blocks
     const int* table;    // [seqs][table_ld] page ids
-    const int* batch;    // [nb] of (sequence, first row, end row, length): Kv4Entry
+    const int* batch;    // [nb] of (sequence, first row, end row, length): Kv4Entry; its shape 4 words before
     int table_ld, pages, layers, heads, dk, dv, width, group, page_log2;
     int nb, rows, each;  // the batch; each: rows of every sequence when they are equal, else 0
+    int shape[2];        // names the sequences' numbers of rows, in order; (0, 0): no batch
     int kernel;          // nh_kv4_debug_kernel
     __host__ __device__ int page() const { return 1 << page_log2; }
     __host__ __device__ int groups() const { return width / group; }

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
     const Kv4Entry entry = kv4_batch(c, b);
     const int row0 = entry.row0, nrows = entry.row1 - row0, seq = entry.seq;
     const int first = entry.len - nrows, r0 = tile * 16 * RT;
-    if (first < 0 || r0 >= nrows * per || entry.row1 > c.rows) return;  // (a state that no extend of this shape leaves)
+    if (!kv4_current(c) || first < 0 || r0 >= nrows * per || entry.row1 > c.rows) return;
     const int r1 = min(r0 + 16 * RT, nrows * per) - 1;
     const int plo = first + r0 / per, phi = first + r1 / per;
 
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
     if (b >= c.nb) return;
     const Kv4Entry entry = kv4_batch(c, b);
     const int row0 = entry.row0, nrows = entry.row1 - row0, first = entry.len - nrows, r0 = tile * KP_ROWS;
-    if (first < 0 || r0 >= nrows * per || entry.row1 > c.rows) return;
+    if (!kv4_current(c) || first < 0 || r0 >= nrows * per || entry.row1 > c.rows) return;
     const int r1 = min(r0 + KP_ROWS, nrows * per) - 1;
     const int plo = first + r0 / per, phi = first + r1 / per;
     const int w0 = min(r0 + wave * 32, r1), w1 = min(w0 + 31, r1);  // this wavefront's rows

@@ -93,6 +93,13 @@ __device__ __forceinline__ int kv4_find(const Kv4View& c, int& unit, int lane, F
     unit = __builtin_amdgcn_readfirstlane(unit);
     return __builtin_amdgcn_readfirstlane(b);
 }
+// The batch on the device is of the rows that this launch was made for: not so
+// where a captured launch is replayed after an extend of other rows, or when
+// the batch is over, whose grid and plan fit nothing that is there.
+__device__ __forceinline__ bool kv4_current(const Kv4View& c) {
+    const int2 s = *reinterpret_cast<const int2*>(c.batch - 4);
+    return s.x == c.shape[0] && s.y == c.shape[1];
+}
 __device__ __forceinline__ Kv4Entry kv4_batch(const Kv4View& c, int b) {
     const int4 e = reinterpret_cast<const int4*>(c.batch)[b];
     return Kv4Entry{e.x, e.y, e.z, e.w};

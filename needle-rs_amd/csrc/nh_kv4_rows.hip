@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4View c, int layer, const 
     const Kv4Entry e = kv4_batch(c, b);
     const int first = e.len - (e.row1 - e.row0);  // the position of row row0
     const int pos0 = ((first >> 5) + unit) << 5, lo = max(first - pos0, 0), hi = min(e.len - 1 - pos0, 31);
-    if (first < 0 || lo > hi || e.row1 > c.rows) return;  // (a captured append after an extend of other rows)
+    if (!kv4_current(c) || first < 0 || lo > hi || e.row1 > c.rows) return;
     const int pg = kv4_page(c, e.seq, pos0);
     if (pg < 0) return;
 #pragma unroll 1
