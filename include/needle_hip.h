@@ -447,9 +447,11 @@ int nh_kv4_read(nh_kv4* c, int layer, const int* seqs, const int* pos, const int
  * (Session::attend's span, crates/needle-engine/src/model.rs:62-66, by
  * position).  lse (f32 [rows][heads], or NULL): the log of the summed
  * exponentials, to join with other keys.  Scores, weights' sums and products
- * are held in f32; f32 and f16 calls carry 22 bits of a weight, bf16 calls 11
- * (f16 and bf16 calls of many rows 11 of it and of a key's and a value's step x
- * code).  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used by
+ * are held in f32; f32 and f16 calls carry 22 bits of a weight x its value's
+ * step, bf16 calls 11, none finer than 2^-40 of the largest step.  f16 and bf16
+ * calls of many rows carry 11 of the weight and of a key's and a value's step x
+ * code, none finer than 2^-26 of the largest step among the keys up to the rows
+ * (so steps down to 2^-20 of that have all 11).  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used by
  * the work queued on `stream` only (its size depends on the batch's lengths:
  * asked after the extend; 0: it may be NULL). */
 int64_t nh_kv4_attend_ws_bytes(const nh_kv4* c, int heads, int sink, int ring);

@@ -512,11 +512,18 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
 // ------------------------------------------------------------------ prompts
 // Many rows: a workgroup of eight wavefronts takes 256 rows, 32 a wavefront, and
 // the chunks' codes are turned into f16 operands once for all of them, through
-// LDS, two chunks in turn.  Keys and values are kept as step x code there, in
-// units of a power of two above the largest step (one more AND-and-multiply for
-// two codes; rounded to 11 bits), their lows go through the same small products
-// as above, so the rounding is relative to a group's range and not to its
-// offset.  32 x 32 MFMAs: a lane holds 16 scores of its row, the other half of
+// LDS, two chunks in turn.  Keys and values are kept as step x code there,
+// rounded to 11 bits, their lows go through the same small products as above, so
+// the rounding is relative to a group's range and not to its offset.  A code
+// under a mask and 0x6400 is the f16 number 1024 + c; one fused multiply-add
+// with the step and -1024 steps leaves step x code, for two codes at a time (an
+// AND-OR and the multiply-add).  Steps are in units of a power of two over
+// the largest step of the range (below 2^6 of them, so that 1024 steps and 240
+// steps are f16 numbers): those down to 2^-20 of it keep their 11 bits, smaller
+// ones are good to 2^-27 of it a dim.  (Codes as subnormals times steps, as they
+// were, lost bits from 2^-5 of the largest step on: a row 10,000 times the others
+// took 5 % off every result that did not see it.)
+// 32 x 32 MFMAs: a lane holds 16 scores of its row, the other half of
 // them is 32 lanes away.  The weights' sum is one more row of the lows' product.
 //
 // Two sequences' 2,000 rows after 6,000 keys, 32 heads over 8 of 128, bf16 (427
@@ -583,10 +590,12 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
         return layer + ((unsigned)pg < (unsigned)c.pages ? pg : 0) * page_bytes + (uint32_t)(slot >> 5) * L::CHUNK;
     };
 
-    // The references: powers of two above every step of the keys (and values)
+    // The references: powers of two, 2^ref above every step of the keys (and values)
     // of this range, and whether a value is NaN.  One look at the steps ahead of
-    // the loop: inside it they took a third of the instructions.
-    int kref, vref;
+    // the loop: inside it they took a third of the instructions.  The operands' units are
+    // 2^unit: 64 steps of the largest's size, fewer where the format's smallest
+    // step, 2^-24, keeps its bits without (so that the queries' sums fit, below).
+    int kunit, vunit;
     bool nan;
     {
         const uint32_t x2 = 2 * (lane & (16 * NG - 1));  // two steps a lane
@@ -635,15 +644,20 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
             top[1] = max(top[1], st[1][w]);
             bads |= sbad[w];
         }
-        kref = __builtin_amdgcn_readfirstlane((int)(top[0] >> 10)) - 14;
-        vref = __builtin_amdgcn_readfirstlane((int)(top[1] >> 10)) - 14;
+        const int kref = __builtin_amdgcn_readfirstlane((int)(top[0] >> 10)) - 14;
+        const int vref = __builtin_amdgcn_readfirstlane((int)(top[1] >> 10)) - 14;
+        kunit = max(kref - 6, -10);
+        vunit = max(vref - 6, -10);
         nan = __builtin_amdgcn_readfirstlane(bads) != 0;
     }
-    const float kmul = pow2i(14 - kref), vmul = pow2i(14 - vref);
+    const float kmul = pow2i(-kunit), vmul = pow2i(-vunit);
 
-    // The queries, scaled to just under 2^5, and their sums in units that make the
+    // The queries, scaled to just under 2^a, and their sums in units that make the
     // lows' product another term of the scores' own accumulator: scores are z cz,
-    // z = up (q . step c) 2^(-10 - ref) + low (up sum q 2^(-10 - ref)).
+    // z = up (q . step c) 2^-unit + low (up sum q 2^-unit).  The sum of 64 is just under
+    // 2^(a + 6 - unit): a takes it to 2^15, so that its two f16 parts hold 22 bits of it,
+    // and is -1 at least (unit >= -10), where elements down to 2^-8 of the row's largest
+    // keep 11 bits (smaller ones are good to 2^-20 of it).
     h8 q[NX], qs = {};
     float cz;
     {
@@ -668,19 +682,20 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
         }
         most = halves_max(most);
         const int ef = max((int)(__builtin_bit_cast(uint32_t, most) >> 23 & 255u), 15);
-        const float up = __builtin_bit_cast(float, (uint32_t)(258 - ef) << 23);
-        cz = (a.scale * KA_LOG2E) * pow2i(10 + kref) * __builtin_bit_cast(float, (uint32_t)(ef - 4) << 23);
+        const int size = min(9 + kunit, 15);  // (a)
+        const int up = size + 126 - ef;
+        cz = __builtin_amdgcn_ldexpf(a.scale * KA_LOG2E, kunit - up);
 #pragma unroll
         for (int j = 0; j < NX; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float y = (float)x[j][e] * up;
+                const float y = __builtin_amdgcn_ldexpf((float)x[j][e], up);
                 sums[j * 16 / G] += y;
                 q[j][e] = (_Float16)(y * (e & 2 ? 0.0625f : 1.0f));
             }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const float s = (sums[g] + __shfl_xor(sums[g], 32, 64)) * pow2i(-10 - kref);
+            const float s = (sums[g] + __shfl_xor(sums[g], 32, 64)) * pow2i(-kunit);
             const _Float16 hi = (_Float16)s, lo = (_Float16)(s - (float)hi);
             qs[g] = half == 0 ? hi : lo;
         }
@@ -725,19 +740,19 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
             }
         }
     };
-    // Codes under a mask times scaled steps: c 2^-24 x step 2^(14 - ref) (16 times
-    // that under the upper mask), two at a time.
-    auto times = [](uint32_t codes, uint32_t steps) {
-        const h2 y = __builtin_bit_cast(h2, codes) * __builtin_bit_cast(h2, steps);
+    // Codes under a mask times scaled steps s (16 c s under the upper mask), two at a
+    // time: (1024 + c) s - 1024 s, rounded once.
+    auto times = [](uint32_t codes, h2 steps) {
+        const h2 y = __builtin_elementwise_fma(__builtin_bit_cast(h2, codes | 0x64006400u), steps, steps * (_Float16)-1024.0f);
         return __builtin_bit_cast(uint32_t, y);
     };
     auto unpack = [&](const Raw& x, int i, Image& to) {
         const int key0 = span.at(i) * KA_CHUNK;
         if (does_k) {
             float s = f16_value(x.ks) * kmul;
-            s = s > 65504.0f ? 65504.0f : s;  // (a hidden key's; NaN stays, a key's reader has to see it)
-            const h2 s2 = {(_Float16)s, (_Float16)s};
-            const uint32_t sw = __builtin_bit_cast(uint32_t, s2), w = x.k, z = w >> 8;
+            s = s > 63.96875f ? 63.96875f : s;  // (a hidden key's; NaN stays, a key's reader has to see it)
+            const h2 sw = {(_Float16)s, (_Float16)s};
+            const uint32_t w = x.k, z = w >> 8;
             const u32x4 y = {times(w & 0x000f000fu, sw), times(w & 0x00f000f0u, sw), times(z & 0x000f000fu, sw),
                              times(z & 0x00f000f0u, sw)};
             to.k[2 * kj + (kg >> 1)][(kg & 1) * 32 + 16 * kt + o] = y;
@@ -751,11 +766,11 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
 #pragma unroll
                 for (int t = 0; t < 4; ++t) s[t] = key0 + 16 * vt + 4 * kg + t <= phi && s[t] == s[t] ? s[t] : 0.0f;
             }
-            uint32_t sw[2];
+            h2 sw[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const f32x2 y = {s[2 * t], s[2 * t + 1]};
-                sw[t] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, h2));
+                sw[t] = __builtin_convertvector(y, h2);
             }
             const uint32_t w0 = vi ? x.v[0] >> 8 : x.v[0], w1 = vi ? x.v[1] >> 8 : x.v[1];
             const uint2 even = {times(w0 & 0x000f000fu, sw[0]), times(w1 & 0x000f000fu, sw[1])};
@@ -895,7 +910,7 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
     // Row `m32` of the lows' product is in reg m % 4 + 4 (m / 8) of half m / 4 % 2.
     const float l = __shfl(accl[4], m32, 64);  // m = 8
     if (l != l) m = l;
-    const float unit = pow2i(10 + vref);
+    const float unit = pow2i(vunit);
     if (r0 + wave * 32 + m32 > r1) return;
     const int64_t row = row0 + token, head = kvh * per + r - token * per;
     const bool last = plan.splits == 1;
