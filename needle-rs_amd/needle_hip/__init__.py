@@ -653,21 +653,20 @@ class Session:
             raise ValueError("a session rolls back at most 32 drafts")
         if len(self) + n + 1 > self.cap:
             raise ValueError("the drafts and the next token do not fit the session's capacity")
-        # (all that the check could refuse, before anything is fed)
-        if not 0.0 <= temperature < float("inf") or temperature > 0.0 and u is None:
-            raise NeedleHipError(-1, "a temperature is 0 (greedy), or positive with uniforms")
         with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream()):
             target = torch.empty((1, n + 1, width), dtype=torch.float32, device="cuda")
             x = torch.from_numpy(toks.view(np.int32)).cuda().view(1, n)
             if u is not None:
-                u = torch.as_tensor(u, dtype=torch.float32).to(target.device).reshape(1, n + 1)
+                u = torch.as_tensor(u, dtype=torch.float32).to(target.device).reshape(1, n + 1).contiguous()
             if probs is not None:
                 probs = probs.reshape(1, n, width)
+            # (all that the check could refuse, before anything is fed)
+            check = _DraftCheck(target, x, u, probs, temperature=temperature)
             _check(_lib.nh_forward(self.h, _hptr(toks), 0, _dptr(target), _stream()))
             if n:
                 _check(_lib.nh_forward_outputs(self.h, _hptr(toks), n, OUT_ALL_LOGITS, target[0, 1].data_ptr(), n * width,
                                                _stream()))
-            tokens = verify_drafts(target, x, u, probs=probs, temperature=temperature)[1]
+            tokens = check.run()[1]
             new = [t for t in tokens[0].tolist() if t >= 0]
             self.rollback(n + 1 - len(new))
             self.forward(new[-1:])
@@ -743,4 +742,4 @@ def seeded_normals(sizes, seed: int = 0):
     return outs
 
 
-from .kv4 import KvCache4, verify_drafts  # noqa: E402,F401
+from .kv4 import KvCache4, _DraftCheck, verify_drafts  # noqa: E402,F401

@@ -228,6 +228,49 @@ def _plain(t, dtype, shape, index, what):
         raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on the logits' device")
 
 
+class _DraftCheck:
+    """One check of drafts, its arguments looked over and its outputs and
+    workspace there; `run` queues it on the current stream.  What can be refused
+    is refused here, so that a session is fed after it."""
+
+    def __init__(self, logits, drafts, u=None, probs=None, counts=None, temperature=1.0):
+        if not nh._ready:
+            nh.init()
+        if len(logits.shape) != 3 or len(drafts.shape) != 2:
+            raise ValueError("logits are [batch][n + 1][vocab], drafts [batch][n]")
+        batch, rows, vocab = logits.shape
+        n, index = rows - 1, logits.get_device()
+        ldl, ldp = _row_stride(logits, index, "logits"), 0
+        _plain(drafts, torch.int32, (batch, n), index, "drafts")
+        if u is not None:
+            _plain(u, torch.float32, (batch, n + 1), index, "u")
+        if counts is not None:
+            _plain(counts, torch.int32, (batch,), index, "counts")
+        if probs is not None:
+            if probs.shape != (batch, n, vocab):
+                raise ValueError("probs are [batch][n][vocab]")
+            ldp = _row_stride(probs, index, "probs") if batch * n else vocab
+        if index != torch.cuda.current_device():
+            raise ValueError("the tensors are on another device than the current one")
+        temperature = C.c_float(float(temperature)).value  # (as the entry takes it)
+        if not 0.0 <= temperature < float("inf") or temperature > 0.0 and u is None:
+            raise nh.NeedleHipError(-1, "a temperature is 0 (greedy), or positive with uniforms")
+        ws_bytes = nh._lib.nh_verify_drafts_ws_bytes(batch, n, vocab)
+        if ws_bytes < 0:
+            nh._check(int(ws_bytes))
+        self.accepted = torch.empty(batch, dtype=torch.int32, device=logits.device)
+        self.tokens = torch.empty((batch, n + 1), dtype=torch.int32, device=logits.device)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
+        self._held = (logits, drafts, counts, probs, u, ws)
+        self._args = (logits.data_ptr(), _TYPES[logits.dtype], ldl, _ptr(drafts), _ptr(counts), _ptr(probs),
+                      _TYPES[probs.dtype] if probs is not None else 0, ldp, _ptr(u), temperature, batch, n, vocab,
+                      self.accepted.data_ptr(), self.tokens.data_ptr(), _ptr(ws), ws_bytes)
+
+    def run(self):
+        nh._check(nh._lib.nh_verify_drafts(*self._args, nh._stream()))
+        return self.accepted, self.tokens
+
+
 def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor | None = None,
                   probs: torch.Tensor | None = None, counts: torch.Tensor | None = None, temperature: float = 1.0,
                   stream=None):
@@ -238,34 +281,5 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor | 
     none); counts [batch]: drafts of each sequence (None: n); temperature 0:
     greedy.  Rows of logits and probs may be padded (a view of wider rows), not
     repeated (an expanded row)."""
-    if not nh._ready:
-        nh.init()
-    if len(logits.shape) != 3 or len(drafts.shape) != 2:
-        raise ValueError("logits are [batch][n + 1][vocab], drafts [batch][n]")
-    batch, rows, vocab = logits.shape
-    n, index = rows - 1, logits.get_device()
-
-    ldl, ldp = _row_stride(logits, index, "logits"), 0
-    _plain(drafts, torch.int32, (batch, n), index, "drafts")
-    if u is not None:
-        _plain(u, torch.float32, (batch, n + 1), index, "u")
-    if counts is not None:
-        _plain(counts, torch.int32, (batch,), index, "counts")
-    if probs is not None:
-        if probs.shape != (batch, n, vocab):
-            raise ValueError("probs are [batch][n][vocab]")
-        ldp = _row_stride(probs, index, "probs") if probs.numel() else vocab
-    if index != torch.cuda.current_device():
-        raise ValueError("the tensors are on another device than the current one")
-    ws_bytes = nh._lib.nh_verify_drafts_ws_bytes(batch, n, vocab)
-    if ws_bytes < 0:
-        nh._check(int(ws_bytes))
     with _on(stream):
-        accepted = torch.empty(batch, dtype=torch.int32, device=logits.device)
-        tokens = torch.empty((batch, n + 1), dtype=torch.int32, device=logits.device)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
-    nh._check(nh._lib.nh_verify_drafts(logits.data_ptr(), _TYPES[logits.dtype], ldl, _ptr(drafts), _ptr(counts),
-                                       _ptr(probs), _TYPES[probs.dtype] if probs is not None else 0, ldp, _ptr(u),
-                                       float(temperature), batch, n, vocab, accepted.data_ptr(), tokens.data_ptr(),
-                                       _ptr(ws), ws_bytes, nh._stream(stream)))
-    return accepted, tokens
+        return _DraftCheck(logits, drafts, u, probs, counts, temperature).run()
