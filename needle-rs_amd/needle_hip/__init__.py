@@ -510,6 +510,7 @@ class Session:
 
     def __init__(self, model: Model, cap: int, handle=None):
         self.model = model
+        self._span = None  # (sink, ring) of set_attend
         if handle is None:
             h = C.c_void_p()
             _check(_lib.nh_session_new(model.h, int(cap), C.byref(h)))
@@ -522,6 +523,7 @@ class Session:
 
     def reset(self):
         _check(_lib.nh_session_reset(self.h))
+        self._span = None
 
     def _width(self, outputs):
         return self.model.d_model if outputs in (OUT_HIDDEN, OUT_LAST_HIDDEN) else self.model.out_rows
@@ -586,11 +588,14 @@ class Session:
         """Session::clone (model.rs:53-55)."""
         h = C.c_void_p()
         _check(_lib.nh_session_clone(self.h, _stream(stream), C.byref(h)))
-        return Session(self.model, self.cap, handle=h.value)
+        made = Session(self.model, self.cap, handle=h.value)
+        made._span = self._span
+        return made
 
     def set_attend(self, sink: int, ring: int):
         """Session::attend = Some((sink, ring)) (model.rs:62-66); ring 0: None."""
         _check(_lib.nh_session_set_attend(self.h, int(sink), int(ring)))
+        self._span = (int(sink), int(ring)) if ring > 0 else None
 
     def debug_spin_limit(self, limit: int):
         """Test hook: the polls a bounded in-kernel wait makes before giving up."""
@@ -645,8 +650,10 @@ class Session:
         (the kept drafts and the next one), all of them in the session, whose
         logits are those after the last.  The drafts' rows take the prefill
         combine, a step the decode combine, so a near tie may be picked
-        otherwise than by steps.  Under a span a refused draft has taken the KV
-        slot of the position a ring before it, as any rolled back position has."""
+        otherwise than by steps.  Under a span that the drafts reach the end of, a
+        refused one would have taken the KV slot of a position that later queries
+        still see: there the drafts are fed to a clone, and the kept ones to the
+        session, as if nothing else had been."""
         toks = np.ascontiguousarray(np.asarray(drafts, dtype=np.uint32).reshape(-1))
         n, width = toks.size, self.model.out_rows
         if n > 32:
@@ -663,12 +670,18 @@ class Session:
             # (all that the check could refuse, before anything is fed)
             check = _DraftCheck(target, x, u, probs, temperature=temperature)
             _check(_lib.nh_forward(self.h, _hptr(toks), 0, _dptr(target), _stream()))
+            # (positions below sink + ring have slots of their own; a single draft's slot is the next token's)
+            apart = n > 1 and self._span is not None and len(self) + n > sum(self._span)
+            fed = self.clone() if apart else self
             if n:
-                _check(_lib.nh_forward_outputs(self.h, _hptr(toks), n, OUT_ALL_LOGITS, target[0, 1].data_ptr(), n * width,
+                _check(_lib.nh_forward_outputs(fed.h, _hptr(toks), n, OUT_ALL_LOGITS, target[0, 1].data_ptr(), n * width,
                                                _stream()))
             tokens = check.run()[1]
             new = [t for t in tokens[0].tolist() if t >= 0]
-            self.rollback(n + 1 - len(new))
+            if not apart:
+                self.rollback(n + 1 - len(new))
+            elif len(new) > 1:
+                self.forward(new[:-1], OUT_NONE)
             self.forward(new[-1:])
         return new
 

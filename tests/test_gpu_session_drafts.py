@@ -69,3 +69,56 @@ def test_session_drafts_with_probabilities(nh, other_stream, sure):
         kept_all += kept
         refused += n - kept
     assert kept_all > 3 and (refused > 3) == sure
+
+
+@pytest.mark.parametrize("sink,ring,fed", [(6, 40, 100), (0, 33, 40), (10, 64, 50), (118, 256, 60)])
+def test_refused_drafts_under_a_span_leave_no_trace(nh, sink, ring, fed):
+    """Drafts that are all refused, before and after the ring is full: the session goes on bit by bit as one that was
+    only ever fed the picked tokens, one at a time."""
+    rng = np.random.default_rng(9)
+    m = nh.Model.from_archive(archive(85))
+    s = m.session(256)
+    s.set_attend(sink, ring)
+    s.forward(o.random_tokens(fed, 300, seed=86))
+    plain = s.clone()
+    for step in range(16):
+        best = int(plain.forward([]).argmax())
+        n = int(rng.integers(1, 21))
+        drafts = rng.integers(0, 300, n)
+        drafts[0] = (best + 1 + int(rng.integers(0, 298))) % 300
+        assert s.verify_drafts(drafts) == [best]
+        plain.forward([best])
+        assert torch.equal(s.forward([]), plain.forward([])), step
+    assert len(s) == len(plain) == fed + 16
+
+
+def test_kept_drafts_under_a_span(nh):
+    """Some kept, some refused, by greedy picks: each step as a clone that is fed the kept drafts and the next token."""
+    rng = np.random.default_rng(10)
+    m = nh.Model.from_archive(archive(87))
+    s = m.session(256)
+    s.set_attend(5, 48)
+    s.forward(o.random_tokens(70, 300, seed=88))
+    kept_all = 0
+    for step in range(12):
+        n = int(rng.integers(1, 9))
+        c, like = s.clone(), s.clone()
+        drafts = s.clone().generate_greedy(n)[0].astype(np.int64)
+        if n > 2:
+            drafts[int(rng.integers(1, n))] = int(rng.integers(0, 300))
+        first = c.forward([]).cpu().numpy()
+        rows = c.forward(drafts, nh.OUT_ALL_LOGITS).cpu().numpy()
+        accepted, tokens = ref.verify(np.concatenate((first[None], rows))[None], drafts[None].astype(np.int32), None,
+                                      temperature=0.0)
+        want = tokens[0, :int(accepted[0]) + 1].tolist()
+        assert s.verify_drafts(drafts) == want
+        if n == 1:  # its slot is the next token's, so it is fed in place, and kept as it was fed
+            like.forward(drafts, nh.OUT_ALL_LOGITS)
+            like.rollback(2 - len(want))
+        elif len(want) > 1:
+            like.forward(want[:-1], nh.OUT_NONE)
+        like.forward(want[-1:])
+        assert len(s) == len(like)
+        assert torch.equal(s.forward([]), like.forward([])), step
+        kept_all += len(want) - 1
+    assert kept_all > 5
