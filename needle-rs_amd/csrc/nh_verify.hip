@@ -191,7 +191,9 @@ __global__ __launch_bounds__(VR_THREADS) void k_verify_rows(VerifyArgs a) {
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < VR_WAVES; ++w) m = fmaxf(m, sv[w]);
-        const float ch = (float)a.c, cl = ch < __builtin_inff() ? (float)(a.c - (double)ch) : 0.0f;
+        // (a temperature below 2^-127 has a factor past f32: held at its end, so that the maximum's 0 times it is 0)
+        constexpr float END = 3.402823466e38f;
+        const float ch = a.c < (double)END ? (float)a.c : END, cl = ch < END ? (float)(a.c - (double)ch) : 0.0f;
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < VR_EACH; ++k) {

@@ -36,3 +36,14 @@ def test_uniforms_past_the_whole(nh, vocab, with_probs):
         u[:, 1] = past
         kept, tokens = check(nh, logits, drafts, u, q)
         assert np.array_equal(tokens[np.arange(24), kept], last)
+
+
+@pytest.mark.parametrize("with_probs", [False, True])
+@pytest.mark.parametrize("temperature", [1e-45, 1e-40, 4e-39, 5e-39, 1e-20, 1e30, 3e38])
+def test_temperatures_of_any_size(nh, temperature, with_probs):
+    """From the smallest f32 to its end: next to greedy, then next to even."""
+    logits, drafts, u, q = case(11, 6, 3, 5000, 1.0, with_probs)
+    drafts[::2] = logits[::2, :3].argmax(-1)
+    kept, tokens = check(nh, logits, drafts, u, q, temperature=float(np.float32(temperature)))
+    if temperature < 1:
+        assert (kept[::2] == 3).all() and np.array_equal(tokens[::2, 3], logits[::2, 3].argmax(-1))
