@@ -741,9 +741,12 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
         }
     };
     // Codes under a mask times scaled steps s (16 c s under the upper mask), two at a
-    // time: (1024 + c) s - 1024 s, rounded once.
-    auto times = [](uint32_t codes, h2 steps) {
-        const h2 y = __builtin_elementwise_fma(__builtin_bit_cast(h2, codes | 0x64006400u), steps, steps * (_Float16)-1024.0f);
+    // time: (1024 + c) s - 1024 s, rounded once.  (Two literals do not fit an
+    // AND-OR: the second one stays in a register, which the empty asm keeps it in.)
+    uint32_t k1024 = 0x64006400u;
+    asm("" : "+v"(k1024));
+    auto times = [&](uint32_t codes, h2 steps) {
+        const h2 y = __builtin_elementwise_fma(__builtin_bit_cast(h2, codes | k1024), steps, steps * (_Float16)-1024.0f);
         return __builtin_bit_cast(uint32_t, y);
     };
     auto unpack = [&](const Raw& x, int i, Image& to) {
