@@ -451,7 +451,7 @@ int nh_kv4_read(nh_kv4* c, int layer, const int* seqs, const int* pos, const int
  * step, bf16 calls 11, none finer than 2^-40 of the largest step.  f16 and bf16
  * calls of many rows carry 11 of the weight and of a key's and a value's step x
  * code, none finer than 2^-26 of the largest step among the keys up to the rows
- * (so steps down to 2^-20 of that have all 11).  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used by
+ * (so steps down to 2^-19 of that have all 11).  DEVICE ws, 16-byte aligned, of nh_kv4_attend_ws_bytes bytes, used by
  * the work queued on `stream` only (its size depends on the batch's lengths:
  * asked after the extend; 0: it may be NULL). */
 int64_t nh_kv4_attend_ws_bytes(const nh_kv4* c, int heads, int sink, int ring);
@@ -470,11 +470,13 @@ int nh_kv4_debug_kernel(nh_kv4* c, int kernel);
  * probabilities, q(x) = 1); `counts` (or NULL: n) says how many drafts of a
  * sequence there are.  The token after the kept ones is drawn at the uniform
  * u[b (n+1) + n], the first t whose cumulative weight exceeds u times the
- * whole (the last that weighs anything for u >= 1): of max(p - q, 0) where a draft was refused (p without x when probs is
- * NULL, and p itself where nothing is left), else of p.  Temperature 0: a draft is
- * kept if it is the argmax (nh_argmax), the next token is the argmax, and u may
- * be NULL.  A NaN logit is never chosen; of a row without a finite or +inf
- * logit token 0 is taken; a draft outside the vocabulary is refused.
+ * whole (the last that weighs anything for u >= 1): of max(p - q, 0) where a
+ * draft was refused (p without x when probs is NULL, and p itself where nothing
+ * is left), else of p.  Temperature 0: a draft is kept if it is the argmax
+ * (nh_argmax), the next token is the argmax, and u may be NULL.  A NaN logit is
+ * never chosen, but as a greedy row's first one (a NaN x[0] gives 0 there, as
+ * nh_argmax has it); of a row without a finite or +inf logit token 0 is taken; a
+ * draft outside the vocabulary is refused.
  * All DEVICE: logits[(b (n+1) + i) ldl + t] of `type` (row n: after the last
  * draft), u f32, accepted[b] = kept drafts, tokens[b][n+1] = the kept drafts,
  * the next token, then -1.  ws: 16-byte aligned, of

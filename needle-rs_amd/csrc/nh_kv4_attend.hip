@@ -517,20 +517,20 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
 // the rounding is relative to a group's range and not to its offset.  A code
 // under a mask and 0x6400 is the f16 number 1024 + c; one fused multiply-add
 // with the step and -1024 steps leaves step x code, for two codes at a time (an
-// AND-OR and the multiply-add).  Steps are in units of a power of two over
-// the largest step of the range (below 2^6 of them, so that 1024 steps and 240
-// steps are f16 numbers): those down to 2^-20 of it keep their 11 bits, smaller
-// ones are good to 2^-27 of it a dim.  (Codes as subnormals times steps, as they
-// were, lost bits from 2^-5 of the largest step on: a row 10,000 times the others
-// took 5 % off every result that did not see it.)
+// AND-OR and the multiply-add).  The power of two over the largest step of the
+// range is 2^6 there, so that 1024 steps and 240 steps are f16 numbers: steps down
+// to 2^-20 of that power keep their 11 bits, smaller ones leave step x code good
+// to 2^-27 of it.  (Codes as subnormals times steps lose bits from 2^-5 on: a row
+// 10,000 times the others took 5 % off every result that did not see it, for 1 %
+// of the time.)
 // 32 x 32 MFMAs: a lane holds 16 scores of its row, the other half of
 // them is 32 lanes away.  The weights' sum is one more row of the lows' product.
 //
 // Two sequences' 2,000 rows after 6,000 keys, 32 heads over 8 of 128, bf16 (427
-// GFLOP): 570 us, 750 TFLOP/s; the kernel above takes 1,450, an operand's masks,
-// steps and lows serving 16 rows there and 256 here.  A large library product
-// runs at 1,130 to 1,180.  The matrix cores are busy 37 % of the time, the vector
-// units (exponentials, maxima, weights to f16) 42 %, one wavefront's chain of
+// GFLOP): 573 us, 745 TFLOP/s (up to 584 by card); the kernel above takes 1,450,
+// an operand's masks, steps and lows serving 16 rows there and 256 here.  A large
+// library product runs at 1,130 to 1,180.  The matrix cores are busy 37 % of the
+// time, the vector units (exponentials, maxima, weights to f16) 43 %, one wavefront's chain of
 // scores, maximum, weights and sums being what neither hides from the other.
 constexpr int KP_WAVES = 8;
 constexpr int KP_ROWS = 32 * KP_WAVES;
