@@ -527,7 +527,7 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
 // them is 32 lanes away.  The weights' sum is one more row of the lows' product.
 //
 // Two sequences' 2,000 rows after 6,000 keys, 32 heads over 8 of 128, bf16 (427
-// GFLOP): 573 us, 745 TFLOP/s (up to 584 by card); the kernel above takes 1,450,
+// GFLOP): 573 us, 745 TFLOP/s (up to 591 by card); the kernel above takes 1,450,
 // an operand's masks, steps and lows serving 16 rows there and 256 here.  A large
 // library product runs at 1,130 to 1,180.  The matrix cores are busy 37 % of the
 // time, the vector units (exponentials, maxima, weights to f16) 43 %, one wavefront's chain of
