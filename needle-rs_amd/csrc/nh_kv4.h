@@ -1,5 +1,5 @@
-// The 4-bit key/value cache: its layout in HBM, what its kernels are given,
-// and their launchers.
+// The 4-bit key/value cache: its layout in HBM, what its kernels are given
+// beside the view that the paged caches share (nh_kv.h), and their launchers.
 //
 // Format.  A row of keys (or values) of one head is cut into groups of 32 or
 // 64 along the head; per group low = f16(min), step = f16((max - min) *
@@ -31,27 +31,15 @@
 // with another, so rows are written without reading their neighbours.
 #pragma once
 
-#include "nh_internal.h"
+#include "nh_kv.h"
 
 namespace nh {
 
-enum Kv4Type { KV4_F32 = 0, KV4_F16 = 1, KV4_BF16 = 2 };  // NH_F32 ..
-
 constexpr int KV4_LANES = 16;
 
-struct Kv4Entry {
-    int seq, row0, row1, len;
-};
-
-struct Kv4View {
-    uint8_t* data;       // [pages][layers][heads] blocks
-    const int* table;    // [seqs][table_ld] page ids
-    const int* batch;    // [nb] of (sequence, first row, end row, length): Kv4Entry; its shape 4 words before
-    int table_ld, pages, layers, heads, dk, dv, width, group, page_log2;
-    int nb, rows, each;  // the batch; each: rows of every sequence when they are equal, else 0
-    int shape[2];        // names the sequences' numbers of rows, in order; (0, 0): no batch
-    int kernel;          // nh_kv4_debug_kernel
-    __host__ __device__ int page() const { return 1 << page_log2; }
+struct Kv4View : KvView {
+    int width, group;
+    int kernel;  // nh_kv4_debug_kernel
     __host__ __device__ int groups() const { return width / group; }
     // bytes of 32 positions, and of one (page, layer, head)
     __host__ __device__ uint32_t chunk() const { return 32u * (width + 8 * groups()); }
@@ -59,27 +47,6 @@ struct Kv4View {
     __host__ __device__ size_t page_bytes() const { return block() * heads * layers; }
 };
 
-// Values of the device's int32 state: (index, value) pairs.
-struct Kv4Patch {
-    static constexpr int MAX = 480;
-    int n;
-    uint32_t at[MAX];
-    int v[MAX];
-};
-// Pages to copy whole.
-struct Kv4Pairs {
-    static constexpr int MAX = 480;
-    int n;
-    int from[MAX], to[MAX];
-};
-// Rows to read: entry i is rows row0[i] .. row0[i + 1] - 1 of the output,
-// positions pos[i] .. of sequence seq[i]; unit0: the first of the chunks that
-// they lie in, in the launch.
-struct Kv4Spans {
-    static constexpr int MAX = 240;
-    int n;
-    int seq[MAX], pos[MAX], row0[MAX + 1], unit0[MAX + 1];
-};
 // The chunks of 32 that positions pos .. pos + n - 1 lie in.
 __host__ __device__ inline int kv4_chunks(int pos, int n) { return n ? ((pos + n - 1) >> 5) - (pos >> 5) + 1 : 0; }
 // Runs of positions to move into fresh pages: positions src .. of sequence
@@ -102,13 +69,11 @@ struct Kv4AttendArgs {
     void* ws;
 };
 
-hipError_t launch_kv4_patch(int* state, const Kv4Patch& p, hipStream_t s);
-hipError_t launch_kv4_pairs(const Kv4View& c, const Kv4Pairs& p, hipStream_t s);
 hipError_t launch_kv4_runs(const Kv4View& c, const int* state, const Kv4Runs& r, hipStream_t s);
 hipError_t launch_kv4_append(const Kv4View& c, const int* row0, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int type,
                              hipStream_t s);
 // layer < 0: all, [layers][rows]; `rows` rows a layer in the output, this launch's from `row`.
-hipError_t launch_kv4_read(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,
+hipError_t launch_kv4_read(const Kv4View& c, int layer, const KvSpans& p, int64_t rows, int64_t row, void* k, void* v,
                            int type, hipStream_t s);
 // Bytes of workspace an attention call of the batch needs; row0: the host's copy
 // of the sequences' first rows; longest: the batch's longest sequence.

@@ -106,13 +106,13 @@ struct KaChunk {
 // NW wavefronts a workgroup, each every NW-th chunk of the range; RT tiles of 16 rows.
 template <int TYPE, int W, int G, int RT, int NW>
 __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
-    typedef typename Kv4Elem<TYPE>::T T;
+    typedef typename KvElem<TYPE>::T T;
     constexpr int NG = W / G, NB = W / 64, NJ = W / 32, GJ = G / 32, GI = G / 16;
-    constexpr int PARTS = TYPE == KV4_F32 ? 2 : 1;   // f16 halves of a query element
+    constexpr int PARTS = TYPE == KV_F32 ? 2 : 1;   // f16 halves of a query element
     // ..  and of a weight.  One leaves up to three roundings of an f16 output (4.6e-4
     // of it instead of 2.1e-4, 20 keys; 131,072 keys: 38.6 us, 41.0 with two), but
     // a tenth of a bf16 output's one.
-    constexpr int WPARTS = TYPE == KV4_BF16 ? 1 : 2;
+    constexpr int WPARTS = TYPE == KV_BF16 ? 1 : 2;
     // The MFMAs take a subnormal as it is, but line its products up by the exponent
     // of the smallest normal number: up to 2^-17 of the largest product is cut off
     // (2^-20 with normal operands, both measured).  Calls that carry 22 bits bring
@@ -139,13 +139,13 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
         b = tile / plan.tiles_each;
         tile -= b * plan.tiles_each;
     } else {
-        b = kv4_find(c, tile, lane, [&](const Kv4Entry& e) { return ((e.row1 - e.row0) * per + 16 * RT - 1) / (16 * RT); });
+        b = kv_find(c, tile, lane, [&](const KvEntry& e) { return ((e.row1 - e.row0) * per + 16 * RT - 1) / (16 * RT); });
     }
     if (b >= c.nb) return;
-    const Kv4Entry entry = kv4_batch(c, b);
+    const KvEntry entry = kv_batch(c, b);
     const int row0 = entry.row0, nrows = entry.row1 - row0, seq = entry.seq;
     const int first = entry.len - nrows, r0 = tile * 16 * RT;
-    if (!kv4_current(c) || first < 0 || r0 >= nrows * per || entry.row1 > c.rows) return;
+    if (!kv_current(c) || first < 0 || r0 >= nrows * per || entry.row1 > c.rows) return;
     const int r1 = min(r0 + 16 * RT, nrows * per) - 1;
     const int plo = first + r0 / per, phi = first + r1 / per;
 
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
                 for (int e = 0; e < 8; ++e) x[j][e] = (float)y[e];
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][e] = d + e < c.dk ? Kv4Elem<TYPE>::get(src + d + e) : 0.0f;
+                for (int e = 0; e < 8; ++e) x[j][e] = d + e < c.dk ? KvElem<TYPE>::get(src + d + e) : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[j][e]));
@@ -497,7 +497,7 @@ __global__ __launch_bounds__(NW * 64, W <= 128 ? 2 : 1) void k_kv4_attend(Kv4Vie
             const int t = r / per, head = kvh * per + r - t * per;
             const int64_t row = row0 + t;
             if (plan.splits == 1) {
-                Kv4Elem<TYPE>::put(reinterpret_cast<T*>(a.out) + row * a.ldo + (int64_t)head * c.dv + d, v / sum);
+                KvElem<TYPE>::put(reinterpret_cast<T*>(a.out) + row * a.ldo + (int64_t)head * c.dv + d, v / sum);
                 if (a.lse && d == 0) a.lse[row * a.heads + head] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
             } else {
                 const int64_t at = ((int64_t)split * c.rows + row) * a.heads + head;
@@ -544,7 +544,7 @@ __device__ __forceinline__ float halves_max(float v) {
 
 template <int TYPE, int W, int G>
 __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
-    typedef typename Kv4Elem<TYPE>::T T;
+    typedef typename KvElem<TYPE>::T T;
     typedef Kv4Lay<W, G> L;
     constexpr int NG = L::NG, NJ = W / 32, NX = W / 16, ND = W / 32;
     struct Image {  // a chunk's operands, 16 bytes a lane each
@@ -560,11 +560,11 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
         b = tile / plan.tiles_each;
         tile = plan.tiles_each - 1 - (tile - b * plan.tiles_each);  // the longest first
     } else
-        b = kv4_find(c, tile, lane, [&](const Kv4Entry& e) { return ((e.row1 - e.row0) * per + KP_ROWS - 1) / KP_ROWS; });
+        b = kv_find(c, tile, lane, [&](const KvEntry& e) { return ((e.row1 - e.row0) * per + KP_ROWS - 1) / KP_ROWS; });
     if (b >= c.nb) return;
-    const Kv4Entry entry = kv4_batch(c, b);
+    const KvEntry entry = kv_batch(c, b);
     const int row0 = entry.row0, nrows = entry.row1 - row0, first = entry.len - nrows, r0 = tile * KP_ROWS;
-    if (!kv4_current(c) || first < 0 || r0 >= nrows * per || entry.row1 > c.rows) return;
+    if (!kv_current(c) || first < 0 || r0 >= nrows * per || entry.row1 > c.rows) return;
     const int r1 = min(r0 + KP_ROWS, nrows * per) - 1;
     const int plo = first + r0 / per, phi = first + r1 / per;
     const int w0 = min(r0 + wave * 32, r1), w1 = min(w0 + 31, r1);  // this wavefront's rows
@@ -963,7 +963,7 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
 constexpr int KA_SPLITS = 512;
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, int splits) {
-    typedef typename Kv4Elem<TYPE>::T T;
+    typedef typename KvElem<TYPE>::T T;
     __shared__ float f[KA_SPLITS], sv[4][256], st[4], ss[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t n = (int64_t)c.rows * a.heads, at = blockIdx.x;
@@ -1010,7 +1010,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, in
     __syncthreads();
     if (tid < c.dv) {
         T* out = reinterpret_cast<T*>(a.out) + at / a.heads * a.ldo + at % a.heads * c.dv;
-        Kv4Elem<TYPE>::put(out + tid, ((sv[0][tid] + sv[1][tid]) + (sv[2][tid] + sv[3][tid])) / sum);
+        KvElem<TYPE>::put(out + tid, ((sv[0][tid] + sv[1][tid]) + (sv[2][tid] + sv[3][tid])) / sum);
     }
     if (a.lse && tid == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
 }
@@ -1021,7 +1021,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, in
 constexpr int KA_FEW = 8;
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_kv4_join_few(Kv4View c, Kv4AttendArgs a, int splits) {
-    typedef typename Kv4Elem<TYPE>::T T;
+    typedef typename KvElem<TYPE>::T T;
     const int64_t n = (int64_t)c.rows * a.heads, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n * c.dv) return;
     const int64_t at = i / c.dv;
@@ -1046,7 +1046,7 @@ __global__ __launch_bounds__(256) void k_kv4_join_few(Kv4View c, Kv4AttendArgs a
         sum = some ? __builtin_fmaf(l[s], g, sum) : sum;
         o = some ? __builtin_fmaf(v[s], g, o) : o;
     }
-    Kv4Elem<TYPE>::put(reinterpret_cast<T*>(a.out) + at / a.heads * a.ldo + at % a.heads * c.dv + d, o / sum);
+    KvElem<TYPE>::put(reinterpret_cast<T*>(a.out) + at / a.heads * a.ldo + at % a.heads * c.dv + d, o / sum);
     if (a.lse && d == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
 }
 
@@ -1121,7 +1121,7 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
 
     // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at
     // 256 dims its sums do not fit the registers.
-    if (type == KV4_F32 || c.width > 128 || c.kernel == 1 || base == 0) return s;
+    if (type == KV_F32 || c.width > 128 || c.kernel == 1 || base == 0) return s;
     const int64_t steps = (chunks_of(s.rows, true) + s.splits * s.waves - 1) / (s.splits * s.waves);
     const double step = s.rows == 32 ? 1.8 : c.width == 64 ? 0.9 : 1.74;
     const double plain = 4.0 + std::max(1.0, (double)(base * s.splits) / (double)slots) * (4.0 + (double)steps * step) +
@@ -1143,15 +1143,15 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
 
 size_t kv4_attend_ws(const Kv4View& c, const int* row0, int heads, int sink, int ring, int longest) {
     // (enough for a call of any type)
-    const int s = std::max(shape_of(c, row0, KV4_F32, heads, sink, ring, longest).splits,
-                           shape_of(c, row0, KV4_F16, heads, sink, ring, longest).splits);
+    const int s = std::max(shape_of(c, row0, KV_F32, heads, sink, ring, longest).splits,
+                           shape_of(c, row0, KV_F16, heads, sink, ring, longest).splits);
     return s > 1 ? (size_t)s * c.rows * heads * (c.dv + 2) * 4 : 0;
 }
 
 template <int TYPE, int W, int G>
 static hipError_t attend_shaped(const Kv4View& c, const int* row0, const Kv4AttendArgs& a, int longest, hipStream_t s) {
     const KaShape shape = shape_of(c, row0, TYPE, a.heads, a.sink, a.ring, longest);
-    const size_t es = sizeof(typename Kv4Elem<TYPE>::T);
+    const size_t es = sizeof(typename KvElem<TYPE>::T);
     KaPlan plan;
     plan.tiles_each = shape.tiles_each;
     plan.splits = shape.splits;
@@ -1160,7 +1160,7 @@ static hipError_t attend_shaped(const Kv4View& c, const int* row0, const Kv4Atte
     if (shape.tiles * c.heads > 0x7fffffff || (int64_t)c.rows * a.heads > 0x7fffffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(shape.tiles * c.heads), plan.splits);
     bool done = false;
-    if constexpr (W <= 128 && TYPE != KV4_F32)
+    if constexpr (W <= 128 && TYPE != KV_F32)
         if (shape.prompt) {
             hipLaunchKernelGGL((k_kv4_prompt<TYPE, W, G>), grid, dim3(KP_WAVES * 64), 0, s, c, a, plan);
             done = true;
@@ -1193,9 +1193,9 @@ static hipError_t attend_typed(const Kv4View& c, const int* row0, const Kv4Atten
 }
 
 hipError_t launch_kv4_attend(const Kv4View& c, const int* row0, const Kv4AttendArgs& a, int longest, hipStream_t s) {
-    return a.type == KV4_F32   ? attend_typed<KV4_F32>(c, row0, a, longest, s)
-           : a.type == KV4_F16 ? attend_typed<KV4_F16>(c, row0, a, longest, s)
-                               : attend_typed<KV4_BF16>(c, row0, a, longest, s);
+    return a.type == KV_F32   ? attend_typed<KV_F32>(c, row0, a, longest, s)
+           : a.type == KV_F16 ? attend_typed<KV_F16>(c, row0, a, longest, s)
+                               : attend_typed<KV_BF16>(c, row0, a, longest, s);
 }
 
 }  // namespace nh

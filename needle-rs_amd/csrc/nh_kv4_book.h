@@ -1,6 +1,7 @@
-// The pages of a 4-bit key/value cache, on the host: which sequence holds
-// which pages, how many sequences share a page, which pages are free.  Plain
-// C++ without HIP; nh_kv4.cpp mirrors the tables on the device.
+// The pages of a key/value cache (of the 4-bit one and the 8-bit one alike), on
+// the host: which sequence holds which pages, how many sequences share a page,
+// which pages are free.  Plain C++ without HIP; nh_kv_host.h mirrors the tables
+// on the device.
 //
 // A sequence is a list of page ids and a length.  Branches share pages by
 // count; a page is written only by its single holder, so a sequence that is

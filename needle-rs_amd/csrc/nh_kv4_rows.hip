@@ -4,18 +4,6 @@
 
 namespace nh {
 
-// ------------------------------------------------------------------ state
-__global__ __launch_bounds__(512) void k_kv4_patch(int* __restrict__ state, Kv4Patch p) {
-    const int i = threadIdx.x;
-    if (i < p.n) state[p.at[i]] = p.v[i];
-}
-
-hipError_t launch_kv4_patch(int* state, const Kv4Patch& p, hipStream_t s) {
-    static_assert(Kv4Patch::MAX <= 512 && sizeof(Kv4Patch) <= 4000, "one block, one argument segment");
-    hipLaunchKernelGGL(k_kv4_patch, dim3(1), dim3(512), 0, s, state, p);
-    return hipGetLastError();
-}
-
 // ------------------------------------------------------------------- rows
 // Of one group: low, step and the reciprocal the codes are taken with.
 struct Kv4Group {
@@ -55,9 +43,9 @@ __device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Group& g) {
 // store with two rows a lane in flight; both rows' loads issued first was slower
 // (19 us: twice the code for rows that are mostly fetched once).
 template <int TYPE, int W, int G, bool VALUES>
-__device__ __forceinline__ void kv4_pack_row(const typename Kv4Elem<TYPE>::T* __restrict__ x, int dim, bool vec, uint8_t* img,
+__device__ __forceinline__ void kv4_pack_row(const typename KvElem<TYPE>::T* __restrict__ x, int dim, bool vec, uint8_t* img,
                                              int slot, int lane, bool live) {
-    typedef typename Kv4Elem<TYPE>::T T;
+    typedef typename KvElem<TYPE>::T T;
     typedef T Vec __attribute__((ext_vector_type(8)));
     typedef Kv4Lay<W, G> L;
 #pragma unroll
@@ -70,7 +58,7 @@ __device__ __forceinline__ void kv4_pack_row(const typename Kv4Elem<TYPE>::T* __
             for (int e = 0; e < 8; ++e) v[e] = (float)y[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = live && d + e < dim ? Kv4Elem<TYPE>::get(x + d + e) : 0.0f;
+            for (int e = 0; e < 8; ++e) v[e] = live && d + e < dim ? KvElem<TYPE>::get(x + d + e) : 0.0f;
         }
         float mn = __builtin_inff(), mx = -__builtin_inff();
         int bad = 0;
@@ -147,8 +135,8 @@ struct Kv4Rows {  // the rows of an append, or of a read
 __host__ __device__ inline int kv4_most_chunks(int rows) { return rows ? (rows + 30) / 32 + 1 : 0; }
 
 template <int TYPE, int W, int G>
-__global__ __launch_bounds__(256) void k_kv4_append(Kv4View c, int layer, const typename Kv4Elem<TYPE>::T* __restrict__ k,
-                                                    const typename Kv4Elem<TYPE>::T* __restrict__ v, Kv4Rows a) {
+__global__ __launch_bounds__(256) void k_kv4_append(Kv4View c, int layer, const typename KvElem<TYPE>::T* __restrict__ k,
+                                                    const typename KvElem<TYPE>::T* __restrict__ v, Kv4Rows a) {
     typedef Kv4Lay<W, G> L;
     __shared__ __align__(16) uint8_t img[L::CHUNK];
     const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.x % c.heads;
@@ -157,13 +145,13 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4View c, int layer, const 
         b = unit / a.each;
         unit -= b * a.each;
     } else
-        b = kv4_find(c, unit, lane, [](const Kv4Entry& e) { return kv4_most_chunks(e.row1 - e.row0); });
+        b = kv_find(c, unit, lane, [](const KvEntry& e) { return kv4_most_chunks(e.row1 - e.row0); });
     if (b >= c.nb) return;
-    const Kv4Entry e = kv4_batch(c, b);
+    const KvEntry e = kv_batch(c, b);
     const int first = e.len - (e.row1 - e.row0);  // the position of row row0
     const int pos0 = ((first >> 5) + unit) << 5, lo = max(first - pos0, 0), hi = min(e.len - 1 - pos0, 31);
-    if (!kv4_current(c) || first < 0 || lo > hi || e.row1 > c.rows) return;
-    const int pg = kv4_page(c, e.seq, pos0);
+    if (!kv_current(c) || first < 0 || lo > hi || e.row1 > c.rows) return;
+    const int pg = kv_page(c, e.seq, pos0);
     if (pg < 0) return;
 #pragma unroll 1
     for (int s0 = lo; s0 <= hi; s0 += 16) {
@@ -180,14 +168,14 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4View c, int layer, const 
 
 template <int TYPE>
 static bool can_take8(const void* p, int64_t ld, int dim) {
-    const size_t es = sizeof(typename Kv4Elem<TYPE>::T);
+    const size_t es = sizeof(typename KvElem<TYPE>::T);
     return dim % 8 == 0 && (uintptr_t)p % 16 == 0 && ld * es % 16 == 0;
 }
 
 template <int TYPE, int G>
 static hipError_t append_typed(const Kv4View& c, const int* row0, int layer, const void* k, const void* v, int64_t ldk,
                                int64_t ldv, hipStream_t s) {
-    typedef const typename Kv4Elem<TYPE>::T* P;
+    typedef const typename KvElem<TYPE>::T* P;
     Kv4Rows a{ldk, ldv, can_take8<TYPE>(k, ldk, c.dk), can_take8<TYPE>(v, ldv, c.dv), kv4_most_chunks(c.each)};
     int64_t units = (int64_t)a.each * c.nb;
     if (!a.each)
@@ -209,17 +197,17 @@ static hipError_t append_typed(const Kv4View& c, const int* row0, int layer, con
 
 hipError_t launch_kv4_append(const Kv4View& c, const int* row0, int layer, const void* k, const void* v, int64_t ldk,
                              int64_t ldv, int type, hipStream_t s) {
-    return type == KV4_F32   ? append_typed<KV4_F32>(c, row0, layer, k, v, ldk, ldv, s)
-           : type == KV4_F16 ? append_typed<KV4_F16>(c, row0, layer, k, v, ldk, ldv, s)
-                             : append_typed<KV4_BF16>(c, row0, layer, k, v, ldk, ldv, s);
+    return type == KV_F32   ? append_typed<KV_F32>(c, row0, layer, k, v, ldk, ldv, s)
+           : type == KV_F16 ? append_typed<KV_F16>(c, row0, layer, k, v, ldk, ldv, s)
+                             : append_typed<KV_BF16>(c, row0, layer, k, v, ldk, ldv, s);
 }
 
 // Eight dims of a row of keys, or of values, out of a chunk's image.  step * code
 // is exact in f32, so the fma rounds once, as the product and the sum do.
 template <int TYPE, int W, int G, bool VALUES>
-__device__ __forceinline__ void kv4_unpack8(const uint8_t* img, int slot, int t, typename Kv4Elem<TYPE>::T* __restrict__ to,
+__device__ __forceinline__ void kv4_unpack8(const uint8_t* img, int slot, int t, typename KvElem<TYPE>::T* __restrict__ to,
                                             int dim, bool vec) {
-    typedef typename Kv4Elem<TYPE>::T T;
+    typedef typename KvElem<TYPE>::T T;
     typedef T Vec __attribute__((ext_vector_type(8)));
     typedef Kv4Lay<W, G> L;
     const int g = t * 8 / G;
@@ -242,7 +230,7 @@ __device__ __forceinline__ void kv4_unpack8(const uint8_t* img, int slot, int t,
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         T z;
-        Kv4Elem<TYPE>::put(&z, __builtin_fmaf(step, (float)code[e], low));
+        KvElem<TYPE>::put(&z, __builtin_fmaf(step, (float)code[e], low));
         y[e] = z;
     }
     if (vec)
@@ -257,16 +245,16 @@ __device__ __forceinline__ void kv4_unpack8(const uint8_t* img, int slot, int t,
 // thread, then 8 dims a lane out of it.  Bound by what it writes: the 7,485 rows
 // above in 10 us (4 TB/s), 8 layers of 4,122 (177 MB) in 35 (5 TB/s).
 template <int TYPE, int W, int G>
-__global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, Kv4Spans p, int64_t rows, int64_t row_at,
-                                                  typename Kv4Elem<TYPE>::T* __restrict__ k,
-                                                  typename Kv4Elem<TYPE>::T* __restrict__ v, Kv4Rows a) {
+__global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, KvSpans p, int64_t rows, int64_t row_at,
+                                                  typename KvElem<TYPE>::T* __restrict__ k,
+                                                  typename KvElem<TYPE>::T* __restrict__ v, Kv4Rows a) {
     typedef Kv4Lay<W, G> L;
     __shared__ __align__(16) uint8_t img[L::CHUNK];
     const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.x % c.heads;
-    const int unit = blockIdx.x / c.heads, b = kv4_span(p.unit0, p.n, unit, lane);
+    const int unit = blockIdx.x / c.heads, b = kv_span(p.unit0, p.n, unit, lane);
     const int first = p.pos[b], end = first + p.row0[b + 1] - p.row0[b];
     const int pos0 = ((first >> 5) + unit - p.unit0[b]) << 5, lo = max(first - pos0, 0), hi = min(end - 1 - pos0, 31);
-    const int pg = kv4_page(c, p.seq[b], pos0);
+    const int pg = kv_page(c, p.seq[b], pos0);
     if (pg < 0) return;
     const uint8_t* from = kv4_block(c, pg, layer0 + (int)blockIdx.y, head) + (uint32_t)((pos0 & (c.page() - 1)) >> 5) * L::CHUNK;
     for (uint32_t i = tid; i < L::CHUNK / 16; i += 256)
@@ -282,9 +270,9 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, int layer0, Kv4Span
 }
 
 template <int TYPE, int G>
-static hipError_t read_typed(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,
+static hipError_t read_typed(const Kv4View& c, int layer, const KvSpans& p, int64_t rows, int64_t row, void* k, void* v,
                              hipStream_t s) {
-    typedef typename Kv4Elem<TYPE>::T* P;
+    typedef typename KvElem<TYPE>::T* P;
     const Kv4Rows a{0, 0, can_take8<TYPE>(k, c.dk, c.dk), can_take8<TYPE>(v, c.dv, c.dv), 0};
     const int64_t blocks = (int64_t)p.unit0[p.n] * c.heads;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
@@ -295,37 +283,21 @@ static hipError_t read_typed(const Kv4View& c, int layer, const Kv4Spans& p, int
 }
 
 template <int TYPE>
-static hipError_t read_typed(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,
+static hipError_t read_typed(const Kv4View& c, int layer, const KvSpans& p, int64_t rows, int64_t row, void* k, void* v,
                              hipStream_t s) {
     return c.group == 32 ? read_typed<TYPE, 32>(c, layer, p, rows, row, k, v, s)
                          : read_typed<TYPE, 64>(c, layer, p, rows, row, k, v, s);
 }
 
-hipError_t launch_kv4_read(const Kv4View& c, int layer, const Kv4Spans& p, int64_t rows, int64_t row, void* k, void* v,
+hipError_t launch_kv4_read(const Kv4View& c, int layer, const KvSpans& p, int64_t rows, int64_t row, void* k, void* v,
                            int type, hipStream_t s) {
-    static_assert(sizeof(Kv4Spans) <= 3900, "the argument segment");
-    return type == KV4_F32   ? read_typed<KV4_F32>(c, layer, p, rows, row, k, v, s)
-           : type == KV4_F16 ? read_typed<KV4_F16>(c, layer, p, rows, row, k, v, s)
-                             : read_typed<KV4_BF16>(c, layer, p, rows, row, k, v, s);
+    static_assert(sizeof(KvSpans) <= 3900, "the argument segment");
+    return type == KV_F32   ? read_typed<KV_F32>(c, layer, p, rows, row, k, v, s)
+           : type == KV_F16 ? read_typed<KV_F16>(c, layer, p, rows, row, k, v, s)
+                             : read_typed<KV_BF16>(c, layer, p, rows, row, k, v, s);
 }
 
 // ------------------------------------------------------------------ pages
-// Whole pages, every layer and head: 16 bytes a thread (8 pages of 20 layers, 2.6
-// MB in and out, 3.0 us: a launch's latency).
-__global__ __launch_bounds__(256) void k_kv4_pairs(Kv4View c, Kv4Pairs p) {
-    const size_t n = c.page_bytes() / 16;
-    const uint4* from = reinterpret_cast<const uint4*>(c.data) + (size_t)p.from[blockIdx.y] * n;
-    uint4* to = reinterpret_cast<uint4*>(c.data) + (size_t)p.to[blockIdx.y] * n;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) to[i] = from[i];
-}
-
-hipError_t launch_kv4_pairs(const Kv4View& c, const Kv4Pairs& p, hipStream_t s) {
-    static_assert(sizeof(Kv4Pairs) <= 3900, "the argument segment");
-    const size_t blocks = (c.page_bytes() / 16 + 255) / 256;
-    hipLaunchKernelGGL(k_kv4_pairs, dim3((unsigned)(blocks < 1024 ? blocks : 1024), p.n), dim3(256), 0, s, c, p);
-    return hipGetLastError();
-}
-
 // A workgroup writes one run's positions of one chunk of a fresh page, for one
 // (layer, head): gathered into LDS, then stored as an append stores them.  The
 // fresh pages belong to this sequence alone and no position shares a byte with
@@ -336,12 +308,12 @@ __global__ __launch_bounds__(128) void k_kv4_runs(Kv4View c, const int* __restri
     typedef Kv4Lay<W, G> L;
     __shared__ __align__(16) uint8_t img[L::CHUNK];
     const int tid = threadIdx.x, lane = tid & 63, l = tid & 15;
-    const int unit = blockIdx.x, m = kv4_span(r.unit0, r.n, unit, lane);
+    const int unit = blockIdx.x, m = kv_span(r.unit0, r.n, unit, lane);
     const int dst = r.dst[m], pos0 = ((dst >> 5) + unit - r.unit0[m]) << 5;
     const int lo = max(dst - pos0, 0), hi = min(dst + r.count[m] - 1 - pos0, 31), src0 = r.src[m] - dst + pos0;
     const int to = state[r.fresh[m] + (pos0 >> c.page_log2)], mask = c.page() - 1;
     for (int slot = lo + (tid >> 4); slot <= hi; slot += 8) {
-        const int src = src0 + slot, from = kv4_page(c, r.seq[m], src);
+        const int src = src0 + slot, from = kv_page(c, r.seq[m], src);
         if (from < 0) continue;
         const uint8_t* a = kv4_block(c, from, (int)blockIdx.y, (int)blockIdx.z) + (uint32_t)((src & mask) >> 5) * L::CHUNK;
         const int s = src & 31;

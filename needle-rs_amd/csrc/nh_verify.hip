@@ -25,7 +25,7 @@
 #include <algorithm>
 
 #include "../../include/needle_hip.h"
-#include "nh_kv4_device.h"
+#include "nh_kv_device.h"
 
 namespace nh {
 
@@ -134,7 +134,7 @@ __device__ __forceinline__ double wave_sum(double v) { return lane_f64(wave_scan
 // of many by far less; 16 a thread are summed in f32, the rest in f64.
 template <int LT, bool GREEDY>
 __global__ __launch_bounds__(VR_THREADS) void k_verify_rows(VerifyArgs a) {
-    typedef typename Kv4Elem<LT>::T T;
+    typedef typename KvElem<LT>::T T;
     constexpr int VEC = 16 / sizeof(T);
     typedef T Vec __attribute__((ext_vector_type(VEC)));
     __shared__ float sv[VR_WAVES];
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(VR_THREADS) void k_verify_rows(VerifyArgs a) {
             for (int e = 0; e < VEC; ++e) v[k + e] = (float)y[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[k + e] = t + e < n ? Kv4Elem<LT>::get(x + t + e) : __builtin_nanf("");
+            for (int e = 0; e < VEC; ++e) v[k + e] = t + e < n ? KvElem<LT>::get(x + t + e) : __builtin_nanf("");
         }
     }
     VerifySlice* to = a.slices + row * a.nslices + slice;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(VR_THREADS) void k_verify_rows(VerifyArgs a) {
             const float l = v[k], d = l - m;
             const float t = d * ch;
             float r = __builtin_fmaf(d, cl, __builtin_fmaf(d, ch, -t));
-            if constexpr (LT == KV4_F32) {
+            if constexpr (LT == KV_F32) {
                 const float b = d - l;
                 r = __builtin_fmaf((l - (d - b)) - (m + b), ch, r);
             }
@@ -233,8 +233,8 @@ template <int LT, int PT, bool GREEDY, bool RESIDUE>
 __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs a) {
     constexpr int VP_THREADS = RESIDUE ? 256 : 1024, VP_WAVES = VP_THREADS / 64;
     constexpr int SUB = VR_SLICE / (VP_THREADS * VP_EACH);  // strips of a slice
-    typedef typename Kv4Elem<LT>::T T;
-    typedef typename Kv4Elem<PT>::T P;
+    typedef typename KvElem<LT>::T T;
+    typedef typename KvElem<PT>::T P;
     __shared__ double s_sum, ss[2][VP_WAVES];
     __shared__ float s_max;
     __shared__ int s_kept, s_best, s_slice, s_pick, s_last, s_left, s_out;
@@ -266,11 +266,11 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
             double sl0 = 0.0;
             if (!GREEDY && lane < a.nslices) ml = sl[lane].max, sl0 = sl[lane].sum;
             const float ui = GREEDY ? 0.0f : u[i];
-            const float first = GREEDY ? Kv4Elem<LT>::get(logits + i * a.ldl) : 0.0f;
+            const float first = GREEDY ? KvElem<LT>::get(logits + i * a.ldl) : 0.0f;
             const int x = i < cnt ? drafts[i] : 0;
             const bool in = (unsigned)x < (unsigned)a.vocab;
-            const float lx = !GREEDY && in ? Kv4Elem<LT>::get(logits + i * a.ldl + x) : 0.0f;
-            const double q = RESIDUE && in && i < cnt ? (double)Kv4Elem<PT>::get(probs + i * a.ldp + x) : 1.0;
+            const float lx = !GREEDY && in ? KvElem<LT>::get(logits + i * a.ldl + x) : 0.0f;
+            const double q = RESIDUE && in && i < cnt ? (double)KvElem<PT>::get(probs + i * a.ldp + x) : 1.0;
             draft = x;
             if constexpr (GREEDY) {
                 for (int k = lane; k < a.nslices; k += 64) verify_best(m, best, sl[k].max, sl[k].best);
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
                 for (int k = 0; k < VP_EACH; ++k) l[k] = (float)y[k];
             } else {
 #pragma unroll
-                for (int k = 0; k < VP_EACH; ++k) l[k] = t + k < a.vocab ? Kv4Elem<LT>::get(x + t + k) : __builtin_nanf("");
+                for (int k = 0; k < VP_EACH; ++k) l[k] = t + k < a.vocab ? KvElem<LT>::get(x + t + k) : __builtin_nanf("");
             }
             if (RESIDUE && left) {
                 if (whole && a.paligned) {
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(RESIDUE ? 256 : 1024) void k_verify_pick(VerifyArgs
                     for (int k = 0; k < VP_EACH; ++k) d[k] = (float)y[k];
                 } else {
 #pragma unroll
-                    for (int k = 0; k < VP_EACH; ++k) d[k] = t + k < a.vocab ? Kv4Elem<PT>::get(q + t + k) : 0.0f;
+                    for (int k = 0; k < VP_EACH; ++k) d[k] = t + k < a.vocab ? KvElem<PT>::get(q + t + k) : 0.0f;
                 }
             }
         };
@@ -503,21 +503,21 @@ static void launch_verify(const VerifyArgs& a, hipStream_t s) {
     const dim3 rows((unsigned)((int64_t)a.batch * (a.n + 1) * a.nslices)), one(a.batch), t(VR_THREADS), many(256), few(1024);
     if (a.c == 0.0) {
         hipLaunchKernelGGL((k_verify_rows<LT, true>), rows, t, 0, s, a);
-        hipLaunchKernelGGL((k_verify_pick<LT, KV4_F32, true, false>), one, few, 0, s, a);
+        hipLaunchKernelGGL((k_verify_pick<LT, KV_F32, true, false>), one, few, 0, s, a);
     } else {
         hipLaunchKernelGGL((k_verify_rows<LT, false>), rows, t, 0, s, a);
         if (a.probs)
             hipLaunchKernelGGL((k_verify_pick<LT, PT, false, true>), dim3(a.batch * a.nslices), many, 0, s, a);
         else
-            hipLaunchKernelGGL((k_verify_pick<LT, KV4_F32, false, false>), one, few, 0, s, a);
+            hipLaunchKernelGGL((k_verify_pick<LT, KV_F32, false, false>), one, few, 0, s, a);
     }
 }
 
 template <int LT>
 static hipError_t launch_verify(const VerifyArgs& a, int ptype, hipStream_t s) {
-    if (ptype == KV4_F32) launch_verify<LT, KV4_F32>(a, s);
-    else if (ptype == KV4_F16) launch_verify<LT, KV4_F16>(a, s);
-    else launch_verify<LT, KV4_BF16>(a, s);
+    if (ptype == KV_F32) launch_verify<LT, KV_F32>(a, s);
+    else if (ptype == KV_F16) launch_verify<LT, KV_F16>(a, s);
+    else launch_verify<LT, KV_BF16>(a, s);
     return hipGetLastError();
 }
 
@@ -577,9 +577,9 @@ int nh_verify_drafts(const void* logits, int type, int64_t ldl, const int32_t* d
     a.c = temperature > 0.0f ? 1.4426950408889634074 / (double)temperature : 0.0;
     const hipStream_t st = (hipStream_t)stream;
     const int pt = probs ? probs_type : NH_F32;
-    const hipError_t e = type == NH_F32   ? nh::launch_verify<nh::KV4_F32>(a, pt, st)
-                         : type == NH_F16 ? nh::launch_verify<nh::KV4_F16>(a, pt, st)
-                                          : nh::launch_verify<nh::KV4_BF16>(a, pt, st);
+    const hipError_t e = type == NH_F32   ? nh::launch_verify<nh::KV_F32>(a, pt, st)
+                         : type == NH_F16 ? nh::launch_verify<nh::KV_F16>(a, pt, st)
+                                          : nh::launch_verify<nh::KV_BF16>(a, pt, st);
     if (e != hipSuccess) return fail(NH_EDEVICE, std::string("verify: ") + hipGetErrorString(e));
     return NH_OK;
 }
