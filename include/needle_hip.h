@@ -41,6 +41,7 @@ typedef struct nh_weights nh_weights; /* every matmul weight of a .cact archive 
 typedef struct nh_model nh_model;     /* a loaded model for the decode step (Model) */
 typedef struct nh_session nh_session; /* one sequence's decoding state in HBM (Session) */
 typedef struct nh_kv4 nh_kv4;         /* a paged key/value cache held in 4 bits */
+typedef struct nh_rope nh_rope;       /* a plan of rotary positions */
 
 /* ---- runtime ----------------------------------------------------------- */
 /* Select the device and prepare the code tables.  No reference counterpart
@@ -461,6 +462,45 @@ int nh_kv4_attend(const nh_kv4* c, int layer, const void* q, int64_t ldq, int he
  * (1), by that of many where it takes the call's type and dims (2), or by the
  * one that the shapes make the quicker (0, as made). */
 int nh_kv4_debug_kernel(nh_kv4* c, int kernel);
+
+/* ---- rotary positions ---------------------------------------------------- */
+/* No reference counterpart as an operator: its model turns its keys and
+ * queries inside its layers (Tables, crates/needle-engine/src/infer.rs:869-960).
+ * For models of a caller's own, beside the caches.
+ *
+ * Pair i of a head's first 2 `pairs` dims, (i, i + pairs) or (2 i, 2 i + 1),
+ * turns by position x frequency[i]: y_a = x_a c - x_b s, y_b = x_b c + x_a s with
+ * c = f32(amplitude cos), s = f32(amplitude sin) and every product and sum
+ * rounded to f32; the other dims stay.  Angles are worked out at any 32-bit
+ * position to 2^-33 of a turn (negative ones turn backwards), so there is no
+ * table and no longest context. */
+#define NH_ROPE_HALF 0
+#define NH_ROPE_INTERLEAVED 1
+#define NH_ROPE_PLAIN 0  /* theta^(-2 i / dim) */
+#define NH_ROPE_LINEAR 1 /* all frequencies divided by the factor */
+#define NH_ROPE_BASE 2   /* theta times factor^(dim / (dim - 2)): the slowest pair slowed by the factor, the quickest kept */
+#define NH_ROPE_PARTS 3  /* by a ramp over the pairs' indices, from that of `high` turns in the original length (kept) to
+                          * that of `low` turns (divided); amplitude 0.1 ln(factor) + 1 */
+#define NH_ROPE_BANDS 4  /* by a ramp over the pairs' turns in the original length: `high` and more kept, `low` and fewer divided */
+/* The frequencies of dim / 2 pairs (HOST freqs, radians a position) and the
+ * amplitude for a context `factor` times the original length.  Host arithmetic
+ * in 64 bits: no device is needed.  factor is read by all scalings but PLAIN,
+ * original, low and high by PARTS and BANDS. */
+int nh_rope_freqs(int dim, double theta, int scaling, double factor, double original, double low, double high,
+                  double* freqs, double* amplitude);
+/* A plan of HOST freqs[pairs] (any, |f| <= 10^6).  The only call that
+ * allocates; a plan belongs to the device it was made on and is read only:
+ * calls on several streams may share it. */
+int nh_rope_new(const double* freqs, int pairs, double amplitude, int layout, nh_rope** r);
+int nh_rope_free(nh_rope* r);
+/* Turns DEVICE q[row * ldq + head * dim + d] and k (kv_heads 0: none) of `type`
+ * by the rows' positions pos[rows] (DEVICE) into q_out, k_out, in one launch.
+ * q_out may be q, k_out k (the dims that do not turn are then not touched);
+ * otherwise inputs and outputs share no element.  transposed: the rotation
+ * the other way (amplitude kept), which takes outputs' gradients to inputs'. */
+int nh_rope_apply(const nh_rope* r, const int32_t* pos, int64_t rows, int dim, const void* q, int64_t ldq, int heads,
+                  void* q_out, int64_t ldqo, const void* k, int64_t ldk, int kv_heads, void* k_out, int64_t ldko, int type,
+                  int transposed, void* stream);
 
 /* ---- drafted tokens ----------------------------------------------------- */
 /* No reference counterpart (generate.rs:87-139 picks one token a step).

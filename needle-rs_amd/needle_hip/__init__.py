@@ -109,6 +109,10 @@ SIGNATURES = {
     "nh_kv4_attend": (I, [P, I, P, C.c_int64, I, C.c_float, I, I, P, C.c_int64, P, I, P, C.c_uint64, P]),
     "nh_verify_drafts_ws_bytes": (C.c_int64, [I, I, I]),
     "nh_verify_drafts": (I, [P, I, C.c_int64, P, P, P, I, C.c_int64, P, C.c_float, I, I, I, P, P, P, C.c_uint64, P]),
+    "nh_rope_freqs": (I, [I, C.c_double, I, C.c_double, C.c_double, C.c_double, C.c_double, P, P]),
+    "nh_rope_new": (I, [P, I, C.c_double, I, P]),
+    "nh_rope_free": (I, [P]),
+    "nh_rope_apply": (I, [P, P, C.c_int64, I, P, C.c_int64, I, P, C.c_int64, P, C.c_int64, I, P, C.c_int64, I, I, P]),
     "nh_normal": (I, [C.c_uint32, C.c_uint32, C.c_uint64, P]),
     "nh_split": (I, [C.c_uint32, C.c_uint32, P]),
 }
@@ -756,3 +760,4 @@ def seeded_normals(sizes, seed: int = 0):
 
 
 from .kv4 import KvCache4, _DraftCheck, verify_drafts  # noqa: E402,F401
+from .rope import Rope  # noqa: E402,F401
