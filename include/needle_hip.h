@@ -41,6 +41,7 @@ typedef struct nh_weights nh_weights; /* every matmul weight of a .cact archive 
 typedef struct nh_model nh_model;     /* a loaded model for the decode step (Model) */
 typedef struct nh_session nh_session; /* one sequence's decoding state in HBM (Session) */
 typedef struct nh_kv4 nh_kv4;         /* a paged key/value cache held in 4 bits */
+typedef struct nh_kv8 nh_kv8;         /* a paged key/value cache held in 8 bits */
 typedef struct nh_rope nh_rope;       /* a plan of rotary positions */
 
 /* ---- runtime ----------------------------------------------------------- */
@@ -501,6 +502,69 @@ int nh_rope_free(nh_rope* r);
 int nh_rope_apply(const nh_rope* r, const int32_t* pos, int64_t rows, int dim, const void* q, int64_t ldq, int heads,
                   void* q_out, int64_t ldqo, const void* k, int64_t ldk, int kv_heads, void* k_out, int64_t ldko, int type,
                   int transposed, void* stream);
+
+/* ---- an 8-bit key/value cache -------------------------------------------- */
+/* No reference counterpart.  The 4-bit cache's pages, sequences, batches,
+ * captured steps and refusals (above), with keys and values as whole numbers
+ * -127 .. 127 times an f32 step for each block of 16 positions and head:
+ *   step = max|x| f32(1/127) over the block's rows of the call that stores its
+ *   first position, code = rint(x (1 / step)) held to +-127, all in f32;
+ *   rows that join a begun block double its step until it is their own max|x|
+ *   f32(1/127) at least, and the codes that were there are divided by as much (ties to
+ *   even): off by at most a step in all.  A step below 2^-120 counts as 0.
+ * A key or value row with a NaN or an infinity reads as NaN, takes no part in
+ * its block's step, and makes NaN of what a query that sees it gets.  No
+ * compaction: positions that moved to other blocks would be rounded again. */
+/* layers x kv_heads heads of qk_dim keys and v_dim values (1 to 256 each);
+ * `pages` pages of `page` (64, 128 or 256) positions; up to `seqs` sequences of
+ * up to `cap` positions (rounded up to pages).  One position of a layer's head
+ * takes WK + WV + 2 bytes, (64, 64), (128, 128), (192, 128) or (256, 256) the
+ * first that holds both dims.  The only call that
+ * allocates. */
+int nh_kv8_new(int layers, int kv_heads, int qk_dim, int v_dim, int page, int pages, int seqs, int cap, nh_kv8** c);
+int nh_kv8_free(nh_kv8* c);
+/* As the 4-bit cache's calls of the same names. */
+int64_t nh_kv8_bytes(const nh_kv8* c);
+int nh_kv8_free_pages(const nh_kv8* c);
+int nh_kv8_seq_new(nh_kv8* c);
+int nh_kv8_seq_len(const nh_kv8* c, int seq);
+int nh_kv8_seq_free(nh_kv8* c, int seq);
+int nh_kv8_seq_truncate(nh_kv8* c, int seq, int len);
+int nh_kv8_seq_fork(nh_kv8* c, int seq, int n, int* branches);
+int nh_kv8_seq_copy(nh_kv8* c, int seq, void* stream);
+int nh_kv8_extend(nh_kv8* c, const int* seqs, const int* rows, int n, void* stream);
+int nh_kv8_rows(const nh_kv8* c);
+/* rows[i] (>= 0) query rows for each of n distinct sequences (HOST arrays),
+ * which become the batch without being positions of it: every row sees its
+ * whole sequence, as a decoder's rows see their encoder's states.  No position
+ * is added, append is refused, and attend's rows follow the sequences' lengths
+ * at the call; a sequence may be empty, and its rows' outputs are 0 then (lse
+ * -inf).  Refused under stream capture; a captured attend follows it as it
+ * follows an extend. */
+int nh_kv8_ask(nh_kv8* c, const int* seqs, const int* rows, int n, void* stream);
+/* The batch's rows into one layer, as nh_kv4_append.  With a rope (of at most
+ * qk_dim dims, of the cache's device) the keys are turned first, in f32, to
+ * their positions in their sequences, or to DEVICE pos[rows] if given; `heads`
+ * query heads in DEVICE q are turned with them into q_out (q itself, or apart
+ * from it), in the same launch; heads 0: keys alone. */
+int nh_kv8_append(nh_kv8* c, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int type,
+                  const nh_rope* rope, const int32_t* pos, const void* q, int64_t ldq, int heads, void* q_out,
+                  int64_t ldqo, void* stream);
+/* As nh_kv4_read. */
+int nh_kv8_read(nh_kv8* c, int layer, const int* seqs, const int* pos, const int* rows, int n, void* k, void* v,
+                int type, void* stream);
+/* Attention of the batch's rows, as nh_kv4_attend; under nh_kv8_ask every row
+ * is at its sequence's last position, so it sees all of it, with a ring > 0 the
+ * first `sink` and the last `ring` positions.  Scores, weights' sums and
+ * products are held in f32.  f16 and bf16 queries enter as they are, f32 ones
+ * to 2^-24 of a row's largest; f32 and f16 calls carry 22 bits of a weight x
+ * its value's step, bf16 calls and calls of many f16 rows 11 (of many rows also
+ * of a value's step x code), none finer than 2^-40 of the largest step. */
+int64_t nh_kv8_attend_ws_bytes(const nh_kv8* c, int heads, int sink, int ring);
+int nh_kv8_attend(const nh_kv8* c, int layer, const void* q, int64_t ldq, int heads, float scale, int sink, int ring,
+                  void* out, int64_t ldo, float* lse, int type, void* ws, uint64_t ws_bytes, void* stream);
+/* No reference counterpart (a test hook): as nh_kv4_debug_kernel. */
+int nh_kv8_debug_kernel(nh_kv8* c, int kernel);
 
 /* ---- drafted tokens ----------------------------------------------------- */
 /* No reference counterpart (generate.rs:87-139 picks one token a step).

@@ -45,6 +45,19 @@ struct KvSpans {
     int seq[MAX], pos[MAX], row0[MAX + 1], unit0[MAX + 1];
 };
 
+// Results of `splits` ranges of keys to join: ws holds, range by range, (maximum,
+// sum) of each of n (row, head), base 2, then their sums of weighted values.
+constexpr int KV_SPLITS = 512;  // at most
+constexpr int KV_FEW = 8;       // ranges that the join takes a thread an element
+struct KvJoin {
+    void* out;
+    float* lse;  // or null
+    const float* ws;
+    int64_t n, ldo;
+    int heads, dv, splits;
+};
+
+hipError_t launch_kv_join(const KvJoin& a, int type, hipStream_t s);
 hipError_t launch_kv_patch(int* state, const KvPatch& p, hipStream_t s);
 hipError_t launch_kv_pairs(uint8_t* data, size_t page_bytes, const KvPairs& p, hipStream_t s);
 

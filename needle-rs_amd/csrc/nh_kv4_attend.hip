@@ -25,45 +25,19 @@
 // sequence has all the keys the two are about equal: 131,072 keys (151 MB, f16) 41
 // us with the join.  Few keys are latency: 374 of them 7.8 us.
 #include <algorithm>
-#include <type_traits>
 
 #include "nh_kv4_device.h"
+#include "nh_kv_attend.h"
 
 namespace nh {
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-
 constexpr int KA_CHUNK = 32;   // keys of a step of a wavefront; a page holds whole chunks
-constexpr float KA_LOG2E = 1.44269504088896340736f;
 
 // The value of lane `I` of each row of 16 lanes (DPP row_newbcast).
 template <int I>
 __device__ __forceinline__ float row_bcast(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + I, 0xF, 0xF, true));
 }
-// Maximum and sum over the four lane groups of a row's lane.
-__device__ __forceinline__ float groups_max(float v) {
-    const uint32_t x = __builtin_bit_cast(uint32_t, v);
-    auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    const float y = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
-    const uint32_t z = __builtin_bit_cast(uint32_t, y);
-    auto b = __builtin_amdgcn_permlane16_swap(z, z, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
-}
-__device__ __forceinline__ float groups_sum(float v) {
-    const uint32_t x = __builtin_bit_cast(uint32_t, v);
-    auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    const float y = __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
-    const uint32_t z = __builtin_bit_cast(uint32_t, y);
-    auto b = __builtin_amdgcn_permlane16_swap(z, z, false, false);
-    return __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
-}
-
-// 2^e for -126 <= e <= 127.
-__device__ __forceinline__ float pow2i(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
-
 template <int I, int N, class F>
 __device__ __forceinline__ void static_for(F f) {
     if constexpr (I < N) {
@@ -72,27 +46,7 @@ __device__ __forceinline__ void static_for(F f) {
     }
 }
 
-struct KaPlan {
-    int splits;      // key ranges of a sequence; more than one: partial results go to the workspace
-    int tiles_each;  // row tiles of every sequence when they are equal, else 0
-    int aligned;     // rows of q can be read 8 elements at a time
-    int out_aligned; // rows of out can be written 4 elements at a time
-};
-
-// The chunks that a tile of rows at positions lo .. hi sees: [0, ns) and [w, n).
-struct KaSpan {
-    int ns, w, n;
-    __device__ __forceinline__ KaSpan(int lo, int hi, int sink, int ring) {
-        n = hi / KA_CHUNK + 1;
-        ns = 0, w = 0;
-        if (ring) {
-            ns = min((int)(((int64_t)sink + KA_CHUNK - 1) / KA_CHUNK), n);
-            w = max(ns, max(0, lo - ring + 1) / KA_CHUNK);
-        }
-    }
-    __device__ __forceinline__ int count() const { return ns + n - w; }
-    __device__ __forceinline__ int at(int i) const { return i < ns ? i : i - ns + w; }
-};
+typedef KaSpanOf<KA_CHUNK> KaSpan;
 
 // What a lane loads of a chunk: two tiles of 16 keys.
 template <int W, int NG>
@@ -536,12 +490,6 @@ constexpr int KP_WAVES = 8;
 constexpr int KP_ROWS = 32 * KP_WAVES;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ float halves_max(float v) {
-    const uint32_t x = __builtin_bit_cast(uint32_t, v);
-    auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
-}
-
 template <int TYPE, int W, int G>
 __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4AttendArgs a, KaPlan plan) {
     typedef typename KvElem<TYPE>::T T;
@@ -957,99 +905,6 @@ __global__ __launch_bounds__(KP_WAVES * 64) void k_kv4_prompt(Kv4View c, Kv4Atte
     }
 }
 
-// The key ranges' partial results of one (row, head), joined by a workgroup: the
-// ranges' factors first, then a wavefront every fourth range, eight loads at a
-// time (one wavefront in turn over the 256 ranges of a long sequence took 170 us).
-constexpr int KA_SPLITS = 512;
-template <int TYPE>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, Kv4AttendArgs a, int splits) {
-    typedef typename KvElem<TYPE>::T T;
-    __shared__ float f[KA_SPLITS], sv[4][256], st[4], ss[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t n = (int64_t)c.rows * a.heads, at = blockIdx.x;
-    const float* ml = reinterpret_cast<const float*>(a.ws);
-    const float* po = ml + 2 * n * splits + at * c.dv;
-    float top = -__builtin_inff();
-    for (int s = tid; s < splits; s += 256) {
-        f[s] = ml[2 * (s * n + at)];
-        top = fmaxf(top, f[s]);
-    }
-#pragma unroll
-    for (int h = 1; h < 64; h <<= 1) top = fmaxf(top, lane_xor(top, h, lane));
-    if (lane == 0) st[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(st[0], st[1]), fmaxf(st[2], st[3]));
-    const float zero = top == -__builtin_inff() ? 0.0f : top;
-    float sum = 0.0f;
-    for (int s = tid; s < splits; s += 256) {
-        // -1: a range without keys, which wrote no sums.  NaN: scores were, and the row's results are.
-        const float g = f[s] == -__builtin_inff() ? -1.0f : __builtin_amdgcn_exp2f(f[s] - zero);
-        f[s] = g;
-        sum += g < 0.0f ? 0.0f : ml[2 * (s * n + at) + 1] * g;
-    }
-#pragma unroll
-    for (int h = 1; h < 64; h <<= 1) sum += lane_xor(sum, h, lane);
-    if (lane == 0) ss[wave] = sum;
-    __syncthreads();
-    sum = (ss[0] + ss[1]) + (ss[2] + ss[3]);
-    for (int x = 0; x * 64 < c.dv; ++x) {
-        const int d = x * 64 + lane;
-        float v = 0.0f;
-        for (int s0 = wave; s0 < splits; s0 += 32) {
-            float y[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = s0 + 4 * k < splits && d < c.dv ? po[(s0 + 4 * k) * n * c.dv + d] : 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float g = s0 + 4 * k < splits ? f[s0 + 4 * k] : -1.0f;
-                v = g < 0.0f ? v : __builtin_fmaf(y[k], g, v);
-            }
-        }
-        sv[wave][d & 255] = v;
-    }
-    __syncthreads();
-    if (tid < c.dv) {
-        T* out = reinterpret_cast<T*>(a.out) + at / a.heads * a.ldo + at % a.heads * c.dv;
-        KvElem<TYPE>::put(out + tid, ((sv[0][tid] + sv[1][tid]) + (sv[2][tid] + sv[3][tid])) / sum);
-    }
-    if (a.lse && tid == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
-}
-
-// The same for few ranges, a thread an element of the output: many rows are many
-// elements, and a workgroup a (row, head) would mostly wait for its barriers (32,768
-// of two ranges).
-constexpr int KA_FEW = 8;
-template <int TYPE>
-__global__ __launch_bounds__(256) void k_kv4_join_few(Kv4View c, Kv4AttendArgs a, int splits) {
-    typedef typename KvElem<TYPE>::T T;
-    const int64_t n = (int64_t)c.rows * a.heads, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n * c.dv) return;
-    const int64_t at = i / c.dv;
-    const int d = (int)(i - at * c.dv);
-    const float* ml = reinterpret_cast<const float*>(a.ws);
-    const float* po = ml + 2 * n * splits + i;
-    float m[KA_FEW], l[KA_FEW], v[KA_FEW], top = -__builtin_inff();
-#pragma unroll
-    for (int s = 0; s < KA_FEW; ++s) {
-        const int64_t x = s < splits ? s : 0;
-        m[s] = s < splits ? ml[2 * (x * n + at)] : -__builtin_inff();
-        l[s] = ml[2 * (x * n + at) + 1];
-        v[s] = po[x * n * c.dv];
-        top = fmaxf(top, m[s]);
-    }
-    const float zero = top == -__builtin_inff() ? 0.0f : top;
-    float sum = 0.0f, o = 0.0f;
-#pragma unroll
-    for (int s = 0; s < KA_FEW; ++s) {
-        const float g = __builtin_amdgcn_exp2f(m[s] - zero);
-        const bool some = m[s] != -__builtin_inff();  // (a range without keys wrote no sums)
-        sum = some ? __builtin_fmaf(l[s], g, sum) : sum;
-        o = some ? __builtin_fmaf(v[s], g, o) : o;
-    }
-    KvElem<TYPE>::put(reinterpret_cast<T*>(a.out) + at / a.heads * a.ldo + at % a.heads * c.dv + d, o / sum);
-    if (a.lse && d == 0) a.lse[at] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
-}
-
 // The shape of a call: which kernel, its rows a tile and wavefronts, key ranges.
 struct KaShape {
     bool prompt;
@@ -1117,7 +972,7 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
     // 17.1), of four, whose join is larger beside its work, four.
     int64_t want = base ? std::max<int64_t>(1, slots / base) : 1;
     if (slots == 512 && want == 1 && base * 8 < slots * 5 && chunks >= 64) want = 2;  // (two workgroups share a CU)
-    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, KA_SPLITS), chunks / ((s.waves == 8 ? 2 : 4) * s.waves)));
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, KV_SPLITS), chunks / ((s.waves == 8 ? 2 : 4) * s.waves)));
 
     // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at
     // 256 dims its sums do not fit the registers.
@@ -1133,7 +988,7 @@ static KaShape shape_of(const Kv4View& c, const int* row0, int type, int heads, 
     const int64_t most = chunks_of(KP_ROWS, false), middle = chunks_of(KP_ROWS, true);
     const double each = c.width == 64 ? 1.0 : 1.3;
     double best = 0.0;
-    for (int64_t n = 1; n <= KA_FEW * 4 && (n == 1 || most / n >= 16); ++n) {
+    for (int64_t n = 1; n <= KV_FEW * 4 && (n == 1 || most / n >= 16); ++n) {
         const int64_t rounds = (p.tiles * c.heads * n + 255) / 256;
         const double us = 18.0 + (double)rounds * (double)(((rounds == 1 ? most : middle) + n - 1) / n) * each + ka_join_us(c, heads, n);
         if (n == 1 || us < best) best = us, p.splits = (int)n;
@@ -1173,11 +1028,11 @@ static hipError_t attend_shaped(const Kv4View& c, const int* row0, const Kv4Atte
             if (shape.rows == 32) kern = k_kv4_attend<TYPE, W, G, 2, 4>;
         hipLaunchKernelGGL(kern, grid, dim3(shape.waves * 64), 0, s, c, a, plan);
     }
-    if (plan.splits > KA_FEW)
-        hipLaunchKernelGGL(k_kv4_join<TYPE>, dim3((unsigned)(c.rows * a.heads)), dim3(256), 0, s, c, a, plan.splits);
-    else if (plan.splits > 1)
-        hipLaunchKernelGGL(k_kv4_join_few<TYPE>, dim3((unsigned)(((int64_t)c.rows * a.heads * c.dv + 255) / 256)), dim3(256), 0, s, c, a,
-                           plan.splits);
+    if (plan.splits > 1) {
+        if (const hipError_t e = hipGetLastError()) return e;
+        return launch_kv_join({a.out, a.lse, reinterpret_cast<const float*>(a.ws), (int64_t)c.rows * a.heads, a.ldo, a.heads, c.dv, plan.splits},
+                              TYPE, s);
+    }
     return hipGetLastError();
 }
 

@@ -207,6 +207,22 @@ struct Kv4Book {
         return 0;
     }
 
+    // rows[i] rows for each sequence that are queries alone: the batch, and no positions.
+    int ask(const int* s, const int* rows, int n) {
+        int64_t total = 0;
+        for (int i = 0; i < n; ++i) {
+            if (!live(s[i])) return refuse(INVALID, "no such sequence");
+            if (rows[i] < 0) return refuse(INVALID, "a negative number of rows");
+            total += rows[i];
+        }
+        if (!distinct(s, n)) return refuse(INVALID, "a sequence is named twice");
+        if (total > INT32_MAX) return refuse(INVALID, "too many rows");
+        batch_seq.assign(s, s + n);
+        batch_row0.assign(1, 0);
+        for (int i = 0; i < n; ++i) batch_row0.push_back(batch_row0.back() + rows[i]);
+        return 0;
+    }
+
     // Sequence s[i] keeps its positions of counts[i] ascending, disjoint
     // ranges [ranges[2 j], ranges[2 j + 1]), closed up.  Leading pages that
     // stay whole stay; the others' kept positions move to fresh pages.  `moves`

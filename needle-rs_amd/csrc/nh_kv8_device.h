@@ -1,0 +1,24 @@
+// Device helpers of the 8-bit cache's kernels.
+#pragma once
+
+#include "nh_kv8.h"
+#include "nh_kv_device.h"
+
+namespace nh {
+
+// A chunk of the cache: where its parts lie, in bytes from its start.
+template <int WK, int WV>
+struct Kv8Lay {
+    static constexpr int NJ = WK / 64, NV = WV / 16;
+    static constexpr uint32_t VALUES = 64 * WK, RECORD = 64 * (WK + WV), CHUNK = RECORD + sizeof(Kv8Record);
+    // dims 64 j + 16 kg + 0 .. 15 of position 16 t + o
+    static __device__ __forceinline__ uint32_t k_piece(int t, int j, int lane) { return (uint32_t)(t * NJ + j) * 1024 + lane * 16; }
+    // dim 16 n + o, all positions of lane (o, kg); 4 positions of block t at + 4 t
+    static __device__ __forceinline__ uint32_t v_piece(int n, int lane) { return VALUES + (uint32_t)n * 1024 + lane * 16; }
+};
+
+__device__ __forceinline__ uint8_t* kv8_block(const Kv8View& c, int page, int layer, int head) {
+    return c.data + (((size_t)page * c.layers + layer) * c.heads + head) * c.block();
+}
+
+}  // namespace nh

@@ -109,6 +109,24 @@ SIGNATURES = {
     "nh_kv4_attend": (I, [P, I, P, C.c_int64, I, C.c_float, I, I, P, C.c_int64, P, I, P, C.c_uint64, P]),
     "nh_verify_drafts_ws_bytes": (C.c_int64, [I, I, I]),
     "nh_verify_drafts": (I, [P, I, C.c_int64, P, P, P, I, C.c_int64, P, C.c_float, I, I, I, P, P, P, C.c_uint64, P]),
+    "nh_kv8_new": (I, [I] * 8 + [P]),
+    "nh_kv8_free": (I, [P]),
+    "nh_kv8_bytes": (C.c_int64, [P]),
+    "nh_kv8_free_pages": (I, [P]),
+    "nh_kv8_seq_new": (I, [P]),
+    "nh_kv8_seq_len": (I, [P, I]),
+    "nh_kv8_seq_free": (I, [P, I]),
+    "nh_kv8_seq_truncate": (I, [P, I, I]),
+    "nh_kv8_seq_fork": (I, [P, I, I, P]),
+    "nh_kv8_seq_copy": (I, [P, I, P]),
+    "nh_kv8_extend": (I, [P, P, P, I, P]),
+    "nh_kv8_ask": (I, [P, P, P, I, P]),
+    "nh_kv8_rows": (I, [P]),
+    "nh_kv8_append": (I, [P, I, P, P, C.c_int64, C.c_int64, I, P, P, P, C.c_int64, I, P, C.c_int64, P]),
+    "nh_kv8_read": (I, [P, I, P, P, P, I, P, P, I, P]),
+    "nh_kv8_debug_kernel": (I, [P, I]),
+    "nh_kv8_attend_ws_bytes": (C.c_int64, [P, I, I, I]),
+    "nh_kv8_attend": (I, [P, I, P, C.c_int64, I, C.c_float, I, I, P, C.c_int64, P, I, P, C.c_uint64, P]),
     "nh_rope_freqs": (I, [I, C.c_double, I, C.c_double, C.c_double, C.c_double, C.c_double, P, P]),
     "nh_rope_new": (I, [P, I, C.c_double, I, P]),
     "nh_rope_free": (I, [P]),
@@ -760,4 +778,5 @@ def seeded_normals(sizes, seed: int = 0):
 
 
 from .kv4 import KvCache4, _DraftCheck, verify_drafts  # noqa: E402,F401
+from .kv8 import KvCache8  # noqa: E402,F401
 from .rope import Rope  # noqa: E402,F401

@@ -9,7 +9,7 @@ import torch
 
 import needle_hip as nh
 
-from .kv4 import _TYPES, _on
+from .kvcache import _TYPES, _on
 
 _LAYOUTS = {"half": 0, "interleaved": 1}  # NH_ROPE_HALF, NH_ROPE_INTERLEAVED
 # NH_ROPE_LINEAR .., and the turns (low, high) where none are given
