@@ -80,75 +80,61 @@ __device__ __forceinline__ void kv8_take8(const typename KvElem<TYPE>::T* __rest
 
 // ----------------------------------------------------------------- append
 struct Kv8AppendPlan {
-    int each;               // chunks of every sequence, when all have the same rows (the most), else 0
-    int veck, vecv;         // rows of k, of v can be taken 8 (4) elements at a time
-    int k_share, v_share, q_share;  // heads a workgroup takes
-    int k_parts, v_parts, q_parts;  // workgroups a chunk
-    RopePlan rope;          // of the queries
-    int wide;               // .. 4 pairs a thread
+    int blocks_each, chunks_each;  // blocks of 16 and chunks of 64 of every sequence, when all have the same rows (the most), else 0
+    int veck, vecv;                // rows of k can be taken 8, rows of v 4 elements at a time
+    int k_parts, q_parts;          // workgroups a block for the heads of the keys, of the queries
+    int q_share;                   // query heads a workgroup takes
+    int k_grid, v_grid;            // workgroups of the keys, of the values; the queries' come after them
+    RopePlan rope;                 // of the queries
+    int wide, widek;               // .. and of the keys: four pairs a thread
 };
+constexpr int KV8_HEADS = 4;  // of the keys a workgroup takes, a wavefront each
 
-__host__ __device__ inline int kv8_most_chunks(int rows) { return rows ? (rows + 62) / 64 + 1 : 0; }
+// The most blocks (chunks) of 2^LOG positions that rows of a sequence can lie in.
+template <int LOG>
+__host__ __device__ inline int kv8_most(int rows) {
+    return rows ? ((rows + (1 << LOG) - 2) >> LOG) + 1 : 0;
+}
+
+// Unit `unit` of all sequences' blocks of 2^LOG positions: the new rows in it.
+struct Kv8Unit {
+    bool some;
+    int seq, pos0, lo, hi;  // slots lo .. hi of the block from pos0 on
+    int64_t row0;           // the row of slot 0
+};
+template <int LOG>
+__device__ __forceinline__ Kv8Unit kv8_unit(const Kv8View& c, int unit, int each, int lane) {
+    Kv8Unit u;
+    u.some = false;
+    int b;
+    if (each) {
+        b = unit / each;
+        unit -= b * each;
+    } else
+        b = kv_find(c, unit, lane, [](const KvEntry& e) { return kv8_most<LOG>(e.row1 - e.row0); });
+    if (b >= c.nb) return u;
+    const KvEntry e = kv_batch(c, b);
+    const int first = e.len - (e.row1 - e.row0);  // the position of row row0
+    u.seq = e.seq;
+    u.pos0 = ((first >> LOG) + unit) << LOG;
+    u.lo = max(first - u.pos0, 0);
+    u.hi = min(e.len - 1 - u.pos0, (1 << LOG) - 1);
+    u.row0 = (int64_t)e.row0 + u.pos0 - first;
+    u.some = kv_current(c) && first >= 0 && u.lo <= u.hi && e.row1 <= c.rows;
+    return u;
+}
 
 // One block of keys by one wavefront: lane (o, kg) has position o, 16 dims of
-// each 64 from 16 kg on: the bytes that it stores are one piece of its own.
-template <int TYPE, int WK, int WV, int TURN>
-__device__ __forceinline__ void kv8_put_keys(const typename KvElem<TYPE>::T* __restrict__ x, int dim, bool vec, uint8_t* chunk,
-                                             int t, int lo, int hi, int lane, const RopeView& r, const float2* cs) {
+// each 64 from 16 kg on (v, 0 where there is none): the bytes that it stores are
+// one piece of its own.
+template <int WK, int WV>
+__device__ __forceinline__ void kv8_put_keys(float (&v)[WK / 64][16], uint8_t* chunk, int t, int lo, int hi, int lane) {
     typedef Kv8Lay<WK, WV> L;
-    const int o = lane & 15, kg = lane >> 4;
+    const int o = lane & 15;
     const bool live = o >= lo && o <= hi;
     Kv8Record* rec = reinterpret_cast<Kv8Record*>(chunk + L::RECORD);
     const float old = lo ? rec->ks[t] : 0.0f;
     const uint32_t old_bad = lo ? rec->kbad[t] & ((1u << lo) - 1u) : 0u;
-    float v[L::NJ][16];
-#pragma unroll
-    for (int j = 0; j < L::NJ; ++j)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const int d = 64 * j + 16 * kg + 8 * g;
-            float* y = v[j] + 8 * g;
-            if (!live) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = 0.0f;
-                continue;
-            }
-            kv8_take8<TYPE>(x, d, dim, vec, y);
-            if constexpr (TURN == 1) {  // pairs (i, i + pairs)
-                if (d < 2 * r.pairs) {
-                    float z[8];
-                    // (eight dims on one side of the pairs, or some on each)
-                    const bool whole = r.pairs % 8 == 0;
-                    if (whole)
-                        kv8_take8<TYPE>(x, d < r.pairs ? d + r.pairs : d - r.pairs, dim, vec, z);
-                    else
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int at = d + e < r.pairs ? d + e + r.pairs : d + e - r.pairs;
-                            z[e] = d + e < 2 * r.pairs ? KvElem<TYPE>::get(x + at) : 0.0f;
-                        }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const bool second = d + e >= r.pairs;
-                        const int i = second ? d + e - r.pairs : d + e;
-                        if (i < r.pairs) {
-                            const float2 w = cs[i];
-                            const float2 both = second ? rope_turn(z[e], y[e], w) : rope_turn(y[e], z[e], w);
-                            y[e] = second ? both.y : both.x;
-                        }
-                    }
-                }
-            } else if constexpr (TURN == 2) {  // neighbours
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const int i = (d + e) / 2;
-                    if (i < r.pairs) {
-                        const float2 both = rope_turn(y[e], y[e + 1], cs[i]);
-                        y[e] = both.x, y[e + 1] = both.y;
-                    }
-                }
-            }
-        }
     float most = 0.0f;
     int bad = 0;
 #pragma unroll
@@ -194,10 +180,11 @@ __device__ __forceinline__ void kv8_put_keys(const typename KvElem<TYPE>::T* __r
 }
 
 // One block of values: lane (c, a) has dims 4 c .. of positions 4 a ..: turned
-// four by four, its words are whole too.
+// four by four, its words are whole too.  A whole chunk's go to `img`, which its
+// workgroup stores 16 bytes a lane.
 template <int TYPE, int WK, int WV>
 __device__ __forceinline__ void kv8_put_values(const typename KvElem<TYPE>::T* __restrict__ x, int64_t ld, int dim, bool vec,
-                                               uint8_t* chunk, int t, int lo, int hi, int lane) {
+                                               uint8_t* chunk, uint8_t* img, int t, int lo, int hi, int lane) {
     typedef typename KvElem<TYPE>::T T;
     typedef T Vec __attribute__((ext_vector_type(4)));
     typedef Kv8Lay<WK, WV> L;
@@ -214,12 +201,10 @@ __device__ __forceinline__ void kv8_put_values(const typename KvElem<TYPE>::T* _
     for (int r = 0; r < 4; ++r) {
         const int slot = 4 * a + r;
         const bool live = slot >= lo && slot <= hi;
-        int wrong = 0;
-        float top = 0.0f;
+        const T* p = x + (int64_t)slot * ld;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const int d = 64 * n + 4 * c;
-            const T* p = x + (int64_t)slot * ld;
             if (vec) {
                 Vec y = {};
                 if (live && d < dim) y = *reinterpret_cast<const Vec*>(p + d);
@@ -229,17 +214,26 @@ __device__ __forceinline__ void kv8_put_values(const typename KvElem<TYPE>::T* _
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[n][r][e] = live && d + e < dim ? KvElem<TYPE>::get(p + d + e) : 0.0f;
             }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        int wrong = 0;
+        float top = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 wrong |= !(fabsf(v[n][r][e]) < __builtin_inff());
                 top = fmaxf(top, fabsf(v[n][r][e]));
             }
-        }
         // (the row's sixteen lanes)
         const uint64_t which = __ballot(wrong != 0);
         bad[r] = (which >> (16 * a) & 0xffffu) != 0;
+        if (which) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) bads |= (which >> (16 * g) & 0xffffu) ? 1u << (4 * g + r) : 0u;
+            for (int g = 0; g < 4; ++g) bads |= (which >> (16 * g) & 0xffffu) ? 1u << (4 * g + r) : 0u;
+        }
         most = fmaxf(most, bad[r] ? 0.0f : top);
     }
     most = wave_max(most, lane);
@@ -251,11 +245,16 @@ __device__ __forceinline__ void kv8_put_values(const typename KvElem<TYPE>::T* _
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int d = 4 * c + e;  // of 64
-                uint32_t* p = reinterpret_cast<uint32_t*>(chunk + L::v_piece(4 * n + (d >> 4), 16 * a + (d & 15)) + 4 * t);
+                const uint32_t at = L::v_piece(4 * n + (d >> 4), 16 * a + (d & 15)) + 4 * t;
                 uint32_t y[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) y[r] = kv8_code(bad[r] ? 0.0f : v[n][r][e], s.inv);
                 uint32_t w = low_bytes(y[0], y[1], y[2], y[3]);
+                if (img) {
+                    *reinterpret_cast<uint32_t*>(img + at - L::VALUES) = w;
+                    continue;
+                }
+                uint32_t* p = reinterpret_cast<uint32_t*>(chunk + at);
                 if (before) {
                     uint32_t was = *p;
                     if (s.down) was = kv8_halved(was, s.down);
@@ -272,76 +271,188 @@ __device__ __forceinline__ void kv8_put_values(const typename KvElem<TYPE>::T* _
     }
 }
 
-// A workgroup takes one chunk of a sequence's new rows and some heads of the
-// keys, of the values or of the queries.  A wavefront has a block: its step is a
-// maximum over its own lanes, no workgroup shares a block, and no barrier is
-// needed but the one behind the table of cosines and sines of the chunk's
-// positions, worked out once for the workgroup's heads.
+// How keys find the other of a pair: interleaved, both are a lane's; in halves too
+// where there are 64 or 128 pairs; else by LDS.
+constexpr int KV8_APART = 1, KV8_NEIGHBOURS = 2, KV8_HALVES = 3;
+
+// The cosines and sines of a block's new rows, shared out over the threads:
+// [16][kv8_angles_ld] (rows apart by 16 bytes of the banks).
+__host__ __device__ __forceinline__ int kv8_angles_ld(int pairs) { return pairs + 2 - (pairs & 1); }
+__device__ __forceinline__ void kv8_angles(const Kv8Append& a, const Kv8Unit& u, float2* cs) {
+    const int pairs = a.r.pairs, ld = kv8_angles_ld(pairs);
+    for (int i = threadIdx.x; i < (u.hi - u.lo + 1) * pairs; i += 256) {
+        const int slot = u.lo + i / pairs, pair = i % pairs;
+        cs[slot * ld + pair] = rope_cos_sin(a.r.turns[pair], a.pos ? a.pos[u.row0 + slot] : u.pos0 + slot, a.r.amplitude);
+    }
+}
+
+// Rows of some heads' keys turned into LDS, f32 [head][16][LD]: a thread takes V
+// pairs (i, i + pairs) (or V dims behind them) of one row, for all the heads.
+template <int TYPE, int V, int LD>
+__device__ __forceinline__ void kv8_turn_keys(const typename KvElem<TYPE>::T* __restrict__ k, int64_t ld, int dim, int heads,
+                                              const Kv8Unit& u, int pairs, const float2* cs, float* to) {
+    typedef typename KvElem<TYPE>::T T;
+    typedef T Vec __attribute__((ext_vector_type(V)));
+    typedef float Out __attribute__((ext_vector_type(V)));
+    const int turned = pairs / V, units = turned + (dim - 2 * pairs) / V;
+    for (int i = threadIdx.x; i < (u.hi - u.lo + 1) * units; i += 256) {
+        const int slot = u.lo + i / units, n = i % units;
+        const bool turns = n < turned;
+        const int d0 = turns ? n * V : 2 * pairs + (n - turned) * V, d1 = turns ? d0 + pairs : d0;
+        const T* x = k + (u.row0 + slot) * ld;
+        float* y = to + slot * LD;
+        Vec x0[KV8_HEADS], x1[KV8_HEADS];
+#pragma unroll
+        for (int h = 0; h < KV8_HEADS; ++h) {
+            x0[h] = *reinterpret_cast<const Vec*>(x + (int64_t)min(h, heads - 1) * dim + d0);
+            x1[h] = *reinterpret_cast<const Vec*>(x + (int64_t)min(h, heads - 1) * dim + d1);
+        }
+        float2 w[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = turns ? cs[slot * kv8_angles_ld(pairs) + n * V + e] : float2{1.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < KV8_HEADS; ++h) {
+            Out y0, y1;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float2 z = rope_turn((float)x0[h][e], (float)x1[h][e], w[e]);
+                y0[e] = turns ? z.x : (float)x0[h][e], y1[e] = z.y;
+            }
+            *reinterpret_cast<Out*>(y + h * 16 * LD + d0) = y0;
+            if (turns) *reinterpret_cast<Out*>(y + h * 16 * LD + d1) = y1;
+        }
+    }
+}
+
+// A workgroup takes
+//   a block of 16 positions and four heads of the keys, a wavefront a head.  Turned
+//   keys: the block's cosines and sines through LDS, shared out over the threads;
+//   where a pair's dims are not one lane's, the heads' rows go through LDS too;
+//   a chunk of 64 positions and one head of the values, a wavefront a block;
+//   a block of 16 positions and some heads of the queries.
+// A block's step is a maximum over one wavefront's lanes, and no two workgroups
+// share a block, so rows that join one are stored by reading, halving and writing
+// it.
 template <int TYPE, int WK, int WV, int TURN>
 __global__ __launch_bounds__(256) void k_kv8_append(Kv8View c, Kv8Append a, Kv8AppendPlan p) {
     typedef typename KvElem<TYPE>::T T;
     typedef Kv8Lay<WK, WV> L;
-    extern __shared__ float2 cs[];  // [64][pairs + 1]
+    constexpr int LD = WK + 4;
+    extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int parts = p.k_parts + p.v_parts + p.q_parts;
-    int part = blockIdx.x % parts, unit = blockIdx.x / parts, b;
-    if (p.each) {
-        b = unit / p.each;
-        unit -= b * p.each;
-    } else
-        b = kv_find(c, unit, lane, [](const KvEntry& e) { return kv8_most_chunks(e.row1 - e.row0); });
-    if (b >= c.nb) return;
-    const KvEntry e = kv_batch(c, b);
-    const int first = e.len - (e.row1 - e.row0);  // the position of row row0
-    const int pos0 = ((first >> 6) + unit) << 6, lo = max(first - pos0, 0), hi = min(e.len - 1 - pos0, 63);
-    if (!kv_current(c) || first < 0 || lo > hi || e.row1 > c.rows) return;
-    const int64_t row0 = (int64_t)e.row0 + pos0 - first;  // of slot 0
-
-    if constexpr (TURN != 0) {
-        if (part >= p.k_parts + p.v_parts) {
-            const int h0 = (part - p.k_parts - p.v_parts) * p.q_share, h1 = min(h0 + p.q_share, a.q.heads);
-            const RopeArgs q{a.r, nullptr, a.q, RopeRows{}, 0, c.dk, 0};
-            for (int i = tid; i < (hi - lo + 1) * p.rope.units; i += 256) {
-                const int slot = lo + i / p.rope.units, u = i % p.rope.units;
-                const int64_t row = row0 + slot;
-                const int pos = a.pos ? a.pos[row] : pos0 + slot;
-                if (p.wide)
-                    rope_rows<TYPE, 4, TURN == 2>(q, p.rope, row, u, pos, h0, h1);
-                else
-                    rope_rows<TYPE, 1, TURN == 2>(q, p.rope, row, u, pos, h0, h1);
-            }
-            return;
-        }
-    }
-    const int pg = kv_page(c, e.seq, pos0);
-    if (pg < 0) return;
-    const uint32_t at = (uint32_t)((pos0 & (c.page() - 1)) >> 6) * L::CHUNK;
-    const bool keys = part < p.k_parts;
-    if (!keys) part -= p.k_parts;
-    const int share = keys ? p.k_share : p.v_share;
-    const int h0 = part * share, h1 = min(h0 + share, c.heads);
-    if constexpr (TURN != 0) {
-        if (keys) {
-            const int n = (hi - lo + 1) * a.r.pairs;
-            for (int i = tid; i < n; i += 256) {
-                const int slot = lo + i / a.r.pairs, pair = i % a.r.pairs;
-                cs[slot * (a.r.pairs + 1) + pair] =
-                    rope_cos_sin(a.r.turns[pair], a.pos ? a.pos[row0 + slot] : pos0 + slot, a.r.amplitude);
-            }
+    int bid = blockIdx.x;
+    if (bid < p.k_grid) {
+        const int h0 = bid % p.k_parts * KV8_HEADS, heads = min(KV8_HEADS, c.heads - h0);
+        const Kv8Unit u = kv8_unit<4>(c, bid / p.k_parts, p.blocks_each, lane);
+        if (!u.some) return;
+        const int pg = kv_page(c, u.seq, u.pos0);
+        if (pg < 0) return;
+        const T* k = reinterpret_cast<const T*>(a.k) + (int64_t)h0 * c.dk;
+        float v[L::NJ][16];
+        const int o = lane & 15, kg = lane >> 4;
+        const bool live = o >= u.lo && o <= u.hi;
+        if constexpr (TURN == KV8_APART) {
+            float* rows = reinterpret_cast<float*>(lds);
+            float2* cs = reinterpret_cast<float2*>(rows + KV8_HEADS * 16 * LD);
+            kv8_angles(a, u, cs);
             __syncthreads();
-        }
-    }
-    const int t = wave, blo = max(lo - 16 * t, 0), bhi = min(hi - 16 * t, 15);
-    if (blo > bhi) return;
-    for (int h = h0; h < h1; ++h) {
-        uint8_t* chunk = kv8_block(c, pg, a.layer, h) + at;
-        if (keys) {
-            const int slot = 16 * t + (lane & 15);
-            const T* x = reinterpret_cast<const T*>(a.k) + (row0 + slot) * a.ldk + (int64_t)h * c.dk;
-            kv8_put_keys<TYPE, WK, WV, TURN>(x, c.dk, p.veck, chunk, t, blo, bhi, lane, a.r, cs + slot * (a.r.pairs + 1));
+            if (p.widek)
+                kv8_turn_keys<TYPE, 4, LD>(k, a.ldk, c.dk, heads, u, a.r.pairs, cs, rows);
+            else
+                kv8_turn_keys<TYPE, 1, LD>(k, a.ldk, c.dk, heads, u, a.r.pairs, cs, rows);
+            __syncthreads();
+            if (wave >= heads) return;
+            const float* x = rows + (wave * 16 + o) * LD;
+#pragma unroll
+            for (int j = 0; j < L::NJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = 64 * j + 16 * kg + 4 * i;
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(x + d);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[j][4 * i + e] = live && d + e < c.dk ? y[e] : 0.0f;
+                }
         } else {
-            const T* x = reinterpret_cast<const T*>(a.v) + (row0 + 16 * t) * a.ldv + (int64_t)h * c.dv;
-            kv8_put_values<TYPE, WK, WV>(x, a.ldv, c.dv, p.vecv, chunk, t, blo, bhi, lane);
+            const T* x = k + (u.row0 + o) * a.ldk + (int64_t)min(wave, heads - 1) * c.dk;
+#pragma unroll
+            for (int j = 0; j < L::NJ; ++j)
+#pragma unroll
+                for (int g = 0; g < 2; ++g) kv8_take8<TYPE>(x, 64 * j + 16 * kg + 8 * g, live ? c.dk : 0, p.veck, v[j] + 8 * g);
+            if constexpr (TURN != 0) {
+                float2* cs = reinterpret_cast<float2*>(lds);
+                kv8_angles(a, u, cs);
+                __syncthreads();
+                const float2* w = cs + o * kv8_angles_ld(a.r.pairs);
+                if (live) {
+                    if constexpr (TURN == KV8_NEIGHBOURS) {
+#pragma unroll
+                        for (int j = 0; j < L::NJ; ++j)
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                const int i = (64 * j + 16 * kg + e) / 2;
+                                if (i < a.r.pairs) {
+                                    const float2 z = rope_turn(v[j][e], v[j][e + 1], w[i]);
+                                    v[j][e] = z.x, v[j][e + 1] = z.y;
+                                }
+                            }
+                    } else {  // (KV8_HALVES: pairs is a multiple of 64, so both of a pair are this lane's)
+                        const auto turn = [&](float (&y)[16], float (&z)[16], int j) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float2 both = rope_turn(y[e], z[e], w[64 * j + 16 * kg + e]);
+                                y[e] = both.x, z[e] = both.y;
+                            }
+                        };
+                        if (a.r.pairs == 64) {
+                            if constexpr (L::NJ >= 2) turn(v[0], v[1], 0);
+                        } else if constexpr (L::NJ >= 4) {
+                            turn(v[0], v[2], 0);
+                            turn(v[1], v[3], 1);
+                        }
+                    }
+                }
+            }
+            if (wave >= heads) return;
+        }
+        uint8_t* chunk = kv8_block(c, pg, a.layer, h0 + wave) + (uint32_t)((u.pos0 & (c.page() - 1)) >> 6) * L::CHUNK;
+        kv8_put_keys<WK, WV>(v, chunk, u.pos0 >> 4 & 3, u.lo, u.hi, lane);
+        return;
+    }
+    bid -= p.k_grid;
+    if (bid < p.v_grid) {
+        const int h = bid % c.heads;
+        const Kv8Unit u = kv8_unit<6>(c, bid / c.heads, p.chunks_each, lane);
+        if (!u.some) return;
+        const int pg = kv_page(c, u.seq, u.pos0);
+        if (pg < 0) return;
+        uint8_t* chunk = kv8_block(c, pg, a.layer, h) + (uint32_t)((u.pos0 & (c.page() - 1)) >> 6) * L::CHUNK;
+        const bool whole = u.lo == 0 && u.hi == 63;
+        const int t = wave, lo = max(u.lo - 16 * t, 0), hi = min(u.hi - 16 * t, 15);
+        if (lo <= hi) {
+            const T* x = reinterpret_cast<const T*>(a.v) + (u.row0 + 16 * t) * a.ldv + (int64_t)h * c.dv;
+            kv8_put_values<TYPE, WK, WV>(x, a.ldv, c.dv, p.vecv, chunk, whole ? lds : nullptr, t, lo, hi, lane);
+        }
+        if (whole) {
+            __syncthreads();
+            for (int i = tid; i < 4 * WV; i += 256)
+                reinterpret_cast<u32x4*>(chunk + L::VALUES)[i] = reinterpret_cast<const u32x4*>(lds)[i];
+        }
+        return;
+    }
+    if constexpr (TURN != 0) {
+        bid -= p.v_grid;
+        const int h0 = bid % p.q_parts * p.q_share, h1 = min(h0 + p.q_share, a.q.heads);
+        const Kv8Unit u = kv8_unit<4>(c, bid / p.q_parts, p.blocks_each, lane);
+        if (!u.some) return;
+        const RopeArgs q{a.r, nullptr, a.q, RopeRows{}, 0, c.dk, 0};
+        for (int i = tid; i < (u.hi - u.lo + 1) * p.rope.units; i += 256) {
+            const int slot = u.lo + i / p.rope.units, n = i % p.rope.units;
+            const int64_t row = u.row0 + slot;
+            const int pos = a.pos ? a.pos[row] : u.pos0 + slot;
+            if (p.wide)
+                rope_rows<TYPE, 4, TURN == KV8_NEIGHBOURS>(q, p.rope, row, n, pos, h0, h1);
+            else
+                rope_rows<TYPE, 1, TURN == KV8_NEIGHBOURS>(q, p.rope, row, n, pos, h0, h1);
         }
     }
 }
@@ -349,46 +460,57 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8View c, Kv8Append a, Kv8A
 template <int TYPE, int WK, int WV>
 static hipError_t append_typed(const Kv8View& c, const int* row0, const Kv8Append& a, hipStream_t s) {
     const size_t es = sizeof(typename KvElem<TYPE>::T);
-    Kv8AppendPlan p;
-    p.each = kv8_most_chunks(c.each);
-    int64_t units = (int64_t)p.each * c.nb;
-    if (!p.each)
-        for (int b = 0; b < c.nb; ++b) units += kv8_most_chunks(row0[b + 1] - row0[b]);
+    Kv8AppendPlan p = {};
+    p.blocks_each = kv8_most<4>(c.each);
+    p.chunks_each = kv8_most<6>(c.each);
+    int64_t blocks = (int64_t)p.blocks_each * c.nb, chunks = (int64_t)p.chunks_each * c.nb;
+    if (!c.each)
+        for (int b = 0; b < c.nb; ++b) {
+            blocks += kv8_most<4>(row0[b + 1] - row0[b]);
+            chunks += kv8_most<6>(row0[b + 1] - row0[b]);
+        }
     p.veck = c.dk % 8 == 0 && (uintptr_t)a.k % 16 == 0 && a.ldk * es % 16 == 0 && c.dk * es % 16 == 0;
     p.vecv = c.dv % 4 == 0 && (uintptr_t)a.v % (4 * es) == 0 && a.ldv % 4 == 0;
     const bool turn = a.r.turns != nullptr;
-    p.k_share = p.v_share = 1;
-    p.q_share = 0;
-    p.k_parts = (c.heads + p.k_share - 1) / p.k_share;
-    p.v_parts = (c.heads + p.v_share - 1) / p.v_share;
-    p.q_parts = 0;
-    p.rope = RopePlan{};
-    p.wide = 0;
-    if (turn && a.q.heads) {
-        const RopeArgs q{a.r, nullptr, a.q, RopeRows{}, 0, c.dk, 0};
-        p.wide = rope_takes4(q, es);
-        p.rope = rope_plan(q, p.wide ? 4 : 1);
-        p.q_share = std::min(a.q.heads, 8);
-        p.q_parts = (a.q.heads + p.q_share - 1) / p.q_share;
+    p.k_parts = (c.heads + KV8_HEADS - 1) / KV8_HEADS;
+    const int64_t k_grid = blocks * p.k_parts, v_grid = chunks * c.heads;
+    if (turn) {
+        const RopeArgs k{a.r, nullptr, {a.k, nullptr, a.ldk, 4, c.heads}, RopeRows{}, 0, c.dk, 0};
+        p.widek = rope_takes4(k, es);
+        if (a.q.heads) {
+            const RopeArgs q{a.r, nullptr, a.q, RopeRows{}, 0, c.dk, 0};
+            p.wide = rope_takes4(q, es);
+            p.rope = rope_plan(q, p.wide ? 4 : 1);
+            p.q_share = std::min(a.q.heads, 8);
+            p.q_parts = (a.q.heads + p.q_share - 1) / p.q_share;
+        }
     }
-    const int64_t blocks = units * (p.k_parts + p.v_parts + p.q_parts);
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const size_t lds = turn ? (size_t)64 * (a.r.pairs + 1) * sizeof(float2) : 0;
-    auto kern = !turn              ? k_kv8_append<TYPE, WK, WV, 0>
-                : a.r.interleaved ? k_kv8_append<TYPE, WK, WV, 2>
-                                  : k_kv8_append<TYPE, WK, WV, 1>;
+    const int64_t grid = k_grid + v_grid + blocks * p.q_parts;
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    p.k_grid = (int)k_grid;
+    p.v_grid = (int)v_grid;
+    const int how = !turn ? 0 : a.r.interleaved ? KV8_NEIGHBOURS : a.r.pairs % 64 == 0 ? KV8_HALVES : KV8_APART;
+    // keys' rows and angles, or a chunk's values
+    const size_t angles = turn ? (size_t)16 * kv8_angles_ld(a.r.pairs) * sizeof(float2) : 0;
+    const size_t lds = std::max<size_t>(64 * WV, angles + (how == KV8_APART ? (size_t)KV8_HEADS * 16 * (WK + 4) * 4 : 0));
+    auto kern = how == 0                ? k_kv8_append<TYPE, WK, WV, 0>
+                : how == KV8_NEIGHBOURS ? k_kv8_append<TYPE, WK, WV, KV8_NEIGHBOURS>
+                                        : k_kv8_append<TYPE, WK, WV, KV8_APART>;
+    if constexpr (WK >= 128)
+        if (how == KV8_HALVES) kern = k_kv8_append<TYPE, WK, WV, KV8_HALVES>;
     if (lds > 65536) {
         // (more than a kernel may have without being asked for it)
         if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds))
             return e;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, s, c, a, p);
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, s, c, a, p);
     return hipGetLastError();
 }
 
 // ------------------------------------------------------------------- read
 // A workgroup reads one head's rows of one chunk, a wavefront a block: keys as
-// their lanes hold them, values four positions by four dims.
+// their lanes hold them, values four positions by four dims, their pieces 16 bytes
+// a lane by LDS.
 template <int TYPE, int WK, int WV>
 __global__ __launch_bounds__(256) void k_kv8_read(Kv8View c, int layer0, KvSpans p, int64_t rows, int64_t row_at,
                                                   typename KvElem<TYPE>::T* __restrict__ k,
@@ -407,6 +529,10 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8View c, int layer0, KvSpans
     const uint8_t* chunk = kv8_block(c, pg, layer0 + (int)blockIdx.y, head) + (uint32_t)((pos0 & (c.page() - 1)) >> 6) * L::CHUNK;
     const Kv8Record* rec = reinterpret_cast<const Kv8Record*>(chunk + L::RECORD);
     const int64_t row = (int64_t)blockIdx.y * rows + row_at + p.row0[b] + (pos0 - first);  // of slot 0
+    __shared__ __align__(16) uint8_t img[64 * WV];
+    for (int i = tid; i < 4 * WV; i += 256)
+        reinterpret_cast<u32x4*>(img)[i] = reinterpret_cast<const u32x4*>(chunk + L::VALUES)[i];
+    __syncthreads();
     if (16 * t > hi || 16 * t + 15 < lo) return;
     const float nan = __builtin_nanf("");
     {
@@ -446,7 +572,7 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8View c, int layer0, KvSpans
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            w[e] = *reinterpret_cast<const uint32_t*>(chunk + L::v_piece(4 * n + (cc >> 2), 16 * a + 4 * (cc & 3) + e) + 4 * t);
+            w[e] = *reinterpret_cast<const uint32_t*>(img + L::v_piece(4 * n + (cc >> 2), 16 * a + 4 * (cc & 3) + e) - L::VALUES + 4 * t);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int in = 4 * a + r, slot = 16 * t + in;

@@ -65,7 +65,7 @@ class KvCache8(PagedCache):
                 raise ValueError("q and k differ in type")
             if out is None:
                 with _on(stream):
-                    out = torch.empty((self._rows, heads, self.qk_dim), dtype=t, device=self.device)
+                    out = torch.empty_like(q, memory_format=torch.contiguous_format)
                 ldo = heads * self.qk_dim
             else:
                 ldo = self._rows_of(out, heads, self.qk_dim, "out")

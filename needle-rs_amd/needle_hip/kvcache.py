@@ -61,6 +61,14 @@ class PagedCache:
         self.device = torch.device("cuda", torch.cuda.current_device())
         self._index = self.device.index
         self._rows = 0  # the batch's
+        self._like = {}
+
+    def _empty(self, shape, dtype):
+        """torch.empty on the cache's device, a microsecond sooner: like a tensor that is there."""
+        t = self._like.get(dtype)
+        if t is None:
+            t = self._like[dtype] = torch.empty(0, dtype=dtype, device=self.device)
+        return t.new_empty(shape)
 
     # ---- sequences
     def new_seq(self) -> int:
@@ -145,8 +153,7 @@ class PagedCache:
         n = sum(x for x in r if x > 0)
         shape = (n, self.kv_heads) if layer is not None else (self.layers, n, self.kv_heads)
         with _on(stream):
-            k = torch.empty((*shape, self.qk_dim), dtype=dtype, device=self.device)
-            v = torch.empty((*shape, self.v_dim), dtype=dtype, device=self.device)
+            k, v = self._empty((*shape, self.qk_dim), dtype), self._empty((*shape, self.v_dim), dtype)
         nh._check(self._c.read(self.h, -1 if layer is None else int(layer), ps, pp, pr, count, k.data_ptr(),
                                       v.data_ptr(), _TYPES[dtype], nh._stream(stream)))
         return k, v
@@ -162,7 +169,7 @@ class PagedCache:
         ldq = self._rows_of(q, heads, self.qk_dim, "q")
         with _on(stream):
             if out is None:
-                out, ldo = torch.empty((self._rows, heads, self.v_dim), dtype=q.dtype, device=self.device), heads * self.v_dim
+                out, ldo = q.new_empty((self._rows, heads, self.v_dim)), heads * self.v_dim
             else:
                 ldo = self._rows_of(out, heads, self.v_dim, "out")
                 if out.dtype != q.dtype:
@@ -173,7 +180,7 @@ class PagedCache:
             n = self._c.attend_ws_bytes(self.h, heads, int(sink), int(ring))
             if n < 0:
                 nh._check(int(n))
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+            ws = self._empty((n,), torch.uint8) if n else None
         nh._check(self._c.attend(self.h, int(layer), q.data_ptr(), ldq, heads,
                                         float(self.qk_dim ** -0.5 if scale is None else scale), int(sink), int(ring),
                                         out.data_ptr(), ldo, _ptr(lse), _TYPES[q.dtype], _ptr(ws), n, nh._stream(stream)))

@@ -16,15 +16,16 @@ _LAYOUTS = {"half": 0, "interleaved": 1}  # NH_ROPE_HALF, NH_ROPE_INTERLEAVED
 _SCALINGS = {"linear": (1, None), "base": (2, None), "parts": (3, (1.0, 32.0)), "bands": (4, (1.0, 4.0))}
 
 
-def _row_stride(t: torch.Tensor, rows: int, dim, index: int, what: str) -> int:
+def _row_stride(t: torch.Tensor, rows: int, dim: int, index: int, dtype, what: str) -> int:
     """The row stride of [rows][heads][dim]; a row lies in one piece."""
-    if len(t.shape) != 3 or t.shape[0] != rows or (dim is not None and t.shape[2] != dim):
-        raise ValueError(f"{what} is [{rows}][heads][{'dim' if dim is None else dim}], not {list(t.shape)}")
-    if t.get_device() != index or t.dtype not in _TYPES:
-        raise ValueError(f"{what} is f32, f16 or bf16 on the plan's device")
-    _, heads, dim = t.shape
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != rows or shape[2] != dim:
+        raise ValueError(f"{what} is [{rows}][heads][{dim}], not {list(shape)}")
+    if t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{what} is of q's type, f32, f16 or bf16, on the plan's device")
+    heads = shape[1]
     ld, of_head, of_dim = t.stride()
-    if (dim > 1 and of_dim != 1) or (heads > 1 and of_head != dim):
+    if (of_dim != 1 and dim > 1) or (of_head != dim and heads > 1):
         raise ValueError(f"a row of {what} is not contiguous")
     return ld if rows > 1 else heads * dim
 
@@ -74,7 +75,7 @@ class Rope:
         self._index = self.device.index
 
     def _positions(self, positions: torch.Tensor, rows: int):
-        if positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous() or \
+        if positions.dtype is not torch.int32 or positions.shape != (rows,) or not positions.is_contiguous() or \
                 positions.get_device() != self._index:
             raise ValueError(f"positions: contiguous int32 [{rows}] on {self.device}")
         return positions.data_ptr()
@@ -87,30 +88,43 @@ class Rope:
         new ones); q itself and k itself turn in place.  transposed: gradients of
         the outputs to the inputs' (the same angles backwards).  Returns q's
         rows, with k the pair."""
-        rows = q.shape[0]
+        if len(q.shape) != 3:
+            raise ValueError(f"q is [rows][heads][dim], not {list(q.shape)}")
+        rows, heads, dim = q.shape
+        dtype, index = q.dtype, self._index
+        if dtype not in _TYPES:
+            raise ValueError("q is f32, f16 or bf16")
         pos = self._positions(positions, rows)
-        given = (q,) if k is None else (q, k)
-        outs = (None,) * len(given) if out is None else (out,) if k is None else tuple(out)
-        if len(outs) != len(given):
-            raise ValueError("one out for each of q and k")
-        args, made = [], []
-        dim = q.shape[2] if len(q.shape) == 3 else None
-        with _on(stream):
-            for x, y, what in zip(given, outs, ("q", "k")):
-                ld = _row_stride(x, rows, dim, self._index, what)
-                if x.dtype != q.dtype:
-                    raise ValueError("q and k differ in type")
-                if y is None:
-                    y = torch.empty(x.shape, dtype=x.dtype, device=self.device)
-                elif y.dtype != x.dtype or y.shape != x.shape:
-                    raise ValueError(f"{what} and its out differ in type or shape")
-                made.append(y)
-                args += (x.data_ptr(), ld, x.shape[1], y.data_ptr(), _row_stride(y, rows, dim, self._index, "out"))
+        ldq = _row_stride(q, rows, dim, index, dtype, "q")
+        ldk = kv_heads = 0
+        if k is not None:
+            ldk = _row_stride(k, rows, dim, index, dtype, "k")
+            kv_heads = k.shape[1]
+        if out is None:
+            with _on(stream):
+                out = qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+                ldqo = heads * dim
+                if k is not None:
+                    ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+                    ldko, out = kv_heads * dim, (qo, ko)
+        else:
+            if k is None:
+                qo = out
+            else:
+                qo, ko = out
+                if ko.shape != k.shape:
+                    raise ValueError("k and its out differ in shape")
+                ldko = _row_stride(ko, rows, dim, index, dtype, "out")
+            if qo.shape != q.shape:
+                raise ValueError("q and its out differ in shape")
+            ldqo = _row_stride(qo, rows, dim, index, dtype, "out")
         if k is None:
-            args += (None, 0, 0, None, 0)
-        nh._check(nh._lib.nh_rope_apply(self.h, pos, rows, dim, *args, _TYPES[q.dtype], int(bool(transposed)),
-                                        nh._stream(stream)))
-        return made[0] if k is None else tuple(made)
+            args = (None, 0, 0, None, 0)
+        else:
+            args = (k.data_ptr(), ldk, kv_heads, ko.data_ptr(), ldko)
+        nh._check(nh._lib.nh_rope_apply(self.h, pos, rows, dim, q.data_ptr(), ldq, heads, qo.data_ptr(), ldqo, *args, _TYPES[dtype],
+                                        1 if transposed else 0, nh._stream(stream)))
+        return out
 
     def __del__(self):
         if getattr(self, "h", None) and nh is not None and nh._lib is not None:
