@@ -19,11 +19,9 @@
 #include <algorithm>
 
 #include "nh_kv8_device.h"
-#include "nh_kv_attend.h"
 
 namespace nh {
 
-typedef KaSpanOf<KV8_CHUNK> Ka8Span;
 typedef int i32x4_ __attribute__((ext_vector_type(4)));
 
 // What a lane loads of a chunk.
@@ -33,15 +31,6 @@ struct Ka8Chunk {
     f32x4 ks, vs;
     u32x4 bad;  // 4 u16 of the keys, 4 of the values
 };
-
-// Four codes as f16: bytes 0, 1 and 2, 3.
-__device__ __forceinline__ h2 codes2(uint32_t w, uint32_t which) {
-    return __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, which)) + (_Float16)-1152.0f;
-}
-__device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
-    const h2 w = codes2(a, 0x04010400u), x = codes2(a, 0x04030402u), y = codes2(b, 0x04010400u), z = codes2(b, 0x04030402u);
-    return h8{w[0], w[1], x[0], x[1], y[0], y[1], z[0], z[1]};
-}
 
 // NW wavefronts a workgroup, each every NW-th chunk of the range; RT tiles of 16 rows.
 template <int TYPE, int WK, int WV, int RT, int NW>
@@ -372,8 +361,9 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
     }
 }
 
-// The shape of a call: its rows a tile and wavefronts, key ranges.
+// The shape of a call: which kernel, its rows a tile and wavefronts, key ranges.
 struct Ka8Shape {
+    bool prompt;
     int rows, waves, tiles_each, splits;
     int64_t tiles;
 };
@@ -393,6 +383,15 @@ static Ka8Shape shape_of(const Kv8View& c, const int* row0, int type, int heads,
     const int per = heads / c.heads;
     const int64_t tokens = c.nb ? (c.rows + c.nb - 1) / c.nb : 0;
     Ka8Shape s;
+    s.prompt = false;
+    if (type != KV_F32 && c.wk <= 128 && c.kernel != 1 && c.nb && ((int64_t)c.rows * per / c.nb >= 128 || c.kernel == 2)) {
+        s.prompt = true;
+        s.waves = 0;
+        s.splits = 1;
+        tiles_of(c, row0, per, 128, s);
+        if (s.tiles * c.heads > 256) tiles_of(c, row0, per, 256, s);
+        return s;
+    }
     tiles_of(c, row0, per, 16, s);
     const int64_t base = s.tiles * c.heads;
     s.waves = c.wk <= 128 && base <= 256 ? 8 : 4;
@@ -412,6 +411,13 @@ size_t kv8_attend_ws(const Kv8View& c, const int* row0, int heads, int sink, int
     return s > 1 ? (size_t)s * c.rows * heads * (c.dv + 2) * 4 : 0;
 }
 
+static hipError_t joined(const Kv8View& c, const Kv8AttendArgs& a, const KaPlan& plan, int type, hipStream_t s) {
+    if (const hipError_t e = hipGetLastError()) return e;
+    if (plan.splits == 1) return hipSuccess;
+    return launch_kv_join({a.out, a.lse, reinterpret_cast<const float*>(a.ws), (int64_t)c.rows * a.heads, a.ldo, a.heads, c.dv, plan.splits},
+                          type, s);
+}
+
 template <int TYPE, int WK, int WV>
 static hipError_t attend_shaped(const Kv8View& c, const int* row0, const Kv8AttendArgs& a, int longest, hipStream_t s) {
     const Ka8Shape shape = shape_of(c, row0, TYPE, a.heads, a.sink, a.ring, longest);
@@ -423,16 +429,16 @@ static hipError_t attend_shaped(const Kv8View& c, const int* row0, const Kv8Atte
     plan.out_aligned = c.dv % 4 == 0 && (uintptr_t)a.out % 16 == 0 && a.ldo * es % 16 == 0;
     if (shape.tiles * c.heads > 0x7fffffff || (int64_t)c.rows * a.heads > 0x7fffffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(shape.tiles * c.heads), plan.splits);
+    if constexpr (WK <= 128 && TYPE != KV_F32)
+        if (shape.prompt) {
+            if (const hipError_t e = launch_kv8_prompt(c, a, plan, shape.tiles * c.heads, shape.rows, s)) return e;
+            return joined(c, a, plan, TYPE, s);
+        }
     auto kern = k_kv8_attend<TYPE, WK, WV, 1, 4>;
     if constexpr (WK <= 128)
         if (shape.waves == 8) kern = k_kv8_attend<TYPE, WK, WV, 1, 8>;
     hipLaunchKernelGGL(kern, grid, dim3(shape.waves * 64), 0, s, c, a, plan);
-    if (plan.splits > 1) {
-        if (const hipError_t e = hipGetLastError()) return e;
-        return launch_kv_join({a.out, a.lse, reinterpret_cast<const float*>(a.ws), (int64_t)c.rows * a.heads, a.ldo, a.heads, c.dv, plan.splits},
-                              TYPE, s);
-    }
-    return hipGetLastError();
+    return joined(c, a, plan, TYPE, s);
 }
 
 template <int TYPE>

@@ -2,7 +2,7 @@
 #pragma once
 
 #include "nh_kv8.h"
-#include "nh_kv_device.h"
+#include "nh_kv_attend.h"
 
 namespace nh {
 
@@ -19,6 +19,17 @@ struct Kv8Lay {
 
 __device__ __forceinline__ uint8_t* kv8_block(const Kv8View& c, int page, int layer, int head) {
     return c.data + (((size_t)page * c.layers + layer) * c.heads + head) * c.block();
+}
+
+typedef KaSpanOf<KV8_CHUNK> Ka8Span;
+
+// Four codes as f16: bytes 0, 1 and 2, 3.
+__device__ __forceinline__ h2 codes2(uint32_t w, uint32_t which) {
+    return __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, which)) + (_Float16)-1152.0f;
+}
+__device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
+    const h2 w = codes2(a, 0x04010400u), x = codes2(a, 0x04030402u), y = codes2(b, 0x04010400u), z = codes2(b, 0x04030402u);
+    return h8{w[0], w[1], x[0], x[1], y[0], y[1], z[0], z[1]};
 }
 
 }  // namespace nh
