@@ -511,8 +511,16 @@ static hipError_t append_typed(const Kv8View& c, const int* row0, const Kv8Appen
 // A workgroup reads one head's rows of one chunk, a wavefront a block: keys as
 // their lanes hold them, values four positions by four dims, their pieces 16 bytes
 // a lane by LDS.
-template <int TYPE, int WK, int WV>
-__global__ __launch_bounds__(256) void k_kv8_read(Kv8View c, int layer0, KvSpans p, int64_t rows, int64_t row_at,
+// Few spans are few arguments: a launch's are read from host memory (3.9 KB of them
+// make a microsecond of a read of 8 rows).
+struct Kv8FewSpans {
+    static constexpr int MAX = 16;
+    int n;
+    int seq[MAX], pos[MAX], row0[MAX + 1], unit0[MAX + 1];
+};
+
+template <int TYPE, int WK, int WV, class Spans>
+__global__ __launch_bounds__(256) void k_kv8_read(Kv8View c, int layer0, Spans p, int64_t rows, int64_t row_at,
                                                   typename KvElem<TYPE>::T* __restrict__ k,
                                                   typename KvElem<TYPE>::T* __restrict__ v, int veck, int vecv) {
     typedef typename KvElem<TYPE>::T T;
@@ -599,8 +607,17 @@ static hipError_t read_typed(const Kv8View& c, int layer, const KvSpans& p, int6
     const int veck = c.dk % 8 == 0 && (uintptr_t)k % 16 == 0, vecv = c.dv % 4 == 0 && (uintptr_t)v % (4 * sizeof(T)) == 0;
     const int64_t blocks = (int64_t)p.unit0[p.n] * c.heads;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_kv8_read<TYPE, WK, WV>), dim3((unsigned)blocks, layer < 0 ? c.layers : 1), dim3(256), 0, s, c,
-                       layer < 0 ? 0 : layer, p, rows, row, (T*)k, (T*)v, veck, vecv);
+    const dim3 grid((unsigned)blocks, layer < 0 ? c.layers : 1);
+    if (p.n <= Kv8FewSpans::MAX) {
+        Kv8FewSpans few;
+        few.n = p.n;
+        for (int i = 0; i < p.n; ++i) few.seq[i] = p.seq[i], few.pos[i] = p.pos[i];
+        for (int i = 0; i <= p.n; ++i) few.row0[i] = p.row0[i], few.unit0[i] = p.unit0[i];
+        hipLaunchKernelGGL((k_kv8_read<TYPE, WK, WV, Kv8FewSpans>), grid, dim3(256), 0, s, c, layer < 0 ? 0 : layer, few, rows, row,
+                           (T*)k, (T*)v, veck, vecv);
+    } else
+        hipLaunchKernelGGL((k_kv8_read<TYPE, WK, WV, KvSpans>), grid, dim3(256), 0, s, c, layer < 0 ? 0 : layer, p, rows, row, (T*)k,
+                           (T*)v, veck, vecv);
     return hipGetLastError();
 }
 

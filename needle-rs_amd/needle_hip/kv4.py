@@ -35,7 +35,7 @@ class KvCache4(PagedCache):
         counts, pc, _ = _ints([len(r) for r in ranges])
         flat, pf, _ = _ints([x for r in ranges for pair in r for x in pair])
         nh._check(nh._lib.nh_kv4_seq_compact(self.h, ps, n, pc, pf, nh._stream(stream)))
-        self._rows = self.rows
+        self._batch(self.rows)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, stream=None):
         """The batch's keys [rows][kv_heads][qk_dim] and values [rows][kv_heads][v_dim]

@@ -6,7 +6,7 @@ import torch
 
 import needle_hip as nh
 
-from .kvcache import _TYPES, PagedCache, _ints, _on
+from .kvcache import _TYPES, PagedCache, _ints, _like, _on
 from .rope import Rope
 
 
@@ -33,7 +33,7 @@ class KvCache8(PagedCache):
         if n != m:
             raise ValueError("one number of rows for each sequence")
         nh._check(self._c.ask(self.h, ps, pr, n, nh._stream(stream)))
-        self._rows = sum(r)
+        self._batch(sum(r))
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rope: Rope | None = None,
                positions: torch.Tensor | None = None, q: torch.Tensor | None = None, out: torch.Tensor | None = None,
@@ -65,7 +65,7 @@ class KvCache8(PagedCache):
                 raise ValueError("q and k differ in type")
             if out is None:
                 with _on(stream):
-                    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                    out = _like(q)
                 ldo = heads * self.qk_dim
             else:
                 ldo = self._rows_of(out, heads, self.qk_dim, "out")

@@ -33,6 +33,11 @@ def _on(stream):
     return torch.cuda.stream(stream) if stream is not None else _here
 
 
+def _like(t):
+    """A new contiguous tensor like t."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -60,8 +65,13 @@ class PagedCache:
         self.page, self.pages = int(page), int(pages)
         self.device = torch.device("cuda", torch.cuda.current_device())
         self._index = self.device.index
-        self._rows = 0  # the batch's
         self._like = {}
+        self._batch(0)
+
+    def _batch(self, rows: int):
+        """Another batch, of so many rows."""
+        self._rows = rows
+        self._ws_bytes = {}  # of attend, by what it depends on beside the batch
 
     def _empty(self, shape, dtype):
         """torch.empty on the cache's device, a microsecond sooner: like a tensor that is there."""
@@ -81,24 +91,24 @@ class PagedCache:
     def free(self, seq: int):
         """Gives back the pages that no branch shares."""
         nh._check(self._c.seq_free(self.h, int(seq)))
-        self._rows = self.rows  # (the batch may be over)
+        self._batch(self.rows)  # (it may be over)
 
     def truncate(self, seq: int, length: int):
         """Forgets positions `length` and on."""
         nh._check(self._c.seq_truncate(self.h, int(seq), int(length)))
-        self._rows = self.rows
+        self._batch(self.rows)
 
     def fork(self, seq: int, n: int = 1) -> list:
         """n branches that share the sequence's pages until they are written."""
         out = (C.c_int * max(int(n), 1))()
         nh._check(self._c.seq_fork(self.h, int(seq), int(n), C.addressof(out)))
-        self._rows = self.rows
+        self._batch(self.rows)
         return out[:n]
 
     def copy(self, seq: int, stream=None) -> int:
         """A branch with pages of its own."""
         made = nh._check(self._c.seq_copy(self.h, int(seq), nh._stream(stream)))
-        self._rows = self.rows
+        self._batch(self.rows)
         return made
 
     @property
@@ -118,7 +128,7 @@ class PagedCache:
         if n != m:
             raise ValueError("one number of rows for each sequence")
         nh._check(self._c.extend(self.h, ps, pr, n, nh._stream(stream)))
-        self._rows = sum(r)
+        self._batch(sum(r))
 
     @property
     def rows(self) -> int:
@@ -177,9 +187,12 @@ class PagedCache:
             if lse is not None and (lse.dtype != torch.float32 or lse.shape != (q.shape[0], heads) or
                                     not lse.is_contiguous() or lse.get_device() != self._index):
                 raise ValueError("lse is a contiguous f32 [rows][heads]")
-            n = self._c.attend_ws_bytes(self.h, heads, int(sink), int(ring))
-            if n < 0:
-                nh._check(int(n))
+            n = self._ws_bytes.get((heads, sink, ring))
+            if n is None:
+                n = self._c.attend_ws_bytes(self.h, heads, int(sink), int(ring))
+                if n < 0:
+                    nh._check(int(n))
+                self._ws_bytes[heads, sink, ring] = n
             ws = self._empty((n,), torch.uint8) if n else None
         nh._check(self._c.attend(self.h, int(layer), q.data_ptr(), ldq, heads,
                                         float(self.qk_dim ** -0.5 if scale is None else scale), int(sink), int(ring),
@@ -189,6 +202,7 @@ class PagedCache:
     def debug_kernel(self, kernel: int):
         """Attention by one of its kernels (nh_kv4_debug_kernel, nh_kv8_debug_kernel); tests only."""
         nh._check(self._c.debug_kernel(self.h, int(kernel)))
+        self._ws_bytes = {}
 
     def __del__(self):
         if getattr(self, "h", None) and nh is not None and nh._lib is not None:

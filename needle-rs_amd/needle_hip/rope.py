@@ -9,7 +9,7 @@ import torch
 
 import needle_hip as nh
 
-from .kvcache import _TYPES, _on
+from .kvcache import _TYPES, _like, _on
 
 _LAYOUTS = {"half": 0, "interleaved": 1}  # NH_ROPE_HALF, NH_ROPE_INTERLEAVED
 # NH_ROPE_LINEAR .., and the turns (low, high) where none are given
@@ -102,10 +102,10 @@ class Rope:
             kv_heads = k.shape[1]
         if out is None:
             with _on(stream):
-                out = qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+                out = qo = _like(q)
                 ldqo = heads * dim
                 if k is not None:
-                    ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+                    ko = _like(k)
                     ldko, out = kv_heads * dim, (qo, ko)
         else:
             if k is None:
