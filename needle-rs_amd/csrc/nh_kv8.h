@@ -77,9 +77,11 @@ hipError_t launch_kv8_append(const Kv8View& c, const int* row0, const Kv8Append&
 // layer < 0: all, [layers][rows]; `rows` rows a layer in the output, this launch's from `row`.
 hipError_t launch_kv8_read(const Kv8View& c, int layer, const KvSpans& p, int64_t rows, int64_t row, void* k, void* v,
                            int type, hipStream_t s);
-// Attention by the kernel of many rows (f16 and bf16, dims up to 128): `tiles` workgroups of `rows` rows a range.
+// Attention by the kernel of many rows (f16 and bf16, dims up to 128): `tiles`
+// workgroups of KP8_ROWS rows a range of keys.
+constexpr int KP8_ROWS = 256;
 struct KaPlan;
-hipError_t launch_kv8_prompt(const Kv8View& c, const Kv8AttendArgs& a, const KaPlan& plan, int64_t tiles, int rows, hipStream_t s);
+hipError_t launch_kv8_prompt(const Kv8View& c, const Kv8AttendArgs& a, const KaPlan& plan, int64_t tiles, hipStream_t s);
 // Bytes of workspace an attention call of the batch needs; row0: the host's copy
 // of the sequences' first rows; longest: the batch's longest sequence.
 size_t kv8_attend_ws(const Kv8View& c, const int* row0, int heads, int sink, int ring, int longest);

@@ -22,7 +22,7 @@
 
 namespace nh {
 
-typedef int i32x4_ __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // What a lane loads of a chunk.
 template <int WK, int WV>
@@ -32,8 +32,8 @@ struct Ka8Chunk {
     u32x4 bad;  // 4 u16 of the keys, 4 of the values
 };
 
-// NW wavefronts a workgroup, each every NW-th chunk of the range; RT tiles of 16 rows.
-template <int TYPE, int WK, int WV, int RT, int NW>
+// NW wavefronts a workgroup, each every NW-th chunk of the range.
+template <int TYPE, int WK, int WV, int NW>
 __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8View c, Kv8AttendArgs a, KaPlan plan) {
     typedef typename KvElem<TYPE>::T T;
     typedef Kv8Lay<WK, WV> L;
@@ -56,96 +56,88 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
         b = tile / plan.tiles_each;
         tile -= b * plan.tiles_each;
     } else {
-        b = kv_find(c, tile, lane, [&](const KvEntry& e) { return ((e.row1 - e.row0) * per + 16 * RT - 1) / (16 * RT); });
+        b = kv_find(c, tile, lane, [&](const KvEntry& e) { return ((e.row1 - e.row0) * per + 15) / 16; });
     }
     if (b >= c.nb) return;
     const KvEntry entry = kv_batch(c, b);
     const int row0 = entry.row0, nrows = entry.row1 - row0, seq = entry.seq;
-    const int first = entry.len - (c.ask ? 1 : nrows), r0 = tile * 16 * RT;
+    const int first = entry.len - (c.ask ? 1 : nrows), r0 = tile * 16;
     if (!kv_current(c) || (!c.ask && first < 0) || r0 >= nrows * per || entry.row1 > c.rows) return;
-    const int r1 = min(r0 + 16 * RT, nrows * per) - 1;
+    const int r1 = min(r0 + 16, nrows * per) - 1;
     const int plo = first + (c.ask ? 0 : r0 / per), phi = first + (c.ask ? 0 : r1 / per);
 
     // The queries: f16 operands scaled by a power of two to just under 2^15, or digits.
-    h8 q[RT][NJ][2];
-    i32x4_ qd[RT][3][NJ];
-    float cq[RT];
-    int pos[RT];
+    h8 q[NJ][2];
+    i32x4 qd[3][NJ];
+    float cq;
+    const int r = min(r0 + o, r1), token = r / per, pos = first + (c.ask ? 0 : token);
+    const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(row0 + token) * a.ldq + (int64_t)(kvh * per + r - token * per) * c.dk;
+    float x[NJ][16], most = 0.0f;
+    bool nan = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = min(r0 + rt * 16 + o, r1), t = r / per;
-        pos[rt] = first + (c.ask ? 0 : t);
-        const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(row0 + t) * a.ldq + (int64_t)(kvh * per + r - t * per) * c.dk;
-        float x[NJ][16], most = 0.0f;
-        bool nan = false;
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int d = j * 64 + kg * 16 + g * 8;
+            if (plan.aligned) {
+                typedef T Vec __attribute__((ext_vector_type(8)));
+                Vec y = {};
+                if (d < c.dk) y = *reinterpret_cast<const Vec*>(src + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][8 * g + e] = (float)y[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][8 * g + e] = d + e < c.dk ? KvElem<TYPE>::get(src + d + e) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                most = fmaxf(most, fabsf(x[j][8 * g + e]));
+                nan |= x[j][8 * g + e] != x[j][8 * g + e];
+            }
+        }
+    if constexpr (DIGITS) {
+        most = nan ? __builtin_inff() : most;
+        most = groups_max(most);
+        // |x| <= most, as a whole number of at most 127 (2^16 + 2^8 + 1)
+        const float full = 8355711.0f;
+        const bool fine = most < __builtin_inff(), some = most > 0x1p-100f;
+        const float up = fine && some ? full / most : 0.0f;
+        // z = 2^-8 of the sum of whole numbers x codes
+        cq = fine ? (a.scale * KA_LOG2E) * (some ? most * (256.0f / full) : 0.0f) : __builtin_nanf("");
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int d = j * 64 + kg * 16 + g * 8;
-                if (plan.aligned) {
-                    typedef T Vec __attribute__((ext_vector_type(8)));
-                    Vec y = {};
-                    if (d < c.dk) y = *reinterpret_cast<const Vec*>(src + d);
+            for (int w = 0; w < 4; ++w) {
+                uint32_t d0 = 0, d1 = 0, d2 = 0;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[j][8 * g + e] = (float)y[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[j][8 * g + e] = d + e < c.dk ? KvElem<TYPE>::get(src + d + e) : 0.0f;
+                for (int e = 0; e < 4; ++e) {
+                    const int n = (int)rintf(__builtin_amdgcn_fmed3f(x[j][4 * w + e] * up, -full, full));
+                    const int lo = (int8_t)n, n1 = (n - lo) >> 8, mid = (int8_t)n1, hi = (n1 - mid) >> 8;
+                    d0 |= (uint32_t)(uint8_t)hi << (8 * e);
+                    d1 |= (uint32_t)(uint8_t)mid << (8 * e);
+                    d2 |= (uint32_t)(uint8_t)lo << (8 * e);
                 }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    most = fmaxf(most, fabsf(x[j][8 * g + e]));
-                    nan |= x[j][8 * g + e] != x[j][8 * g + e];
-                }
+                qd[0][j][w] = (int)d0;
+                qd[1][j][w] = (int)d1;
+                qd[2][j][w] = (int)d2;
             }
-        if constexpr (DIGITS) {
-            most = nan ? __builtin_inff() : most;
-            most = groups_max(most);
-            // |x| <= most, as a whole number of at most 127 (2^16 + 2^8 + 1)
-            const float full = 8355711.0f;
-            const bool fine = most < __builtin_inff(), some = most > 0x1p-100f;
-            const float up = fine && some ? full / most : 0.0f;
-            // z = 2^-8 of the sum of whole numbers x codes
-            cq[rt] = fine ? (a.scale * KA_LOG2E) * (some ? most * (256.0f / full) : 0.0f) : __builtin_nanf("");
+    } else {
+        most = groups_max(most);
+        const int ef = max((int)(__builtin_bit_cast(uint32_t, most) >> 23 & 255u), 15);
+        const float up = __builtin_bit_cast(float, (uint32_t)(268 - ef) << 23);
+        cq = (a.scale * KA_LOG2E) * __builtin_bit_cast(float, (uint32_t)(ef - 14) << 23);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint32_t d0 = 0, d1 = 0, d2 = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int n = (int)rintf(__builtin_amdgcn_fmed3f(x[j][4 * w + e] * up, -full, full));
-                        const int lo = (int8_t)n, n1 = (n - lo) >> 8, mid = (int8_t)n1, hi = (n1 - mid) >> 8;
-                        d0 |= (uint32_t)(uint8_t)hi << (8 * e);
-                        d1 |= (uint32_t)(uint8_t)mid << (8 * e);
-                        d2 |= (uint32_t)(uint8_t)lo << (8 * e);
-                    }
-                    qd[rt][0][j][w] = (int)d0;
-                    qd[rt][1][j][w] = (int)d1;
-                    qd[rt][2][j][w] = (int)d2;
-                }
-        } else {
-            most = groups_max(most);
-            const int ef = max((int)(__builtin_bit_cast(uint32_t, most) >> 23 & 255u), 15);
-            const float up = __builtin_bit_cast(float, (uint32_t)(268 - ef) << 23);
-            cq[rt] = (a.scale * KA_LOG2E) * __builtin_bit_cast(float, (uint32_t)(ef - 14) << 23);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) q[rt][j][e / 8][e % 8] = (_Float16)(x[j][e] * up);
-        }
+            for (int e = 0; e < 16; ++e) q[j][e / 8][e % 8] = (_Float16)(x[j][e] * up);
     }
 
-    f32x4 acc[RT][NV];
-    float m[RT], l[RT];
+    f32x4 acc[NV];
+    float m, l;
+    m = -__builtin_inff();
+    l = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -__builtin_inff();
-        l[rt] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) acc[rt][i] = f32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < NV; ++i) acc[i] = f32x4{0, 0, 0, 0};
     // The weights are kept as 2^15 p, and with their steps as the f16 operand 2^15 p
     // step / 2^eref, 2^eref above every step seen so far: at most 2^15, and exact to
     // 11 bits down to 2^-29 of it.
@@ -188,97 +180,86 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
             const float down = pow2i(max(eref - et, -126));
             eref = et;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int k = 0; k < NV; ++k) acc[rt][k] *= down;
+            for (int k = 0; k < NV; ++k) acc[k] *= down;
         }
         const float wscale = pow2i(-eref);
         float vstep[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) vstep[t] = key0 + 16 * t <= phi ? x.vs[t] * wscale : 0.0f;
-        f32x4 z[RT][4];
+        f32x4 z[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             if constexpr (DIGITS) {
-                i32x4_ n[RT][3] = {};
+                i32x4 n[3] = {};
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    const i32x4_ k = __builtin_bit_cast(i32x4_, x.k[t][j] ^ 0x80808080u);
+                    const i32x4 k = __builtin_bit_cast(i32x4, x.k[t][j] ^ 0x80808080u);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int d = 0; d < 3; ++d) n[rt][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, qd[rt][d][j], n[rt][d], 0, 0, 0);
+                    for (int d = 0; d < 3; ++d) n[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, qd[d][j], n[d], 0, 0, 0);
                 }
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        z[rt][t][r] = __builtin_fmaf((float)n[rt][2][r], 0x1p-8f, (float)(n[rt][0][r] * 256 + n[rt][1][r]));
+                for (int r = 0; r < 4; ++r)
+                    z[t][r] = __builtin_fmaf((float)n[2][r], 0x1p-8f, (float)(n[0][r] * 256 + n[1][r]));
             } else {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) z[rt][t] = f32x4{0, 0, 0, 0};
+                z[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
                         const h8 k = codes8(x.k[t][j][2 * g], x.k[t][j][2 * g + 1]);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) z[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rt][j][g], z[rt][t], 0, 0, 0);
+                        z[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[j][g], z[t], 0, 0, 0);
                     }
             }
         }
-        h8 pw[RT][2][WPARTS];
+        h8 pw[2][WPARTS];
+        const bool fresh = m == -__builtin_inff();  // no key seen yet
+        const float base = fresh ? 0.0f : m;
+        float s[4][4];  // 15 + log2 of the weight against the maximum so far
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const bool fresh = m[rt] == -__builtin_inff();  // no key seen yet
-            const float base = fresh ? 0.0f : m[rt];
-            float s[4][4];  // 15 + log2 of the weight against the maximum so far
+        for (int t = 0; t < 4; ++t) {
+            const float f = cq * x.ks[t];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][r] = __builtin_fmaf(z[t][r], f, 15.0f - base);
+        }
+        if (!plain) {
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const float f = cq[rt] * x.ks[t];
+                const uint32_t bad = (t & 2 ? bad1 : bad0) >> (16 * (t & 1)) >> (4 * kg);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][r] = __builtin_fmaf(z[rt][t][r], f, 15.0f - base);
-            }
-            if (!plain) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const uint32_t bad = (t & 2 ? bad1 : bad0) >> (16 * (t & 1)) >> (4 * kg);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = key0 + 16 * t + 4 * kg + r;
-                        const bool seen = (j <= pos[rt]) & ((j < sink) | (j > pos[rt] - ring));
-                        s[t][r] = !seen ? -__builtin_inff() : bad >> r & 1 ? __builtin_nanf("") : s[t][r];
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    const int j = key0 + 16 * t + 4 * kg + r;
+                    const bool seen = (j <= pos) & ((j < sink) | (j > pos - ring));
+                    s[t][r] = !seen ? -__builtin_inff() : bad >> r & 1 ? __builtin_nanf("") : s[t][r];
                 }
             }
-            float most = s[0][0];
+        }
+        float most = s[0][0];
 #pragma unroll
-            for (int k = 1; k < 16; ++k) most = fmaxf(most, s[k / 4][k % 4]);
-            most = groups_max(most);
-            if (__any(most > 15.0f || fresh)) {
-                // A new maximum (the first: whatever it is).
-                const float over = most == -__builtin_inff() ? 0.0f : fresh ? most - 15.0f : fmaxf(most - 15.0f, 0.0f);
-                const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
-                m[rt] = fresh && most == -__builtin_inff() ? m[rt] : base + over;
-                l[rt] *= keep;
+        for (int k = 1; k < 16; ++k) most = fmaxf(most, s[k / 4][k % 4]);
+        most = groups_max(most);
+        if (__any(most > 15.0f || fresh)) {
+            // A new maximum (the first: whatever it is).
+            const float over = most == -__builtin_inff() ? 0.0f : fresh ? most - 15.0f : fmaxf(most - 15.0f, 0.0f);
+            const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
+            m = fresh && most == -__builtin_inff() ? m : base + over;
+            l *= keep;
 #pragma unroll
-                for (int k = 0; k < NV; ++k) acc[rt][k] *= keep;
+            for (int k = 0; k < NV; ++k) acc[k] *= keep;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) s[k / 4][k % 4] -= over;
-            }
+            for (int k = 0; k < 16; ++k) s[k / 4][k % 4] -= over;
+        }
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-                const f32x2 p = {__builtin_amdgcn_exp2f(s[k / 4][k % 4]), __builtin_amdgcn_exp2f(s[k / 4][k % 4 + 1])};
-                l[rt] += p[0];
-                l[rt] += p[1];
-                const f32x2 w = {p[0] * vstep[k / 4], p[1] * vstep[k / 4]};
-                const h2 hi = __builtin_convertvector(w, h2);
-                pw[rt][k / 8][0][k % 8] = hi[0], pw[rt][k / 8][0][k % 8 + 1] = hi[1];
-                if constexpr (WPARTS == 2) {
-                    const f32x2 rest = {w[0] - (float)hi[0], w[1] - (float)hi[1]};
-                    const h2 lo = __builtin_convertvector(rest, h2);
-                    pw[rt][k / 8][1][k % 8] = lo[0], pw[rt][k / 8][1][k % 8 + 1] = lo[1];
-                }
+        for (int k = 0; k < 16; k += 2) {
+            const f32x2 p = {__builtin_amdgcn_exp2f(s[k / 4][k % 4]), __builtin_amdgcn_exp2f(s[k / 4][k % 4 + 1])};
+            l += p[0];
+            l += p[1];
+            const f32x2 w = {p[0] * vstep[k / 4], p[1] * vstep[k / 4]};
+            const h2 hi = __builtin_convertvector(w, h2);
+            pw[k / 8][0][k % 8] = hi[0], pw[k / 8][0][k % 8 + 1] = hi[1];
+            if constexpr (WPARTS == 2) {
+                const f32x2 rest = {w[0] - (float)hi[0], w[1] - (float)hi[1]};
+                const h2 lo = __builtin_convertvector(rest, h2);
+                pw[k / 8][1][k % 8] = lo[0], pw[k / 8][1][k % 8 + 1] = lo[1];
             }
         }
 #pragma unroll
@@ -287,10 +268,8 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
             for (int h = 0; h < 2; ++h) {
                 const h8 v = codes8(x.v[n][2 * h], x.v[n][2 * h + 1]);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int p = 0; p < WPARTS; ++p)
-                        acc[rt][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pw[rt][h][p], acc[rt][n], 0, 0, 0);
+                for (int p = 0; p < WPARTS; ++p)
+                    acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pw[h][p], acc[n], 0, 0, 0);
             }
     };
 
@@ -315,48 +294,44 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
         }
     }
 
-    // The wavefronts' sums joined, 16 rows at a time.
+    // The wavefronts' sums joined.
     const float unit = pow2i(eref);
+    l = groups_sum(l);
+    if (l != l) m = l;  // NaN scores: the row's, whatever other ranges hold
+    if (kg == 0) sm[wave][o] = m, sl[wave][o] = l * 0x1p-15f;
+    __syncthreads();
+    float high = sm[0][o];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        l[rt] = groups_sum(l[rt]);
-        if (l[rt] != l[rt]) m[rt] = l[rt];  // NaN scores: the row's, whatever other ranges hold
-        if (rt) __syncthreads();
-        if (kg == 0) sm[wave][o] = m[rt], sl[wave][o] = l[rt] * 0x1p-15f;
-        __syncthreads();
-        float most = sm[0][o];
+    for (int w = 1; w < NW; ++w) high = fmaxf(high, sm[w][o]);
+    const float base = high == -__builtin_inff() ? 0.0f : high;
+    const float f = __builtin_amdgcn_exp2f(m - base) * 0x1p-15f;
 #pragma unroll
-        for (int w = 1; w < NW; ++w) most = fmaxf(most, sm[w][o]);
-        const float base = most == -__builtin_inff() ? 0.0f : most;
-        const float f = __builtin_amdgcn_exp2f(m[rt] - base) * 0x1p-15f;
+    for (int n = 0; n < NV; ++n) *reinterpret_cast<f32x4*>(&so[wave][o][16 * n + 4 * kg]) = acc[n] * f * unit;
+    __syncthreads();
+    for (int at = tid; at < 16 * WV; at += NW * 64) {
+        const int rr = at / WV, d = at % WV;
+        if (r0 + rr > r1 || d >= c.dv) continue;
+        float top = sm[0][rr];
 #pragma unroll
-        for (int n = 0; n < NV; ++n) *reinterpret_cast<f32x4*>(&so[wave][o][16 * n + 4 * kg]) = acc[rt][n] * f * unit;
-        __syncthreads();
-        for (int x = tid; x < 16 * WV; x += NW * 64) {
-            const int rr = x / WV, d = x % WV, r = r0 + rt * 16 + rr;
-            if (r > r1 || d >= c.dv) continue;
-            float top = sm[0][rr];
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, sm[w][rr]);
+        const float zero = top == -__builtin_inff() ? 0.0f : top;
+        float sum = 0.0f, v = 0.0f;
 #pragma unroll
-            for (int w = 1; w < NW; ++w) top = fmaxf(top, sm[w][rr]);
-            const float zero = top == -__builtin_inff() ? 0.0f : top;
-            float sum = 0.0f, v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                sum = __builtin_fmaf(sl[w][rr], __builtin_amdgcn_exp2f(sm[w][rr] - zero), sum);
-                v += so[w][rr][d];
-            }
-            const int t = r / per, head = kvh * per + r - t * per;
-            const int64_t row = row0 + t;
-            if (plan.splits == 1) {
-                // (no key seen: 0)
-                KvElem<TYPE>::put(reinterpret_cast<T*>(a.out) + row * a.ldo + (int64_t)head * c.dv + d, sum == 0.0f ? 0.0f : v / sum);
-                if (a.lse && d == 0) a.lse[row * a.heads + head] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
-            } else {
-                const int64_t at = ((int64_t)split * c.rows + row) * a.heads + head;
-                float* ml = reinterpret_cast<float*>(a.ws);
-                ml[2 * ((int64_t)plan.splits * c.rows * a.heads) + at * c.dv + d] = v;
-                if (d == 0) ml[2 * at] = sum == sum ? top : sum, ml[2 * at + 1] = sum;
-            }
+        for (int w = 0; w < NW; ++w) {
+            sum = __builtin_fmaf(sl[w][rr], __builtin_amdgcn_exp2f(sm[w][rr] - zero), sum);
+            v += so[w][rr][d];
+        }
+        const int t = (r0 + rr) / per, head = kvh * per + r0 + rr - t * per;
+        const int64_t row = row0 + t;
+        if (plan.splits == 1) {
+            // (no key seen: 0)
+            KvElem<TYPE>::put(reinterpret_cast<T*>(a.out) + row * a.ldo + (int64_t)head * c.dv + d, sum == 0.0f ? 0.0f : v / sum);
+            if (a.lse && d == 0) a.lse[row * a.heads + head] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
+        } else {
+            const int64_t part = ((int64_t)split * c.rows + row) * a.heads + head;
+            float* ml = reinterpret_cast<float*>(a.ws);
+            ml[2 * ((int64_t)plan.splits * c.rows * a.heads) + part * c.dv + d] = v;
+            if (d == 0) ml[2 * part] = sum == sum ? top : sum, ml[2 * part + 1] = sum;
         }
     }
 }
@@ -379,29 +354,67 @@ static void tiles_of(const Kv8View& c, const int* row0, int per, int rows, Ka8Sh
         for (int b = 0; b < c.nb; ++b) s.tiles += ((int64_t)(row0[b + 1] - row0[b]) * per + rows - 1) / rows;
 }
 
+// Which kernel is the quicker depends on the rows, the keys and how both fill the
+// chip, so both are estimated, in us, from what was measured of each at 128 (64)
+// dims of bf16:
+//  rows   4 in all and 5 (3) a round of 512 workgroups of four wavefronts, 2.2 (1.4) a
+//         step of a wavefront: 64 keys of 16 rows
+//  prompt 4 in all and 8 (6) a round of a workgroup a CU, 2.0 (1.75) for 64 keys of
+//         256 rows
+//  join   4, and the partial results' bytes there and back at 2 TB/s
+// 32 heads over 8 of 128 dims, rows / prompt: a sequence of 4,000 keys 512 rows 85 / 75,
+// 1,024 142 / 111, 2,048 240 / 134; four of 1,500 keys 128 rows 43 / 56, 256 73 / 57; 16
+// of 2,000 keys 32 rows 52 / 68, 64 rows 96 / 73.  16 heads of 64: 16 sequences of 2,000
+// keys 128 rows 54 / 59, 256 99 / 65; four of 1,500 512 rows 44 / 50, 1,024 67 / 51.
+static double ka_join_us(const Kv8View& c, int heads, int64_t splits) {
+    return splits > 1 ? 4.0 + (double)c.rows * heads * (double)splits * (c.dv + 2) * 8 / 2e6 : 0.0;
+}
+
 static Ka8Shape shape_of(const Kv8View& c, const int* row0, int type, int heads, int sink, int ring, int longest) {
     const int per = heads / c.heads;
     const int64_t tokens = c.nb ? (c.rows + c.nb - 1) / c.nb : 0;
+    // The chunks that a tile of `rows` rows sees: the last tile's, and a middle one's.
+    auto chunks_of = [&](int rows, bool middle) -> int64_t {
+        const int64_t keys = longest - (middle && !c.ask ? tokens / 2 : 0), wide = c.ask ? 1 : std::min<int64_t>(tokens, rows / per + 1);
+        return ((ring ? std::min<int64_t>(keys, (int64_t)sink + ring + wide + 2 * KV8_CHUNK) : keys) + KV8_CHUNK - 1) / KV8_CHUNK;
+    };
     Ka8Shape s;
     s.prompt = false;
-    if (type != KV_F32 && c.wk <= 128 && c.kernel != 1 && c.nb && ((int64_t)c.rows * per / c.nb >= 128 || c.kernel == 2)) {
-        s.prompt = true;
-        s.waves = 0;
-        s.splits = 1;
-        tiles_of(c, row0, per, 128, s);
-        if (s.tiles * c.heads > 256) tiles_of(c, row0, per, 256, s);
-        return s;
-    }
     tiles_of(c, row0, per, 16, s);
     const int64_t base = s.tiles * c.heads;
+    // Eight wavefronts where the tiles leave CUs idle (one of 4,000 keys of 8 tiles: 23 us
+    // for 27): they meet in LDS and not in the workspace.
     s.waves = c.wk <= 128 && base <= 256 ? 8 : 4;
+    // Ranges of keys until every CU has its eight wavefronts (four at more than 128 dims,
+    // by their registers), a chunk each at least; two ranges are not worth the join (8
+    // tiles of 1,000 keys 10.7 us, in two 12.1; 4,000 keys in seven 12.1 for 23, 16,000 in
+    // 31 14.5 for 71).
     const int64_t slots = s.waves == 8 || c.wk > 128 ? 256 : 512;
-    const int64_t wide = std::min<int64_t>(tokens, s.rows / per + 1);
-    const int64_t keys = ring ? std::min<int64_t>(longest, (int64_t)sink + ring + wide + 2 * KV8_CHUNK) : longest;
-    const int64_t chunks = (keys + KV8_CHUNK - 1) / KV8_CHUNK;
-    const int64_t want = base ? std::max<int64_t>(1, slots / base) : 1;
-    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, KV_SPLITS), chunks / (2 * s.waves)));
-    return s;
+    const int64_t chunks = chunks_of(s.rows, false);
+    const int64_t most = std::min<int64_t>(std::min<int64_t>(base ? std::max<int64_t>(1, slots / base) : 1, KV_SPLITS), chunks / s.waves);
+    s.splits = most < 2 || (chunks < 4 * s.waves && most < 3) ? 1 : (int)most;
+
+    // f32 calls keep 22 bits of a weight, which the prompt kernel does not; at more than
+    // 128 dims its sums do not fit the registers, and it counts a page's bytes in 32 bits.
+    if (type == KV_F32 || c.wk > 128 || c.kernel == 1 || base == 0) return s;
+    if ((uint64_t)c.block() * c.heads * c.layers >> 32) return s;
+    const bool wide = c.wk == 128;
+    const double steps = (double)((chunks_of(s.rows, true) + s.splits * s.waves - 1) / (s.splits * s.waves));
+    const double plain = 4.0 + std::max(1.0, (double)(base * s.splits) / (double)slots) * (wide ? 5.0 + 2.2 * steps : 3.0 + 1.4 * steps) +
+                         ka_join_us(c, heads, s.splits);
+    Ka8Shape p;
+    p.prompt = true;
+    p.waves = 0;
+    tiles_of(c, row0, per, KP8_ROWS, p);
+    const int64_t last = chunks_of(KP8_ROWS, false), middle = chunks_of(KP8_ROWS, true);
+    double best = 0.0;
+    for (int64_t n = 1; n <= KV_FEW * 4 && (n == 1 || last / n >= 8); ++n) {
+        const int64_t rounds = (p.tiles * c.heads * n + 255) / 256;
+        const double each = (double)(((rounds == 1 ? last : middle) + n - 1) / n);
+        const double us = 4.0 + (double)rounds * (wide ? 8.0 + 2.0 * each : 6.0 + 1.75 * each) + ka_join_us(c, heads, n);
+        if (n == 1 || us < best) best = us, p.splits = (int)n;
+    }
+    return best < plain || c.kernel == 2 ? p : s;
 }
 
 size_t kv8_attend_ws(const Kv8View& c, const int* row0, int heads, int sink, int ring, int longest) {
@@ -431,12 +444,12 @@ static hipError_t attend_shaped(const Kv8View& c, const int* row0, const Kv8Atte
     const dim3 grid((unsigned)(shape.tiles * c.heads), plan.splits);
     if constexpr (WK <= 128 && TYPE != KV_F32)
         if (shape.prompt) {
-            if (const hipError_t e = launch_kv8_prompt(c, a, plan, shape.tiles * c.heads, shape.rows, s)) return e;
+            if (const hipError_t e = launch_kv8_prompt(c, a, plan, shape.tiles * c.heads, s)) return e;
             return joined(c, a, plan, TYPE, s);
         }
-    auto kern = k_kv8_attend<TYPE, WK, WV, 1, 4>;
+    auto kern = k_kv8_attend<TYPE, WK, WV, 4>;
     if constexpr (WK <= 128)
-        if (shape.waves == 8) kern = k_kv8_attend<TYPE, WK, WV, 1, 8>;
+        if (shape.waves == 8) kern = k_kv8_attend<TYPE, WK, WV, 8>;
     hipLaunchKernelGGL(kern, grid, dim3(shape.waves * 64), 0, s, c, a, plan);
     return joined(c, a, plan, TYPE, s);
 }

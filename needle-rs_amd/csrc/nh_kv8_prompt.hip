@@ -4,8 +4,8 @@
 
 namespace nh {
 
-// Many rows: a workgroup of four or eight wavefronts takes 32 rows a wavefront, and
-// the chunks' codes are turned into f16 operands once for all of them, through
+// Many rows: a workgroup of eight wavefronts takes 32 rows a wavefront, and the
+// chunks' codes are turned into f16 operands once for all of them, through
 // LDS.  32 x 32 MFMAs: a lane holds 16 of its row's scores with 32 keys, the other
 // half of them is 32 lanes away.
 //
@@ -16,6 +16,8 @@ namespace nh {
 // a row's weights x steps keep their 11 bits down to 2^-22 of the largest of them.  A
 // step below 2^-60 of the largest that the rows see counts as that.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int KP8_WAVES = 8;
+static_assert(KP8_ROWS == 32 * KP8_WAVES, "32 rows a wavefront");
 
 template <int W>
 struct Kp8Image {  // a chunk's operands, 16 bytes a lane each
@@ -26,16 +28,15 @@ struct Kp8Image {  // a chunk's operands, 16 bytes a lane each
     int first, pad;
 };
 
-template <int TYPE, int W, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void k_kv8_prompt(Kv8View c, Kv8AttendArgs a, KaPlan plan) {
+template <int TYPE, int W>
+__global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8AttendArgs a, KaPlan plan) {
     typedef typename KvElem<TYPE>::T T;
     typedef Kv8Lay<W, W> L;
     typedef Kp8Image<W> Image;
-    constexpr int NX = W / 16, ND = W / 32, ROWS = 32 * NW;
-    // A wavefront turns EACH pieces of the keys and of the values, or (APART) one of either.
-    constexpr int EACH = NX > NW ? NX / NW : 1;
+    constexpr int NX = W / 16, ND = W / 32, ROWS = KP8_ROWS, NW = KP8_WAVES;
+    // A wavefront turns a piece of the keys and one of the values, or (APART) one of either.
     constexpr bool APART = NX < NW;
-    static_assert(NX % EACH == 0 && (APART ? 2 * NX == NW : NX == EACH * NW), "every piece is turned once");
+    static_assert(APART ? 2 * NX == NW : NX == NW, "every piece is turned once");
     extern __shared__ __align__(16) uint8_t lds8[];
     Image* img = reinterpret_cast<Image*>(lds8);
 
@@ -106,10 +107,10 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv8_prompt(Kv8View c, Kv8AttendA
     const int page_log2 = c.page_log2, pages = c.pages, in_page = (c.page() >> 6) - 1;
     auto page_of = [&](int i) { return table[(span.at(min(i, last)) * KV8_CHUNK >> page_log2) + lane0]; };
     const uint8_t* base = kv8_block(c, 0, a.layer, kvh);
-    const uint32_t page_bytes = (uint32_t)(c.block() * c.heads * c.layers);  // (below 2^32: the launcher)
+    const uint32_t page_bytes = (uint32_t)(c.block() * c.heads * c.layers);  // (below 2^32: shape_of)
 
     struct Raw {
-        u32x4 k[EACH], v[EACH];
+        u32x4 k, v;
         uint32_t rec;  // a word of the record each lane: 4 steps of the keys, 4 of the values, 4 of marks
     };
     // Where chunk i lies (past the end: the last one again), and its loads.
@@ -118,31 +119,24 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv8_prompt(Kv8View c, Kv8AttendA
         return base + (uint64_t)known * page_bytes + (uint32_t)((span.at(min(i, last)) & in_page) * L::CHUNK);
     };
     auto load = [&](Raw& x, const uint8_t* p) {
-#pragma unroll
-        for (int u = 0; u < EACH; ++u) {
-            const int n = (wave & (NX / EACH - 1)) * EACH + u;
-            if (!APART || wave < NX) x.k[u] = *reinterpret_cast<const u32x4*>(p + n * 1024 + lane * 16);
-            if (!APART || wave >= NX) x.v[u] = *reinterpret_cast<const u32x4*>(p + L::v_piece(n, lane));
-        }
+        const int n = wave & (NX - 1);
+        if (!APART || wave < NX) x.k = *reinterpret_cast<const u32x4*>(p + n * 1024 + lane * 16);
+        if (!APART || wave >= NX) x.v = *reinterpret_cast<const u32x4*>(p + L::v_piece(n, lane));
         x.rec = *reinterpret_cast<const uint32_t*>(p + L::RECORD + 4 * (lane & 15));
     };
     // Step `step` of six of turning: two of a piece of the keys, four of one of the values.
     auto turn = [&](const Raw& x, Image& to, int step) {
-#pragma unroll
-        for (int u = 0; u < EACH; ++u) {
-            const int n = (wave & (NX / EACH - 1)) * EACH + u;
-            if (step < 2) {
-                // piece (t, j), 16 dims of position 16 t + o: the halves of the product's step 4 j + kg
-                const int t = n / L::NJ, j = n % L::NJ;
-                to.k[t >> 1][4 * j + kg][32 * step + 16 * (t & 1) + o] =
-                    __builtin_bit_cast(u32x4, codes8(x.k[u][2 * step], x.k[u][2 * step + 1]));
-            } else if (step < 6) {
-                // dim 16 n + o, four positions of a block
-                const int t = step - 2;
-                const h2 y = codes2(x.v[u][t], 0x04010400u), w = codes2(x.v[u][t], 0x04030402u);
-                const uint2 both = {__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, w)};
-                reinterpret_cast<uint2*>(&to.v[n >> 1][t][32 * (kg & 1) + 16 * (n & 1) + o])[kg >> 1] = both;
-            }
+        const int n = wave & (NX - 1);
+        if (step < 2) {
+            // piece (t, j), 16 dims of position 16 t + o: the halves of the product's step 4 j + kg
+            const int t = n / L::NJ, j = n % L::NJ;
+            to.k[t >> 1][4 * j + kg][32 * step + 16 * (t & 1) + o] = __builtin_bit_cast(u32x4, codes8(x.k[2 * step], x.k[2 * step + 1]));
+        } else if (step < 6) {
+            // dim 16 n + o, four positions of a block
+            const int t = step - 2;
+            const h2 y = codes2(x.v[t], 0x04010400u), w = codes2(x.v[t], 0x04030402u);
+            const uint2 both = {__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, w)};
+            reinterpret_cast<uint2*>(&to.v[n >> 1][t][32 * (kg & 1) + 16 * (n & 1) + o])[kg >> 1] = both;
         }
     };
     float top = 0.0f;  // the largest step so far
@@ -369,21 +363,21 @@ __global__ __launch_bounds__(NW * 64, 2) void k_kv8_prompt(Kv8View c, Kv8AttendA
 }
 
 template <int TYPE, int W>
-static hipError_t prompt_shaped(const Kv8View& c, const Kv8AttendArgs& a, const KaPlan& plan, int64_t tiles, int rows, hipStream_t s) {
-    auto kern = rows == 128 ? k_kv8_prompt<TYPE, W, 4> : k_kv8_prompt<TYPE, W, 8>;
+static hipError_t prompt_shaped(const Kv8View& c, const Kv8AttendArgs& a, const KaPlan& plan, int64_t tiles, hipStream_t s) {
+    auto kern = k_kv8_prompt<TYPE, W>;
     const int lds = 3 * (int)sizeof(Kp8Image<W>);
     // (more than a kernel may have without being asked for it)
     if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds))
         return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)tiles, plan.splits), dim3(2 * rows), lds, s, c, a, plan);
+    hipLaunchKernelGGL(kern, dim3((unsigned)tiles, plan.splits), dim3(KP8_WAVES * 64), lds, s, c, a, plan);
     return hipGetLastError();
 }
 
-hipError_t launch_kv8_prompt(const Kv8View& c, const Kv8AttendArgs& a, const KaPlan& plan, int64_t tiles, int rows, hipStream_t s) {
+hipError_t launch_kv8_prompt(const Kv8View& c, const Kv8AttendArgs& a, const KaPlan& plan, int64_t tiles, hipStream_t s) {
     if (a.type == KV_F32 || c.wk > 128) return hipErrorInvalidValue;
     if (c.wk == 64)
-        return a.type == KV_F16 ? prompt_shaped<KV_F16, 64>(c, a, plan, tiles, rows, s) : prompt_shaped<KV_BF16, 64>(c, a, plan, tiles, rows, s);
-    return a.type == KV_F16 ? prompt_shaped<KV_F16, 128>(c, a, plan, tiles, rows, s) : prompt_shaped<KV_BF16, 128>(c, a, plan, tiles, rows, s);
+        return a.type == KV_F16 ? prompt_shaped<KV_F16, 64>(c, a, plan, tiles, s) : prompt_shaped<KV_BF16, 64>(c, a, plan, tiles, s);
+    return a.type == KV_F16 ? prompt_shaped<KV_F16, 128>(c, a, plan, tiles, s) : prompt_shaped<KV_BF16, 128>(c, a, plan, tiles, s);
 }
 
 }  // namespace nh
