@@ -519,8 +519,7 @@ int nh_rope_apply(const nh_rope* r, const int32_t* pos, int64_t rows, int dim, c
  * `pages` pages of `page` (64, 128 or 256) positions; up to `seqs` sequences of
  * up to `cap` positions (rounded up to pages).  One position of a layer's head
  * takes WK + WV + 2 bytes, (64, 64), (128, 128), (192, 128) or (256, 256) the
- * first that holds both dims.  The only call that
- * allocates. */
+ * first that holds both dims.  The only call that allocates. */
 int nh_kv8_new(int layers, int kv_heads, int qk_dim, int v_dim, int page, int pages, int seqs, int cap, nh_kv8** c);
 int nh_kv8_free(nh_kv8* c);
 /* As the 4-bit cache's calls of the same names. */
@@ -558,8 +557,12 @@ int nh_kv8_read(nh_kv8* c, int layer, const int* seqs, const int* pos, const int
  * first `sink` and the last `ring` positions.  Scores, weights' sums and
  * products are held in f32.  f16 and bf16 queries enter as they are, f32 ones
  * to 2^-24 of a row's largest; f32 and f16 calls carry 22 bits of a weight x
- * its value's step, bf16 calls and calls of many f16 rows 11 (of many rows also
- * of a value's step x code), none finer than 2^-40 of the largest step. */
+ * its value's step, bf16 calls and calls of many f16 rows 11, none finer than
+ * 2^-40 of the largest step (of many rows 2^-33 of the row's largest weight x
+ * step, and a step below 2^-60 of the largest weighs as that).  A row's sum of
+ * weights x values, before its division by the weights' sum, has to fit f32.
+ * NH_EDEVICE from 2^23 tiles of 16 rows x heads on (nh_kv8_append: 2^29 rows x
+ * heads): more than a launch takes. */
 int64_t nh_kv8_attend_ws_bytes(const nh_kv8* c, int heads, int sink, int ring);
 int nh_kv8_attend(const nh_kv8* c, int layer, const void* q, int64_t ldq, int heads, float scale, int sink, int ring,
                   void* out, int64_t ldo, float* lse, int type, void* ws, uint64_t ws_bytes, void* stream);

@@ -33,7 +33,8 @@
 
 namespace nh {
 
-constexpr int KV8_BLOCK = 16, KV8_CHUNK = 64;
+constexpr int KV8_CHUNK = 64;
+constexpr int64_t KV8_THREADS = 0xffffffff;  // that a launch can have in x
 
 struct Kv8Record {
     float ks[4], vs[4];

@@ -486,7 +486,7 @@ static hipError_t append_typed(const Kv8View& c, const int* row0, const Kv8Appen
         }
     }
     const int64_t grid = k_grid + v_grid + blocks * p.q_parts;
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    if (grid > KV8_THREADS / 256) return hipErrorInvalidValue;
     p.k_grid = (int)k_grid;
     p.v_grid = (int)v_grid;
     const int how = !turn ? 0 : a.r.interleaved ? KV8_NEIGHBOURS : a.r.pairs % 64 == 0 ? KV8_HALVES : KV8_APART;
@@ -606,7 +606,7 @@ static hipError_t read_typed(const Kv8View& c, int layer, const KvSpans& p, int6
     typedef typename KvElem<TYPE>::T T;
     const int veck = c.dk % 8 == 0 && (uintptr_t)k % 16 == 0, vecv = c.dv % 4 == 0 && (uintptr_t)v % (4 * sizeof(T)) == 0;
     const int64_t blocks = (int64_t)p.unit0[p.n] * c.heads;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    if (blocks > KV8_THREADS / 256) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks, layer < 0 ? c.layers : 1);
     if (p.n <= Kv8FewSpans::MAX) {
         Kv8FewSpans few;

@@ -11,7 +11,7 @@ namespace nh {
 
 template <int TYPE, int V, bool INTER>
 __global__ __launch_bounds__(256) void k_rope(RopeArgs a, RopePlan p) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / p.units;
+    const int64_t i = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x, row = i / p.units;
     const int u = (int)(i - row * p.units);
     if (row >= a.rows) return;
     const int h0 = blockIdx.y * p.share;
@@ -25,11 +25,12 @@ static hipError_t rope_wide(const RopeArgs& a, hipStream_t s) {
     const int64_t threads = a.rows * p.units;
     // Heads are shared out until every SIMD has four wavefronts: angles are worked
     // out again for each share, so no further.
-    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>((heads + 3) / 4, 262144 / std::max<int64_t>(threads, 1)));
+    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(std::min((heads + 3) / 4, 65535), 262144 / std::max<int64_t>(threads, 1)));
     p.share = (int)((heads + shares - 1) / shares);
-    const int64_t blocks = (threads + 255) / 256;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks, (heads + p.share - 1) / p.share);
+    // (a launch has fewer than 2^32 threads in x: beyond 2^30 they go on in z)
+    const int64_t blocks = (threads + 255) / 256, x = std::min<int64_t>(blocks, 1 << 22);
+    if (blocks > x * 65535) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)x, (heads + p.share - 1) / p.share, (unsigned)((blocks + x - 1) / std::max<int64_t>(x, 1)));
     if (a.r.interleaved)
         hipLaunchKernelGGL((k_rope<TYPE, V, true>), grid, dim3(256), 0, s, a, p);
     else
