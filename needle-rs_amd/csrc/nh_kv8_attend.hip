@@ -58,13 +58,22 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
     } else {
         b = kv_find(c, tile, lane, [&](const KvEntry& e) { return ((e.row1 - e.row0) * per + 15) / 16; });
     }
-    if (b >= c.nb) return;
-    const KvEntry entry = kv_batch(c, b);
+    // (the entry and the shape in one wait, no branch between them)
+    const KvEntry entry = kv_batch(c, min(b, c.nb - 1));
+    const bool current = kv_current(c);
     const int row0 = entry.row0, nrows = entry.row1 - row0, seq = entry.seq;
     const int first = entry.len - (c.ask ? 1 : nrows), r0 = tile * 16;
-    if (!kv_current(c) || (!c.ask && first < 0) || r0 >= nrows * per || entry.row1 > c.rows) return;
+    if ((b >= c.nb) | !current | (!c.ask & (first < 0)) | (r0 >= nrows * per) | (entry.row1 > c.rows)) return;
     const int r1 = min(r0 + 16, nrows * per) - 1;
     const int plo = first + (c.ask ? 0 : r0 / per), phi = first + (c.ask ? 0 : r1 / per);
+
+    const Ka8Span span(plo, phi, a.sink, a.ring);
+    const int sink = a.ring ? a.sink : 0x7fffffff, ring = a.ring;
+    const int per_split = max((span.count() + plan.splits - 1) / plan.splits, NW);
+    const int c0 = split * per_split, c1 = min(c0 + per_split, span.count());
+    const int* table = c.table + (size_t)seq * c.table_ld;
+    auto page_of = [&](int i) { return i < c1 ? table[span.at(i) * KV8_CHUNK >> c.page_log2] : 0; };
+    int chunk = c0 + wave, p0 = page_of(chunk), p1 = page_of(chunk + NW);
 
     // The queries: f16 operands scaled by a power of two to just under 2^15, or digits.
     h8 q[NJ][2];
@@ -72,8 +81,7 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
     float cq;
     const int r = min(r0 + o, r1), token = r / per, pos = first + (c.ask ? 0 : token);
     const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(row0 + token) * a.ldq + (int64_t)(kvh * per + r - token * per) * c.dk;
-    float x[NJ][16], most = 0.0f;
-    bool nan = false;
+    T raw[NJ][16];
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -84,16 +92,41 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
                 Vec y = {};
                 if (d < c.dk) y = *reinterpret_cast<const Vec*>(src + d);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][8 * g + e] = (float)y[e];
+                for (int e = 0; e < 8; ++e) raw[j][8 * g + e] = y[e];
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][8 * g + e] = d + e < c.dk ? KvElem<TYPE>::get(src + d + e) : 0.0f;
+                for (int e = 0; e < 8; ++e) raw[j][8 * g + e] = d + e < c.dk ? src[d + e] : (T)0.0f;
             }
+        }
+
+    // (the first chunk is on its way while the queries are turned into operands)
+    auto load = [&](Chunk& to, int i, int pg) {
+        if (i >= c1) return;
+        const int slot = span.at(i) * KV8_CHUNK & (c.page() - 1);
+        // (a page id comes from the cache's own table; a bad one is not followed)
+        const uint8_t* p = kv8_block(c, (unsigned)pg < (unsigned)c.pages ? pg : 0, a.layer, kvh) + (uint32_t)(slot >> 6) * L::CHUNK;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                most = fmaxf(most, fabsf(x[j][8 * g + e]));
-                nan |= x[j][8 * g + e] != x[j][8 * g + e];
-            }
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) to.k[t][j] = *reinterpret_cast<const u32x4*>(p + L::k_piece(t, j, lane));
+        to.ks = *reinterpret_cast<const f32x4*>(p + L::RECORD);
+        to.vs = *reinterpret_cast<const f32x4*>(p + L::RECORD + 16);
+        to.bad = *reinterpret_cast<const u32x4*>(p + L::RECORD + 32);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) to.v[n] = *reinterpret_cast<const u32x4*>(p + L::v_piece(n, lane));
+    };
+    Chunk two[2];
+    load(two[0], chunk, p0);
+
+    float x[NJ][16], most = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            x[j][e] = (float)raw[j][e];
+            most = fmaxf(most, fabsf(x[j][e]));
+            nan |= x[j][e] != x[j][e];
         }
     if constexpr (DIGITS) {
         most = nan ? __builtin_inff() : most;
@@ -142,28 +175,6 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
     // step / 2^eref, 2^eref above every step seen so far: at most 2^15, and exact to
     // 11 bits down to 2^-29 of it.
     int eref = -126;
-
-    const Ka8Span span(plo, phi, a.sink, a.ring);
-    const int sink = a.ring ? a.sink : 0x7fffffff, ring = a.ring;
-    const int per_split = max((span.count() + plan.splits - 1) / plan.splits, NW);
-    const int c0 = split * per_split, c1 = min(c0 + per_split, span.count());
-
-    const int* table = c.table + (size_t)seq * c.table_ld;
-    auto page_of = [&](int i) { return i < c1 ? table[span.at(i) * KV8_CHUNK >> c.page_log2] : 0; };
-    auto load = [&](Chunk& x, int i, int pg) {
-        const int slot = span.at(i) * KV8_CHUNK & (c.page() - 1);
-        // (a page id comes from the cache's own table; a bad one is not followed)
-        const uint8_t* p = kv8_block(c, (unsigned)pg < (unsigned)c.pages ? pg : 0, a.layer, kvh) + (uint32_t)(slot >> 6) * L::CHUNK;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) x.k[t][j] = *reinterpret_cast<const u32x4*>(p + L::k_piece(t, j, lane));
-        x.ks = *reinterpret_cast<const f32x4*>(p + L::RECORD);
-        x.vs = *reinterpret_cast<const f32x4*>(p + L::RECORD + 16);
-        x.bad = *reinterpret_cast<const u32x4*>(p + L::RECORD + 32);
-#pragma unroll
-        for (int n = 0; n < NV; ++n) x.v[n] = *reinterpret_cast<const u32x4*>(p + L::v_piece(n, lane));
-    };
 
     auto compute = [&](const Chunk& x, int i) {
         const int key0 = span.at(i) * KV8_CHUNK;
@@ -275,22 +286,13 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
 
     // The loads of the next chunk are in flight during this one's arithmetic, the
     // page id of the one after it is on its way.
-    {
-        Chunk x[2];
-        int i = c0 + wave;
-        auto fetch = [&](Chunk& to, int at, int pg) {
-            if (at < c1) load(to, at, pg);
-        };
-        int p0 = page_of(i), p1 = page_of(i + NW);
-        fetch(x[0], i, p0);
-        while (i < c1) {
+    while (chunk < c1) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k, i += NW) {
-                if (i >= c1) break;
-                fetch(x[k ^ 1], i + NW, p1);
-                p1 = page_of(i + 2 * NW);
-                compute(x[k], i);
-            }
+        for (int k = 0; k < 2; ++k, chunk += NW) {
+            if (chunk >= c1) break;
+            load(two[k ^ 1], chunk + NW, p1);
+            p1 = page_of(chunk + 2 * NW);
+            compute(two[k], chunk);
         }
     }
 

@@ -65,7 +65,7 @@ __device__ __forceinline__ int kv_find(const KvView& c, int& unit, int lane, F u
 // the batch is over, whose grid and plan fit nothing that is there.
 __device__ __forceinline__ bool kv_current(const KvView& c) {
     const int2 s = *reinterpret_cast<const int2*>(c.batch - 4);
-    return s.x == c.shape[0] && s.y == c.shape[1];
+    return (s.x == c.shape[0]) & (s.y == c.shape[1]);
 }
 __device__ __forceinline__ KvEntry kv_batch(const KvView& c, int b) {
     const int4 e = reinterpret_cast<const int4*>(c.batch)[b];
