@@ -310,29 +310,41 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
 #pragma unroll
     for (int n = 0; n < NV; ++n) *reinterpret_cast<f32x4*>(&so[wave][o][16 * n + 4 * kg]) = acc[n] * f * unit;
     __syncthreads();
-    for (int at = tid; at < 16 * WV; at += NW * 64) {
-        const int rr = at / WV, d = at % WV;
+    // (four dims of a row a thread)
+    for (int at = tid; at < 4 * WV; at += NW * 64) {
+        const int rr = at / (WV / 4), d = 4 * (at % (WV / 4));
         if (r0 + rr > r1 || d >= c.dv) continue;
         float top = sm[0][rr];
 #pragma unroll
         for (int w = 1; w < NW; ++w) top = fmaxf(top, sm[w][rr]);
         const float zero = top == -__builtin_inff() ? 0.0f : top;
-        float sum = 0.0f, v = 0.0f;
+        float sum = 0.0f;
+        f32x4 v = {};
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             sum = __builtin_fmaf(sl[w][rr], __builtin_amdgcn_exp2f(sm[w][rr] - zero), sum);
-            v += so[w][rr][d];
+            v += *reinterpret_cast<const f32x4*>(&so[w][rr][d]);
         }
         const int t = (r0 + rr) / per, head = kvh * per + r0 + rr - t * per;
         const int64_t row = row0 + t;
         if (plan.splits == 1) {
-            // (no key seen: 0)
-            KvElem<TYPE>::put(reinterpret_cast<T*>(a.out) + row * a.ldo + (int64_t)head * c.dv + d, sum == 0.0f ? 0.0f : v / sum);
+            T* out = reinterpret_cast<T*>(a.out) + row * a.ldo + (int64_t)head * c.dv + d;
+            v *= sum == 0.0f ? 0.0f : 1.0f / sum;  // (no key seen: 0)
+            if (plan.out_aligned) {
+                typedef T Vec4 __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<Vec4*>(out) = __builtin_convertvector(v, Vec4);
+            } else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < c.dv) out[e] = (T)v[e];
             if (a.lse && d == 0) a.lse[row * a.heads + head] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
         } else {
             const int64_t part = ((int64_t)split * c.rows + row) * a.heads + head;
             float* ml = reinterpret_cast<float*>(a.ws);
-            ml[2 * ((int64_t)plan.splits * c.rows * a.heads) + part * c.dv + d] = v;
+            float* out = ml + 2 * ((int64_t)plan.splits * c.rows * a.heads) + part * c.dv + d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < c.dv) out[e] = v[e];
             if (d == 0) ml[2 * part] = sum == sum ? top : sum, ml[2 * part + 1] = sum;
         }
     }
