@@ -16,6 +16,14 @@
 // kg) the scores of its row o with keys 16 t + 4 kg + 0..3, and a lane's 16 bytes
 // of values are of those very keys, so a weight never leaves its lane, and a
 // row's maximum, sum and correction are one lane's scalars.
+//
+// One row a head is bound by the cache's bytes: 64 sequences of up to 8,192 keys, 32
+// heads over 8 of 128, bf16 (818 MB) 155 us, 5.2 TB/s, as a large copy; one of 131,072
+// keys (269 MB) 52 to 62 with the 4.5 of its join.  Few keys are bound by latency (374 of
+// them 6.5 us on the GPU), so the first chunk's loads start before the queries are
+// operands.  More rows are bound by vector instructions, some 285 for 64 keys of 16
+// rows at 64 dims, 128 of them for codes turned into f16: four sequences' 448 rows over
+// 1,500 keys, 16 heads of 64, 30 us with the vector units three quarters busy.
 #include <algorithm>
 
 #include "nh_kv8_device.h"
@@ -376,10 +384,10 @@ static void tiles_of(const Kv8View& c, const int* row0, int per, int rows, Ka8Sh
 //  prompt 4 in all and 8 (6) a round of a workgroup a CU, 2.0 (1.75) for 64 keys of
 //         256 rows
 //  join   4, and the partial results' bytes there and back at 2 TB/s
-// 32 heads over 8 of 128 dims, rows / prompt: a sequence of 4,000 keys 512 rows 85 / 75,
-// 1,024 142 / 111, 2,048 240 / 134; four of 1,500 keys 128 rows 43 / 56, 256 73 / 57; 16
-// of 2,000 keys 32 rows 52 / 68, 64 rows 96 / 73.  16 heads of 64: 16 sequences of 2,000
-// keys 128 rows 54 / 59, 256 99 / 65; four of 1,500 512 rows 44 / 50, 1,024 67 / 51.
+// 32 heads over 8 of 128 dims, rows / prompt: a sequence of 4,000 keys 512 rows 75 / 74,
+// 1,024 130 / 110, 2,048 220 / 135; four of 1,500 keys 128 rows 37 / 62, 256 67 / 56; 16
+// of 2,000 keys 32 rows 46 / 63, 64 rows 85 / 71.  16 heads of 64: 16 sequences of 2,000
+// keys 128 rows 53 / 58, 256 92 / 64; four of 1,500 512 rows 39 / 49, 1,024 62 / 51.
 static double ka_join_us(const Kv8View& c, int heads, int64_t splits) {
     return splits > 1 ? 4.0 + (double)c.rows * heads * (double)splits * (c.dv + 2) * 8 / 2e6 : 0.0;
 }
