@@ -491,7 +491,8 @@ int nh_rope_freqs(int dim, double theta, int scaling, double factor, double orig
                   double* freqs, double* amplitude);
 /* A plan of HOST freqs[pairs] (any, |f| <= 10^6).  The only call that
  * allocates; a plan belongs to the device it was made on and is read only:
- * calls on several streams may share it. */
+ * calls on several streams may share it, and graphs that captured them, which
+ * it has to outlive. */
 int nh_rope_new(const double* freqs, int pairs, double amplitude, int layout, nh_rope** r);
 int nh_rope_free(nh_rope* r);
 /* Turns DEVICE q[row * ldq + head * dim + d] and k (kv_heads 0: none) of `type`
@@ -556,7 +557,7 @@ int nh_kv8_read(nh_kv8* c, int layer, const int* seqs, const int* pos, const int
  * is at its sequence's last position, so it sees all of it, with a ring > 0 the
  * first `sink` and the last `ring` positions.  Scores, weights' sums and
  * products are held in f32.  f16 and bf16 queries enter as they are, f32 ones
- * to 2^-24 of a row's largest; f32 and f16 calls carry 22 bits of a weight x
+ * to 2^-24 of a row's largest (one below 2^-100 as 0); f32 and f16 calls carry 22 bits of a weight x
  * its value's step, bf16 calls and calls of many f16 rows 11, none finer than
  * 2^-40 of the largest step (of many rows 2^-33 of the row's largest weight x
  * step, and a step below 2^-60 of the largest weighs as that).  A row's sum of

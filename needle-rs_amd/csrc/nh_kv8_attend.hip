@@ -462,7 +462,7 @@ static hipError_t attend_shaped(const Kv8View& c, const int* row0, const Kv8Atte
     plan.splits = shape.splits;
     plan.aligned = c.dk % 8 == 0 && (uintptr_t)a.q % 16 == 0 && a.ldq * es % 16 == 0 && c.dk * es % 16 == 0;
     plan.out_aligned = c.dv % 4 == 0 && (uintptr_t)a.out % 16 == 0 && a.ldo * es % 16 == 0;
-    if (shape.tiles * c.heads > KV8_THREADS / 512 || (int64_t)c.rows * a.heads > 0x7fffffff) return hipErrorInvalidValue;
+    if (shape.tiles * c.heads > KV8_THREADS / 512 || (int64_t)c.rows * a.heads > 0x7fffff00) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(shape.tiles * c.heads), plan.splits);
     if constexpr (WK <= 128 && TYPE != KV_F32)
         if (shape.prompt) {

@@ -153,6 +153,75 @@ def test_many_rows_in_a_graph(nh):
             at += n
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("qk,v,turned,layout", [(64, 64, 48, "half"), (128, 128, 128, "half"), (128, 96, 64, "interleaved"),
+                                                (256, 256, 32, "half"), (45, 51, 44, "half")])
+def test_rows_at_odd_addresses(nh, qk, v, turned, layout, dtype):
+    """k, v, q and every output an element behind an aligned address, rows of an odd stride: the bits of contiguous rows."""
+    rng = np.random.default_rng(qk + v)
+    kv, heads, rows = 2, 4, [5, 70]
+    plan, n = nh.Rope(turned, layout=layout), sum(rows)
+
+    def odd(x):
+        wide = torch.full((n, x.shape[1] * x.shape[2] + 3), 5.0, dtype=x.dtype, device="cuda")
+        view = wide[:, 1:1 + x.shape[1] * x.shape[2]].unflatten(1, x.shape[1:])
+        view.copy_(x)
+        return wide, view
+
+    k, w, q = (rows_of(rng, n, h, d, dtype).cuda() for h, d in ((kv, qk), (kv, v), (heads, qk)))
+    got = []
+    for move in (lambda x: (None, x), odd):
+        c = nh.KvCache8(1, kv, qk, v, pages=4, seqs=2, cap=128)
+        ids = [c.new_seq(), c.new_seq()]
+        c.extend(ids, rows)
+        turned_to, out = move(torch.zeros_like(q)), move(torch.zeros(n, heads, v, dtype=T[dtype], device="cuda"))
+        c.append(0, move(k)[1], move(w)[1], rope=plan, q=move(q)[1], out=turned_to[1])
+        result = [*c.read(0, ids, [0, 0], rows), turned_to[1].clone()]
+        for kernel in (1, 2):
+            c.debug_kernel(kernel)
+            c.attend(0, turned_to[1], out=out[1])
+            result.append(out[1].clone())
+        got.append(result)
+        for wide, view in (turned_to, out):
+            if wide is not None:
+                assert bool((wide[:, 0] == 5.0).all()) and bool((wide[:, -2:] == 5.0).all())
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size_k,size_v", [(1.0, 1e-25), (1.0, 1e30), (1e28, 1.0), (1e-28, 1e-20)])
+def test_attention_over_small_and_large_numbers(nh, size_k, size_v, dtype):
+    rng = np.random.default_rng(70)
+    n, rows = 700, 300
+    k, v = rows_of(rng, n, 2, 64, dtype, size_k), rows_of(rng, n, 2, 64, dtype, size_v)
+    q = rows_of(rng, rows, 4, 64, dtype, 1 / size_k)
+    c = nh.KvCache8(1, 2, 64, 64, pages=12, seqs=1, cap=n)
+    s = c.new_seq()
+    for m, a in ((n - rows, 0), (rows, n - rows)):
+        c.extend([s], [m])
+        c.append(0, k[a:a + m].cuda(), v[a:a + m].cuda())
+    held = [ref.quantize(plain(x), (n - rows,)) for x in (k, v)]
+    for kernel in (0, 1, 2):
+        c.debug_kernel(kernel)
+        check_attend(c, 0, q, [held[0]], [held[1]], [rows], dtype, kernel=kernel, many=dtype != "f32")
+
+
+def test_reads_of_many_spans(nh):
+    """Spans by the hundred, of the same sequences again and again, some empty, over one another."""
+    rng, pick = np.random.default_rng(60), random.Random(60)
+    lens = [300, 64, 1, 129]
+    c, ids, ks, vs = filled(nh, rng, lens, 2, 48, 64, 64, "f32", layers=2, last=[5, 0, 1, 100])
+    for count in (1, 15, 16, 17, 100, 700):
+        which = [pick.randrange(4) for _ in range(count)]
+        first = [pick.randrange(lens[i]) for i in which]
+        rows = [pick.randrange(min(lens[i] - a, 40) + 1) for i, a in zip(which, first)]
+        k, v = c.read(None, [ids[i] for i in which], first, rows, torch.float32)
+        for got, side in ((k, ks), (v, vs)):
+            for layer in (0, 1):
+                want = np.concatenate([side[layer][i][a:a + r] for i, a, r in zip(which, first, rows)])
+                assert np.array_equal(plain(got[layer]), want), count
+
+
 def test_two_graphs_on_two_streams(nh):
     """Steps of two caches captured apart and replayed at once: neither's workspace is the other's."""
     made = []
