@@ -557,11 +557,12 @@ int nh_kv8_read(nh_kv8* c, int layer, const int* seqs, const int* pos, const int
  * is at its sequence's last position, so it sees all of it, with a ring > 0 the
  * first `sink` and the last `ring` positions.  Scores, weights' sums and
  * products are held in f32.  f16 and bf16 queries enter as they are, f32 ones
- * to 2^-24 of a row's largest (one below 2^-100 as 0); f32 and f16 calls carry 22 bits of a weight x
- * its value's step, bf16 calls and calls of many f16 rows 11, none finer than
- * 2^-40 of the largest step (of many rows 2^-33 of the row's largest weight x
- * step, and a step below 2^-60 of the largest weighs as that).  A row's sum of
- * weights x values, before its division by the weights' sum, has to fit f32.
+ * to 2^-24 of a row's largest (one below 2^-100 as 0); f32 and f16 calls carry
+ * 22 bits of a weight x its value's step, bf16 calls and calls of many f16 rows
+ * 11, none finer than 2^-40 of the largest step (of many rows 2^-33 of the row's
+ * largest weight x step, and a step below 2^-60 of the largest weighs as that).
+ * A row's sum of weights x values, before its division by the weights' sum, has
+ * to fit f32.
  * NH_EDEVICE from 2^23 tiles of 16 rows x heads on (nh_kv8_append: 2^29 rows x
  * heads): more than a launch takes. */
 int64_t nh_kv8_attend_ws_bytes(const nh_kv8* c, int heads, int sink, int ring);

@@ -9,9 +9,12 @@
 // factor of 16 x 16 scores.  In the same way a weight takes its value's step, and
 // the second product's operands are codes too.  A byte c + 128 under 0x64 is the
 // f16 number 1152 + c (one byte permutation for two), from which one packed
-// addition takes 1152: exact.  f32 queries go the other way: their rows as whole
-// numbers of 23 bits in three signed digits of 8, times the codes in the i8
-// MFMAs, which are exact and take the bytes as they are.
+// addition takes 1152: exact.  That is done to the values; a key's byte alone is the
+// f16 subnormal (128 + c) 2^-24, and the products' sums start at -128 2^-24 times the
+// query's own sum: 30.0 us became 28.8 in the last example below.  (Sums of weights and
+// values would lose to the offset what their signs cancel.)  f32 queries go the other
+// way: their rows as whole numbers of 23 bits in three signed digits of 8, times the
+// codes in the i8 MFMAs, which are exact and take the bytes as they are.
 // The products are transposed, keys (or dims) by rows: S^T = K Q^T leaves lane (o,
 // kg) the scores of its row o with keys 16 t + 4 kg + 0..3, and a lane's 16 bytes
 // of values are of those very keys, so a weight never leaves its lane, and a
@@ -19,11 +22,11 @@
 //
 // One row a head is bound by the cache's bytes: 64 sequences of up to 8,192 keys, 32
 // heads over 8 of 128, bf16 (818 MB) 155 us, 5.2 TB/s, as a large copy; one of 131,072
-// keys (269 MB) 52 to 62 with the 4.5 of its join.  Few keys are bound by latency (374 of
+// keys (269 MB) 50 to 60 with the 4.5 of its join.  Few keys are bound by latency (374 of
 // them 6.5 us on the GPU), so the first chunk's loads start before the queries are
-// operands.  More rows are bound by vector instructions, some 285 for 64 keys of 16
-// rows at 64 dims, 128 of them for codes turned into f16: four sequences' 448 rows over
-// 1,500 keys, 16 heads of 64, 30 us with the vector units three quarters busy.
+// operands.  More rows are bound by vector instructions, some 250 for 64 keys of 16
+// rows at 64 dims, 96 of them for codes turned into f16: four sequences' 448 rows over
+// 1,500 keys, 16 heads of 64, 28.8 us with the vector units three quarters busy.
 #include <algorithm>
 
 #include "nh_kv8_device.h"
@@ -86,7 +89,7 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
     // The queries: f16 operands scaled by a power of two to just under 2^15, or digits.
     h8 q[NJ][2];
     i32x4 qd[3][NJ];
-    float cq;
+    float cq, offset = 0.0f;
     const int r = min(r0 + o, r1), token = r / per, pos = first + (c.ask ? 0 : token);
     const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(row0 + token) * a.ldq + (int64_t)(kvh * per + r - token * per) * c.dk;
     T raw[NJ][16];
@@ -171,6 +174,12 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) q[j][e / 8][e % 8] = (_Float16)(x[j][e] * up);
+        // what the keys' 128 too many make of a row's scores
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) offset += (float)q[j][e / 8][e % 8];
+        offset = groups_sum(offset) * -0x1p-17f;
     }
 
     f32x4 acc[NV];
@@ -220,12 +229,12 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
                 for (int r = 0; r < 4; ++r)
                     z[t][r] = __builtin_fmaf((float)n[2][r], 0x1p-8f, (float)(n[0][r] * 256 + n[1][r]));
             } else {
-                z[t] = f32x4{0, 0, 0, 0};
+                z[t] = f32x4{offset, offset, offset, offset};
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
-                        const h8 k = codes8(x.k[t][j][2 * g], x.k[t][j][2 * g + 1]);
+                        const h8 k = bytes8(x.k[t][j][2 * g], x.k[t][j][2 * g + 1]);
                         z[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[j][g], z[t], 0, 0, 0);
                     }
             }
@@ -236,7 +245,7 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
         float s[4][4];  // 15 + log2 of the weight against the maximum so far
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const float f = cq * x.ks[t];
+            const float f = DIGITS ? cq * x.ks[t] : cq * x.ks[t] * 0x1p24f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][r] = __builtin_fmaf(z[t][r], f, 15.0f - base);
         }

@@ -31,5 +31,12 @@ __device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
     const h2 w = codes2(a, 0x04010400u), x = codes2(a, 0x04030402u), y = codes2(b, 0x04010400u), z = codes2(b, 0x04030402u);
     return h8{w[0], w[1], x[0], x[1], y[0], y[1], z[0], z[1]};
 }
+// The same, 128 more and 2^-24 times as large: a byte alone is an f16 subnormal,
+// which the matrix instructions take exactly.
+__device__ __forceinline__ uint32_t bytes2(uint32_t w, uint32_t which) { return __builtin_amdgcn_perm(w, w, which); }
+__device__ __forceinline__ h8 bytes8(uint32_t a, uint32_t b) {
+    const u32x4 w = {bytes2(a, 0x0c010c00u), bytes2(a, 0x0c030c02u), bytes2(b, 0x0c010c00u), bytes2(b, 0x0c030c02u)};
+    return __builtin_bit_cast(h8, w);
+}
 
 }  // namespace nh

@@ -117,7 +117,8 @@ def attend_bound(q, k, v, o, scale, dtype, many=False):
     2^-20 of the largest (d of them, and 16 roundings of sums), an f32 query's
     whole numbers are off by 2^-24 of the row's largest each (the products are
     exact, their sum is rounded twice); a score off by e changes a weight by e,
-    numerator and denominator alike.  The weights: 11 bits (22 in f32 and f16
+    numerator and denominator alike: 2 delta.  A key of few rows enters as code + 128, so
+    the largest product is up to 255 / 127 of a code's: 4.016 delta.  The weights: 11 bits (22 in f32 and f16
     calls of few rows), f16 values of many rows 11 bits of their own; 32
     products of an MFMA cut off at 2^-20 of its largest, the largest of all
     MFMAs adding up to at most 1; a rounding a key in the running sums."""
@@ -131,4 +132,4 @@ def attend_bound(q, k, v, o, scale, dtype, many=False):
     vmax = np.abs(v).max() if v.size else 0.0
     weight = 2.0 ** -11 * (2 if many else 1) if dtype == "bf16" or many else 2.0 ** -21
     rounding = half_step(dtype) * np.abs(o) * 1.01 + (2.0 ** -24 if dtype == "f16" else 0.0)
-    return rounding + vmax * (weight + 2.0 ** -15 + 4 * delta + 4 * (len(k) + 64) * 2.0 ** -24) + 1e-30
+    return rounding + vmax * (weight + 2.0 ** -15 + 4.016 * delta + 4 * (len(k) + 64) * 2.0 ** -24) + 1e-30
