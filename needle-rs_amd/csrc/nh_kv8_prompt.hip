@@ -16,8 +16,8 @@ namespace nh {
 // a row's weights x steps keep their 11 bits down to 2^-22 of the largest of them.  A
 // step below 2^-60 of the largest that the rows see counts as that.
 //
-// 2 x 2,000 rows after 6,000 keys, 32 heads over 8 of 128 (427 GFLOP), bf16: 445 to 460
-// us, 930 to 960 TFLOP/s, where a large product reaches 1,320 to 1,370.  The matrix
+// 2 x 2,000 rows after 6,000 keys, 32 heads over 8 of 128 (427 GFLOP), bf16: 440 to 460
+// us, 930 to 970 TFLOP/s, where a large product reaches 1,320 to 1,370.  The matrix
 // cores are busy for half of the cycles: a row's 32 exponentials, and as many sums and
 // products, are vector work for nearly as long as its products, and two wavefronts a SIMD
 // do not overlap them whole.  With the turning of the codes and the records taken out
