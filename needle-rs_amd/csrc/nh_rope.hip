@@ -5,7 +5,7 @@
 //   (2 i, 2 i + 1); transposed: s with the other sign, which is the gradient.
 //
 // Bytes bound it: a thread takes four pairs of a row, works their angles out once (f64
-// series, some 60 instructions a pair) and turns them in every head of its share, four
+// series, about 40 instructions a pair) and turns them in every head of its share, four
 // heads' loads in flight.  6,001 rows of 32 + 8 heads of 128 in bf16 (123 MB) 25 us, 4.9
 // TB/s; 4,096 rows of 24 + 24 heads of 96, 32 dims turned by neighbours, in place (76
 // MB) 15.1, 5.0 TB/s; a copy of 1 GiB has 5.2.  8 rows: 3.0 to 3.4 us, a launch and
