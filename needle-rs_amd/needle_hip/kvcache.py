@@ -160,10 +160,11 @@ class PagedCache:
             raise ValueError("f32, f16 or bf16")
         if layer is not None and int(layer) < 0:
             raise ValueError("no such layer")
-        n = sum(x for x in r if x > 0)
+        n = max(sum(r), 0)  # (a negative number among them is refused below)
         shape = (n, self.kv_heads) if layer is not None else (self.layers, n, self.kv_heads)
         with _on(stream):
-            k, v = self._empty((*shape, self.qk_dim), dtype), self._empty((*shape, self.v_dim), dtype)
+            k = self._empty((*shape, self.qk_dim), dtype)
+            v = torch.empty_like(k) if self.v_dim == self.qk_dim else self._empty((*shape, self.v_dim), dtype)
         nh._check(self._c.read(self.h, -1 if layer is None else int(layer), ps, pp, pr, count, k.data_ptr(),
                                       v.data_ptr(), _TYPES[dtype], nh._stream(stream)))
         return k, v
