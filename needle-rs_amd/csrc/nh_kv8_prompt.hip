@@ -14,7 +14,12 @@ namespace nh {
 // weights themselves is that of p' / step, 16 keys at a time.  The reference is the
 // row's largest score + log2 step (within 2^7, so that it is hardly ever moved), so
 // a row's weights x steps keep their 11 bits down to 2^-22 of the largest of them.  A
-// step below 2^-60 of the largest that the rows see counts as that.
+// step below 2^-60 of the largest that the rows see counts as that (2^-125 where that
+// is more), so 1 / step passes what a row was given its reference at by 2^60 at most.
+// The sum is held in a unit 2^-e of the row's own, chosen anew where its reference
+// moves, as the sum or the largest new weight is then: steps of any size before and
+// after one another leave it within f32.  (A unit fixed by the first 64 keys lost it
+// where later steps were 2^120 times as large.)
 //
 // 2 x 2,000 rows after 6,000 keys, 32 heads over 8 of 128 (427 GFLOP), bf16: 440 to 460
 // us, 930 to 970 TFLOP/s, where a large product reaches 1,320 to 1,370.  The matrix
@@ -36,10 +41,10 @@ static_assert(KP8_ROWS == 32 * KP8_WAVES, "32 rows a wavefront");
 template <int W>
 struct Kp8Image {  // a chunk's operands, 16 bytes a lane each
     u32x4 k[2][W / 16][64], v[W / 32][4][64];
-    float ks[4], lv[4], rv[4];  // the keys' steps; log2 of the values' (inf: a marked row among them), 2^first over them
+    float ks[4], lv[4], rv[4];  // the keys' steps; log2 of the values' (inf: a marked row among them), 1 over them
     float marked_lv[4];         // log2 of the steps of blocks with marked rows too
     uint32_t marks[2];          // rows of the keys or the values, a bit each
-    int first, pad;
+    int pad[2];
 };
 
 template <int TYPE, int W>
@@ -75,7 +80,7 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
 
     const int r = min(r0 + wave * 32 + m32, r1), token = r / per, pos = first + (c.ask ? 0 : token);
     h8 q[NX];
-    float cq, m = -__builtin_inff(), l = 0.0f;
+    float cq, m = -__builtin_inff(), l = 0.0f, unit = 1.0f;  // (l: the weights' sum x unit, 2^e)
     f32x16 acc[ND];
     {
         const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(row0 + token) * a.ldq + (int64_t)(kvh * per + r - token * per) * c.dk;
@@ -154,8 +159,6 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
         }
     };
     float top = 0.0f;  // the largest step so far
-    int ref = 0;       // the first chunk's exponent
-    bool none = true;
     auto record = [&](const Raw& x, int i, Image& to) {
         if (wave != 0) return;
         const int key0 = span.at(min(i, last)) * KV8_CHUNK;
@@ -164,10 +167,7 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
         const float vs = lane >= 4 && lane < 8 && key0 + 16 * (lane - 4) <= phi ? mine : 0.0f;
         float most = fmaxf(vs, quad_xor1(vs));
         top = fmaxf(top, fmaxf(most, quad_xor2(most)));
-        // (nothing but zeros so far: as steps of 2^-60)
-        const float least = top > 0.0f ? fmaxf(top * 0x1p-60f, 0x1p-125f) : 0x1p-60f;
-        if (none) ref = __builtin_amdgcn_readlane((int)(__builtin_bit_cast(uint32_t, fmaxf(top, least)) >> 23), 4) - 127;
-        none = false;
+        const float least = fmaxf(top * 0x1p-60f, 0x1p-125f);
         // (words 8, 9 and 10, 11: the keys' and the values' marks of two blocks each)
         const uint32_t marks = x.rec | __builtin_bit_cast(uint32_t, quad_xor2(mine));
         const uint32_t m0 = (uint32_t)__builtin_amdgcn_readlane((int)marks, 8), m1 = (uint32_t)__builtin_amdgcn_readlane((int)marks, 9);
@@ -177,10 +177,9 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
             const float v = fmaxf(vs, least), lv = __builtin_amdgcn_logf(v);
             to.lv[t] = (t & 2 ? m1 : m0) >> (16 * (t & 1)) & 0xffffu ? __builtin_inff() : lv;
             to.marked_lv[t] = lv;
-            to.rv[t] = __builtin_amdgcn_ldexpf(__builtin_amdgcn_rcpf(v), ref);
+            to.rv[t] = __builtin_amdgcn_rcpf(v);
         }
         if (lane < 2) to.marks[lane] = lane ? m1 : m0;
-        to.first = ref;
     };
     auto whole_turn = [&](const Raw& x, int i, Image& to) {
 #pragma unroll
@@ -189,6 +188,7 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
         record(x, i, to);
     };
 
+    auto exponent = [](float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127; };
     float s[16], limit = -__builtin_inff();  // (a score past it moves the reference; none yet: any)
     f32x16 z;
     h8 p[2], kx[NX], vx[2 * ND];
@@ -222,11 +222,23 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
             const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(-over);
             m = fresh && most == -__builtin_inff() ? m : (fresh ? 0.0f : m) + over;
             limit = m == -__builtin_inff() ? m : 15.0f;
-            l *= keep;
 #pragma unroll
             for (int d = 0; d < ND; ++d) acc[d] *= keep;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] -= over;
+            // The sum's unit: log2 of the weights' sum so far, or of the largest weight among
+            // these keys, whichever is more (-inf: no key yet).
+            float of[2] = {s[0], s[8]};
+#pragma unroll
+            for (int e = 1; e < 8; ++e) of[0] = fmaxf(of[0], s[e]), of[1] = fmaxf(of[1], s[8 + e]);
+            const float now_l = fmaxf(of[0] - now.marked_lv[2 * tk], of[1] - now.marked_lv[2 * tk + 1]);
+            const int e0 = exponent(unit);
+            const float was = fresh ? -__builtin_inff() : __builtin_amdgcn_logf(l) - (float)e0 - over;
+            // (both halves of the row hold sums of their own, in one unit)
+            const float both = halves_max(fmaxf(now_l, was));
+            const int e1 = both == -__builtin_inff() ? e0 : (int)rintf(fminf(fmaxf(-both, -126.0f), 126.0f));
+            l = fresh ? 0.0f : l * __builtin_amdgcn_exp2f((float)(e1 - e0) - over);
+            unit = pow2i(e1);
         }
     };
     // Half `tk` of a chunk, in two parts whose instructions are written down in the
@@ -255,8 +267,8 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
             p[j >> 2][2 * j % 8] = w2[0], p[j >> 2][2 * j % 8 + 1] = w2[1];
             __builtin_amdgcn_sched_barrier(0);
         }
-        l = __builtin_fmaf(sum[0], rv[0], l);
-        l = __builtin_fmaf(sum[1], rv[1], l);
+        l = __builtin_fmaf(sum[0], rv[0] * unit, l);
+        l = __builtin_fmaf(sum[1], rv[1] * unit, l);
     };
     // (scores of half `tk` of `with`, keys of half `kt` of `keys`)
     auto sums_part = [&](const Image& with, int tk, const Image& keys, int kt, auto also) {
@@ -332,13 +344,13 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
         }
     }
 
-    const int unit = c0 < c1 ? __builtin_amdgcn_readfirstlane(img[0].first) : 0;
+    const int up = exponent(unit);
     const float sum = l + __shfl_xor(l, 32, 64);
     if (r0 + wave * 32 + m32 > r1) return;
     const int64_t row = row0 + token, head = kvh * per + r - token * per;
     const bool alone = plan.splits == 1;
-    // the sums are of p / (step 2^-unit); the reference counts the step, and 2^8
-    const float at_ref = m - (float)unit - 8.0f;
+    // the sums are of p / step x 2^up; the reference counts the step, and 2^8
+    const float at_ref = m - (float)up - 8.0f;
     const float scale = alone ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
     T* out = reinterpret_cast<T*>(a.out) + row * a.ldo + head * c.dv;
     const int64_t at = ((int64_t)split * c.rows + row) * a.heads + head;
@@ -351,7 +363,7 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
             const int dim = 32 * d + 8 * (e >> 2) + 4 * half;
             float y[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = __builtin_amdgcn_ldexpf(acc[d][e + k] * scale, unit);
+            for (int k = 0; k < 4; ++k) y[k] = __builtin_amdgcn_ldexpf(acc[d][e + k] * scale, up);
             if (alone) {
                 typedef T Vec4 __attribute__((ext_vector_type(4)));
                 if (plan.out_aligned && dim + 4 <= c.dv) {
