@@ -199,10 +199,14 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
         const uint32_t bad0 = __builtin_amdgcn_readfirstlane((int)(x.bad[0] | x.bad[2]));
         const uint32_t bad1 = __builtin_amdgcn_readfirstlane((int)(x.bad[1] | x.bad[3]));
         const bool plain = whole && !(bad0 | bad1);
-        // The steps' reference: raised when a step passes it (of a block that the tile sees).
-        float top = x.vs[0];
+        // The steps' reference: raised when a step passes it (of a block that the tile sees;
+        // others' steps, past the rows or under no window, count as 0).
+        f32x4 vs = x.vs;
+        if (!whole) {
 #pragma unroll
-        for (int t = 1; t < 4; ++t) top = fmaxf(top, key0 + 16 * t <= phi ? x.vs[t] : 0.0f);
+            for (int t = 0; t < 4; ++t) vs[t] = ka8_sees(key0 + 16 * t, plo, phi, sink, ring) ? vs[t] : 0.0f;
+        }
+        const float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
         const int et = __builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, top) >> 23)) - 126;
         if (et > eref) {
             const float down = pow2i(max(eref - et, -126));
@@ -213,7 +217,7 @@ __global__ __launch_bounds__(NW * 64, WK <= 128 ? 2 : 1) void k_kv8_attend(Kv8Vi
         const float wscale = pow2i(-eref);
         float vstep[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) vstep[t] = key0 + 16 * t <= phi ? x.vs[t] * wscale : 0.0f;
+        for (int t = 0; t < 4; ++t) vstep[t] = vs[t] * wscale;
         f32x4 z[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {

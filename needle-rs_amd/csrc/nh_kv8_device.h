@@ -23,6 +23,11 @@ __device__ __forceinline__ uint8_t* kv8_block(const Kv8View& c, int page, int la
 
 typedef KaSpanOf<KV8_CHUNK> Ka8Span;
 
+// Whether rows at positions lo .. hi see any of the 16 from `block` on.
+__device__ __forceinline__ bool ka8_sees(int block, int lo, int hi, int sink, int ring) {
+    return (block <= hi) & ((block < sink) | (block + 15 > lo - ring));
+}
+
 // Four codes as f16: bytes 0, 1 and 2, 3.
 __device__ __forceinline__ h2 codes2(uint32_t w, uint32_t which) {
     return __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, which)) + (_Float16)-1152.0f;

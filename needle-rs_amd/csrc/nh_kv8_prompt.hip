@@ -164,7 +164,7 @@ __global__ __launch_bounds__(KP8_WAVES * 64, 2) void k_kv8_prompt(Kv8View c, Kv8
         const int key0 = span.at(min(i, last)) * KV8_CHUNK;
         // lane 4 + t: the step of block t's values, 0 of hidden ones; the quad's largest
         const float mine = __builtin_bit_cast(float, x.rec);
-        const float vs = lane >= 4 && lane < 8 && key0 + 16 * (lane - 4) <= phi ? mine : 0.0f;
+        const float vs = lane >= 4 && lane < 8 && ka8_sees(key0 + 16 * (lane - 4), plo, phi, sink, ring) ? mine : 0.0f;
         float most = fmaxf(vs, quad_xor1(vs));
         top = fmaxf(top, fmaxf(most, quad_xor2(most)));
         const float least = fmaxf(top * 0x1p-60f, 0x1p-125f);

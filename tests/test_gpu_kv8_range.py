@@ -1,5 +1,5 @@
 """Attention over the 8-bit cache where blocks of values differ in size by more than any exponent of the kernels' own
-spans: steps up to 2^110, zeros before them."""
+spans: steps up to 2^110, zeros before them, large blocks that a window hides."""
 import numpy as np
 import pytest
 import torch
@@ -81,3 +81,22 @@ def test_rows_of_their_own_beside_all_sizes(nh, sizes):
             # the scores' error alone: the bound of a value of 1
             score = ref.attend_bound(plain(q), hk[:z], np.ones_like(hv[:z]), 0 * o[a:z], 0.125, "bf16", True).max()
             assert np.abs(plain(lse[a:z]) - l[a:z]).max() <= score + 2.0 ** -20, (kernel, a)
+
+
+@pytest.mark.parametrize("size", [1e6, 1e13, 1e20, 1e30])
+@pytest.mark.parametrize("rows,heads,dim", [(1, 2, 64), (5, 2, 128), (300, 4, 64), (3, 2, 256)])
+def test_large_blocks_that_a_window_hides(nh, rows, heads, dim, size):
+    """Blocks that no row of the call sees, in chunks of which it sees other blocks, are as if they were not there."""
+    rng = np.random.default_rng(rows + dim)
+    n, sink, ring = 400, 20, 40
+    v = rows_of(rng, n, 2, dim, "bf16").float()
+    v[32:n - 48] *= size  # (positions 360 .. 399 and the sink's 0 .. 19 are seen; blocks from 32 to 351 are not)
+    k, v = rows_of(rng, n, 2, dim, "bf16"), v.to(torch.bfloat16)
+    c, s, hk, hv = held_of(nh, k, v)
+    q = rows_of(rng, rows, heads, dim, "bf16")
+    hidden = hv.copy()
+    hidden[32:n - 48] = 0
+    c.ask([s], [rows])
+    for kernel in (0, 1, 2):
+        c.debug_kernel(kernel)
+        check_attend(c, 0, q, [hk], [hidden], [rows], "bf16", sink, ring, ask=True, many=True)
