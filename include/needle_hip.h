@@ -534,6 +534,15 @@ int nh_kv8_seq_fork(nh_kv8* c, int seq, int n, int* branches);
 int nh_kv8_seq_copy(nh_kv8* c, int seq, void* stream);
 int nh_kv8_extend(nh_kv8* c, const int* seqs, const int* rows, int n, void* stream);
 int nh_kv8_rows(const nh_kv8* c);
+/* Tells the device, on `stream`, that the batch is over.  A fork, a truncate or a
+ * free of one of the batch's sequences ends it on the host alone; until the next
+ * extend, ask or copy the device still has it, and a captured append that is
+ * replayed in between stores its rows again, which here may double the step of
+ * a begun block and round its kept rows anew, shared ones too.  After this call
+ * such a replay does nothing.  Nothing is done while the batch lasts, or where
+ * no append of this cache was captured; else refused under stream capture.
+ * (The Python cache calls it after each of the three.) */
+int nh_kv8_end_batch(nh_kv8* c, void* stream);
 /* rows[i] (>= 0) query rows for each of n distinct sequences (HOST arrays),
  * which become the batch without being positions of it: every row sees its
  * whole sequence, as a decoder's rows see their encoder's states.  No position

@@ -11,6 +11,7 @@ using namespace nh::kv;
 
 struct nh_kv8 : nh::KvHost {
     nh::Kv8View v{};
+    bool captured = false;  // a graph holds an append
     nh_kv8() { view = &v; }
 };
 
@@ -76,6 +77,16 @@ int nh_kv8_ask(nh_kv8* c, const int* seqs, const int* rows, int n, void* stream)
 
 int nh_kv8_rows(const nh_kv8* c) { return rows(c); }
 
+// A replayed append of a batch that is over would round the kept rows of its
+// begun blocks anew: without the batch's shape it does nothing.
+int nh_kv8_end_batch(nh_kv8* c, void* stream) {
+    if (int rc = check(c)) return rc;
+    if (!c->captured) return NH_OK;
+    hipStream_t st = (hipStream_t)stream;
+    if (int rc = check_eager(st)) return rc;
+    return guarded([&]() -> int { return drop_batch(c, st); });
+}
+
 int nh_kv8_append(nh_kv8* c, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int type,
                   const nh_rope* rope, const int32_t* pos, const void* q, int64_t ldq, int heads, void* q_out,
                   int64_t ldqo, void* stream) {
@@ -96,6 +107,11 @@ int nh_kv8_append(nh_kv8* c, int layer, const void* k, const void* v, int64_t ld
     nh::Kv8Append a{k, v, ldk, ldv, layer, {}, pos, {}};
     if (rope) a.r = rope->v;
     if (heads) a.q = nh::RopeRows{q, q_out, ldq, ldqo, heads};
+    if (!c->captured) {
+        hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing((hipStream_t)stream, &s) != hipSuccess) (void)hipGetLastError();
+        c->captured = s != hipStreamCaptureStatusNone;
+    }
     NH_TRY(nh::launch_kv8_append(c->v, c->book.batch_row0.data(), a, type, (hipStream_t)stream), "kv8 append");
     return NH_OK;
 }

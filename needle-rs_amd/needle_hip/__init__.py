@@ -122,6 +122,7 @@ SIGNATURES = {
     "nh_kv8_extend": (I, [P, P, P, I, P]),
     "nh_kv8_ask": (I, [P, P, P, I, P]),
     "nh_kv8_rows": (I, [P]),
+    "nh_kv8_end_batch": (I, [P, P]),
     "nh_kv8_append": (I, [P, I, P, P, C.c_int64, C.c_int64, I, P, P, P, C.c_int64, I, P, C.c_int64, P]),
     "nh_kv8_read": (I, [P, I, P, P, P, I, P, P, I, P]),
     "nh_kv8_debug_kernel": (I, [P, I]),

@@ -19,11 +19,33 @@ class KvCache8(PagedCache):
     rows of queries alone, each of which sees its whole sequence (a decoder's
     rows and their encoder's states)."""
 
-    _CALLS = PagedCache._CALLS + ("ask",)
+    _CALLS = PagedCache._CALLS + ("ask", "end_batch")
 
     def __init__(self, layers: int, kv_heads: int, qk_dim: int, v_dim: int, pages: int, seqs: int, cap: int, page: int = 64):
         self._make("kv8", layers, kv_heads, qk_dim, v_dim, pages, page,
                    (int(layers), int(kv_heads), int(qk_dim), int(v_dim), int(page), int(pages), int(seqs), int(cap)))
+
+    def _changed(self, call, args, stream):
+        """A call that may end the batch: the device is told (before it, end_batch checks for a capture alone)."""
+        st = nh._stream(stream)
+        nh._check(self._c.end_batch(self.h, st))
+        made = call(*args)
+        nh._check(self._c.end_batch(self.h, st))
+        return made
+
+    def free(self, seq: int, stream=None):
+        """Gives back the pages that no branch shares.  free, truncate and fork do device work only where an
+        append was captured, whose replays then store nothing until the next extend."""
+        self._changed(super().free, (seq,), stream)
+
+    def truncate(self, seq: int, length: int, stream=None):
+        """Forgets positions `length` and on.  Rows that are kept beside them in a block of 16 stay as they
+        are held: a step that a forgotten row has doubled is not halved again."""
+        self._changed(super().truncate, (seq, length), stream)
+
+    def fork(self, seq: int, n: int = 1, stream=None) -> list:
+        """n branches that share the sequence's pages until they are written."""
+        return self._changed(super().fork, (seq, n), stream)
 
     def ask(self, seqs, rows, stream=None):
         """rows[i] query rows for each sequence; they become the batch, and no
