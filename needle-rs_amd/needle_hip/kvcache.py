@@ -46,7 +46,8 @@ class PagedCache:
     """A paged cache of keys and values, shared by many sequences.  A step:
     `extend` names its sequences and their new rows; then, for every layer,
     `append` stores the rows' keys and values and `attend` attends with their
-    queries.  The formats: KvCache4, KvCache8."""
+    queries.  For serving: no call records gradients.  The formats: KvCache4,
+    KvCache8."""
 
     _CALLS = ("free", "bytes", "free_pages", "seq_new", "seq_len", "seq_free", "seq_truncate", "seq_fork", "seq_copy",
               "extend", "rows", "append", "read", "debug_kernel", "attend_ws_bytes", "attend")

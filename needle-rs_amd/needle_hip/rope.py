@@ -87,13 +87,17 @@ class Rope:
         wider matrix's columns.  out: a tensor, with k a pair of them (None:
         new ones); q itself and k itself turn in place.  transposed: gradients of
         the outputs to the inputs' (the same angles backwards).  Returns q's
-        rows, with k the pair."""
+        rows, with k the pair.  The call records no gradients: rows that would
+        need them are refused (a torch.autograd.Function calls apply forwards and
+        transposed backwards; detach() or torch.no_grad() otherwise)."""
         if len(q.shape) != 3:
             raise ValueError(f"q is [rows][heads][dim], not {list(q.shape)}")
         rows, heads, dim = q.shape
         dtype, index = q.dtype, self._index
         if dtype not in _TYPES:
             raise ValueError("q is f32, f16 or bf16")
+        if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+            raise ValueError("apply records no gradients: detach q and k, or turn their gradients with transposed=True")
         pos = self._positions(positions, rows)
         ldq = _row_stride(q, rows, dim, index, dtype, "q")
         ldk = kv_heads = 0
