@@ -513,6 +513,11 @@ int nh_rope_apply(const nh_rope* r, const int32_t* pos, int64_t rows, int dim, c
  *   rows that join a begun block double its step until it is their own max|x|
  *   f32(1/127) at least, and the codes that were there are divided by as much (ties to
  *   even): off by at most a step in all.  A step below 2^-120 counts as 0.
+ * So what a block holds depends on how its rows were shared out over calls, and on
+ * rows that a truncate forgot: a step that they doubled stays, with the rounding
+ * of what is kept, until the block's first position is stored anew (in the 4-bit
+ * cache no row touches another).  Drafts fed to a fork leave no trace in the
+ * sequence: its begun page is copied first.
  * A key or value row with a NaN or an infinity reads as NaN, takes no part in
  * its block's step, and makes NaN of what a query that sees it gets.  No
  * compaction: positions that moved to other blocks would be rounded again. */
