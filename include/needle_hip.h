@@ -560,7 +560,10 @@ int nh_kv8_ask(nh_kv8* c, const int* seqs, const int* rows, int n, void* stream)
  * qk_dim dims, of the cache's device) the keys are turned first, in f32, to
  * their positions in their sequences, or to DEVICE pos[rows] if given; `heads`
  * query heads in DEVICE q are turned with them into q_out (q itself, or apart
- * from it), in the same launch; heads 0: keys alone. */
+ * from it), in the same launch; heads 0: keys alone.  NH_EDEVICE: more than a
+ * launch takes, some 2^31 workgroups (for each block of 16 positions with new
+ * rows one for 4 kv heads and one for 8 query heads, for each 64 positions one a
+ * kv head). */
 int nh_kv8_append(nh_kv8* c, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int type,
                   const nh_rope* rope, const int32_t* pos, const void* q, int64_t ldq, int heads, void* q_out,
                   int64_t ldqo, void* stream);
@@ -577,8 +580,8 @@ int nh_kv8_read(nh_kv8* c, int layer, const int* seqs, const int* pos, const int
  * largest weight x step, and a step below 2^-60 of the largest weighs as that).
  * A row's sum of weights x values, before its division by the weights' sum, has
  * to fit f32.
- * NH_EDEVICE from 2^23 tiles of 16 rows x heads on (nh_kv8_append: 2^29 rows x
- * heads): more than a launch takes. */
+ * NH_EDEVICE: more than a launch takes, which is 2^31 rows x heads or 2^23 tiles
+ * (for each sequence and kv head, 16 of its rows x query heads). */
 int64_t nh_kv8_attend_ws_bytes(const nh_kv8* c, int heads, int sink, int ring);
 int nh_kv8_attend(const nh_kv8* c, int layer, const void* q, int64_t ldq, int heads, float scale, int sink, int ring,
                   void* out, int64_t ldo, float* lse, int type, void* ws, uint64_t ws_bytes, void* stream);

@@ -84,7 +84,7 @@ struct Kv8AppendPlan {
     int veck, vecv;                // rows of k can be taken 8, rows of v 4 elements at a time
     int k_parts, q_parts;          // workgroups a block for the heads of the keys, of the queries
     int q_share;                   // query heads a workgroup takes
-    int k_grid, v_grid;            // workgroups of the keys, of the values; the queries' come after them
+    int k_grid, v_grid, grid;      // workgroups of the keys, of the values, of all: the queries' come after them
     RopePlan rope;                 // of the queries
     int wide, widek;               // .. and of the keys: four pairs a thread
 };
@@ -345,7 +345,8 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8View c, Kv8Append a, Kv8A
     constexpr int LD = WK + 4;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int bid = blockIdx.x;
+    int bid = blockIdx.y * gridDim.x + blockIdx.x;
+    if (bid >= p.grid) return;
     if (bid < p.k_grid) {
         const int h0 = bid % p.k_parts * KV8_HEADS, heads = min(KV8_HEADS, c.heads - h0);
         const Kv8Unit u = kv8_unit<4>(c, bid / p.k_parts, p.blocks_each, lane);
@@ -491,9 +492,12 @@ static hipError_t append_typed(const Kv8View& c, const int* row0, const Kv8Appen
         }
     }
     const int64_t grid = k_grid + v_grid + blocks * p.q_parts;
-    if (grid > KV8_THREADS / 256) return hipErrorInvalidValue;
+    // (beyond the threads of a launch in x they go on in y)
+    const int64_t x = grid > KV8_THREADS / 256 ? 1 << 22 : grid, y = (grid + x - 1) / x;
+    if (grid > INT32_MAX - x) return hipErrorInvalidValue;
     p.k_grid = (int)k_grid;
     p.v_grid = (int)v_grid;
+    p.grid = (int)grid;
     const int how = !turn ? 0 : a.r.interleaved ? KV8_NEIGHBOURS : a.r.pairs % 64 == 0 ? KV8_HALVES : KV8_APART;
     // keys' rows and angles, or a chunk's values
     const size_t angles = turn ? (size_t)16 * kv8_angles_ld(a.r.pairs) * sizeof(float2) : 0;
@@ -508,7 +512,7 @@ static hipError_t append_typed(const Kv8View& c, const int* row0, const Kv8Appen
         if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds))
             return e;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, s, c, a, p);
+    hipLaunchKernelGGL(kern, dim3((unsigned)x, (unsigned)y), dim3(256), lds, s, c, a, p);
     return hipGetLastError();
 }
 
