@@ -100,3 +100,30 @@ def test_large_blocks_that_a_window_hides(nh, rows, heads, dim, size):
     for kernel in (0, 1, 2):
         c.debug_kernel(kernel)
         check_attend(c, 0, q, [hk], [hidden], [rows], "bf16", sink, ring, ask=True, many=True)
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_rows_beside_large_values_of_later_rows(nh, kernel):
+    """A border of blocks 10^6 times as large inside a tile of rows: rows in tiles before it keep the bound of what they
+    see, rows of its own tile lose what is finer than 2^-40 of the largest step (2^-60, many rows)."""
+    rng = np.random.default_rng(12)
+    n, last = 200, 100
+    k, v = rows_of(rng, n, 1, 64, "bf16"), rows_of(rng, n, 1, 64, "bf16")
+    v[:32] *= 1e-6
+    v[160:] *= 1e6
+    c = nh.KvCache8(1, 1, 64, 64, pages=4, seqs=1, cap=256)
+    c.debug_kernel(kernel)
+    s = c.new_seq()
+    q = rows_of(rng, n, 1, 64, "bf16")
+    hk, hv = (ref.quantize(plain(x), (n - last,)) for x in (k, v))
+    o, _ = ref.attend(plain(q), hk, hv, 0.125)
+    for a, z in ((0, n - last), (n - last, n)):
+        c.extend([s], [z - a])
+        c.append(0, k[a:z].cuda(), v[a:z].cuda())
+        got = plain(c.attend(0, q[a:z].cuda())).astype(np.float64)
+        tile = 256 if kernel == 2 else 16
+        for r in range(a, z):
+            end = min(a + ((r - a) // tile + 1) * tile, z)  # of the row's tile
+            steps = np.abs(hv[:end]).max() / 127
+            limit = ref.attend_bound(plain(q), hk[:r + 1], hv[:r + 1], o[r], 0.125, "bf16", True)
+            assert (np.abs(got[r - a] - o[r]) <= limit + 127 * steps * 2.0 ** -(60 if kernel == 2 else 40)).all(), r
