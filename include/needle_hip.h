@@ -573,12 +573,16 @@ int nh_kv8_read(nh_kv8* c, int layer, const int* seqs, const int* pos, const int
 /* Attention of the batch's rows, as nh_kv4_attend; under nh_kv8_ask every row
  * is at its sequence's last position, so it sees all of it, with a ring > 0 the
  * first `sink` and the last `ring` positions.  Scores, weights' sums and
- * products are held in f32.  f16 and bf16 queries enter as they are, f32 ones
- * to 2^-24 of a row's largest (one below 2^-100 as 0); f32 and f16 calls carry
- * 22 bits of a weight x its value's step, bf16 calls and calls of many f16 rows
- * 11, none finer than 2^-40 of the largest step (of many rows 2^-33 of the row's
- * largest weight x step, and a step below 2^-60 of the largest weighs as that).
- * A row's sum of weights x values, before its division by the weights' sum, has
+ * products are held in f32.  f16 and bf16 queries enter as they are (an element
+ * below 2^-31 of its row's largest loses bits), f32 ones to 2^-24 of a row's
+ * largest (one below 2^-100 as 0); 16-bit calls of few rows take a key's code as
+ * code + 128 and start its score at what that adds, so the partial sums are rounded
+ * at up to twice their size.  f32 and f16 calls carry 22 bits of a weight x its
+ * value's step, bf16 calls and calls of many f16 rows 11, none finer than 2^-40 of
+ * the largest step (of many rows 2^-33 of the row's largest weight x step, and a
+ * step below 2^-60 of the largest weighs as that); the largest step is that of the
+ * blocks that any row worked on with this one sees (up to 16 rows x heads of a
+ * sequence, of many rows 256).  A row's sum of weights x values, before its division by the weights' sum, has
  * to fit f32.
  * NH_EDEVICE: more than a launch takes, which is 2^31 rows x heads or 2^23 tiles
  * (for each sequence and kv head, 16 of its rows x query heads). */

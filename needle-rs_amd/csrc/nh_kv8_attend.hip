@@ -11,7 +11,7 @@
 // f16 number 1152 + c (one byte permutation for two), from which one packed
 // addition takes 1152: exact.  That is done to the values; a key's byte alone is the
 // f16 subnormal (128 + c) 2^-24, and the products' sums start at -128 2^-24 times the
-// query's own sum: 30.0 us became 28.8 in the last example below.  (Sums of weights and
+// query's own sum: 30.0 us became 28.6 in the last example below.  (Sums of weights and
 // values would lose to the offset what their signs cancel.)  f32 queries go the other
 // way: their rows as whole numbers of 23 bits in three signed digits of 8, times the
 // codes in the i8 MFMAs, which are exact and take the bytes as they are.
@@ -22,11 +22,14 @@
 //
 // One row a head is bound by the cache's bytes: 64 sequences of up to 8,192 keys, 32
 // heads over 8 of 128, bf16 (818 MB) 155 us, 5.2 TB/s, as a large copy; one of 131,072
-// keys (269 MB) 50 to 60 with the 4.5 of its join.  Few keys are bound by latency (374 of
+// keys (269 MB) 50 to 60 with the 4.5 of its join.  The 64 at other dims and in f32: 192 +
+// 128 dims 184 (f32 191), 256 + 256 290 (303), 128 + 128 f32 154, 5.3 to 5.6 TB/s.  Few keys are bound by latency (374 of
 // them 6.5 us on the GPU), so the first chunk's loads start before the queries are
 // operands.  More rows are bound by vector instructions, some 250 for 64 keys of 16
 // rows at 64 dims, 96 of them for codes turned into f16: four sequences' 448 rows over
-// 1,500 keys, 16 heads of 64, 28.8 us with the vector units three quarters busy.
+// 1,500 keys, 16 heads of 64, 28.6 us with the vector units three quarters busy.  512 rows
+// after 4,000 keys, 32 heads over 8 (the only kernel for f32, and for more than 128 dims, at
+// one wavefront a SIMD): 128 dims f32 89, 192 + 128 bf16 118 (f32 145), 256 + 256 177 (232).
 #include <algorithm>
 
 #include "nh_kv8_device.h"
@@ -401,6 +404,8 @@ static void tiles_of(const Kv8View& c, const int* row0, int per, int rows, Ka8Sh
 // 1,024 130 / 110, 2,048 220 / 135; four of 1,500 keys 128 rows 37 / 62, 256 67 / 56; 16
 // of 2,000 keys 32 rows 46 / 63, 64 rows 85 / 71.  16 heads of 64: 16 sequences of 2,000
 // keys 128 rows 53 / 58, 256 92 / 64; four of 1,500 512 rows 39 / 49, 1,024 62 / 51.
+// (Both kernels were swept at these two head shapes, causal and of even batches alone, before
+// the first one's keys became subnormals, which took 2 to 4 percent off it.)
 static double ka_join_us(const Kv8View& c, int heads, int64_t splits) {
     return splits > 1 ? 4.0 + (double)c.rows * heads * (double)splits * (c.dv + 2) * 8 / 2e6 : 0.0;
 }

@@ -21,8 +21,8 @@ namespace nh {
 // after one another leave it within f32.  (A unit fixed by the first 64 keys lost it
 // where later steps were 2^120 times as large.)
 //
-// 2 x 2,000 rows after 6,000 keys, 32 heads over 8 of 128 (427 GFLOP), bf16: 440 to 460
-// us, 930 to 970 TFLOP/s, where a large product reaches 1,320 to 1,370.  The matrix
+// 2 x 2,000 rows after 6,000 keys, 32 heads over 8 of 128 (427 GFLOP), bf16: 440 to 470
+// us, 910 to 970 TFLOP/s, where a large product reaches 1,320 to 1,370.  The matrix
 // cores are busy for half of the cycles: a row's 32 exponentials, and as many sums and
 // products, are vector work for nearly as long as its products, and two wavefronts a SIMD
 // do not overlap them whole.  With the turning of the codes and the records taken out
@@ -32,7 +32,7 @@ namespace nh {
 // wavefronts on images of 32 keys (530), sums by dot products (477), two chunks of
 // loads in registers (463) and exponentials put off by half a chunk (453 for 452).
 // At 64 dims there are half as many products for as many exponentials: 16 x 512 rows
-// over 2,000 keys, 16 heads, 123 to 138 us; a wavefront alone takes 3,000 cycles for 64
+// over 2,000 keys, 16 heads, 112 to 138 us; a wavefront alone takes 3,000 cycles for 64
 // keys, and more than two a SIMD have no registers (four wavefronts, three a SIMD: 154).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int KP8_WAVES = 8;

@@ -334,8 +334,9 @@ __device__ __forceinline__ void kv8_turn_keys(const typename KvElem<TYPE>::T* __
 // share a block, so rows that join one are stored by reading, halving and writing
 // it.
 // Bytes bound it: 7,490 rows of three prompts, 8 heads of 128 + 128 turned with 32
-// query heads, bf16 (169 MB) 34 to 37 us, 4.6 to 5 TB/s; a row of each of 8 sequences
-// 5.1 us, latency.  All three roles in one workgroup kept 386 scalar registers spilled
+// query heads, bf16 (169 MB) 34 to 37 us, 4.6 to 5 TB/s; their keys and values alone (46
+// MB) 13.5, turned 18, where a copy would take 8.9: a wavefront has one block's rows in
+// flight and then their codes to work out; a row of each of 8 sequences 5.1 us, latency.  All three roles in one workgroup kept 386 scalar registers spilled
 // and took twice as long; keys' rows through LDS where a lane holds both of a pair cost
 // 4 us of the 34.
 template <int TYPE, int WK, int WV, int TURN>
