@@ -109,8 +109,10 @@ int nh_kv8_append(nh_kv8* c, int layer, const void* k, const void* v, int64_t ld
     if (heads) a.q = nh::RopeRows{q, q_out, ldq, ldqo, heads};
     if (!c->captured) {
         hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing((hipStream_t)stream, &s) != hipSuccess) (void)hipGetLastError();
-        c->captured = s != hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing((hipStream_t)stream, &s) == hipSuccess)
+            c->captured = s != hipStreamCaptureStatusNone;
+        else
+            (void)hipGetLastError();  // (the null stream while another captures: the launch says what it thinks of it)
     }
     NH_TRY(nh::launch_kv8_append(c->v, c->book.batch_row0.data(), a, type, (hipStream_t)stream), "kv8 append");
     return NH_OK;
